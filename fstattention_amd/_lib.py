@@ -7,7 +7,8 @@ from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint3
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libfsta.so")
 
-F32, F16, BF16, F64 = 0, 1, 2, 3
+F32, F16, BF16, F64, FP8 = 0, 1, 2, 3, 4
+PAGED_ALL, PAGED_CAUSAL, PAGED_TREE = 0, 1, 2
 OK, EINVAL, EUNSUPPORTED, EHIP = 0, -1, -2, -3
 FLAG_FAST_PV, FLAG_GENERIC, FLAG_WIDE_WAVES, FLAG_SHARE_TILES, FLAG_STREAM = 1, 2, 4, 8, 16
 
@@ -75,6 +76,12 @@ SIGNATURES = {
     "fsta_medusa_workspace_bytes": (c_size_t, [c_int32, c_int32]),
     "fsta_medusa_tree_ws": (c_int, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_size_t,
                                     c_void_p]),
+    "fsta_paged_write": (c_int, [c_void_p] * 2 + [c_int64] * 4 + [c_void_p] * 7 + [c_int32] * 9 + [c_void_p]),
+    "fsta_paged_read": (c_int, [c_void_p] * 8 + [c_int32] * 9 + [c_void_p]),
+    "fsta_paged_attention_workspace_bytes": (c_size_t, [c_int32] * 6),
+    "fsta_paged_attention": (c_int, [c_void_p] + [c_int64] * 2 + [c_void_p] * 8 + [c_int32] + [c_void_p] * 2 + [c_int32] * 12 +
+                             [c_float, c_void_p, c_size_t, c_void_p]),
+    "fsta_tree_bits": (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
     "fsta_probe_empty_launch": (c_int, [c_int32, c_int32, c_void_p]),
     "fsta_probe_hbm_read": (c_int, [c_void_p, c_size_t, c_int32, c_int32, c_void_p, c_void_p]),
     "fsta_quantize_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int32]),

@@ -32,6 +32,8 @@ SOURCES = [
     "fsta_attention_prefix.hip",
     "fsta_attention_cache.hip",
     "fsta_attention_stream.hip",
+    "fsta_paged_cache.hip",
+    "fsta_paged_attention.hip",
     "fsta_roofline.hip",
 ]
 
@@ -46,7 +48,8 @@ HIPCC_FLAGS = [
 # Kernels of these sources must keep everything in registers: a private array the compiler leaves
 # in scratch memory, or a spill, is reloaded through the same vmcnt queue their gather rings count on.
 NO_SCRATCH = ("fsta_attention_mfma16.hip", "fsta_attention_mfma.hip", "fsta_attention_prefix.hip",
-              "fsta_attention_cache.hip", "fsta_attention_stream.hip", "fsta_attention_generic.hip", "fsta_attention_f32.hip")
+              "fsta_attention_cache.hip", "fsta_attention_stream.hip", "fsta_attention_generic.hip", "fsta_attention_f32.hip",
+              "fsta_paged_attention.hip")
 
 
 def _hipcc() -> str:

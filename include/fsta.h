@@ -28,6 +28,7 @@ extern "C" {
 #define FSTA_F16  1
 #define FSTA_BF16 2
 #define FSTA_F64  3  /* fsta_medusa_tree's probabilities only */
+#define FSTA_FP8  4  /* OCP e4m3 bytes: rows of a paged cache only */
 
 /* return codes */
 #define FSTA_OK            0
@@ -56,6 +57,11 @@ extern "C" {
                                /* fsta_attention_fwd_ws / fsta_attention_workspace_bytes:
                                   cut the shared prefix into n runs of keys (n = 1: never
                                   split; n = 0, i.e. no such flag: the library decides)   */
+
+/* which keys a new token sees in fsta_paged_attention */
+#define FSTA_PAGED_ALL    0  /* every key of its sequence                             */
+#define FSTA_PAGED_CAUSAL 1  /* those up to its own position                          */
+#define FSTA_PAGED_TREE   2  /* those in front of the new tokens, and by its mask row */
 
 /* bits of the status word written by fsta_precompute */
 #define FSTA_PRE_TOO_MANY_ANCESTORS 1u /* a block has more than max_ancestors unique ancestors */
@@ -436,6 +442,79 @@ size_t fsta_medusa_workspace_bytes(int32_t depths, int32_t topk);
 int fsta_medusa_tree_ws(const void* probs, int32_t probs_dtype, int32_t depths, int32_t topk,
                         int32_t n_nodes, int64_t* parent, uint32_t* status,
                         void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * A KV cache in pages, for a batch of sequences of different lengths (no counterpart in the
+ * reference, whose K and V are dense [prefix | tree] tensors, fstattention.py:188-196).
+ *   k_cache, v_cache [num_pages, kv_heads, page_size, head_dim] of cache_dtype: FSTA_F16,
+ *   FSTA_BF16, or FSTA_FP8 with k_exponent, v_exponent [num_pages, kv_heads, page_size] bytes:
+ *   a row's value is byte * 2^(exponent - 127).  page_size a power of two from 16 to 4096,
+ *   head_dim 64 or 128.
+ *   page_table [batch, width] int32: position p of sequence b is row p % page_size of page
+ *   page_table[b][p / page_size].  Entries outside [0, num_pages) name no page: nothing is
+ *   written there, the keys are not attended to and read as zeros.
+ *   kv_lens [batch] int32: positions of a sequence, its new tokens included.
+ *   q_starts [batch + 1] int32, ascending: tokens q_starts[b] .. q_starts[b + 1] - 1 of the packed
+ *   tensors are sequence b's new ones, at its last positions.  The arrays are read on the device
+ *   and kept within the tensors' sizes there; the host never waits for them.
+ * Alignment: tensors 16 bytes (strides multiples of 8 elements, the last dimension contiguous),
+ * arrays and exponents 4 bytes.
+ *
+ * fsta_paged_write: rows k, v [tokens, kv_heads, head_dim] (strides in elements) of the new tokens
+ * go to their places; no place: not written.  FSTA_FP8: exponent = the smallest with max |x| <= 448
+ * 2^(exponent - 127) over the row's finite values, within [17, 247] (127 for a row of zeros); bytes
+ * are rounded to nearest even, infinities and NaNs become NaN.  Two tokens must not have one place.
+ */
+int fsta_paged_write(const void* k, const void* v, int64_t k_token_stride, int64_t k_head_stride,
+                     int64_t v_token_stride, int64_t v_head_stride, void* k_cache, void* v_cache,
+                     uint8_t* k_exponent, uint8_t* v_exponent, const int32_t* page_table,
+                     const int32_t* kv_lens, const int32_t* q_starts, int32_t batch, int32_t width,
+                     int32_t tokens, int32_t num_pages, int32_t page_size, int32_t kv_heads,
+                     int32_t head_dim, int32_t dtype, int32_t cache_dtype, void* stream);
+
+/*
+ * fsta_paged_read: the pages of a batch as dense k, v [batch, kv_heads, max_len, head_dim] of dtype
+ * (16-bit; FSTA_FP8 rows widened, exactly for FSTA_BF16, to the nearest for FSTA_F16); positions at
+ * or past kv_lens and those on no page are zeros.
+ */
+int fsta_paged_read(const void* k_cache, const void* v_cache, const uint8_t* k_exponent,
+                    const uint8_t* v_exponent, const int32_t* page_table, const int32_t* kv_lens,
+                    void* k, void* v, int32_t batch, int32_t width, int32_t max_len, int32_t num_pages,
+                    int32_t page_size, int32_t kv_heads, int32_t head_dim, int32_t dtype,
+                    int32_t cache_dtype, void* stream);
+
+/*
+ * fsta_paged_attention: o[t, h] = sum_p softmax_p(q[t, h] . k_p * sm_scale) v_p over the positions p
+ * of the token's sequence that `mask` (FSTA_PAGED_*) lets it see, with K/V head h / (heads /
+ * kv_heads).  q [tokens, heads, head_dim] of dtype (FSTA_F16, FSTA_BF16; strides in elements), o
+ * contiguous; lse [tokens, heads] float32 or NULL: base-2 log-sum-exp, as fsta_attention_fwd's.  A
+ * token that sees nothing has o = 0 and lse = -inf; rows of tokens of no sequence are not written.
+ * FSTA_PAGED_TREE: the token sees all positions in front of its sequence's new tokens, and the j-th
+ * new one where bit j % 32 of word j / 32 of its row of tree_bits [tokens, tree_words] is set (bits
+ * past the row are 0).  sm_scale > 0.  max_q_len: the most new tokens a sequence has, or 0; it
+ * steers the choice of kernel only.  The workspace (16-byte aligned, always needed) holds the parts
+ * of sequences whose keys are dealt to several workgroups; it is free again when the work queued on
+ * `stream` has run.  tokens * heads < 2^30, batch <= 65536.
+ */
+size_t fsta_paged_attention_workspace_bytes(int32_t batch, int32_t tokens, int32_t max_q_len,
+                                            int32_t heads, int32_t kv_heads, int32_t head_dim);
+int fsta_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                         const void* k_cache, const void* v_cache, const uint8_t* k_exponent,
+                         const uint8_t* v_exponent, const int32_t* page_table, const int32_t* kv_lens,
+                         const int32_t* q_starts, const uint32_t* tree_bits, int32_t tree_words, void* o,
+                         float* lse, int32_t batch, int32_t width, int32_t tokens, int32_t max_q_len,
+                         int32_t num_pages, int32_t page_size, int32_t heads, int32_t kv_heads,
+                         int32_t head_dim, int32_t dtype, int32_t cache_dtype, int32_t mask,
+                         float sm_scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * fsta_tree_bits: parent [tokens] int64, the parent of every node of a batch of trees by its number
+ * within its tree (smaller than the node's own; anything else counts as a root, as in
+ * fsta_lineage_from_parents) -> bits [tokens, words]: bit j of a node's row is set where j is the
+ * node or one of its ancestors (utils.py:66-75's lineage as a mask).  Nodes of no tree: zeros.
+ */
+int fsta_tree_bits(const int64_t* parent, const int32_t* q_starts, int32_t batch, int32_t tokens,
+                   int32_t words, uint32_t* bits, void* stream);
 
 /*
  * Measuring aids (no counterpart in the reference; bench.py reports them beside
