@@ -4,7 +4,7 @@
 // rows sees one K/V head, so every key is read once for the whole group.  A wave owns 32 rows as the columns of
 //     S^T = K_tile . Q^T      and      O^T += V_tile^T . P^T        (32x32x16 matrix instructions, 32 keys a tile)
 // with a float32 base-2 online softmax in between; P stays in the registers the scores came in.  R waves share a tile of keys
-// (row groups), S tiles are worked on at a time (key shares, joined at the end through LDS): (R, S) = (1, 4), (2, 2), (4, 1).
+// (row groups), S tiles are worked on at a time (key shares, joined at the end through LDS): (R, S) = (1, 4), (1, 1), (2, 2), (4, 1).
 // Keys and values come page by page straight into an LDS ring (global -> LDS transfers of 1 KiB); rows that do not exist (past
 // the sequence's end, on a page outside the cache) come from a row of zeros, so that what lies in unused rows of a page can not
 // turn a weight of zero into a NaN.
@@ -16,8 +16,9 @@ namespace {
 
 using namespace mfma;
 
-constexpr int kWaves = 4;
-constexpr int kLeastTiles = 4;            // a run of keys has at least that many tiles
+
+constexpr int kDecodeShares = 4, kDecodeUnits = 1024, kMiddleUnits = 512, kChunkUnits = 256;
+constexpr int kDecodeLeast = 16, kChunkLeast = 8;
 
 enum Mask { kAll = 0, kCausal = 1, kTree = 2 };
 
@@ -34,7 +35,8 @@ struct PagedAttnParams {
     const uint32_t* tree_bits;     // [tokens, tree_words]
     float* part_o;                 // [part][kv_heads][rows][D]
     float* part_lse;               // [part][kv_heads][rows]
-    int32_t tree_words, mask, group, tile_rows, parts, run_units;
+    int32_t tree_words, mask, group, tile_rows, parts;
+    int32_t run_units, least_tiles; // units the launch is cut into where it has fewer, and the least tiles of a run
     float scale_log2e;
 };
 
@@ -51,61 +53,57 @@ struct Cut {
         return (int)(((int64_t)s.fresh * p.group + p.tile_rows - 1) / p.tile_rows);
     }
     __device__ __forceinline__ static int key_tiles(const SeqLens& s) { return max((s.keys + kTileN - 1) / kTileN, 1); }
-    __device__ __forceinline__ uint32_t runs(const SeqLens& s) const {
-        const uint32_t n = ((uint32_t)key_tiles(s) + longest - 1) / longest;
-        return n;
-    }
+    __device__ __forceinline__ uint32_t runs(const SeqLens& s) const { return ((uint32_t)key_tiles(s) + longest - 1) / longest; }
 };
-
-__device__ __forceinline__ Cut make_cut(const PagedAttnParams& p, int lane) {
-    uint64_t cost = 0;
-    for (int c = 0; c < p.batch.batch; c += 64) {
-        const SeqLens s = seq_lens(p.batch, c + lane);
-        // (summed in two pieces; from 2^49 on, where nothing is cut, it may be too small)
-        const uint64_t mine = (uint64_t)Cut::row_tiles(s, p) * (uint64_t)Cut::key_tiles(s);
-        const uint32_t low = (uint32_t)mine & 0xffffffu, high = (uint32_t)min(mine >> 24, (uint64_t)1 << 25);
-        cost += (uint32_t)__builtin_amdgcn_readlane((int)wave_prefix_sum(low), 63);
-        cost += (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)wave_prefix_sum(high), 63) << 24;
-    }
-    cost *= (uint64_t)p.batch.kv_heads;
-    const uint64_t longest = (cost + (uint32_t)p.run_units - 1) / (uint32_t)p.run_units;
-    return Cut{(uint32_t)min(max(longest, (uint64_t)kLeastTiles), (uint64_t)0x7fffffff)};
-}
 
 struct Place {
     SeqLens s;
     int seq, row_tile, run, runs, part;      // part: of the tile's first run, -1 where the keys are not cut
 };
 
-// The item-th (tile of rows, run of keys) of the batch, or with `joins` the item-th tile whose keys are cut; the tiles of a
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)x, lane); }
+
+// The item-th (tile of rows, run of keys) of the batch, or with JOINS the item-th tile whose keys are cut; the tiles of a
 // sequence last ones first (causal: they have most keys).  False: there is no such item.
-template <bool JOINS> __device__ __forceinline__ bool find_item(const PagedAttnParams& p, const Cut& cut, uint32_t item, int lane, Place* out) {
+template <bool JOINS> __device__ __forceinline__ bool find_item(const PagedAttnParams& p, uint32_t item, int lane, Place* out) {
+    const SeqLens first = seq_lens(p.batch, lane);       // (the first 64 sequences' lengths are loaded once)
+    uint64_t cost = 0;
+    for (int c = 0; c < p.batch.batch; c += 64) {
+        const SeqLens s = c ? seq_lens(p.batch, c + lane) : first;
+        // (summed in two pieces; from 2^49 on, where nothing is cut, it may be too small)
+        const uint64_t mine = (uint64_t)Cut::row_tiles(s, p) * (uint64_t)Cut::key_tiles(s);
+        const uint32_t low = (uint32_t)mine & 0xffffffu, high = (uint32_t)min(mine >> 24, (uint64_t)1 << 25);
+        cost += lane_of(wave_prefix_sum(low), 63);
+        cost += (uint64_t)lane_of(wave_prefix_sum(high), 63) << 24;
+    }
+    // (rounded up, in float: a rounding of 2^-24 moves the cut by nothing that counts, and both kernels round alike)
+    const float longest = ceilf((float)cost * (float)p.batch.kv_heads / (float)p.run_units);
+    const Cut cut{(uint32_t)fminf(fmaxf(longest, (float)p.least_tiles), 1073741824.f)};
     uint32_t parts = 0;
     for (int c = 0; c < p.batch.batch; c += 64) {
-        const SeqLens s = seq_lens(p.batch, c + lane);
+        const SeqLens s = c ? seq_lens(p.batch, c + lane) : first;
         const uint32_t tiles = (uint32_t)Cut::row_tiles(s, p), runs = cut.runs(s);
-        const uint32_t mine = JOINS ? (runs > 1 ? tiles : 0u) : tiles * runs;
         const uint32_t cut_items = runs > 1 ? tiles * runs : 0u;
+        const uint32_t mine = !JOINS ? tiles * runs : runs > 1 ? tiles : 0u;
         const uint32_t upto = wave_prefix_sum(mine), parts_upto = wave_prefix_sum(cut_items);
-        const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+        const uint32_t all = lane_of(upto, 63);
         if (item < all) {
             const int who = __builtin_ctzll(__ballot(upto > item));
-            auto of = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, who); };
             out->seq = c + who;
-            out->s.start = (int)of((uint32_t)s.start);
-            out->s.fresh = (int)of((uint32_t)s.fresh);
-            out->s.keys = (int)of((uint32_t)s.keys);
-            const uint32_t n_tiles = of(tiles), n_runs = of(runs);
-            const uint32_t in_seq = item - (of(upto) - of(mine));
+            out->s.start = (int)lane_of((uint32_t)s.start, who);
+            out->s.fresh = (int)lane_of((uint32_t)s.fresh, who);
+            out->s.keys = (int)lane_of((uint32_t)s.keys, who);
+            const uint32_t n_tiles = lane_of(tiles, who), n_runs = lane_of(runs, who);
+            const uint32_t in_seq = item - (lane_of(upto, who) - lane_of(mine, who));
             const uint32_t t = JOINS ? in_seq : in_seq / n_runs;
             out->row_tile = (int)(n_tiles - 1 - t);
             out->run = JOINS ? 0 : (int)(in_seq - t * n_runs);
             out->runs = (int)n_runs;
-            out->part = n_runs > 1 ? (int)(parts + of(parts_upto) - of(cut_items) + t * n_runs) : -1;
+            out->part = n_runs > 1 ? (int)(parts + lane_of(parts_upto, who) - lane_of(cut_items, who) + t * n_runs) : -1;
             return true;
         }
         item -= all;
-        parts += (uint32_t)__builtin_amdgcn_readlane((int)parts_upto, 63);
+        parts += lane_of(parts_upto, 63);
     }
     return false;
 }
@@ -119,27 +117,54 @@ __device__ __forceinline__ int keys_of_tile(const PagedAttnParams& p, const SeqL
 
 // ---- the kernel -----------------------------------------------------------------------------------------------------------
 
-template <int D, int R, bool FP8> struct Shape {
-    static constexpr int S = kWaves / R;
-    static constexpr int kStages = R == 4 ? 4 : 2;
+// 8-bit tiles: up to two row groups read them as they are and widen in registers; four share a widened copy.
+template <int D, int R, int S, bool FP8> struct Shape {
+    static constexpr bool kWiden = FP8 && R > 2;
+    static constexpr int kStages = R == 4 ? 4 : FP8 ? 4 : 2;
     static constexpr int kRowBytes = FP8 ? D : 2 * D;             // a key's or a value's row in the cache
     static constexpr int kDma = 2 * kTileN * kRowBytes / 1024;    // transfers of a tile's K and V
     static constexpr int kPer = kDma / R;                         // of them a wave's
     static constexpr int kPerTile = kPer + (FP8 ? 1 : 0);         // (and one of the exponents)
     static constexpr int kRawBytes = kDma * 1024 + (FP8 ? 256 : 0);
     static constexpr int kWideBytes = 2 * kTileN * D * 2;
-    static constexpr int kShareBytes = kStages * kRawBytes + (FP8 ? kWideBytes : 0);
-    static constexpr size_t kLds = (size_t)S * kShareBytes;
+    static constexpr int kShareBytes = kStages * kRawBytes + (kWiden ? kWideBytes : 0);
+    static constexpr size_t kJoin = (size_t)(S - 1) * R * (32 * D + 64) * 4;
+    static constexpr size_t kLds = (size_t)S * kShareBytes > kJoin ? (size_t)S * kShareBytes : kJoin;
     static_assert(kDma % R == 0, "a wave has whole transfers");
-    static_assert(kLds >= (size_t)(S - 1) * R * (32 * D + 64) * 4, "the join needs that much");
 };
 
-template <bool BF16, int D, int R, bool FP8, bool SPLIT>
-__global__ __launch_bounds__(kWaves * 64, 2) void paged_attn_kernel(PagedAttnParams p) {
-    using SH = Shape<D, R, FP8>;
+// Positions of 16-byte chunks in rows of an 8-bit tile: keys are read 8 bytes from each of 32 rows, values 32 bytes from each
+// of 16 (by the transposing read)
+template <int D> __device__ __forceinline__ int k8_chunk(int row, int c) { return D == 128 ? c ^ ((row >> 1) & 7) : c ^ ((row >> 2) & 3); }
+template <int D> __device__ __forceinline__ int v8_chunk(int row, int c) { return D == 128 ? c ^ (2 * ((row >> 1) & 3)) : c ^ (2 * ((row >> 2) & 1)); }
+
+// 8 e4m3 bytes times a power of two, in the 16-bit type
+template <bool BF16> __device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi, float scale) {
+    u32x4 w;
+    if constexpr (BF16) {
+        w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
+        w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
+        w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
+        w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
+    } else {
+        w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, false));
+        w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, true));
+        w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, false));
+        w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, true));
+    }
+    return w;
+}
+
+// SPLIT: weights go to the matrix cores as pairs of bfloat16, hi + lo
+template <bool BF16, int D, int R, int S, bool FP8, bool SPLIT>
+__global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnParams p) {
+    using SH = Shape<D, R, S, FP8>;
+    constexpr bool kDirect = FP8 && !SH::kWiden;
     using MM = Mma<BF16>;
+    using PV = Mma<BF16 || kDirect>;          // weights times values: 8-bit values are exact in bfloat16 whatever their scale
     using Frag = typename MM::frag;
-    constexpr int S = SH::S, kStages = SH::kStages;
+    using PFrag = typename PV::frag;
+    constexpr int kStages = SH::kStages;
     constexpr int kSteps = D / 16;            // matrix instructions of a tile's scores
     constexpr int kDTiles = D / 32;           // 32-row tiles of O^T
     constexpr float kTrustedSum = BF16 ? 16777216.f : 32768.f;
@@ -155,8 +180,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_attn_kernel(PagedAttnPar
     const uint32_t item = blockIdx.x / (uint32_t)p.batch.kv_heads;
     const int head = (int)(blockIdx.x - item * (uint32_t)p.batch.kv_heads);
     Place at;
-    const Cut cut = make_cut(p, lane);
-    if (!find_item<false>(p, cut, item, lane, &at)) return;
+    if (!find_item<false>(p, item, lane, &at)) return;
     const SeqLens s = at.s;
     const int old = s.keys - s.fresh;         // keys in front of the new tokens (negative: the first new ones have no place)
 
@@ -205,7 +229,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_attn_kernel(PagedAttnPar
         dma_is_v[i] = u >= SH::kDma / 2;
         const int r = (u % (SH::kDma / 2)) * kRowsPerDma + lane / kLanesPerRow;
         const int slot = lane % kLanesPerRow;
-        const int chunk = FP8 ? slot : dma_is_v[i] ? v_chunk<D>(r, slot) : k_chunk<D>(r, slot);
+        const int chunk = SH::kWiden ? slot : FP8 ? (dma_is_v[i] ? v8_chunk<D>(r, slot) : k8_chunk<D>(r, slot)) : dma_is_v[i] ? v_chunk<D>(r, slot) : k_chunk<D>(r, slot);
         dma_row[i] = r;
         dma_off[i] = (uint32_t)((r & 15) * SH::kRowBytes + chunk * 16);
     }
@@ -260,8 +284,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_attn_kernel(PagedAttnPar
     const uint32_t k_lane0 = (uint32_t)(ql * D + k_chunk<D>(ql, half) * 8) * 2;
     const int tr_row = 4 * half + ((lane & 15) >> 2), tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
     const uint32_t v_lane0 = (uint32_t)(tr_row * D + v_chunk<D>(tr_row, tr_col >> 3) * 8 + (tr_col & 7)) * 2;
+    // (8-bit tiles: rows of D bytes; the transposing read hands a lane 8 keys, four from either 8-key half)
+    const uint32_t k8_lane0 = (uint32_t)(ql * D + k8_chunk<D>(ql, 0) * 16 + 8 * half);
+    const int tr8_row = 4 * half + ((lane & 15) >> 1) + ((lane & 8) ? 4 : 0);
+    const uint32_t v8_lane0 = (uint32_t)(tr8_row * D + v8_chunk<D>(tr8_row, (lane >> 4) & 1) * 16 + 8 * (lane & 1));
     const float sc = p.scale_log2e;
     typedef const u32x4 __attribute__((address_space(3))) * lds_u32x4;
+    typedef const u32x2 __attribute__((address_space(3))) * lds_u32x2;
+    typedef const uint32_t __attribute__((address_space(3))) * lds_u32;
+    typedef const uint8_t __attribute__((address_space(3))) * lds_u8;
 
     auto compute = [&](int i, const unsigned char* tile_lds) {
         const int tile = tile0 + share + i * S, first = tile * kTileN;
@@ -270,11 +301,22 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_attn_kernel(PagedAttnPar
         f32x16 sv;
 #pragma unroll
         for (int e = 0; e < 16; ++e) sv[e] = 0.f;
-        const uint32_t k_addr0 = lds_addr(tile_lds) + k_lane0;
+        const uint32_t exps = lds_addr(tile_lds) + SH::kDma * 1024;      // (8-bit tiles read as they are)
+        if constexpr (kDirect) {
+            const uint32_t k_addr0 = lds_addr(tile_lds) + k8_lane0;
+            const float scale = __builtin_bit_cast(float, min((uint32_t)*(lds_u8)(uintptr_t)(exps + ql), 254u) << 23);
 #pragma unroll
-        for (int ks = 0; ks < kSteps; ++ks) {
-            const u32x4 raw = *(lds_u32x4)(uintptr_t)(k_addr0 ^ (uint32_t)(ks << 5));
-            sv = MM::mfma(__builtin_bit_cast(Frag, raw), qf[ks], sv);
+            for (int ks = 0; ks < kSteps; ++ks) {
+                const u32x2 raw = *(lds_u32x2)(uintptr_t)(k_addr0 ^ (uint32_t)(ks << 4));
+                sv = MM::mfma(__builtin_bit_cast(Frag, widen8<BF16>(raw[0], raw[1], scale)), qf[ks], sv);
+            }
+        } else {
+            const uint32_t k_addr0 = lds_addr(tile_lds) + k_lane0;
+#pragma unroll
+            for (int ks = 0; ks < kSteps; ++ks) {
+                const u32x4 raw = *(lds_u32x4)(uintptr_t)(k_addr0 ^ (uint32_t)(ks << 5));
+                sv = MM::mfma(__builtin_bit_cast(Frag, raw), qf[ks], sv);
+            }
         }
         // which of the tile's keys this lane's row sees
         const uint32_t bad = (bad_halves >> (2 * (i % kStages))) & 3u;
@@ -330,38 +372,60 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_attn_kernel(PagedAttnPar
                 sum += pw[e];
             }
         }
-        Frag ph[2], pl[2];
+        l_i += sum;
+        if constexpr (kDirect) {              // the values' powers of two go to the weights (exponents of unused rows may be anything)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t four = *(lds_u32)(uintptr_t)(exps + kTileN + 8 * j + 4 * half);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    pw[4 * j + e] *= __builtin_bit_cast(float, min((four >> (8 * e)) & 255u, 254u) << 23);
+            }
+        }
+        PFrag ph[2], pl[2];
 #pragma unroll
         for (int k2 = 0; k2 < 2; ++k2) {
             u32x4 hi4, lo4;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float a = pw[8 * k2 + 2 * e], b = pw[8 * k2 + 2 * e + 1];
-                const uint32_t hi = MM::pack(a, b);
+                const uint32_t hi = PV::pack(a, b);
                 hi4[e] = hi;
-                if (SPLIT) lo4[e] = MM::pack(a - MM::low(hi), b - MM::high(hi));
+                if (SPLIT) lo4[e] = PV::pack(a - PV::low(hi), b - PV::high(hi));
             }
-            ph[k2] = __builtin_bit_cast(Frag, hi4);
-            if (SPLIT) pl[k2] = __builtin_bit_cast(Frag, lo4);
+            ph[k2] = __builtin_bit_cast(PFrag, hi4);
+            if (SPLIT) pl[k2] = __builtin_bit_cast(PFrag, lo4);
         }
-        l_i += sum;
         // O^T
-        const uint32_t v_addr0 = lds_addr(tile_lds) + (uint32_t)(kTileN * D * 2) + v_lane0;
 #pragma unroll
         for (int dt = 0; dt < kDTiles; ++dt) {
-            const uint32_t addr = v_addr0 ^ (uint32_t)(dt << 6);
-            VPair f0, f1;
-            f0.a = lds_read_tr16(addr);
-            f0.b = lds_read_tr16_at<8 * D * 2>(addr);
-            f1.a = lds_read_tr16_at<16 * D * 2>(addr);
-            f1.b = lds_read_tr16_at<24 * D * 2>(addr);
-            lds_wait();
-            lds_tie(f0.a); lds_tie(f0.b); lds_tie(f1.a); lds_tie(f1.b);
-            o[dt] = MM::mfma(__builtin_bit_cast(Frag, f0), ph[0], o[dt]);
-            o[dt] = MM::mfma(__builtin_bit_cast(Frag, f1), ph[1], o[dt]);
+            PFrag f0, f1;
+            if constexpr (kDirect) {
+                const uint32_t addr = (lds_addr(tile_lds) + (uint32_t)(kTileN * D) + v8_lane0) ^ (uint32_t)(dt << 5);
+                u32x2 a, b;
+                asm volatile("ds_read_b64_tr_b8 %0, %1" : "=v"(a) : "v"(addr) : "memory");
+                asm volatile("ds_read_b64_tr_b8 %0, %1 offset:%2" : "=v"(b) : "v"(addr), "n"(16 * D) : "memory");
+                lds_wait();
+                lds_tie(a); lds_tie(b);
+                f0 = __builtin_bit_cast(PFrag, widen8<true>(a[0], a[1], 1.f));
+                f1 = __builtin_bit_cast(PFrag, widen8<true>(b[0], b[1], 1.f));
+            } else {
+                const uint32_t addr = (lds_addr(tile_lds) + (uint32_t)(kTileN * D * 2) + v_lane0) ^ (uint32_t)(dt << 6);
+                VPair v0, v1;
+                v0.a = lds_read_tr16(addr);
+                v0.b = lds_read_tr16_at<8 * D * 2>(addr);
+                v1.a = lds_read_tr16_at<16 * D * 2>(addr);
+                v1.b = lds_read_tr16_at<24 * D * 2>(addr);
+                lds_wait();
+                lds_tie(v0.a); lds_tie(v0.b); lds_tie(v1.a); lds_tie(v1.b);
+                f0 = __builtin_bit_cast(PFrag, v0);
+                f1 = __builtin_bit_cast(PFrag, v1);
+            }
+            o[dt] = PV::mfma(f0, ph[0], o[dt]);
+            o[dt] = PV::mfma(f1, ph[1], o[dt]);
             if (SPLIT) {
-                o[dt] = MM::mfma(__builtin_bit_cast(Frag, f0), pl[0], o[dt]);
-                o[dt] = MM::mfma(__builtin_bit_cast(Frag, f1), pl[1], o[dt]);
+                o[dt] = PV::mfma(f0, pl[0], o[dt]);
+                o[dt] = PV::mfma(f1, pl[1], o[dt]);
             }
         }
     };
@@ -385,19 +449,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_attn_kernel(PagedAttnPar
             const float scale = __builtin_bit_cast(float, min(E, 254u) << 23);     // (exponents of unused rows may be anything)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint32_t lo = bytes[2 * h], hi = bytes[2 * h + 1];
-                u32x4 w;
-                if constexpr (BF16) {
-                    w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
-                    w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
-                    w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
-                    w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
-                } else {
-                    w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, false));
-                    w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, true));
-                    w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, false));
-                    w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, true));
-                }
+                const u32x4 w = widen8<BF16>(bytes[2 * h], bytes[2 * h + 1], scale);
                 const int rr = r & (kTileN - 1);
                 const int chunk = is_v ? v_chunk<D>(rr, 2 * c + h) : k_chunk<D>(rr, 2 * c + h);
                 lds_write_b128(wide + (uint32_t)((is_v ? kTileN * D * 2 : 0) + rr * D * 2 + chunk * 16), w);
@@ -410,10 +462,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_attn_kernel(PagedAttnPar
         wait_tiles_outstanding<SH::kPerTile>(max(issued - i - 1, 0));
         auto refill = [&]() { if (issued < my_tiles) { issue(issued); ++issued; } };
         if constexpr (R > 1) { ring_barrier(); refill(); }
-        if constexpr (FP8) {
+        if constexpr (SH::kWiden) {
             if (i < my_tiles) widen(i);
-            if constexpr (R > 1) { ring_barrier(); }
-            else lds_wait();
+            ring_barrier();
             if (i < my_tiles) compute(i, ring + kStages * SH::kRawBytes);
         } else {
             if (i < my_tiles) compute(i, ring + (i % kStages) * SH::kRawBytes);
@@ -490,48 +541,86 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_attn_kernel(PagedAttnPar
     }
 }
 
-// Joins the runs of a tile's keys: a workgroup per (tile whose keys are cut, K/V head), a wave per row, two head dims (or one)
-// per lane, in the order of the runs.
-template <bool BF16, int D>
+// Joins the runs of a tile's keys, in an order that the run count alone decides: D / 4 lanes take a row and every SUBS-th run of
+// it, four runs' loads in flight at a time; what they have is joined through LDS.  A workgroup takes ROWS rows at a time of a
+// (tile whose keys are cut, K/V head).
+template <bool BF16, int D, int ROWS>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int kLanes = D / 4, kSubs = 256 / kLanes / ROWS;
+    __shared__ float shared_o[kSubs > 1 ? 256 : 1][5];
+    __shared__ float shared_l[kSubs > 1 ? 256 : 1];
+    const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t item = blockIdx.x / (uint32_t)p.batch.kv_heads;
     const int head = (int)(blockIdx.x - item * (uint32_t)p.batch.kv_heads);
     Place at;
-    const Cut cut = make_cut(p, lane);
-    if (!find_item<true>(p, cut, item, lane, &at)) return;
+    if (!find_item<true>(p, item, lane, &at)) return;
     const int rows = (int)min((int64_t)at.s.fresh * p.group - (int64_t)at.row_tile * p.tile_rows, (int64_t)p.tile_rows);
-    constexpr int kPer = D / 64;
-    const int runs = min(at.runs, p.parts - at.part);
-    for (int r = wave; r < rows; r += 4) {
-        float m = -INFINITY;
-        const int64_t row0 = ((int64_t)at.part * p.batch.kv_heads + head) * p.tile_rows + r, step = (int64_t)p.batch.kv_heads * p.tile_rows;
-        bool nan = false;
-        for (int i = 0; i < runs; ++i) {
-            const float l = p.part_lse[row0 + i * step];
-            nan |= l != l;
-            m = fmaxf(m, l);
-        }
-        float sum = 0.f, acc[kPer];
+    const int runs = max(min(at.runs, p.parts - at.part), 0);
+    const int my = tid / kLanes, sub = my / ROWS, col = 4 * (tid % kLanes);
+    for (int r0 = blockIdx.y * ROWS; r0 < rows; r0 += gridDim.y * ROWS) {
+        const int r = r0 + my % ROWS;
+        float m = -INFINITY, sum = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        if (r < rows) {
+            const int64_t row0 = ((int64_t)at.part * p.batch.kv_heads + head) * p.tile_rows + r, step = (int64_t)p.batch.kv_heads * p.tile_rows;
+            for (int i0 = sub; i0 < runs; i0 += 4 * kSubs) {
+                float l[4];
+                f32x4 x[4];
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
-        for (int i = 0; i < runs; ++i) {
-            const float l = p.part_lse[row0 + i * step];
-            if (l == -INFINITY) continue;
-            const float w = __builtin_amdgcn_exp2f(l - m);
-            sum += w;
-            const float* src = p.part_o + (row0 + i * step) * D + lane * kPer;
+                for (int j = 0; j < 4; ++j) {
+                    const int64_t row = row0 + (int64_t)min(i0 + j * kSubs, runs - 1) * step;
+                    l[j] = p.part_lse[row];
+                    x[j] = *reinterpret_cast<const f32x4*>(p.part_o + row * D + col);
+                }
+                float top = m;
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) acc[e] += w * src[e];
+                for (int j = 0; j < 4; ++j) {
+                    if (i0 + j * kSubs >= runs) l[j] = -INFINITY;
+                    top = fmaxf(top, l[j]);
+                }
+                if (top == -INFINITY && !(l[0] != l[0] || l[1] != l[1] || l[2] != l[2] || l[3] != l[3])) continue;    // nothing seen so far
+                const float back = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+                m = top;
+                sum *= back;
+                acc *= back;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (l[j] == -INFINITY) continue;
+                    const float w = __builtin_amdgcn_exp2f(l[j] - top);      // (a NaN stays one)
+                    sum += w;
+                    acc += x[j] * w;
+                }
+            }
         }
-        const float inv = nan ? __builtin_nanf("") : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+        if constexpr (kSubs > 1) {
+            shared_l[tid] = m;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) shared_o[tid][e] = acc[e];
+            shared_o[tid][4] = sum;
+            __syncthreads();
+            if (sub == 0)
+                for (int other = 1; other < kSubs; ++other) {
+                    const int t = tid + other * ROWS * kLanes;
+                    const float m_b = shared_l[t], sum_b = shared_o[t][4];
+                    if (m_b == -INFINITY && sum_b == 0.f) continue;
+                    const float top = fmaxf(m, m_b);
+                    const float fa = m == -INFINITY && sum == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - top);
+                    const float fb = __builtin_amdgcn_exp2f(m_b - top);
+                    m = top;
+                    sum = sum * fa + sum_b * fb;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[e] = acc[e] * fa + shared_o[t][e] * fb;
+                }
+            __syncthreads();
+        }
+        if (sub > 0 || r >= rows) continue;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const int64_t flat = (int64_t)at.row_tile * p.tile_rows + r;
         const int token = (int)(flat / p.group);
         const int64_t out_row = (int64_t)(at.s.start + token) * (p.batch.kv_heads * p.group) + head * p.group + (flat - (int64_t)token * p.group);
-        if (p.lse && lane == 0) p.lse[out_row] = nan ? __builtin_nanf("") : sum == 0.f ? -INFINITY : m + log2f(sum);
-        uint16_t* dst = static_cast<uint16_t*>(p.o) + out_row * D + lane * kPer;
-        if constexpr (kPer == 2) *reinterpret_cast<uint32_t*>(dst) = Mma<BF16>::pack_out(acc[0] * inv, acc[1] * inv);
-        else *dst = (uint16_t)Mma<BF16>::pack_out(acc[0] * inv, 0.f);
+        if (p.lse && col == 0) p.lse[out_row] = sum == 0.f ? -INFINITY : m + log2f(sum);
+        const u32x2 w = {Mma<BF16>::pack_out(acc[0] * inv, acc[1] * inv), Mma<BF16>::pack_out(acc[2] * inv, acc[3] * inv)};
+        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.o) + out_row * D + col) = w;
     }
 }
 
@@ -540,55 +629,68 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
 // Rows of a workgroup's tile by the most rows a sequence can have: up to 32 rows the keys are all there is to read and its
 // waves share them out; from 128 rows on every wave has rows of its own.
 int rows_of_tile(int64_t most_rows) { return most_rows <= 32 ? 32 : most_rows <= 64 ? 64 : 128; }
-constexpr int kUnitsWanted = 1024;        // (tile, run, K/V head) units a launch is cut into: two per workgroup slot
 
 struct Sizes {
-    int tile_rows;
+    int tile_rows, shares;
+    int64_t most_rows;          // of a sequence, as far as the host knows
     int64_t row_tiles;          // at most, over the batch
-    int64_t run_units, items, parts;
+    int64_t items, parts;
+    int run_units, least_tiles;
 };
 Sizes sizes_of(int32_t batch, int32_t tokens, int32_t max_q_len, int32_t heads, int32_t kv_heads) {
     Sizes z;
     const int group = heads / kv_heads;
-    const int64_t most = max_q_len > 0 && max_q_len < tokens ? max_q_len : tokens;
-    z.tile_rows = rows_of_tile(most * group);
+    z.most_rows = (int64_t)(max_q_len > 0 && max_q_len < tokens ? max_q_len : tokens) * group;
+    z.tile_rows = rows_of_tile(z.most_rows);
     z.row_tiles = ((int64_t)tokens * group + (int64_t)(batch < tokens ? batch : tokens) * (z.tile_rows - 1)) / z.tile_rows;
-    z.run_units = kUnitsWanted;
-    // a run has at least cost / run_units tiles, and a tile of rows one run more than whole ones
-    const int64_t runs = (z.run_units + kv_heads - 1) / kv_heads;
+    z.shares = z.tile_rows == 32 ? kDecodeShares : z.tile_rows == 64 ? 2 : 1;
+    z.run_units = z.tile_rows == 32 ? kDecodeUnits : z.tile_rows == 64 ? kMiddleUnits : kChunkUnits;
+    z.least_tiles = z.tile_rows == 32 ? kDecodeLeast : kChunkLeast;
+    // a run has at least cost / run_units tiles (rounded: 2^-20 more), and a tile of rows one run more than whole ones
+    const int64_t runs = (z.run_units + z.run_units / 1024 + kv_heads) / kv_heads;
     z.items = z.row_tiles + runs;
     z.parts = 2 * runs;         // a cut tile of t key tiles has fewer than 2 t / longest runs
     return z;
 }
 
-template <bool BF16, int D, int R, bool FP8>
+template <bool BF16, int D, int R, int S, bool FP8>
 int launch_units(const PagedAttnParams& p, int64_t units, hipStream_t stream) {
-    // bf16 weights as hi + lo pairs where the matrix cores wait for keys anyway
-    constexpr bool kSplit = BF16 && R < 4;
-    constexpr auto kernel = &paged_attn_kernel<BF16, D, R, FP8, kSplit>;
-    constexpr size_t lds = Shape<D, R, FP8>::kLds;
+    // bfloat16 weights as pairs where the matrix cores wait for keys anyway
+    constexpr bool kSplit = R < 4 && (BF16 || FP8);
+    constexpr auto kernel = &paged_attn_kernel<BF16, D, R, S, FP8, kSplit>;
+    constexpr size_t lds = Shape<D, R, S, FP8>::kLds;
+    if (units * R * S * 64 >= (int64_t)1 << 32) return fail(FSTA_EUNSUPPORTED, "fsta_paged_attention: %d tokens", p.batch.tokens);
     if constexpr (lds > 64 * 1024) {
         const int rc = allow_full_lds<kernel>();
         if (rc != FSTA_OK) return rc;
     }
-    hipLaunchKernelGGL((paged_attn_kernel<BF16, D, R, FP8, kSplit>), dim3((unsigned)units), dim3(kWaves * 64), lds, stream, p);
+    hipLaunchKernelGGL((paged_attn_kernel<BF16, D, R, S, FP8, kSplit>), dim3((unsigned)units), dim3(R * S * 64), lds, stream, p);
     FSTA_HIP_OK(hipGetLastError());
     return FSTA_OK;
 }
 
-template <bool BF16, int D> int launch_attention(const PagedAttnParams& p, bool fp8, const Sizes& z, hipStream_t stream) {
-    const int64_t units = z.items * p.batch.kv_heads;
-    if (units * kWaves * 64 >= (int64_t)1 << 32) return fail(FSTA_EUNSUPPORTED, "fsta_paged_attention: %d tokens", p.batch.tokens);
-    int rc;
-    if (z.tile_rows == 32) rc = fp8 ? launch_units<BF16, D, 1, true>(p, units, stream) : launch_units<BF16, D, 1, false>(p, units, stream);
-    else if (z.tile_rows == 64) rc = fp8 ? launch_units<BF16, D, 2, true>(p, units, stream) : launch_units<BF16, D, 2, false>(p, units, stream);
-    else rc = fp8 ? launch_units<BF16, D, 4, true>(p, units, stream) : launch_units<BF16, D, 4, false>(p, units, stream);
-    if (rc != FSTA_OK) return rc;
-    const int64_t joins = z.run_units;       // fewer cut tiles than that, over all heads
-    const int64_t join_items = (joins + p.batch.kv_heads - 1) / p.batch.kv_heads;
-    hipLaunchKernelGGL((paged_join_kernel<BF16, D>), dim3((unsigned)(join_items * p.batch.kv_heads)), dim3(256), 0, stream, p);
+template <bool BF16, int D, int ROWS> int launch_join(const PagedAttnParams& p, const Sizes& z, hipStream_t stream) {
+    const int64_t items = (z.run_units + z.run_units / 1024 + p.batch.kv_heads) / p.batch.kv_heads;      // more than there are cut tiles
+    const int64_t rows = z.most_rows < z.tile_rows ? z.most_rows : z.tile_rows;
+    const dim3 grid((unsigned)(items * p.batch.kv_heads), (unsigned)((rows + ROWS - 1) / ROWS));
+    hipLaunchKernelGGL((paged_join_kernel<BF16, D, ROWS>), grid, dim3(256), 0, stream, p);
     FSTA_HIP_OK(hipGetLastError());
     return FSTA_OK;
+}
+
+template <bool BF16, int D, bool FP8> int launch_attention(const PagedAttnParams& p, const Sizes& z, hipStream_t stream) {
+    const int64_t units = z.items * p.batch.kv_heads;
+    int rc;
+    if (z.tile_rows == 32) rc = launch_units<BF16, D, 1, kDecodeShares, FP8>(p, units, stream);
+    else if (z.tile_rows == 64) rc = launch_units<BF16, D, 2, 2, FP8>(p, units, stream);
+    else rc = launch_units<BF16, D, 4, 1, FP8>(p, units, stream);
+    if (rc != FSTA_OK) return rc;
+    // nothing is cut where no sequence can have more tiles than the shortest run has
+    const int64_t most_tiles = (((int64_t)p.batch.width << p.batch.page_shift) + kTileN - 1) / kTileN;
+    if (most_tiles <= z.least_tiles) return FSTA_OK;
+    if (z.tile_rows == 32) return launch_join<BF16, D, 1>(p, z, stream);
+    if (z.tile_rows == 64) return launch_join<BF16, D, 2>(p, z, stream);
+    return launch_join<BF16, D, 8>(p, z, stream);
 }
 
 int check_heads(const char* who, int32_t batch, int32_t tokens, int32_t heads, int32_t kv_heads) {
@@ -645,12 +747,16 @@ extern "C" int fsta_paged_attention(const void* q, int64_t q_token_stride, int64
     p.k = k_cache; p.v = v_cache; p.k_exponent = k_exponent; p.v_exponent = v_exponent;
     p.o = o; p.lse = lse;
     p.tree_bits = tree_bits; p.tree_words = mask == FSTA_PAGED_TREE ? tree_words : 0; p.mask = mask;
-    p.group = heads / kv_heads; p.tile_rows = z.tile_rows; p.parts = (int32_t)z.parts; p.run_units = (int32_t)z.run_units;
+    p.group = heads / kv_heads; p.tile_rows = z.tile_rows; p.parts = (int32_t)z.parts; p.run_units = z.run_units; p.least_tiles = z.least_tiles;
     p.scale_log2e = sm_scale * kLog2e;
     p.part_o = static_cast<float*>(workspace);
     p.part_lse = p.part_o + (size_t)z.parts * kv_heads * z.tile_rows * head_dim;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const bool fp8 = cache_dtype == FSTA_FP8;
-    if (dtype == FSTA_BF16) return head_dim == 128 ? launch_attention<true, 128>(p, fp8, z, st) : launch_attention<true, 64>(p, fp8, z, st);
-    return head_dim == 128 ? launch_attention<false, 128>(p, fp8, z, st) : launch_attention<false, 64>(p, fp8, z, st);
+    if (dtype == FSTA_BF16) {
+        if (head_dim == 128) return fp8 ? launch_attention<true, 128, true>(p, z, st) : launch_attention<true, 128, false>(p, z, st);
+        return fp8 ? launch_attention<true, 64, true>(p, z, st) : launch_attention<true, 64, false>(p, z, st);
+    }
+    if (head_dim == 128) return fp8 ? launch_attention<false, 128, true>(p, z, st) : launch_attention<false, 128, false>(p, z, st);
+    return fp8 ? launch_attention<false, 64, true>(p, z, st) : launch_attention<false, 64, false>(p, z, st);
 }
