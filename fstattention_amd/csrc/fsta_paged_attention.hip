@@ -17,7 +17,7 @@ namespace {
 using namespace mfma;
 
 
-constexpr int kDecodeShares = 4, kDecodeUnits = 1024, kMiddleUnits = 512, kChunkUnits = 256;
+constexpr int kDecodeShares = 4, kDecodeUnits = 512, kMiddleUnits = 512, kChunkUnits = 256;
 constexpr int kDecodeLeast = 16, kChunkLeast = 8;
 
 enum Mask { kAll = 0, kCausal = 1, kTree = 2 };
@@ -35,7 +35,7 @@ struct PagedAttnParams {
     const uint32_t* tree_bits;     // [tokens, tree_words]
     float* part_o;                 // [part][kv_heads][rows][D]
     float* part_lse;               // [part][kv_heads][rows]
-    int32_t tree_words, mask, group, tile_rows, parts;
+    int32_t tree_words, mask, group, tile_rows, row_shift, parts;
     int32_t run_units, least_tiles; // units the launch is cut into where it has fewer, and the least tiles of a run
     float scale_log2e;
 };
@@ -49,8 +49,9 @@ __device__ const uint32_t kZeroRow[4] = {0u, 0u, 0u, 0u};
 // for a length.  A run has cost / run_units tiles, cost = all (tile of rows, tile of keys) pairs of the batch.
 struct Cut {
     uint32_t longest;              // tiles of keys in a run
+    // (a batch has fewer than 2^30 rows; tile_rows is a power of two)
     __device__ __forceinline__ static int row_tiles(const SeqLens& s, const PagedAttnParams& p) {
-        return (int)(((int64_t)s.fresh * p.group + p.tile_rows - 1) / p.tile_rows);
+        return (s.fresh * p.group + p.tile_rows - 1) >> p.row_shift;
     }
     __device__ __forceinline__ static int key_tiles(const SeqLens& s) { return max((s.keys + kTileN - 1) / kTileN, 1); }
     __device__ __forceinline__ uint32_t runs(const SeqLens& s) const { return ((uint32_t)key_tiles(s) + longest - 1) / longest; }
@@ -111,8 +112,8 @@ template <bool JOINS> __device__ __forceinline__ bool find_item(const PagedAttnP
 // Number of keys that any row of a tile may see (its rows are tokens first .. last of the sequence's new ones)
 __device__ __forceinline__ int keys_of_tile(const PagedAttnParams& p, const SeqLens& s, int row_tile) {
     if (p.mask != kCausal) return s.keys;
-    const int64_t last_row = min((int64_t)(row_tile + 1) * p.tile_rows, (int64_t)s.fresh * p.group) - 1;
-    return max(s.keys - s.fresh + (int)(last_row / p.group) + 1, 0);
+    const uint32_t last_row = (uint32_t)min((row_tile + 1) << p.row_shift, s.fresh * p.group) - 1u;
+    return max(s.keys - s.fresh + (int)(last_row / (uint32_t)p.group) + 1, 0);
 }
 
 // ---- the kernel -----------------------------------------------------------------------------------------------------------
@@ -155,8 +156,22 @@ template <bool BF16> __device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32
     return w;
 }
 
-// SPLIT: weights go to the matrix cores as pairs of bfloat16, hi + lo
-template <bool BF16, int D, int R, int S, bool FP8, bool SPLIT>
+template <int N, typename F> __device__ __forceinline__ void static_for(F f) {
+    if constexpr (N > 0) {
+        static_for<N - 1>(f);
+        f(std::integral_constant<int, N - 1>{});
+    }
+}
+// Waits until at most N of this wave's LDS accesses are outstanding (they finish in order; scalar loads in between can only make
+// it wait longer).
+template <int N> __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(%0)" : : "n"(N) : "memory"); }
+
+template <bool DIRECT> struct VRaw { VPair x[2]; };        // values of 32 head dims x 32 keys as they come out of LDS
+template <> struct VRaw<true> { u32x2 x[2]; };
+
+// SPLIT: weights go to the matrix cores as pairs of bfloat16, hi + lo.  ONCE: every key is read by one workgroup only, past the
+// caches.
+template <bool BF16, int D, int R, int S, bool FP8, bool SPLIT, bool ONCE>
 __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnParams p) {
     using SH = Shape<D, R, S, FP8>;
     constexpr bool kDirect = FP8 && !SH::kWiden;
@@ -192,14 +207,15 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
     const int steps = (tile1 - tile0 + S - 1) / S;
 
     // this wave's rows
-    const int rows_left = (int)min((int64_t)s.fresh * p.group - (int64_t)at.row_tile * p.tile_rows, (int64_t)p.tile_rows);
-    const int64_t row0 = (int64_t)at.row_tile * p.tile_rows;        // of the tile, among (token, head of the group)
+    const int row0 = at.row_tile << p.row_shift;                    // of the tile, among (token, head of the group)
+    const int rows_left = min(s.fresh * p.group - row0, p.tile_rows);
     const int my_row = group_of_rows * 32 + ql;                     // in the tile
     const bool has_rows = group_of_rows * 32 < rows_left;
-    const int token = (int)((row0 + min(my_row, rows_left - 1)) / p.group);
-    const int q_head = head * p.group + (int)((row0 + min(my_row, rows_left - 1)) - (int64_t)token * p.group);
-    const int first_token = (int)((row0 + group_of_rows * 32) / p.group);
-    const int last_token = (int)((row0 + min(group_of_rows * 32 + 31, rows_left - 1)) / p.group);
+    const uint32_t group = (uint32_t)p.group;
+    const int token = (int)((uint32_t)(row0 + min(my_row, rows_left - 1)) / group);
+    const int q_head = head * p.group + (row0 + min(my_row, rows_left - 1)) - token * p.group;
+    const int first_token = (int)((uint32_t)(row0 + group_of_rows * 32) / group);
+    const int last_token = (int)((uint32_t)(row0 + min(group_of_rows * 32 + 31, rows_left - 1)) / group);
     const int limit = p.mask == kCausal ? old + token : s.keys - 1;                  // this row's last key
     const int low_limit = p.mask == kCausal ? old + first_token : s.keys - 1;        // of the wave's rows, the least and
     const int high_limit = p.mask == kCausal ? old + last_token : s.keys - 1;        // the greatest
@@ -219,7 +235,6 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
     unsigned char* ring = smem + share * SH::kShareBytes;
     constexpr int kLanesPerRow = SH::kRowBytes / 16, kRowsPerDma = 64 / kLanesPerRow;
     const int page_rows = 1 << p.batch.page_shift;
-    const int32_t* table = p.batch.page_table + (size_t)at.seq * p.batch.width;
     uint32_t dma_off[SH::kPer];               // this lane's piece, from the start of its 16 rows
     int dma_row[SH::kPer];
     bool dma_is_v[SH::kPer];
@@ -233,45 +248,62 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
         dma_row[i] = r;
         dma_off[i] = (uint32_t)((r & 15) * SH::kRowBytes + chunk * 16);
     }
-    auto page_of = [&](int tile, int g) {     // page of the tile's 16-key half g
-        const int pos = min(tile * kTileN + 16 * g, s.keys - 1);
-        return __builtin_amdgcn_readfirstlane(table[__builtin_amdgcn_readfirstlane(pos >> p.batch.page_shift)]);
+    // Pages of a tile's two 16-key halves, by scalar loads (through the constant address space: a load the compiler takes for a
+    // vector one it would wait for with vmcnt(0), i.e. for the whole ring), one tile ahead of their use.
+    typedef const int32_t __attribute__((address_space(4))) * const_i32;
+    const const_i32 table = (const_i32)(uintptr_t)(p.batch.page_table + (size_t)at.seq * p.batch.width);
+    auto page_of = [&](int tile, int g) {
+        return table[__builtin_amdgcn_readfirstlane(min(tile * kTileN + 16 * g, s.keys - 1) >> p.batch.page_shift)];
     };
-    auto page_ok = [&](int page) { return (unsigned)page < (unsigned)p.batch.num_pages; };
+    int next_p0 = 0, next_p1 = 0;             // of the share's tile that is issued next
+    auto look_up = [&](int i) {
+        if (i < my_tiles) {
+            next_p0 = page_of(tile0 + share + i * S, 0);
+            next_p1 = page_of(tile0 + share + i * S, 1);
+        }
+    };
+    typedef const void __attribute__((address_space(1))) * global_ptr;
+    typedef void __attribute__((address_space(3))) * lds_ptr;
     uint32_t bad_halves = 0;                  // two bits per slot: halves of its tile on pages outside the cache
     auto issue = [&](int i) {                 // the share's i-th tile into slot i % kStages
         const int tile = tile0 + share + i * S, slot = i % kStages;
         const int first = tile * kTileN;
-        const int p0 = page_of(tile, 0), p1 = page_of(tile, 1);
-        const bool ok0 = page_ok(p0), ok1 = page_ok(p1);
+        const bool ok0 = (unsigned)next_p0 < (unsigned)p.batch.num_pages, ok1 = (unsigned)next_p1 < (unsigned)p.batch.num_pages;
+        const int64_t row_0 = (((int64_t)(ok0 ? next_p0 : 0) * p.batch.kv_heads + head) << p.batch.page_shift) + (first & (page_rows - 1));
+        const int64_t row_1 = (((int64_t)(ok1 ? next_p1 : 0) * p.batch.kv_heads + head) << p.batch.page_shift) + ((first + 16) & (page_rows - 1));
+        look_up(i + 1);
         bad_halves = (bad_halves & ~(3u << (2 * slot))) | ((ok0 ? 0u : 1u) << (2 * slot)) | ((ok1 ? 0u : 2u) << (2 * slot));
-        const bool whole = first + kTileN <= s.keys && ok0 && ok1;
-        const int64_t row_0 = (((int64_t)(ok0 ? p0 : 0) * p.batch.kv_heads + head) << p.batch.page_shift) + (first & (page_rows - 1));
-        const int64_t row_1 = (((int64_t)(ok1 ? p1 : 0) * p.batch.kv_heads + head) << p.batch.page_shift) + ((first + 16) & (page_rows - 1));
         unsigned char* dst = ring + slot * SH::kRawBytes;
+        auto half_of = [&](int j) { return (((group_of_rows * SH::kPer + j) % (SH::kDma / 2)) * kRowsPerDma) / 16; };
+        auto base_of = [&](int j) { return static_cast<const unsigned char*>(dma_is_v[j] ? p.v : p.k) + (half_of(j) ? row_1 : row_0) * SH::kRowBytes; };
+        if (first + kTileN <= s.keys && ok0 && ok1) {
 #pragma unroll
-        for (int j = 0; j < SH::kPer; ++j) {
-            const int u = group_of_rows * SH::kPer + j;
-            const int g = ((u % (SH::kDma / 2)) * kRowsPerDma) / 16;
-            const unsigned char* src = static_cast<const unsigned char*>(dma_is_v[j] ? p.v : p.k) + (g ? row_1 : row_0) * SH::kRowBytes + dma_off[j];
-            if (!whole) {
-                const bool here = first + dma_row[j] < s.keys && (g ? ok1 : ok0);
-                src = here ? src : reinterpret_cast<const unsigned char*>(kZeroRow);
+            for (int j = 0; j < SH::kPer; ++j)
+                __builtin_amdgcn_global_load_lds((global_ptr)(base_of(j) + dma_off[j]), (lds_ptr)(dst + (group_of_rows * SH::kPer + j) * 1024), 16, 0, ONCE ? 2 : 0);
+        } else {
+#pragma unroll
+            for (int j = 0; j < SH::kPer; ++j) {
+                const bool here = first + dma_row[j] < s.keys && (half_of(j) ? ok1 : ok0);
+                const unsigned char* src = here ? base_of(j) + dma_off[j] : reinterpret_cast<const unsigned char*>(kZeroRow);
+                __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(dst + (group_of_rows * SH::kPer + j) * 1024), 16, 0, 0);
             }
-            __builtin_amdgcn_global_load_lds((const void __attribute__((address_space(1)))*)src,
-                                             (void __attribute__((address_space(3)))*)(dst + u * 1024), 16, 0, 0);
         }
         if constexpr (FP8) {                  // exponents of the 32 keys, then of the 32 values, four to a lane
             const int l = lane & 15, g = (l >> 2) & 1;
             const uint8_t* src = ((l & 8) ? p.v_exponent : p.k_exponent) + (g ? row_1 : row_0) + 4 * (l & 3);
             const bool here = first + 16 * g < s.keys && (g ? ok1 : ok0);
             src = here ? src : reinterpret_cast<const uint8_t*>(kZeroRow);
-            __builtin_amdgcn_global_load_lds((const void __attribute__((address_space(1)))*)src,
-                                             (void __attribute__((address_space(3)))*)(dst + SH::kDma * 1024), 4, 0, 0);
+            __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(dst + SH::kDma * 1024), 4, 0, 0);
         }
     };
+    look_up(0);
     // A wave that has a ring of its own refills a slot as soon as it is done with it; waves that share one, behind the next barrier.
+    // (The Q rows are waited for here, behind the first tile's requests: left to their first use inside the loop, the wait would be
+    // one for every transfer on its way, at every tile.)
     int issued = 0;
+    if (my_tiles > 0) { issue(0); issued = 1; }
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks) lds_tie(qf[ks]);
     for (; issued < my_tiles && issued < (R == 1 ? kStages : kStages - 1); ++issued) issue(issued);
 
     float m_i = -INFINITY, l_i = 0.f;
@@ -289,10 +321,6 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
     const int tr8_row = 4 * half + ((lane & 15) >> 1) + ((lane & 8) ? 4 : 0);
     const uint32_t v8_lane0 = (uint32_t)(tr8_row * D + v8_chunk<D>(tr8_row, (lane >> 4) & 1) * 16 + 8 * (lane & 1));
     const float sc = p.scale_log2e;
-    typedef const u32x4 __attribute__((address_space(3))) * lds_u32x4;
-    typedef const u32x2 __attribute__((address_space(3))) * lds_u32x2;
-    typedef const uint32_t __attribute__((address_space(3))) * lds_u32;
-    typedef const uint8_t __attribute__((address_space(3))) * lds_u8;
 
     auto compute = [&](int i, const unsigned char* tile_lds) {
         const int tile = tile0 + share + i * S, first = tile * kTileN;
@@ -301,22 +329,41 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
         f32x16 sv;
 #pragma unroll
         for (int e = 0; e < 16; ++e) sv[e] = 0.f;
+        // (K fragments: all requested, then used as they arrive; LDS reads come back in order)
         const uint32_t exps = lds_addr(tile_lds) + SH::kDma * 1024;      // (8-bit tiles read as they are)
+        uint32_t v_exp[4];
         if constexpr (kDirect) {
             const uint32_t k_addr0 = lds_addr(tile_lds) + k8_lane0;
-            const float scale = __builtin_bit_cast(float, min((uint32_t)*(lds_u8)(uintptr_t)(exps + ql), 254u) << 23);
+            uint32_t E;
+            asm volatile("ds_read_u8 %0, %1" : "=v"(E) : "v"(exps + ql) : "memory");
+            u32x2 raw[kSteps];
 #pragma unroll
-            for (int ks = 0; ks < kSteps; ++ks) {
-                const u32x2 raw = *(lds_u32x2)(uintptr_t)(k_addr0 ^ (uint32_t)(ks << 4));
-                sv = MM::mfma(__builtin_bit_cast(Frag, widen8<BF16>(raw[0], raw[1], scale)), qf[ks], sv);
-            }
+            for (int ks = 0; ks < kSteps; ++ks) raw[ks] = lds_read_b64(k_addr0 ^ (uint32_t)(ks << 4));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v_exp[j] = lds_read_b32(exps + kTileN + 8 * j + 4 * half);
+            wait_lds<kSteps + 4>();
+            lds_tie(E);
+            const float scale = __builtin_bit_cast(float, min(E, 254u) << 23);     // (exponents of unused rows may be anything)
+            static_for<kSteps>([&](auto ks) {
+                constexpr int k = decltype(ks)::value;
+                wait_lds<kSteps + 3 - k>();
+                lds_tie(raw[k]);
+                sv = MM::mfma(__builtin_bit_cast(Frag, widen8<BF16>(raw[k][0], raw[k][1], scale)), qf[k], sv);
+            });
+            lds_wait();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) lds_tie(v_exp[j]);
         } else {
             const uint32_t k_addr0 = lds_addr(tile_lds) + k_lane0;
+            u32x4 raw[kSteps];
 #pragma unroll
-            for (int ks = 0; ks < kSteps; ++ks) {
-                const u32x4 raw = *(lds_u32x4)(uintptr_t)(k_addr0 ^ (uint32_t)(ks << 5));
-                sv = MM::mfma(__builtin_bit_cast(Frag, raw), qf[ks], sv);
-            }
+            for (int ks = 0; ks < kSteps; ++ks) raw[ks] = lds_read_b128(k_addr0 ^ (uint32_t)(ks << 5));
+            static_for<kSteps>([&](auto ks) {
+                constexpr int k = decltype(ks)::value;
+                wait_lds<kSteps - 1 - k>();
+                lds_tie(raw[k]);
+                sv = MM::mfma(__builtin_bit_cast(Frag, raw[k]), qf[k], sv);
+            });
         }
         // which of the tile's keys this lane's row sees
         const uint32_t bad = (bad_halves >> (2 * (i % kStages))) & 3u;
@@ -376,7 +423,7 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
         if constexpr (kDirect) {              // the values' powers of two go to the weights (exponents of unused rows may be anything)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t four = *(lds_u32)(uintptr_t)(exps + kTileN + 8 * j + 4 * half);
+                const uint32_t four = v_exp[j];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     pw[4 * j + e] *= __builtin_bit_cast(float, min((four >> (8 * e)) & 255u, 254u) << 23);
@@ -396,38 +443,49 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
             ph[k2] = __builtin_bit_cast(PFrag, hi4);
             if (SPLIT) pl[k2] = __builtin_bit_cast(PFrag, lo4);
         }
-        // O^T
-#pragma unroll
-        for (int dt = 0; dt < kDTiles; ++dt) {
-            PFrag f0, f1;
+        // O^T (the fragments of the next 32 head dims are requested before the products of these)
+        auto read_v = [&](int dt, VRaw<kDirect>& f) {
             if constexpr (kDirect) {
                 const uint32_t addr = (lds_addr(tile_lds) + (uint32_t)(kTileN * D) + v8_lane0) ^ (uint32_t)(dt << 5);
-                u32x2 a, b;
-                asm volatile("ds_read_b64_tr_b8 %0, %1" : "=v"(a) : "v"(addr) : "memory");
-                asm volatile("ds_read_b64_tr_b8 %0, %1 offset:%2" : "=v"(b) : "v"(addr), "n"(16 * D) : "memory");
-                lds_wait();
-                lds_tie(a); lds_tie(b);
-                f0 = __builtin_bit_cast(PFrag, widen8<true>(a[0], a[1], 1.f));
-                f1 = __builtin_bit_cast(PFrag, widen8<true>(b[0], b[1], 1.f));
+                asm volatile("ds_read_b64_tr_b8 %0, %1" : "=v"(f.x[0]) : "v"(addr) : "memory");
+                asm volatile("ds_read_b64_tr_b8 %0, %1 offset:%2" : "=v"(f.x[1]) : "v"(addr), "n"(16 * D) : "memory");
             } else {
                 const uint32_t addr = (lds_addr(tile_lds) + (uint32_t)(kTileN * D * 2) + v_lane0) ^ (uint32_t)(dt << 6);
-                VPair v0, v1;
-                v0.a = lds_read_tr16(addr);
-                v0.b = lds_read_tr16_at<8 * D * 2>(addr);
-                v1.a = lds_read_tr16_at<16 * D * 2>(addr);
-                v1.b = lds_read_tr16_at<24 * D * 2>(addr);
+                f.x[0].a = lds_read_tr16(addr);
+                f.x[0].b = lds_read_tr16_at<8 * D * 2>(addr);
+                f.x[1].a = lds_read_tr16_at<16 * D * 2>(addr);
+                f.x[1].b = lds_read_tr16_at<24 * D * 2>(addr);
+            }
+        };
+        VRaw<kDirect> raw_v[kDTiles];
+        read_v(0, raw_v[0]);
+        static_for<kDTiles>([&](auto t) {
+            constexpr int dt = decltype(t)::value;
+            if constexpr (dt + 1 < kDTiles) {
+                read_v(dt + 1, raw_v[dt + 1]);
+                wait_lds<kDirect ? 2 : 4>();
+            } else {
                 lds_wait();
-                lds_tie(v0.a); lds_tie(v0.b); lds_tie(v1.a); lds_tie(v1.b);
-                f0 = __builtin_bit_cast(PFrag, v0);
-                f1 = __builtin_bit_cast(PFrag, v1);
             }
-            o[dt] = PV::mfma(f0, ph[0], o[dt]);
-            o[dt] = PV::mfma(f1, ph[1], o[dt]);
+            PFrag f[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if constexpr (kDirect) {
+                    lds_tie(raw_v[dt].x[h]);
+                    f[h] = __builtin_bit_cast(PFrag, widen8<true>(raw_v[dt].x[h][0], raw_v[dt].x[h][1], 1.f));
+                } else {
+                    lds_tie(raw_v[dt].x[h].a);
+                    lds_tie(raw_v[dt].x[h].b);
+                    f[h] = __builtin_bit_cast(PFrag, raw_v[dt].x[h]);
+                }
+            }
+            o[dt] = PV::mfma(f[0], ph[0], o[dt]);
+            o[dt] = PV::mfma(f[1], ph[1], o[dt]);
             if (SPLIT) {
-                o[dt] = PV::mfma(f0, pl[0], o[dt]);
-                o[dt] = PV::mfma(f1, pl[1], o[dt]);
+                o[dt] = PV::mfma(f[0], pl[0], o[dt]);
+                o[dt] = PV::mfma(f[1], pl[1], o[dt]);
             }
-        }
+        });
     };
 
     // 8-bit rows: the share's waves widen the landed tile into the 16-bit layout, once for all row groups
@@ -457,9 +515,11 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
         }
     };
 
+    constexpr int kAhead = R == 1 ? kStages - 1 : kStages - 2;     // tiles that may be on their way behind the one that is waited for
     for (int i = 0; i < steps; ++i) {
         // tile i has landed for everyone who reads it, and everyone is done with the tile before it: its slot is refilled
-        wait_tiles_outstanding<SH::kPerTile>(max(issued - i - 1, 0));
+        if (issued - i - 1 >= kAhead) wait_vmcnt<kAhead * SH::kPerTile>();
+        else wait_tiles_outstanding<SH::kPerTile>(max(issued - i - 1, 0));
         auto refill = [&]() { if (issued < my_tiles) { issue(issued); ++issued; } };
         if constexpr (R > 1) { ring_barrier(); refill(); }
         if constexpr (SH::kWiden) {
@@ -554,7 +614,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
     const int head = (int)(blockIdx.x - item * (uint32_t)p.batch.kv_heads);
     Place at;
     if (!find_item<true>(p, item, lane, &at)) return;
-    const int rows = (int)min((int64_t)at.s.fresh * p.group - (int64_t)at.row_tile * p.tile_rows, (int64_t)p.tile_rows);
+    const int rows = min(at.s.fresh * p.group - (at.row_tile << p.row_shift), p.tile_rows);
     const int runs = max(min(at.runs, p.parts - at.part), 0);
     const int my = tid / kLanes, sub = my / ROWS, col = 4 * (tid % kLanes);
     for (int r0 = blockIdx.y * ROWS; r0 < rows; r0 += gridDim.y * ROWS) {
@@ -615,9 +675,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
         }
         if (sub > 0 || r >= rows) continue;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const int64_t flat = (int64_t)at.row_tile * p.tile_rows + r;
-        const int token = (int)(flat / p.group);
-        const int64_t out_row = (int64_t)(at.s.start + token) * (p.batch.kv_heads * p.group) + head * p.group + (flat - (int64_t)token * p.group);
+        const int flat = (at.row_tile << p.row_shift) + r;
+        const int token = (int)((uint32_t)flat / (uint32_t)p.group);
+        const int64_t out_row = (int64_t)(at.s.start + token) * (p.batch.kv_heads * p.group) + head * p.group + (flat - token * p.group);
         if (p.lse && col == 0) p.lse[out_row] = sum == 0.f ? -INFINITY : m + log2f(sum);
         const u32x2 w = {Mma<BF16>::pack_out(acc[0] * inv, acc[1] * inv), Mma<BF16>::pack_out(acc[2] * inv, acc[3] * inv)};
         *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.o) + out_row * D + col) = w;
@@ -653,20 +713,26 @@ Sizes sizes_of(int32_t batch, int32_t tokens, int32_t max_q_len, int32_t heads, 
     return z;
 }
 
-template <bool BF16, int D, int R, int S, bool FP8>
-int launch_units(const PagedAttnParams& p, int64_t units, hipStream_t stream) {
+template <bool BF16, int D, int R, int S, bool FP8, bool ONCE>
+int launch_units_of(const PagedAttnParams& p, int64_t units, hipStream_t stream) {
     // bfloat16 weights as pairs where the matrix cores wait for keys anyway
     constexpr bool kSplit = R < 4 && (BF16 || FP8);
-    constexpr auto kernel = &paged_attn_kernel<BF16, D, R, S, FP8, kSplit>;
+    constexpr auto kernel = &paged_attn_kernel<BF16, D, R, S, FP8, kSplit, ONCE>;
     constexpr size_t lds = Shape<D, R, S, FP8>::kLds;
     if (units * R * S * 64 >= (int64_t)1 << 32) return fail(FSTA_EUNSUPPORTED, "fsta_paged_attention: %d tokens", p.batch.tokens);
     if constexpr (lds > 64 * 1024) {
         const int rc = allow_full_lds<kernel>();
         if (rc != FSTA_OK) return rc;
     }
-    hipLaunchKernelGGL((paged_attn_kernel<BF16, D, R, S, FP8, kSplit>), dim3((unsigned)units), dim3(R * S * 64), lds, stream, p);
+    hipLaunchKernelGGL((paged_attn_kernel<BF16, D, R, S, FP8, kSplit, ONCE>), dim3((unsigned)units), dim3(R * S * 64), lds, stream, p);
     FSTA_HIP_OK(hipGetLastError());
     return FSTA_OK;
+}
+
+// (a sequence whose rows fit one tile has its keys read once)
+template <bool BF16, int D, int R, int S, bool FP8> int launch_units(const PagedAttnParams& p, int64_t units, const Sizes& z, hipStream_t stream) {
+    return z.most_rows <= z.tile_rows ? launch_units_of<BF16, D, R, S, FP8, true>(p, units, stream)
+                                      : launch_units_of<BF16, D, R, S, FP8, false>(p, units, stream);
 }
 
 template <bool BF16, int D, int ROWS> int launch_join(const PagedAttnParams& p, const Sizes& z, hipStream_t stream) {
@@ -681,9 +747,9 @@ template <bool BF16, int D, int ROWS> int launch_join(const PagedAttnParams& p, 
 template <bool BF16, int D, bool FP8> int launch_attention(const PagedAttnParams& p, const Sizes& z, hipStream_t stream) {
     const int64_t units = z.items * p.batch.kv_heads;
     int rc;
-    if (z.tile_rows == 32) rc = launch_units<BF16, D, 1, kDecodeShares, FP8>(p, units, stream);
-    else if (z.tile_rows == 64) rc = launch_units<BF16, D, 2, 2, FP8>(p, units, stream);
-    else rc = launch_units<BF16, D, 4, 1, FP8>(p, units, stream);
+    if (z.tile_rows == 32) rc = launch_units<BF16, D, 1, kDecodeShares, FP8>(p, units, z, stream);
+    else if (z.tile_rows == 64) rc = launch_units<BF16, D, 2, 2, FP8>(p, units, z, stream);
+    else rc = launch_units<BF16, D, 4, 1, FP8>(p, units, z, stream);
     if (rc != FSTA_OK) return rc;
     // nothing is cut where no sequence can have more tiles than the shortest run has
     const int64_t most_tiles = (((int64_t)p.batch.width << p.batch.page_shift) + kTileN - 1) / kTileN;
@@ -747,7 +813,7 @@ extern "C" int fsta_paged_attention(const void* q, int64_t q_token_stride, int64
     p.k = k_cache; p.v = v_cache; p.k_exponent = k_exponent; p.v_exponent = v_exponent;
     p.o = o; p.lse = lse;
     p.tree_bits = tree_bits; p.tree_words = mask == FSTA_PAGED_TREE ? tree_words : 0; p.mask = mask;
-    p.group = heads / kv_heads; p.tile_rows = z.tile_rows; p.parts = (int32_t)z.parts; p.run_units = z.run_units; p.least_tiles = z.least_tiles;
+    p.group = heads / kv_heads; p.tile_rows = z.tile_rows; p.row_shift = z.tile_rows == 32 ? 5 : z.tile_rows == 64 ? 6 : 7; p.parts = (int32_t)z.parts; p.run_units = z.run_units; p.least_tiles = z.least_tiles;
     p.scale_log2e = sm_scale * kLog2e;
     p.part_o = static_cast<float*>(workspace);
     p.part_lse = p.part_o + (size_t)z.parts * kv_heads * z.tile_rows * head_dim;
