@@ -1,0 +1,470 @@
+// What the kernels of the attention over pages share: their arguments, and what a wave does with a tile of 32 keys.
+#pragma once
+
+#include "fsta_mfma_common.h"
+#include "fsta_paged.h"
+
+namespace fsta {
+namespace paged {
+
+using namespace mfma;
+
+enum Mask { kAll = 0, kCausal = 1, kTree = 2 };
+
+struct PagedAttnParams {
+    PagedBatch batch;
+    const void* q;
+    int64_t q_token_stride, q_head_stride;
+    const void* k;
+    const void* v;
+    const uint8_t* k_exponent;
+    const uint8_t* v_exponent;
+    void* o;                       // [tokens, heads, D]
+    float* lse;                    // [tokens, heads] or null
+    const uint32_t* tree_bits;     // [tokens, tree_words]
+    float* part_o;                 // parts of rows whose keys several workgroups take: [part][rows][D] float32, normalised
+    float* part_lse;               // [part][rows], base 2
+    int32_t tree_words, mask, group, tile_rows, row_shift, parts;
+    int32_t run_units, least_tiles;
+    float scale_log2e;
+};
+
+__device__ static const uint32_t kZeroRow[4] = {0u, 0u, 0u, 0u};
+
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)x, lane); }
+
+// Number of keys that any row of a tile may see (its rows are tokens first .. last of the sequence's new ones)
+__device__ __forceinline__ int keys_of_tile(const PagedAttnParams& p, const SeqLens& s, int row_tile) {
+    if (p.mask != kCausal) return s.keys;
+    const uint32_t last_row = (uint32_t)min((row_tile + 1) << p.row_shift, s.fresh * p.group) - 1u;
+    return max(s.keys - s.fresh + (int)(last_row / (uint32_t)p.group) + 1, 0);
+}
+
+// Positions of 16-byte chunks in rows of an 8-bit tile: keys are read 8 bytes from each of 32 rows, values 32 bytes from each
+// of 16 (by the transposing read)
+template <int D> __device__ __forceinline__ int k8_chunk(int row, int c) { return D == 128 ? c ^ ((row >> 1) & 7) : c ^ ((row >> 2) & 3); }
+template <int D> __device__ __forceinline__ int v8_chunk(int row, int c) { return D == 128 ? c ^ (2 * ((row >> 1) & 3)) : c ^ (2 * ((row >> 2) & 1)); }
+
+// 8 e4m3 bytes times a power of two, in the 16-bit type
+template <bool BF16> __device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi, float scale) {
+    u32x4 w;
+    if constexpr (BF16) {
+        w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
+        w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
+        w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
+        w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
+    } else {
+        w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, false));
+        w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, true));
+        w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, false));
+        w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, true));
+    }
+    return w;
+}
+
+template <int N, typename F> __device__ __forceinline__ void static_for(F f) {
+    if constexpr (N > 0) {
+        static_for<N - 1>(f);
+        f(std::integral_constant<int, N - 1>{});
+    }
+}
+// Waits until at most N of this wave's LDS accesses are outstanding (they finish in order; scalar loads in between can only make
+// it wait longer).
+template <int N> __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(%0)" : : "n"(N) : "memory"); }
+
+template <bool DIRECT> struct VRaw { VPair x[2]; };        // values of 32 head dims x 32 keys as they come out of LDS
+template <> struct VRaw<true> { u32x2 x[2]; };
+
+
+// 32 rows (token, query head) of a wave against tiles of 32 keys, all in registers:
+//     S^T = K_tile . Q^T      O^T += V_tile^T . P^T        (32x32x16 matrix instructions)
+// A lane holds 16 scores of row lane & 31: keys 8 (e / 4) + 4 (lane >> 5) + e % 4, which is also how the transposing reads hand
+// it the values' rows, so that the weights go to the second product from the registers they are in.
+// DIRECT: tiles are 8-bit, widened here.  SPLIT: weights go to the matrix cores as pairs of bfloat16, hi + lo.
+template <bool BF16, int D, bool DIRECT, bool SPLIT> struct RowGroup {
+    using MM = Mma<BF16>;
+    using PV = Mma<BF16 || DIRECT>;           // weights times values: 8-bit values are exact in bfloat16 whatever their scale
+    using Frag = typename MM::frag;
+    using PFrag = typename PV::frag;
+    static constexpr int kSteps = D / 16;     // matrix instructions of a tile's scores
+    static constexpr int kDTiles = D / 32;    // 32-row tiles of O^T
+    static constexpr float kTrustedSum = BF16 || DIRECT ? 16777216.f : 32768.f;
+    static constexpr uint32_t kVBytes = kTileN * D * (DIRECT ? 1 : 2);      // values behind keys
+    static constexpr uint32_t kExps = 2 * kTileN * D;                       // 8-bit tiles: exponents of the keys, of the values
+
+    int ql, half;
+    uint32_t k_lane0, v_lane0;                // this lane's addresses in a tile
+    Frag qf[kSteps];                          // B operand: Q[row][16 ks + 8 half .. + 7]
+    float m_i, l_i;                           // running maximum (base 2), this lane's sum
+    f32x16 o[kDTiles];                        // O[row][32 dt + 8 (e / 4) + 4 half + e % 4]
+
+    __device__ __forceinline__ explicit RowGroup(int lane) : ql(lane & 31), half(lane >> 5) {
+        if constexpr (DIRECT) {               // (the transposing read hands a lane 8 keys, four from either 8-key half)
+            const int row = 4 * half + ((lane & 15) >> 1) + ((lane & 8) ? 4 : 0);
+            k_lane0 = (uint32_t)(ql * D + k8_chunk<D>(ql, 0) * 16 + 8 * half);
+            v_lane0 = (uint32_t)(row * D + v8_chunk<D>(row, (lane >> 4) & 1) * 16 + 8 * (lane & 1));
+        } else {
+            const int row = 4 * half + ((lane & 15) >> 2), col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+            k_lane0 = (uint32_t)(ql * D + k_chunk<D>(ql, half) * 8) * 2;
+            v_lane0 = (uint32_t)(row * D + v_chunk<D>(row, col >> 3) * 8 + (col & 7)) * 2;
+        }
+    }
+    __device__ __forceinline__ void load_q(const uint16_t* row) {
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) {
+            const u32x4 raw = *reinterpret_cast<const u32x4*>(row + 16 * ks + 8 * half);
+            qf[ks] = __builtin_bit_cast(Frag, raw);
+        }
+    }
+    // The loads are waited for here: left to their first use inside the loop over the tiles, that wait would be one for every
+    // transfer on its way, at every tile.
+    __device__ __forceinline__ void await_q() {
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) lds_tie(qf[ks]);
+    }
+    __device__ __forceinline__ void reset() {
+        m_i = -INFINITY;
+        l_i = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < kDTiles; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
+    }
+    __device__ __forceinline__ static bool finite(PFrag f) {
+        constexpr uint32_t kTop = BF16 || DIRECT ? 0x7f80u : 0x7c00u;
+        const u32x4 w = __builtin_bit_cast(u32x4, f);
+        bool ok = true;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ok = ok && (w[e] & kTop) != kTop && (w[e] & (kTop << 16)) != kTop << 16;
+        return ok;
+    }
+    // The values' fragment with everything that is not finite replaced by 0, and where that was +inf (sign 0) / -inf (sign 1) or NaN
+    __device__ __forceinline__ static void sort_out(PFrag f, PFrag& clean, PFrag& plus, PFrag& minus) {
+        constexpr uint32_t kTop = BF16 || DIRECT ? 0x7f80u : 0x7c00u, kOne = BF16 || DIRECT ? 0x3f80u : 0x3c00u;
+        const u32x4 w = __builtin_bit_cast(u32x4, f);
+        u32x4 c, a, b;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            c[e] = a[e] = b[e] = 0u;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t x = (w[e] >> (16 * h)) & 0xffffu;
+                const bool fine = (x & kTop) != kTop, nan = !fine && (x & 0x7fffu) != kTop;
+                c[e] |= (fine ? x : 0u) << (16 * h);
+                a[e] |= (nan || x == kTop ? kOne : 0u) << (16 * h);
+                b[e] |= (nan || x == (kTop | 0x8000u) ? kOne : 0u) << (16 * h);
+            }
+        }
+        clean = __builtin_bit_cast(PFrag, c);
+        plus = __builtin_bit_cast(PFrag, a);
+        minus = __builtin_bit_cast(PFrag, b);
+    }
+
+    // One tile at LDS address `at` (keys, values, exponents).  masked (uniform): word() is the row's bits of the keys it sees.
+    template <typename Word> __device__ __forceinline__ void tile(uint32_t at, float sc, bool masked, Word word) {
+        // S^T (K fragments: all requested, then used as they arrive; LDS reads come back in order)
+        f32x16 sv;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sv[e] = 0.f;
+        uint32_t v_exp[4];
+        if constexpr (DIRECT) {
+            uint32_t E;
+            asm volatile("ds_read_u8 %0, %1" : "=v"(E) : "v"(at + kExps + ql) : "memory");
+            u32x2 raw[kSteps];
+#pragma unroll
+            for (int ks = 0; ks < kSteps; ++ks) raw[ks] = lds_read_b64((at + k_lane0) ^ (uint32_t)(ks << 4));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v_exp[j] = lds_read_b32(at + kExps + kTileN + 8 * j + 4 * half);
+            wait_lds<kSteps + 4>();
+            lds_tie(E);
+            const float scale = __builtin_bit_cast(float, min(E, 254u) << 23);     // (exponents of unused rows may be anything)
+            static_for<kSteps>([&](auto ks) {
+                constexpr int k = decltype(ks)::value;
+                wait_lds<kSteps + 3 - k>();
+                lds_tie(raw[k]);
+                sv = MM::mfma(__builtin_bit_cast(Frag, widen8<BF16>(raw[k][0], raw[k][1], scale)), qf[k], sv);
+            });
+            lds_wait();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) lds_tie(v_exp[j]);
+        } else {
+            u32x4 raw[kSteps];
+#pragma unroll
+            for (int ks = 0; ks < kSteps; ++ks) raw[ks] = lds_read_b128((at + k_lane0) ^ (uint32_t)(ks << 5));
+            static_for<kSteps>([&](auto ks) {
+                constexpr int k = decltype(ks)::value;
+                wait_lds<kSteps - 1 - k>();
+                lds_tie(raw[k]);
+                sv = MM::mfma(__builtin_bit_cast(Frag, raw[k]), qf[k], sv);
+            });
+        }
+        uint32_t mine = ~0u;                  // bit 8 (e / 4) + e % 4: this lane's score e counts
+        if (masked) {
+            mine = word() >> (4 * half);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (!((mine >> (8 * (e / 4) + e % 4)) & 1u)) sv[e] = -INFINITY;
+        }
+        // Weights against the running maximum as it stands (a power of two on a row's weights cancels in O / l); the tile's
+        // own maximum is only looked for when a sum gets large, or at the first tile.
+        float pw[16], sum = 0.f;
+        const float neg_m = m_i == -INFINITY ? 0.f : -m_i;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            pw[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], sc, neg_m));
+            sum += pw[e];
+        }
+        const bool redo = !(sum <= kTrustedSum) || m_i == -INFINITY;
+        if (__ballot(redo) != 0ull) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sv[e]);
+            float a, b;
+            swap_halves(mx, false, a, b);
+            mx = fmaxf(a, b) * sc;
+            const bool raise = mx > m_i + kRescaleSlack || (m_i == -INFINITY && mx > -INFINITY);
+            const float alpha = raise ? __builtin_amdgcn_exp2f(m_i - mx) : 1.f;
+            if (raise) m_i = mx;
+            l_i *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < kDTiles; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+            const float neg = m_i == -INFINITY ? 0.f : -m_i;
+            sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                pw[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], sc, neg));
+                sum += pw[e];
+            }
+        }
+        l_i += sum;
+        if constexpr (DIRECT) {               // the values' powers of two go to the weights
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t four = v_exp[j];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    pw[4 * j + e] *= __builtin_bit_cast(float, min((four >> (8 * e)) & 255u, 254u) << 23);
+            }
+        }
+        PFrag ph[2], pl[2];
+#pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2) {
+            u32x4 hi4, lo4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float a = pw[8 * k2 + 2 * e], b = pw[8 * k2 + 2 * e + 1];
+                const uint32_t hi = PV::pack(a, b);
+                hi4[e] = hi;
+                if (SPLIT) lo4[e] = PV::pack(a - PV::low(hi), b - PV::high(hi));
+            }
+            ph[k2] = __builtin_bit_cast(PFrag, hi4);
+            if (SPLIT) pl[k2] = __builtin_bit_cast(PFrag, lo4);
+        }
+        // O^T (the fragments of the next 32 head dims are requested before the products of these)
+        auto read_v = [&](int dt, VRaw<DIRECT>& f) {
+            const uint32_t addr = (at + kVBytes + v_lane0) ^ (uint32_t)(dt << (DIRECT ? 5 : 6));
+            if constexpr (DIRECT) {
+                asm volatile("ds_read_b64_tr_b8 %0, %1" : "=v"(f.x[0]) : "v"(addr) : "memory");
+                asm volatile("ds_read_b64_tr_b8 %0, %1 offset:%2" : "=v"(f.x[1]) : "v"(addr), "n"(16 * D) : "memory");
+            } else {
+                f.x[0].a = lds_read_tr16(addr);
+                f.x[0].b = lds_read_tr16_at<8 * D * 2>(addr);
+                f.x[1].a = lds_read_tr16_at<16 * D * 2>(addr);
+                f.x[1].b = lds_read_tr16_at<24 * D * 2>(addr);
+            }
+        };
+        VRaw<DIRECT> raw_v[kDTiles];
+        read_v(0, raw_v[0]);
+        static_for<kDTiles>([&](auto t) {
+            constexpr int dt = decltype(t)::value;
+            if constexpr (dt + 1 < kDTiles) {
+                read_v(dt + 1, raw_v[dt + 1]);
+                wait_lds<DIRECT ? 2 : 4>();
+            } else {
+                lds_wait();
+            }
+            PFrag f[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if constexpr (DIRECT) {
+                    lds_tie(raw_v[dt].x[h]);
+                    f[h] = __builtin_bit_cast(PFrag, widen8<true>(raw_v[dt].x[h][0], raw_v[dt].x[h][1], 1.f));
+                } else {
+                    lds_tie(raw_v[dt].x[h].a);
+                    lds_tie(raw_v[dt].x[h].b);
+                    f[h] = __builtin_bit_cast(PFrag, raw_v[dt].x[h]);
+                }
+            }
+            // A value that is not finite must reach the rows that see its key and no other, although a weight of zero times it
+            // is a NaN: where the tile is masked, such values are taken out and put back row by row, by their signs.
+            if (masked && __ballot(!finite(f[0]) || !finite(f[1])) != 0ull) {
+                f32x16 plus_rows, minus_rows;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) plus_rows[e] = minus_rows[e] = 0.f;
+                constexpr uint32_t kOne = BF16 || DIRECT ? 0x3f80u : 0x3c00u;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    PFrag clean, plus, minus;
+                    sort_out(f[h], clean, plus, minus);
+                    f[h] = clean;
+                    u32x4 seen;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int bit = 8 * (2 * h + e / 2) + 2 * (e % 2);
+                        seen[e] = ((mine >> bit) & 1u ? kOne : 0u) | ((mine >> (bit + 1)) & 1u ? kOne << 16 : 0u);
+                    }
+                    plus_rows = PV::mfma(plus, __builtin_bit_cast(PFrag, seen), plus_rows);
+                    minus_rows = PV::mfma(minus, __builtin_bit_cast(PFrag, seen), minus_rows);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    if (plus_rows[e] > 0.f) o[dt][e] += INFINITY;
+                    if (minus_rows[e] > 0.f) o[dt][e] -= INFINITY;
+                }
+            }
+            o[dt] = PV::mfma(f[0], ph[0], o[dt]);
+            o[dt] = PV::mfma(f[1], ph[1], o[dt]);
+            if (SPLIT) {
+                o[dt] = PV::mfma(f[0], pl[0], o[dt]);
+                o[dt] = PV::mfma(f[1], pl[1], o[dt]);
+            }
+        });
+    }
+
+    // Sum over both halves of the lanes that share a row
+    __device__ __forceinline__ float row_sum() const {
+        float a, b;
+        swap_halves(l_i, false, a, b);
+        return a + b;
+    }
+};
+
+// What a wave's rows see of the keys, besides what the tiles themselves say
+struct Sight {
+    int limit, low_limit, high_limit;         // last key of this lane's row; the least and greatest of the wave's rows
+    int old;                                  // keys in front of the new tokens (negative: the first new ones have no place)
+    const uint32_t* bits;                     // this row's mask (trees)
+
+    __device__ __forceinline__ bool whole(const PagedAttnParams& p, int first) const {      // every row sees every key of the tile
+        return first + kTileN - 1 <= low_limit && !(p.mask == kTree && first + kTileN > old);
+    }
+    // bits of the tile's keys; bad: halves of it on pages outside the cache
+    __device__ __forceinline__ uint32_t word(const PagedAttnParams& p, int first, uint32_t bad) const {
+        const int rel = limit - first;
+        uint32_t w = rel >= 31 ? ~0u : rel < 0 ? 0u : (2u << rel) - 1u;
+        if (bad & 1u) w &= 0xffff0000u;
+        if (bad & 2u) w &= 0x0000ffffu;
+        if (p.mask == kTree && first + kTileN > old) {      // keys in front of the new tokens are seen by all, the others by their bit
+            const int number = first - old, wi = number >> 5, sh = number & 31;
+            const uint32_t lo = wi < 0 ? ~0u : wi < p.tree_words ? bits[wi] : 0u;
+            const uint32_t hi = wi + 1 < 0 ? ~0u : wi + 1 < p.tree_words ? bits[wi + 1] : 0u;
+            w &= sh ? (lo >> sh) | (hi << (32 - sh)) : lo;
+        }
+        return w;
+    }
+};
+// Rows first_row .. first_row + 31 of a tile (rows_left of them exist), this lane's `my_row`
+struct Rows { int token, q_head; Sight sight; };
+__device__ __forceinline__ Rows rows_of(const PagedAttnParams& p, const SeqLens& s, int head, int row0, int rows_left, int first_row, int ql) {
+    Rows r;
+    const uint32_t group = (uint32_t)p.group;
+    const int mine = row0 + min(first_row + ql, rows_left - 1);
+    r.token = (int)((uint32_t)mine / group);
+    r.q_head = head * p.group + mine - r.token * p.group;
+    r.sight.old = s.keys - s.fresh;
+    const bool causal = p.mask == kCausal;
+    r.sight.limit = causal ? r.sight.old + r.token : s.keys - 1;
+    r.sight.low_limit = causal ? r.sight.old + (int)((uint32_t)(row0 + first_row) / group) : s.keys - 1;
+    r.sight.high_limit = causal ? r.sight.old + (int)((uint32_t)(row0 + min(first_row + 31, rows_left - 1)) / group) : s.keys - 1;
+    r.sight.bits = p.tree_bits + (int64_t)(s.start + r.token) * p.tree_words;
+    return r;
+}
+
+// Pages by scalar loads, through the constant address space (a load the compiler takes for a vector one it waits for with
+// vmcnt(0), i.e. for the whole ring)
+typedef const int32_t __attribute__((address_space(4))) * const_i32;
+__device__ __forceinline__ const_i32 table_of(const PagedAttnParams& p, int seq) {
+    return (const_i32)(uintptr_t)(p.batch.page_table + (size_t)seq * p.batch.width);
+}
+__device__ __forceinline__ int page_at(const PagedAttnParams& p, const_i32 table, int keys, int pos) {
+    return table[__builtin_amdgcn_readfirstlane(min(pos, keys - 1) >> p.batch.page_shift)];
+}
+
+// Transfers of a tile's keys and values (and exponents) from its pages to a ring slot, as wave `part` of PARTS.
+// WIDENED: an 8-bit tile that is copied into the 16-bit layout afterwards lies in LDS as it does in memory.  ONCE: past the caches.
+template <int D, int PARTS, bool FP8, bool WIDENED, bool ONCE> struct Fetch {
+    static constexpr int kRowBytes = FP8 ? D : 2 * D;             // a key's or a value's row in the cache
+    static constexpr int kDma = 2 * kTileN * kRowBytes / 1024;    // transfers of 1 KiB
+    static constexpr int kPer = kDma / PARTS;                     // of them this wave's
+    static constexpr int kPerTile = kPer + (FP8 ? 1 : 0);         // (and one of the exponents)
+    static constexpr int kBytes = kDma * 1024 + (FP8 ? 256 : 0);
+    static_assert(kDma % PARTS == 0, "a wave has whole transfers");
+    static constexpr int kLanesPerRow = kRowBytes / 16, kRowsPerDma = 64 / kLanesPerRow;
+
+    int first_unit;
+    uint32_t off[kPer];                       // this lane's piece, from the start of its 16 rows
+    __device__ __forceinline__ Fetch(int part, int lane) : first_unit(part * kPer) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int r = row(j, lane), slot = lane % kLanesPerRow;
+            const int chunk = WIDENED ? slot : FP8 ? (is_v(j) ? v8_chunk<D>(r, slot) : k8_chunk<D>(r, slot))
+                                                   : (is_v(j) ? v_chunk<D>(r, slot) : k_chunk<D>(r, slot));
+            off[j] = (uint32_t)((r & 15) * kRowBytes + chunk * 16);
+        }
+    }
+    __device__ __forceinline__ bool is_v(int j) const { return first_unit + j >= kDma / 2; }
+    __device__ __forceinline__ int row(int j, int lane) const { return ((first_unit + j) % (kDma / 2)) * kRowsPerDma + lane / kLanesPerRow; }
+    __device__ __forceinline__ int half_of(int j) const { return (((first_unit + j) % (kDma / 2)) * kRowsPerDma) / 16; }
+
+    // p0, p1: pages of the tile's 16-key halves; returns the halves that are on none
+    __device__ __forceinline__ uint32_t tile(const PagedAttnParams& p, int keys, int head, int first, int p0, int p1, unsigned char* dst, int lane) const {
+        typedef const void __attribute__((address_space(1))) * global_ptr;
+        typedef void __attribute__((address_space(3))) * lds_ptr;
+        const int page_rows = 1 << p.batch.page_shift;
+        const bool ok0 = (unsigned)p0 < (unsigned)p.batch.num_pages, ok1 = (unsigned)p1 < (unsigned)p.batch.num_pages;
+        const int64_t row_0 = (((int64_t)(ok0 ? p0 : 0) * p.batch.kv_heads + head) << p.batch.page_shift) + (first & (page_rows - 1));
+        const int64_t row_1 = (((int64_t)(ok1 ? p1 : 0) * p.batch.kv_heads + head) << p.batch.page_shift) + ((first + 16) & (page_rows - 1));
+        auto base_of = [&](int j) { return static_cast<const unsigned char*>(is_v(j) ? p.v : p.k) + (half_of(j) ? row_1 : row_0) * kRowBytes; };
+        if (first + kTileN <= keys && ok0 && ok1) {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+                __builtin_amdgcn_global_load_lds((global_ptr)(base_of(j) + off[j]), (lds_ptr)(dst + (first_unit + j) * 1024), 16, 0, ONCE ? 2 : 0);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                const bool here = first + row(j, lane) < keys && (half_of(j) ? ok1 : ok0);
+                const unsigned char* src = here ? base_of(j) + off[j] : reinterpret_cast<const unsigned char*>(kZeroRow);
+                __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(dst + (first_unit + j) * 1024), 16, 0, 0);
+            }
+        }
+        if constexpr (FP8) {                  // exponents of the 32 keys, then of the 32 values, four to a lane
+            const int l = lane & 15, g = (l >> 2) & 1;
+            const uint8_t* src = ((l & 8) ? p.v_exponent : p.k_exponent) + (g ? row_1 : row_0) + 4 * (l & 3);
+            const bool here = first + 16 * g < keys && (g ? ok1 : ok0);
+            src = here ? src : reinterpret_cast<const uint8_t*>(kZeroRow);
+            __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(dst + kDma * 1024), 4, 0, 0);
+        }
+        return (ok0 ? 0u : 1u) | (ok1 ? 0u : 2u);
+    }
+};
+
+// At most `tiles` (0 .. MOST) tiles' worth of this wave's transfers outstanding, PER instructions each
+template <int PER, int MOST> __device__ __forceinline__ void wait_tiles(int tiles) {
+    static_assert(MOST * PER < 64, "vmcnt has 6 bits");
+    if (tiles >= MOST) {
+        wait_vmcnt<MOST * PER>();
+    } else {
+        if constexpr (MOST > 0) wait_tiles<PER, MOST - 1>(tiles);
+    }
+}
+
+// A row's 4 consecutive values to the output
+template <bool BF16> __device__ __forceinline__ void store_row(uint16_t* dst, float a, float b, float c, float d) {
+    const u32x2 w = {Mma<BF16>::pack_out(a, b), Mma<BF16>::pack_out(c, d)};
+    *reinterpret_cast<u32x2*>(dst) = w;
+}
+
+}  // namespace paged
+}  // namespace fsta

@@ -231,6 +231,19 @@ def test_many_sequences():
     run(new, keys, 4, 2, 64, torch.bfloat16, 16, 19)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64)])
+@pytest.mark.parametrize("batch,kv_heads,low,high", [(3, 1, 500, 9000), (5, 8, 1, 3000), (70, 2, 1, 1500), (200, 4, 300, 700), (130, 1, 1, 40)])
+def test_keys_dealt_evenly(batch, kv_heads, low, high, dtype, d, fp8):
+    """Lengths of all kinds under the kernel whose workgroups take equal runs of the batch's keys: runs that end inside a head, at
+    its ends, span many sequences, or are empty."""
+    g = torch.Generator().manual_seed(batch + high)
+    new = torch.randint(0, 3, (batch,), generator=g).tolist()
+    keys = [n + int(torch.randint(low, high, (1,), generator=g)) for n in new]
+    keys[batch // 2] = new[batch // 2]
+    run(new, keys, 2 * kv_heads, kv_heads, d, dtype, 64, 60, fp8=fp8)
+
+
 def test_every_position_is_seen_without_a_mask():
     run([5, 70], [64, 333], 4, 2, 128, torch.bfloat16, 16, 20, mode="all")
 
@@ -285,7 +298,7 @@ def test_keys_on_no_page_are_not_seen():
         table = table.clone()
         table[0, 1], table[0, 4], table[1, 0] = -1, 1 << 30, -7
         return table
-    for new in ([1, 1], [33, 40]):
+    for new in ([1, 1], [16, 9], [33, 40]):
         run(new, [150, 90], 4, 2, 64, torch.bfloat16, 16, 28, table=holes)
 
 
@@ -492,6 +505,41 @@ def test_quantised_rows_at_the_ends_of_the_range(dtype):
 
 
 # ---- masks of trees -----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dtype,d,new,keys", [(torch.bfloat16, 128, 5, 40), (torch.float16, 64, 20, 100), (torch.bfloat16, 64, 33, 33),
+                                              (torch.float16, 128, 90, 300)])
+def test_values_that_are_not_finite_reach_the_rows_that_see_them(dtype, d, new, keys, fp8):
+    """A NaN and an infinity of either sign among the new tokens' values, at several head dims: rows that see the key get them,
+    the others what they would have got without."""
+    tab, lens, starts, pages = make_batch([new], [keys], 16, 50)
+    cache = make_cache(pages, 1, 16, d, dtype, 51, fp8)
+    clean = fsta.PagedKV(*(None if t is None else t.clone() for t in cache))
+    place = lambda i: (int(tab[0, (keys - new + i) // 16]), 0, (keys - new + i) % 16)
+    bad = {2: (7, math.nan), 3: (d - 1, math.nan if fp8 else math.inf), new - 1: (33, math.nan if fp8 else -math.inf)}
+    for i, (col, x) in bad.items():
+        if fp8:
+            cache.v.view(torch.uint8)[(*place(i), col)] = 0x7f
+        else:
+            cache.v[(*place(i), col)] = x
+    g = torch.Generator().manual_seed(52)
+    q = torch.randn((new, 2, d), generator=g).to(dtype).cuda()
+    sees = torch.ones((new, new), dtype=torch.bool).tril()
+    sees[4] = False
+    sees[4, 3:5] = True
+    words = -(-new // 32)
+    packed = torch.zeros((new, words * 32), dtype=torch.int64)
+    packed[:, :new] = sees
+    packed = (packed.view(new, words, 32) << torch.arange(32)).sum(-1)
+    bits = torch.where(packed >= 1 << 31, packed - (1 << 32), packed).to(torch.int32).cuda()
+    args = (tab.cuda(), lens.cuda(), starts.cuda(), 0.125)
+    for kwargs, mask in (({}, torch.ones((new, new), dtype=torch.bool).tril()), ({"tree_bits": bits}, sees)):
+        got = fsta.paged_attention(q, cuda(cache), *args, max_q_len=new, **kwargs).cpu()
+        want = fsta.paged_attention(q, cuda(clean), *args, max_q_len=new, **kwargs).cpu()
+        for i, (col, x) in bad.items():
+            want[mask[:, i], :, col] = x
+        torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True)
+
 
 @pytest.mark.parametrize("nodes,window", [([1], 8), ([32, 33, 31], 4), ([64, 1, 200, 0, 7], 16), ([300], None), ([2048, 1000], 3)])
 def test_tree_mask_bits(nodes, window):
