@@ -138,26 +138,28 @@ template <bool BF16, int D, bool DIRECT, bool SPLIT> struct RowGroup {
         for (int e = 0; e < 4; ++e) ok = ok && (w[e] & kTop) != kTop && (w[e] & (kTop << 16)) != kTop << 16;
         return ok;
     }
-    // The values' fragment with everything that is not finite replaced by 0, and where that was +inf (sign 0) / -inf (sign 1) or NaN
-    __device__ __forceinline__ static void sort_out(PFrag f, PFrag& clean, PFrag& plus, PFrag& minus) {
-        constexpr uint32_t kTop = BF16 || DIRECT ? 0x7f80u : 0x7c00u, kOne = BF16 || DIRECT ? 0x3f80u : 0x3c00u;
-        const u32x4 w = __builtin_bit_cast(u32x4, f);
-        u32x4 c, a, b;
+    // The values' fragment with what is not finite replaced by 0
+    __device__ __forceinline__ static PFrag only_finite(PFrag f) {
+        constexpr uint32_t kTop = BF16 || DIRECT ? 0x7f80u : 0x7c00u;
+        u32x4 w = __builtin_bit_cast(u32x4, f);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            c[e] = a[e] = b[e] = 0u;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t x = (w[e] >> (16 * h)) & 0xffffu;
-                const bool fine = (x & kTop) != kTop, nan = !fine && (x & 0x7fffu) != kTop;
-                c[e] |= (fine ? x : 0u) << (16 * h);
-                a[e] |= (nan || x == kTop ? kOne : 0u) << (16 * h);
-                b[e] |= (nan || x == (kTop | 0x8000u) ? kOne : 0u) << (16 * h);
-            }
+            if ((w[e] & kTop) == kTop) w[e] &= 0xffff0000u;
+            if ((w[e] & (kTop << 16)) == kTop << 16) w[e] &= 0xffffu;
         }
-        clean = __builtin_bit_cast(PFrag, c);
-        plus = __builtin_bit_cast(PFrag, a);
-        minus = __builtin_bit_cast(PFrag, b);
+        return __builtin_bit_cast(PFrag, w);
+    }
+    // 1 where it is +inf (sign 0) / -inf (sign 1) or NaN, 0 elsewhere
+    __device__ __forceinline__ static PFrag infinite(PFrag f, uint32_t sign) {
+        constexpr uint32_t kTop = BF16 || DIRECT ? 0x7f80u : 0x7c00u, kOne = BF16 || DIRECT ? 0x3f80u : 0x3c00u;
+        u32x4 w = __builtin_bit_cast(u32x4, f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t x = w[e] ^ (sign << 15 | sign << 31);
+            const uint32_t lo = x & 0xffffu, hi = x >> 16;
+            w[e] = ((lo & 0x7fffu) > kTop || lo == kTop ? kOne : 0u) | ((hi & 0x7fffu) > kTop || hi == kTop ? kOne << 16 : 0u);
+        }
+        return __builtin_bit_cast(PFrag, w);
     }
 
     // One tile at LDS address `at` (keys, values, exponents).  masked (uniform): word() is the row's bits of the keys it sees.
@@ -300,29 +302,28 @@ template <bool BF16, int D, bool DIRECT, bool SPLIT> struct RowGroup {
             // A value that is not finite must reach the rows that see its key and no other, although a weight of zero times it
             // is a NaN: where the tile is masked, such values are taken out and put back row by row, by their signs.
             if (masked && __ballot(!finite(f[0]) || !finite(f[1])) != 0ull) {
-                f32x16 plus_rows, minus_rows;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) plus_rows[e] = minus_rows[e] = 0.f;
                 constexpr uint32_t kOne = BF16 || DIRECT ? 0x3f80u : 0x3c00u;
+#pragma unroll 1
+                for (uint32_t sign = 0; sign < 2; ++sign) {
+                    f32x16 touched;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    PFrag clean, plus, minus;
-                    sort_out(f[h], clean, plus, minus);
-                    f[h] = clean;
-                    u32x4 seen;
+                    for (int e = 0; e < 16; ++e) touched[e] = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int bit = 8 * (2 * h + e / 2) + 2 * (e % 2);
-                        seen[e] = ((mine >> bit) & 1u ? kOne : 0u) | ((mine >> (bit + 1)) & 1u ? kOne << 16 : 0u);
+                    for (int h = 0; h < 2; ++h) {
+                        u32x4 seen;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int bit = 8 * (2 * h + e / 2) + 2 * (e % 2);
+                            seen[e] = ((mine >> bit) & 1u ? kOne : 0u) | ((mine >> (bit + 1)) & 1u ? kOne << 16 : 0u);
+                        }
+                        touched = PV::mfma(infinite(f[h], sign), __builtin_bit_cast(PFrag, seen), touched);
                     }
-                    plus_rows = PV::mfma(plus, __builtin_bit_cast(PFrag, seen), plus_rows);
-                    minus_rows = PV::mfma(minus, __builtin_bit_cast(PFrag, seen), minus_rows);
-                }
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    if (plus_rows[e] > 0.f) o[dt][e] += INFINITY;
-                    if (minus_rows[e] > 0.f) o[dt][e] -= INFINITY;
+                    for (int e = 0; e < 16; ++e)
+                        if (touched[e] > 0.f) o[dt][e] += sign ? -INFINITY : INFINITY;
                 }
+                f[0] = only_finite(f[0]);
+                f[1] = only_finite(f[1]);
             }
             o[dt] = PV::mfma(f[0], ph[0], o[dt]);
             o[dt] = PV::mfma(f[1], ph[1], o[dt]);
@@ -331,6 +332,130 @@ template <bool BF16, int D, bool DIRECT, bool SPLIT> struct RowGroup {
                 o[dt] = PV::mfma(f[1], pl[1], o[dt]);
             }
         });
+    }
+
+    // Weights 2 i and 2 i + 1 against the maximum -neg_m, packed; adds them to the sum
+    __device__ __forceinline__ static uint32_t two_weights(const f32x16& sv, int i, float sc, float neg_m, float& sum) {
+        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[2 * i], sc, neg_m));
+        const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[2 * i + 1], sc, neg_m));
+        sum += a;
+        sum += b;
+        return PV::pack(a, b);
+    }
+    __device__ __forceinline__ bool doubtful(float sum) const { return __ballot(!(sum <= kTrustedSum) || m_i == -INFINITY) != 0ull; }
+    // Where the maximum as it stands is not good enough (a first tile, a large sum): raises it and weighs again
+    __device__ __forceinline__ void raise(const f32x16& sv, float sc, uint32_t (&w)[8], float& sum) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sv[e]);
+        float a, b;
+        swap_halves(mx, false, a, b);
+        mx = fmaxf(a, b) * sc;
+        const bool up = mx > m_i + kRescaleSlack || (m_i == -INFINITY && mx > -INFINITY);
+        const float alpha = up ? __builtin_amdgcn_exp2f(m_i - mx) : 1.f;
+        if (up) m_i = mx;
+        l_i *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < kDTiles; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+        const float neg_m = m_i == -INFINITY ? 0.f : -m_i;
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = two_weights(sv, i, sc, neg_m, sum);
+    }
+    __device__ __forceinline__ static PFrag fragment(const uint32_t (&w)[8], int h) {
+        const u32x4 x = {w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]};
+        return __builtin_bit_cast(PFrag, x);
+    }
+    // Two 16-bit tiles that every row sees whole.  Instructions are issued in this order: the scores of both tiles take turns, so
+    // that none waits for the one in front of it; the weights of the second tile are worked out between the products of the first
+    // tile's values.
+    __device__ __forceinline__ void two_tiles(uint32_t at_a, uint32_t at_b, float sc) {
+        static_assert(!DIRECT && !SPLIT, "16-bit tiles, weights rounded once");
+        constexpr int kFirst = 3;                 // fragments of either tile that are requested ahead
+        u32x4 ka[kSteps], kb[kSteps];
+        auto read_k = [&](int ks) {
+            ka[ks] = lds_read_b128((at_a + k_lane0) ^ (uint32_t)(ks << 5));
+            kb[ks] = lds_read_b128((at_b + k_lane0) ^ (uint32_t)(ks << 5));
+        };
+        VPair va[kDTiles][2], vb[kDTiles][2];
+        auto read_v = [&](uint32_t at, int dt, VPair (&v)[2]) {
+            const uint32_t addr = (at + kVBytes + v_lane0) ^ (uint32_t)(dt << 6);
+            v[0].a = lds_read_tr16(addr);
+            v[0].b = lds_read_tr16_at<8 * D * 2>(addr);
+            v[1].a = lds_read_tr16_at<16 * D * 2>(addr);
+            v[1].b = lds_read_tr16_at<24 * D * 2>(addr);
+        };
+        auto tie_v = [&](VPair (&v)[2]) {
+            lds_tie(v[0].a); lds_tie(v[0].b); lds_tie(v[1].a); lds_tie(v[1].b);
+        };
+        f32x16 sa, sb;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sa[e] = sb[e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < kFirst; ++ks) read_k(ks);
+        static_for<kSteps>([&](auto step) {
+            constexpr int ks = decltype(step)::value;
+            if constexpr (ks + kFirst < kSteps) read_k(ks + kFirst);
+            wait_lds<2 * (kSteps - 1 - ks < kFirst ? kSteps - 1 - ks : kFirst)>();
+            lds_tie(ka[ks]);
+            lds_tie(kb[ks]);
+            sa = MM::mfma(__builtin_bit_cast(Frag, ka[ks]), qf[ks], sa);
+            sb = MM::mfma(__builtin_bit_cast(Frag, kb[ks]), qf[ks], sb);
+            asm volatile("" : "+v"(sa), "+v"(sb));     // (products in this place: left alone, the compiler puts them behind all reads)
+        });
+        // values: half of the head dims requested ahead of the weights, the others behind them
+        constexpr int kHalf = kDTiles / 2;
+#pragma unroll
+        for (int dt = 0; dt < kHalf; ++dt) read_v(at_a, dt, va[dt]);
+        uint32_t wa[8], wb[8];
+        float sum_a = 0.f, sum_b = 0.f, neg_m = m_i == -INFINITY ? 0.f : -m_i;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) wa[i] = two_weights(sa, i, sc, neg_m, sum_a);
+        if (doubtful(sum_a)) raise(sa, sc, wa, sum_a);
+        l_i += sum_a;
+#pragma unroll
+        for (int dt = kHalf; dt < kDTiles; ++dt) read_v(at_a, dt, va[dt]);
+        wait_lds<4 * (kDTiles - kHalf)>();
+#pragma unroll
+        for (int dt = 0; dt < kHalf; ++dt) tie_v(va[dt]);
+        neg_m = m_i == -INFINITY ? 0.f : -m_i;
+        constexpr int kPer = 8 / (2 * kDTiles);        // pairs of weights between two products
+        auto product = [&](auto step) {
+            constexpr int i = decltype(step)::value, dt = (i / (2 * kHalf)) * kHalf + i % kHalf, h = (i / kHalf) % 2;
+            o[dt] = PV::mfma(__builtin_bit_cast(PFrag, va[dt][h]), fragment(wa, h), o[dt]);
+#pragma unroll
+            for (int k = i * kPer; k < (i + 1) * kPer; ++k) {
+                wb[k] = two_weights(sb, k, sc, neg_m, sum_b);
+                asm volatile("" : "+v"(wb[k]), "+v"(o[dt]));
+            }
+        };
+        static_for<kDTiles>(product);
+        lds_wait();
+#pragma unroll
+        for (int dt = kHalf; dt < kDTiles; ++dt) tie_v(va[dt]);
+        static_for<kDTiles>([&](auto step) { product(std::integral_constant<int, kDTiles + decltype(step)::value>{}); });
+#pragma unroll
+        for (int dt = 0; dt < kHalf; ++dt) read_v(at_b, dt, vb[dt]);
+        if (doubtful(sum_b)) raise(sb, sc, wb, sum_b);
+        l_i += sum_b;
+#pragma unroll
+        for (int dt = kHalf; dt < kDTiles; ++dt) read_v(at_b, dt, vb[dt]);
+        wait_lds<4 * (kDTiles - kHalf)>();
+#pragma unroll
+        for (int dt = 0; dt < kHalf; ++dt) tie_v(vb[dt]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int dt = 0; dt < kHalf; ++dt) o[dt] = PV::mfma(__builtin_bit_cast(PFrag, vb[dt][h]), fragment(wb, h), o[dt]);
+        lds_wait();
+#pragma unroll
+        for (int dt = kHalf; dt < kDTiles; ++dt) tie_v(vb[dt]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int dt = kHalf; dt < kDTiles; ++dt) o[dt] = PV::mfma(__builtin_bit_cast(PFrag, vb[dt][h]), fragment(wb, h), o[dt]);
     }
 
     // Sum over both halves of the lanes that share a row
@@ -394,6 +519,8 @@ __device__ __forceinline__ int page_at(const PagedAttnParams& p, const_i32 table
 
 // Transfers of a tile's keys and values (and exponents) from its pages to a ring slot, as wave `part` of PARTS.
 // WIDENED: an 8-bit tile that is copied into the 16-bit layout afterwards lies in LDS as it does in memory.  ONCE: past the caches.
+constexpr int kRawBuffer = 0x00020000;        // buffer resource, word 3: raw 32-bit data
+
 template <int D, int PARTS, bool FP8, bool WIDENED, bool ONCE> struct Fetch {
     static constexpr int kRowBytes = FP8 ? D : 2 * D;             // a key's or a value's row in the cache
     static constexpr int kDma = 2 * kTileN * kRowBytes / 1024;    // transfers of 1 KiB
@@ -403,45 +530,72 @@ template <int D, int PARTS, bool FP8, bool WIDENED, bool ONCE> struct Fetch {
     static_assert(kDma % PARTS == 0, "a wave has whole transfers");
     static constexpr int kLanesPerRow = kRowBytes / 16, kRowsPerDma = 64 / kLanesPerRow;
 
+    static constexpr int kPerHalf = 16 / kRowsPerDma;             // transfers of 16 rows
+    static_assert(kPer % kPerHalf == 0, "a wave has whole halves");
+
     int first_unit;
-    uint32_t off[kPer];                       // this lane's piece, from the start of its 16 rows
-    __device__ __forceinline__ Fetch(int part, int lane) : first_unit(part * kPer) {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const int r = row(j, lane), slot = lane % kLanesPerRow;
-            const int chunk = WIDENED ? slot : FP8 ? (is_v(j) ? v8_chunk<D>(r, slot) : k8_chunk<D>(r, slot))
-                                                   : (is_v(j) ? v_chunk<D>(r, slot) : k_chunk<D>(r, slot));
-            off[j] = (uint32_t)((r & 15) * kRowBytes + chunk * 16);
-        }
+    // This lane's piece of a half's first transfer.  The next ones lie 1 KiB further each, in memory and in LDS; the keys' swizzle
+    // changes by a constant from one to the next, the values' not at all.
+    uint32_t k_off, v_off;
+    // A wave whose transfers are all keys' or all values', of one 16-key half, has one address a tile.
+    static constexpr bool kOneSide = PARTS >= 2, kOneHalf = PARTS >= 4;
+    const unsigned char* side;                // the head's rows of page 0 in the tensor that it fetches from
+    const unsigned char* v_side;              // .. and in v, where it fetches both
+    uint64_t page_bytes;
+    uint32_t turn;                            // what the keys' swizzle changes by
+    __device__ __forceinline__ Fetch(const PagedAttnParams& p, int head, int part, int lane) : first_unit(part * kPer) {
+        const int64_t at = ((int64_t)head << p.batch.page_shift) * kRowBytes;
+        const unsigned char* k = static_cast<const unsigned char*>(p.k) + at;
+        v_side = static_cast<const unsigned char*>(p.v) + at;
+        side = kOneSide && part >= PARTS / 2 ? v_side : k;
+        page_bytes = ((uint64_t)p.batch.kv_heads << p.batch.page_shift) * kRowBytes;
+        const int r = lane / kLanesPerRow, slot = lane % kLanesPerRow;
+        k_off = (uint32_t)(r * kRowBytes + (WIDENED ? slot : FP8 ? k8_chunk<D>(r, slot) : k_chunk<D>(r, slot)) * 16);
+        v_off = (uint32_t)(r * kRowBytes + (WIDENED ? slot : FP8 ? v8_chunk<D>(r, slot) : v_chunk<D>(r, slot)) * 16);
+        if (kOneSide && part >= PARTS / 2) k_off = v_off;
+        turn = WIDENED || (kOneSide && part >= PARTS / 2) ? 0u : 64u;
     }
     __device__ __forceinline__ bool is_v(int j) const { return first_unit + j >= kDma / 2; }
-    __device__ __forceinline__ int row(int j, int lane) const { return ((first_unit + j) % (kDma / 2)) * kRowsPerDma + lane / kLanesPerRow; }
-    __device__ __forceinline__ int half_of(int j) const { return (((first_unit + j) % (kDma / 2)) * kRowsPerDma) / 16; }
+    __device__ __forceinline__ int half_of(int j) const { return ((first_unit + j) % (kDma / 2)) / kPerHalf; }
 
-    // p0, p1: pages of the tile's 16-key halves; returns the halves that are on none
+    // p0, p1: pages of the tile's 16-key halves; returns the halves that are on none.  A half's rows are a buffer of as many bytes
+    // as there are rows: what a lane asks for behind its end the hardware answers with zeros, and no lane needs an address.
     __device__ __forceinline__ uint32_t tile(const PagedAttnParams& p, int keys, int head, int first, int p0, int p1, unsigned char* dst, int lane) const {
         typedef const void __attribute__((address_space(1))) * global_ptr;
         typedef void __attribute__((address_space(3))) * lds_ptr;
-        const int page_rows = 1 << p.batch.page_shift;
+        const uint32_t page_mask = (1u << p.batch.page_shift) - 1u;
         const bool ok0 = (unsigned)p0 < (unsigned)p.batch.num_pages, ok1 = (unsigned)p1 < (unsigned)p.batch.num_pages;
-        const int64_t row_0 = (((int64_t)(ok0 ? p0 : 0) * p.batch.kv_heads + head) << p.batch.page_shift) + (first & (page_rows - 1));
-        const int64_t row_1 = (((int64_t)(ok1 ? p1 : 0) * p.batch.kv_heads + head) << p.batch.page_shift) + ((first + 16) & (page_rows - 1));
-        auto base_of = [&](int j) { return static_cast<const unsigned char*>(is_v(j) ? p.v : p.k) + (half_of(j) ? row_1 : row_0) * kRowBytes; };
-        if (first + kTileN <= keys && ok0 && ok1) {
-#pragma unroll
-            for (int j = 0; j < kPer; ++j)
-                __builtin_amdgcn_global_load_lds((global_ptr)(base_of(j) + off[j]), (lds_ptr)(dst + (first_unit + j) * 1024), 16, 0, ONCE ? 2 : 0);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                const bool here = first + row(j, lane) < keys && (half_of(j) ? ok1 : ok0);
-                const unsigned char* src = here ? base_of(j) + off[j] : reinterpret_cast<const unsigned char*>(kZeroRow);
-                __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(dst + (first_unit + j) * 1024), 16, 0, 0);
-            }
-        }
+#if defined(__HIP_DEVICE_COMPILE__)           // (the host pass knows no buffer resources)
+        auto rows_at = [&](const unsigned char* tensor, int half) {
+            const bool ok = half ? ok1 : ok0;
+            const uint32_t page = (uint32_t)(ok ? (half ? p1 : p0) : 0), in_page = ((uint32_t)first + 16u * half) & page_mask;
+            // (said to be uniform: a resource in vector registers is tried lane by lane)
+            const int rows = __builtin_amdgcn_readfirstlane(ok ? max(min(keys - first - 16 * half, 16), 0) : 0);
+            const uint64_t from = (uint64_t)tensor + page * page_bytes + in_page * (uint32_t)kRowBytes;
+            const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)from) |
+                                  ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(from >> 32)) << 32);
+            return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, rows * kRowBytes, kRawBuffer);
+        };
+        const unsigned char* v_from = kOneSide ? side : v_side;
+        const auto k0 = rows_at(side, kOneHalf ? half_of(0) : 0), k1 = kOneHalf ? k0 : rows_at(side, 1);
+        const auto v0 = kOneSide ? k0 : rows_at(v_from, 0), v1 = kOneSide ? k1 : rows_at(v_from, 1);
+        static_for<kPer>([&](auto index) {
+            constexpr int j = decltype(index)::value, in_half = j % kPerHalf;
+            constexpr bool v = !kOneSide && j >= kDma / 2;
+            constexpr int half = kOneHalf ? 0 : j % (kDma / 2) / kPerHalf;
+            const uint32_t off = v ? v_off : k_off ^ (in_half * turn);
+            lds_ptr to = (lds_ptr)(dst + (first_unit + j - in_half) * 1024);
+            if constexpr (v && half) __builtin_amdgcn_raw_ptr_buffer_load_lds(v1, to, 16, off, 0, in_half * 1024, ONCE ? 2 : 0);
+            else if constexpr (v) __builtin_amdgcn_raw_ptr_buffer_load_lds(v0, to, 16, off, 0, in_half * 1024, ONCE ? 2 : 0);
+            else if constexpr (half) __builtin_amdgcn_raw_ptr_buffer_load_lds(k1, to, 16, off, 0, in_half * 1024, ONCE ? 2 : 0);
+            else __builtin_amdgcn_raw_ptr_buffer_load_lds(k0, to, 16, off, 0, in_half * 1024, ONCE ? 2 : 0);
+        });
+#endif
         if constexpr (FP8) {                  // exponents of the 32 keys, then of the 32 values, four to a lane
             const int l = lane & 15, g = (l >> 2) & 1;
-            const uint8_t* src = ((l & 8) ? p.v_exponent : p.k_exponent) + (g ? row_1 : row_0) + 4 * (l & 3);
+            const int64_t row = ((((int64_t)(g ? (ok1 ? p1 : 0) : (ok0 ? p0 : 0)) * p.batch.kv_heads + head) << p.batch.page_shift)) +
+                                (int64_t)(((uint32_t)first + 16u * g) & page_mask);
+            const uint8_t* src = ((l & 8) ? p.v_exponent : p.k_exponent) + row + 4 * (l & 3);
             const bool here = first + 16 * g < keys && (g ? ok1 : ok0);
             src = here ? src : reinterpret_cast<const uint8_t*>(kZeroRow);
             __builtin_amdgcn_global_load_lds((global_ptr)src, (lds_ptr)(dst + kDma * 1024), 4, 0, 0);

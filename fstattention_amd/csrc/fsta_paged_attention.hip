@@ -88,10 +88,11 @@ template <bool JOINS> __device__ __forceinline__ bool find_item(const PagedAttnP
 // 8-bit tiles: up to two row groups read them as they are and widen in registers; four share a widened copy.
 template <int D, int R, int S, bool FP8> struct Shape {
     static constexpr bool kWiden = FP8 && R > 2;
-    static constexpr int kStages = R == 4 || (FP8 && R == 2) ? 4 : 2;
+    static constexpr int kStep = R == 4 && !FP8 ? 2 : 1;                   // tiles worked on between barriers
+    static constexpr int kStages = R == 4 ? 5 : FP8 && R == 2 ? 4 : 2;
     using Raw = Fetch<D, R, FP8, kWiden, false>;
     static constexpr int kWideBytes = 2 * kTileN * D * 2;
-    static constexpr int kShareBytes = kStages * Raw::kBytes + (kWiden ? kWideBytes : 0);
+    static constexpr int kShareBytes = kStages * Raw::kBytes + (kWiden ? kStep * kWideBytes : 0);
     static constexpr size_t kJoin = (size_t)(S - 1) * R * (32 * D + 64) * 4;
     static constexpr size_t kLds = (size_t)S * kShareBytes > kJoin ? (size_t)S * kShareBytes : kJoin;
 };
@@ -103,7 +104,7 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
     using SH = Shape<D, R, S, FP8>;
     using F = Fetch<D, R, FP8, SH::kWiden, ONCE>;
     using G = RowGroup<BF16, D, FP8 && !SH::kWiden, SPLIT>;
-    constexpr int kStages = SH::kStages, kDTiles = G::kDTiles;
+    constexpr int kStages = SH::kStages, kStep = SH::kStep, kDTiles = G::kDTiles;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
 
     const int tid = threadIdx.x, lane = tid & 63;
@@ -123,7 +124,7 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
     const int tiles = (tile_keys + kTileN - 1) / kTileN;
     const int tile0 = (int)((int64_t)tiles * at.run / at.runs), tile1 = (int)((int64_t)tiles * (at.run + 1) / at.runs);
     const int my_tiles = (tile1 - tile0 - share + S - 1) / S;       // of this share (tile0 + share, + S, ...)
-    const int steps = (tile1 - tile0 + S - 1) / S;
+    const int steps = (tile1 - tile0 + S * kStep - 1) / (S * kStep);
 
     // this wave's rows
     const int row0 = at.row_tile << p.row_shift;                    // of the tile, among (token, head of the group)
@@ -138,19 +139,19 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
 
     // ---- ring of tiles ----------------------------------------------------------------------------------------------------
     unsigned char* ring = smem + share * SH::kShareBytes;
-    const F fetch(group_of_rows, lane);
+    const F fetch(p, head, group_of_rows, lane);
     const const_i32 table = table_of(p, at.seq);
     int next_p0 = 0, next_p1 = 0;             // pages of the share's tile that is fetched next
     auto look_up = [&](int i) {
         if (i < my_tiles) {
             const int first = (tile0 + share + i * S) * kTileN;
             next_p0 = page_at(p, table, s.keys, first);
-            next_p1 = page_at(p, table, s.keys, first + 16);
+            next_p1 = p.batch.page_shift > 4 ? next_p0 : page_at(p, table, s.keys, first + 16);     // (tiles lie at multiples of 32)
         }
     };
     uint32_t bad_halves = 0;                  // two bits per slot: halves of its tile on pages outside the cache
     auto issue = [&](int i) {                 // the share's i-th tile into slot i % kStages
-        const int slot = i % kStages, p0 = next_p0, p1 = next_p1;
+        const int slot = (int)((uint32_t)i % kStages), p0 = next_p0, p1 = next_p1;
         look_up(i + 1);
         const uint32_t bad = fetch.tile(p, s.keys, head, (tile0 + share + i * S) * kTileN, p0, p1, ring + slot * F::kBytes, lane);
         bad_halves = (bad_halves & ~(3u << (2 * slot))) | (bad << (2 * slot));
@@ -160,59 +161,79 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
     if (my_tiles > 0) { issue(0); issued = 1; }
     rows.await_q();
     // A wave that has a ring of its own refills a slot as soon as it is done with it; waves that share one, behind the next barrier.
-    constexpr int kFill = R == 1 ? kStages : kStages - 1;
+    constexpr int kFill = R == 1 ? kStages : kStages - kStep;
     for (; issued < my_tiles && issued < kFill; ++issued) issue(issued);
 
-    auto compute = [&](int i, const unsigned char* tile_lds) {
-        const int first = (tile0 + share + i * S) * kTileN;
-        if (!has_rows || first > mine.sight.high_limit) return;
-        const uint32_t bad = (bad_halves >> (2 * (i % kStages))) & 3u;
-        rows.tile(lds_addr(tile_lds), p.scale_log2e, bad || !mine.sight.whole(p, first), [&] { return mine.sight.word(p, first, bad); });
+    const uint32_t ring_lds = lds_addr(ring), wide_lds = ring_lds + kStages * F::kBytes;
+    auto bad_of = [&](int i) { return (bad_halves >> (2 * (int)((uint32_t)i % kStages))) & 3u; };
+    auto lies_at = [&](int i) { return SH::kWiden ? wide_lds + (uint32_t)((i % kStep) * SH::kWideBytes) : ring_lds + ((uint32_t)i % kStages) * F::kBytes; };
+    auto first_of = [&](int i) { return (tile0 + share + i * S) * kTileN; };
+    auto compute = [&](int i) {
+        const int first = first_of(i);
+        if (first > mine.sight.high_limit) return;
+        const uint32_t bad = bad_of(i);
+        rows.tile(lies_at(i), p.scale_log2e, bad || !mine.sight.whole(p, first), [&] { return mine.sight.word(p, first, bad); });
     };
     // 8-bit rows: the share's waves widen the landed tile into the 16-bit layout, once for all row groups
     auto widen = [&](int i) {
-        const uint32_t raw = lds_addr(ring + (i % kStages) * F::kBytes);
-        const uint32_t wide = lds_addr(ring + kStages * F::kBytes);
+        const uint32_t raw = ring_lds + ((uint32_t)i % kStages) * F::kBytes, wide = lies_at(i);
         constexpr int kPieces = 2 * kTileN * D / 16 / 64 / R;          // 16-byte pieces per lane
+        u32x4 bytes[kPieces];
+        uint32_t E[kPieces];
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) {
+            const int piece = (group_of_rows * kPieces + j) * 64 + lane;
+            bytes[j] = lds_read_b128(raw + piece * 16);
+            asm volatile("ds_read_u8 %0, %1" : "=v"(E[j]) : "v"(raw + F::kDma * 1024 + piece / (D / 16)) : "memory");
+        }
+        lds_wait();
 #pragma unroll
         for (int j = 0; j < kPieces; ++j) {
             const int piece = (group_of_rows * kPieces + j) * 64 + lane;
             const int r = piece / (D / 16), c = piece % (D / 16);      // r: 0..31 keys, 32..63 values
             const bool is_v = r >= kTileN;
-            u32x4 bytes = lds_read_b128(raw + piece * 16);
-            uint32_t E;
-            asm volatile("ds_read_u8 %0, %1" : "=v"(E) : "v"(raw + F::kDma * 1024 + r) : "memory");
-            lds_wait();
-            lds_tie(bytes);
-            lds_tie(E);
-            const float scale = __builtin_bit_cast(float, min(E, 254u) << 23);     // (exponents of unused rows may be anything)
+            lds_tie(bytes[j]);
+            lds_tie(E[j]);
+            const float scale = __builtin_bit_cast(float, min(E[j], 254u) << 23);     // (exponents of unused rows may be anything)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const u32x4 w = widen8<BF16>(bytes[2 * h], bytes[2 * h + 1], scale);
+                const u32x4 w = widen8<BF16>(bytes[j][2 * h], bytes[j][2 * h + 1], scale);
                 const int rr = r & (kTileN - 1);
                 const int chunk = is_v ? v_chunk<D>(rr, 2 * c + h) : k_chunk<D>(rr, 2 * c + h);
                 lds_write_b128(wide + (uint32_t)((is_v ? kTileN * D * 2 : 0) + rr * D * 2 + chunk * 16), w);
             }
         }
     };
-    for (int i = 0; i < steps; ++i) {
-        // tile i has landed for everyone who reads it, and everyone is done with the tile before it: its slot is refilled
-        wait_tiles<F::kPerTile, kFill - 1>(max(issued - i - 1, 0));
-        auto refill = [&] { if (issued < my_tiles) { issue(issued); ++issued; } };
+    for (int step = 0; step < steps; ++step) {
+        // the step's tiles have landed for everyone who reads them, and everyone is done with those before: their slots are refilled
+        const int i = step * kStep, here = min(my_tiles - i, kStep);
+        wait_tiles<F::kPerTile, kFill - kStep>(max(issued - i - here, 0));
         if constexpr (R > 1) {
             ring_barrier();
-            refill();
+#pragma unroll
+            for (int k = 0; k < kStep; ++k)
+                if (issued < my_tiles) { issue(issued); ++issued; }
         }
         if constexpr (SH::kWiden) {
-            if (i < my_tiles) widen(i);
+#pragma unroll 1
+            for (int k = 0; k < here; ++k) widen(i + k);
             ring_barrier();
-            if (i < my_tiles) compute(i, ring + kStages * F::kBytes);
-        } else {
-            if (i < my_tiles) compute(i, ring + (i % kStages) * F::kBytes);
+        }
+        if (has_rows) {
+            if constexpr (kStep == 2) {
+                const int a = first_of(i);
+                if (here == 2 && mine.sight.whole(p, a + kTileN) && (bad_of(i) | bad_of(i + 1)) == 0)
+                    rows.two_tiles(lies_at(i), lies_at(i + 1), p.scale_log2e);
+                else
+#pragma unroll 1
+                    for (int k = 0; k < here; ++k) compute(i + k);
+            } else if (here > 0) {
+                compute(i);
+            }
         }
         if constexpr (R == 1) {
             lds_wait();
-            refill();
+            if (issued < my_tiles) { issue(issued); ++issued; }
         }
     }
 
@@ -257,7 +278,9 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
     const float inv = l_tot > 0.f ? 1.f / l_tot : l_tot == 0.f ? 0.f : l_tot;      // (NaN stays)
     const float lse = l_tot == 0.f ? -INFINITY : m_i + log2f(l_tot);
     if (at.part < 0) {
-        const int64_t out_row = (int64_t)(s.start + mine.token) * (p.batch.kv_heads * p.group) + mine.q_head;
+        // (worked out again: kept over the loop they cost registers that it needs)
+        const int token = (int)((uint32_t)(row0 + my_row) / (uint32_t)p.group);
+        const int64_t out_row = (int64_t)(s.start + token) * (p.batch.kv_heads * p.group) + head * p.group + (row0 + my_row) - token * p.group;
         if (p.lse && half == 0) p.lse[out_row] = lse;
         uint16_t* dst = static_cast<uint16_t*>(p.o) + out_row * D + 4 * half;
 #pragma unroll
