@@ -204,33 +204,43 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
             }
         }
     };
-    for (int step = 0; step < steps; ++step) {
-        // the step's tiles have landed for everyone who reads them, and everyone is done with those before: their slots are refilled
-        const int i = step * kStep, here = min(my_tiles - i, kStep);
-        wait_tiles<F::kPerTile, kFill - kStep>(max(issued - i - here, 0));
+    // A step's tiles have landed for everyone who reads them, and everyone is done with those before: their slots are refilled.
+    auto arrive = [&](int step) {
+        const int i = step * kStep;
+        wait_tiles<F::kPerTile, kFill - kStep>(max(issued - min(i + kStep, my_tiles), 0));
         if constexpr (R > 1) {
             ring_barrier();
 #pragma unroll
             for (int k = 0; k < kStep; ++k)
                 if (issued < my_tiles) { issue(issued); ++issued; }
         }
+    };
+    int step = 0;
+    bool arrived = false;
+    if constexpr (kStep == 2) {               // steps of two tiles that all rows see whole, up to the first that is none (a loop of its
+                                              // own: in one with the others the accumulators are copied at every step)
+        const int whole_keys = has_rows ? min(mine.sight.low_limit + 1, p.mask == kTree ? mine.sight.old : s.keys) : 0;
+        const int whole_steps = min(my_tiles / 2, (whole_keys / kTileN - tile0) / 2);
+        for (; step < whole_steps; ++step) {
+            arrive(step);
+            if ((bad_of(2 * step) | bad_of(2 * step + 1)) != 0) {
+                arrived = true;
+                break;
+            }
+            rows.two_tiles(lies_at(2 * step), lies_at(2 * step + 1), p.scale_log2e);
+        }
+    }
+    for (; step < steps; ++step) {
+        if (!arrived) arrive(step);
+        arrived = false;
+        const int i = step * kStep, here = min(my_tiles - i, kStep);
         if constexpr (SH::kWiden) {
-#pragma unroll 1
             for (int k = 0; k < here; ++k) widen(i + k);
             ring_barrier();
         }
-        if (has_rows) {
-            if constexpr (kStep == 2) {
-                const int a = first_of(i);
-                if (here == 2 && mine.sight.whole(p, a + kTileN) && (bad_of(i) | bad_of(i + 1)) == 0)
-                    rows.two_tiles(lies_at(i), lies_at(i + 1), p.scale_log2e);
-                else
+        if (has_rows)
 #pragma unroll 1
-                    for (int k = 0; k < here; ++k) compute(i + k);
-            } else if (here > 0) {
-                compute(i);
-            }
-        }
+            for (int k = 0; k < here; ++k) compute(i + k);
         if constexpr (R == 1) {
             lds_wait();
             if (issued < my_tiles) { issue(issued); ++issued; }
