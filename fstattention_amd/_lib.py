@@ -78,7 +78,7 @@ SIGNATURES = {
                                     c_void_p]),
     "fsta_paged_write": (c_int, [c_void_p] * 2 + [c_int64] * 4 + [c_void_p] * 7 + [c_int32] * 9 + [c_void_p]),
     "fsta_paged_read": (c_int, [c_void_p] * 8 + [c_int32] * 9 + [c_void_p]),
-    "fsta_paged_attention_workspace_bytes": (c_size_t, [c_int32] * 6),
+    "fsta_paged_attention_workspace_bytes": (c_size_t, [c_int32] * 7),
     "fsta_paged_attention": (c_int, [c_void_p] + [c_int64] * 2 + [c_void_p] * 8 + [c_int32] + [c_void_p] * 2 + [c_int32] * 12 +
                              [c_float, c_void_p, c_size_t, c_void_p]),
     "fsta_tree_bits": (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p]),

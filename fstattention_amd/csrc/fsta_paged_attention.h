@@ -24,8 +24,10 @@ struct PagedAttnParams {
     const uint32_t* tree_bits;     // [tokens, tree_words]
     float* part_o;                 // parts of rows whose keys several workgroups take: [part][rows][D] float32, normalised
     float* part_lse;               // [part][rows], base 2
+    uint32_t* run_length;          // the cut's, behind the parts
     int32_t tree_words, mask, group, tile_rows, row_shift, parts;
-    int32_t run_units, least_tiles;
+    int32_t run_units[3], least_tiles;   // units that a launch may be cut into, the least tiles of a run
+    float slots, unit_cost, cut_cost;    // workgroups that run at once; what a unit and the joining cost, in tiles
     float scale_log2e;
 };
 
@@ -130,13 +132,14 @@ template <bool BF16, int D, bool DIRECT, bool SPLIT> struct RowGroup {
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
     }
-    __device__ __forceinline__ static bool finite(PFrag f) {
-        constexpr uint32_t kTop = BF16 || DIRECT ? 0x7f80u : 0x7c00u;
-        const u32x4 w = __builtin_bit_cast(u32x4, f);
-        bool ok = true;
+    // Sign bits of the halves whose exponent is all ones (adding the exponent's lowest bit carries into the sign's place)
+    __device__ __forceinline__ static uint32_t not_finite(PFrag a, PFrag b) {
+        constexpr uint32_t kTop = BF16 || DIRECT ? 0x7f807f80u : 0x7c007c00u, kLow = BF16 || DIRECT ? 0x00800080u : 0x04000400u;
+        const u32x4 x = __builtin_bit_cast(u32x4, a), y = __builtin_bit_cast(u32x4, b);
+        uint32_t bits = 0u;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ok = ok && (w[e] & kTop) != kTop && (w[e] & (kTop << 16)) != kTop << 16;
-        return ok;
+        for (int e = 0; e < 4; ++e) bits |= ((x[e] & kTop) + kLow) | ((y[e] & kTop) + kLow);
+        return bits & 0x80008000u;
     }
     // The values' fragment with what is not finite replaced by 0
     __device__ __forceinline__ static PFrag only_finite(PFrag f) {
@@ -301,7 +304,7 @@ template <bool BF16, int D, bool DIRECT, bool SPLIT> struct RowGroup {
             }
             // A value that is not finite must reach the rows that see its key and no other, although a weight of zero times it
             // is a NaN: where the tile is masked, such values are taken out and put back row by row, by their signs.
-            if (masked && __ballot(!finite(f[0]) || !finite(f[1])) != 0ull) {
+            if (masked && __ballot(not_finite(f[0], f[1]) != 0u) != 0ull) {
                 constexpr uint32_t kOne = BF16 || DIRECT ? 0x3f80u : 0x3c00u;
 #pragma unroll 1
                 for (uint32_t sign = 0; sign < 2; ++sign) {
@@ -471,6 +474,33 @@ struct Sight {
     int limit, low_limit, high_limit;         // last key of this lane's row; the least and greatest of the wave's rows
     int old;                                  // keys in front of the new tokens (negative: the first new ones have no place)
     const uint32_t* bits;                     // this row's mask (trees)
+    // .. and its first words: a load in front of a tile's weights would wait for every transfer on its way
+    static constexpr int kKept = 8;
+    uint32_t kept[kKept];
+
+    __device__ __forceinline__ void keep(const PagedAttnParams& p) {
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) kept[i] = 0u;
+        if (p.mask == kTree) {
+#pragma unroll
+            for (int i = 0; i < kKept; ++i)
+                if (i < p.tree_words) kept[i] = bits[i];
+        }
+    }
+    __device__ __forceinline__ void await_kept() {
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) lds_tie(kept[i]);
+    }
+    // Word i (uniform); all ones in front of the first: keys in front of the new tokens are seen by all
+    __device__ __forceinline__ uint32_t word_of(const PagedAttnParams& p, int i) const {
+        if (i < 0) return ~0u;
+        if (i >= p.tree_words) return 0u;
+        if (i >= kKept) return bits[i];
+        uint32_t w = 0u;                      // (by masks: a choice among them would put them into memory)
+#pragma unroll
+        for (int k = 0; k < kKept; ++k) w |= kept[k] & (0u - (uint32_t)(i == k));
+        return w;
+    }
 
     __device__ __forceinline__ bool whole(const PagedAttnParams& p, int first) const {      // every row sees every key of the tile
         return first + kTileN - 1 <= low_limit && !(p.mask == kTree && first + kTileN > old);
@@ -481,11 +511,10 @@ struct Sight {
         uint32_t w = rel >= 31 ? ~0u : rel < 0 ? 0u : (2u << rel) - 1u;
         if (bad & 1u) w &= 0xffff0000u;
         if (bad & 2u) w &= 0x0000ffffu;
-        if (p.mask == kTree && first + kTileN > old) {      // keys in front of the new tokens are seen by all, the others by their bit
+        if (p.mask == kTree && first + kTileN > old) {
             const int number = first - old, wi = number >> 5, sh = number & 31;
-            const uint32_t lo = wi < 0 ? ~0u : wi < p.tree_words ? bits[wi] : 0u;
-            const uint32_t hi = wi + 1 < 0 ? ~0u : wi + 1 < p.tree_words ? bits[wi + 1] : 0u;
-            w &= sh ? (lo >> sh) | (hi << (32 - sh)) : lo;
+            const uint32_t lo = word_of(p, wi);
+            w &= sh ? (lo >> sh) | (word_of(p, wi + 1) << (32 - sh)) : lo;
         }
         return w;
     }
@@ -531,10 +560,11 @@ template <int D, int PARTS, bool FP8, bool WIDENED, bool ONCE> struct Fetch {
     static constexpr int kLanesPerRow = kRowBytes / 16, kRowsPerDma = 64 / kLanesPerRow;
 
     static constexpr int kPerHalf = 16 / kRowsPerDma;             // transfers of 16 rows
-    static_assert(kPer % kPerHalf == 0, "a wave has whole halves");
+    static constexpr int kRun = kPer < kPerHalf ? kPer : kPerHalf;   // of them this wave's, one behind the other
+    static_assert(kPer % kRun == 0 && kPerHalf % kRun == 0, "a wave has whole halves, or a part of one");
 
     int first_unit;
-    // This lane's piece of a half's first transfer.  The next ones lie 1 KiB further each, in memory and in LDS; the keys' swizzle
+    // This lane's piece of the wave's first transfer of a half.  The next ones lie 1 KiB further each, in memory and in LDS; the keys' swizzle
     // changes by a constant from one to the next, the values' not at all.
     uint32_t k_off, v_off;
     // A wave whose transfers are all keys' or all values', of one 16-key half, has one address a tile.
@@ -554,6 +584,8 @@ template <int D, int PARTS, bool FP8, bool WIDENED, bool ONCE> struct Fetch {
         v_off = (uint32_t)(r * kRowBytes + (WIDENED ? slot : FP8 ? v8_chunk<D>(r, slot) : v_chunk<D>(r, slot)) * 16);
         if (kOneSide && part >= PARTS / 2) k_off = v_off;
         turn = WIDENED || (kOneSide && part >= PARTS / 2) ? 0u : 64u;
+        const uint32_t skip = (uint32_t)(first_unit % kPerHalf);
+        k_off = (k_off ^ (skip * turn)) + skip * 1024u;
     }
     __device__ __forceinline__ bool is_v(int j) const { return first_unit + j >= kDma / 2; }
     __device__ __forceinline__ int half_of(int j) const { return ((first_unit + j) % (kDma / 2)) / kPerHalf; }
@@ -580,7 +612,7 @@ template <int D, int PARTS, bool FP8, bool WIDENED, bool ONCE> struct Fetch {
         const auto k0 = rows_at(side, kOneHalf ? half_of(0) : 0), k1 = kOneHalf ? k0 : rows_at(side, 1);
         const auto v0 = kOneSide ? k0 : rows_at(v_from, 0), v1 = kOneSide ? k1 : rows_at(v_from, 1);
         static_for<kPer>([&](auto index) {
-            constexpr int j = decltype(index)::value, in_half = j % kPerHalf;
+            constexpr int j = decltype(index)::value, in_half = j % kRun;
             constexpr bool v = !kOneSide && j >= kDma / 2;
             constexpr int half = kOneHalf ? 0 : j % (kDma / 2) / kPerHalf;
             const uint32_t off = v ? v_off : k_off ^ (in_half * turn);

@@ -4,7 +4,7 @@
 // rows sees one K/V head, so every key is read once for the whole group.  A wave owns 32 rows as the columns of
 //     S^T = K_tile . Q^T      and      O^T += V_tile^T . P^T        (32x32x16 matrix instructions, 32 keys a tile)
 // with a float32 base-2 online softmax in between; P stays in the registers the scores came in.  R waves share a tile of keys
-// (row groups), S tiles are worked on at a time (key shares, joined at the end through LDS): (R, S) = (1, 4), (2, 2), (4, 1).
+// (row groups), S tiles are worked on at a time (key shares, joined at the end through LDS): (R, S) = (1, 4), (2, 2), (4, 1), (8, 1).
 // Keys and values come page by page straight into an LDS ring (global -> LDS transfers of 1 KiB); rows that do not exist (past
 // the sequence's end, on a page outside the cache) come from a row of zeros, so that what lies in unused rows of a page can not
 // turn a weight of zero into a NaN.
@@ -15,14 +15,16 @@ namespace {
 
 using namespace paged;
 
-constexpr int kDecodeUnits = 512, kMiddleUnits = 512, kChunkUnits = 256;       // (tile of rows, run of keys, K/V head) units a launch is cut into where it has fewer
 constexpr int kDecodeLeast = 16, kChunkLeast = 8;          // tiles of a run, at least
 
 // ---- who does what --------------------------------------------------------------------------------------------------------
-// Every sequence's rows are cut into tiles of tile_rows and, where the launch would otherwise not fill the GPU, its keys into
-// runs.  The cut is a function of the lengths alone; every wave works it out for itself from the arrays (64 sequences at a
-// time, a lane each: one round trip and a prefix sum), so that no launch has to come before this one and the host never waits
-// for a length.  A run has cost / run_units tiles, cost = all (tile of rows, tile of keys) pairs of the batch.
+// Every sequence's rows are cut into tiles of tile_rows and, where that is faster, its keys into runs of at most `longest` tiles.
+// The cut is a function of the lengths alone; every wave works it out for itself from the arrays (64 sequences at a time, a lane
+// each: one round trip and a few prefix sums), so that no launch has to come before this one and the host never waits for a length.
+// Of four cuts (none, and runs for 1, 2 or 3 rounds' worth of units) the one is taken whose units would be done first: rounds of
+// workgroups times what a unit lasts, its start included, and joining the runs.  (Measured with every cut forced: 32 sequences of
+// 4096 keys, 8 K/V heads, whole 88.7 us, in runs for two rounds 94; 40 sequences 132 whole, 121; 128 tiles of 128 rows 45 us whole and
+// 38 in two runs; 256 of them 51 whole and 66 in two.)
 struct Cut {
     uint32_t longest;              // tiles of keys in a run
     // (a batch has fewer than 2^30 rows; tile_rows is a power of two)
@@ -33,14 +35,51 @@ struct Cut {
     __device__ __forceinline__ uint32_t runs(const SeqLens& s) const { return ((uint32_t)key_tiles(s) + longest - 1) / longest; }
 };
 
+// Largest of the lanes up to and including this one
+__device__ __forceinline__ uint32_t wave_prefix_max(uint32_t x) {
+    auto from = [](uint32_t v, auto ctrl, auto rows) {
+        return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    };
+    x = max(x, from(x, std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{}));   // row_shr:1, 2, 4, 8
+    x = max(x, from(x, std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{}));
+    x = max(x, from(x, std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{}));
+    x = max(x, from(x, std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{}));
+    x = max(x, from(x, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{}));   // row_bcast:15, :31
+    x = max(x, from(x, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{}));
+    return x;
+}
+
 struct Place {
     SeqLens s;
     int seq, row_tile, run, runs, part;      // part: of the tile's first run, -1 where the keys are not cut
 };
 
-// The item-th (tile of rows, run of keys) of the batch, or with JOINS the item-th tile whose keys are cut; the tiles of a
-// sequence last ones first (causal: they have most keys).  False: there is no such item.
-template <bool JOINS> __device__ __forceinline__ bool find_item(const PagedAttnParams& p, uint32_t item, int lane, Place* out) {
+// Tiles of keys in a run.  (In float: a rounding of 2^-24 moves a cut by nothing that counts.)
+__device__ __forceinline__ uint32_t choose(const PagedAttnParams& p, const SeqLens& first, float work) {
+    auto run_of = [&](int units) { return (uint32_t)fminf(fmaxf(ceilf(work / (float)units), (float)p.least_tiles), 1073741824.f); };
+    if (p.batch.batch > 64) return run_of(p.run_units[1]);
+    const uint32_t tiles = (uint32_t)Cut::row_tiles(first, p);
+    const float keys = tiles ? (float)Cut::key_tiles(first) : 0.f;
+    const float most = (float)lane_of(wave_prefix_max((uint32_t)keys), 63);
+    float best = INFINITY;
+    uint32_t longest = 1u << 30;
+#pragma unroll
+    for (int i = -1; i < 3; ++i) {
+        const uint32_t run = i < 0 ? 1u << 30 : run_of(p.run_units[i < 0 ? 0 : i]);
+        const float runs = ceilf(keys * __builtin_amdgcn_rcpf((float)run));
+        const float units = (float)lane_of(wave_prefix_sum(tiles * (uint32_t)runs), 63) * (float)p.batch.kv_heads;
+        const float lasts = fminf(most, (float)run) + p.unit_cost;
+        const float done = (ceilf(units / p.slots) - 1.f) * (work / fmaxf(units, 1.f) + p.unit_cost) + lasts + (most > (float)run ? p.cut_cost : 0.f);
+        if (done < best) {
+            best = done;
+            longest = run;
+        }
+    }
+    return longest;
+}
+
+// The first 64 sequences' lengths, and the cut
+__device__ __forceinline__ SeqLens make_cut(const PagedAttnParams& p, int lane, Cut* cut) {
     const SeqLens first = seq_lens(p.batch, lane);       // (the first 64 sequences' lengths are loaded once)
     uint64_t cost = 0;
     for (int c = 0; c < p.batch.batch; c += 64) {
@@ -51,9 +90,13 @@ template <bool JOINS> __device__ __forceinline__ bool find_item(const PagedAttnP
         cost += lane_of(wave_prefix_sum(low), 63);
         cost += (uint64_t)lane_of(wave_prefix_sum(high), 63) << 24;
     }
-    // (rounded up, in float: a rounding of 2^-24 moves the cut by nothing that counts, and both kernels round alike)
-    const float longest = ceilf((float)cost * (float)p.batch.kv_heads / (float)p.run_units);
-    const Cut cut{(uint32_t)fminf(fmaxf(longest, (float)p.least_tiles), 1073741824.f)};
+    cut->longest = choose(p, first, (float)cost * (float)p.batch.kv_heads);
+    return first;
+}
+
+// The item-th (tile of rows, run of keys) of the batch, or with JOINS the item-th tile whose keys are cut; the tiles of a
+// sequence last ones first (causal: they have most keys).  False: there is no such item.
+template <bool JOINS> __device__ __forceinline__ bool find_item(const PagedAttnParams& p, const SeqLens& first, const Cut& cut, uint32_t item, int lane, Place* out) {
     uint32_t parts = 0;
     for (int c = 0; c < p.batch.batch; c += 64) {
         const SeqLens s = c ? seq_lens(p.batch, c + lane) : first;
@@ -88,8 +131,8 @@ template <bool JOINS> __device__ __forceinline__ bool find_item(const PagedAttnP
 // 8-bit tiles: up to two row groups read them as they are and widen in registers; four share a widened copy.
 template <int D, int R, int S, bool FP8> struct Shape {
     static constexpr bool kWiden = FP8 && R > 2;
-    static constexpr int kStep = R == 4 && !FP8 ? 2 : 1;                   // tiles worked on between barriers
-    static constexpr int kStages = R == 4 ? 5 : FP8 && R == 2 ? 4 : 2;
+    static constexpr int kStep = R >= 4 && !FP8 ? 2 : 1;                   // tiles worked on between barriers
+    static constexpr int kStages = R == 8 ? 9 : R == 4 ? 5 : FP8 && R == 2 ? 4 : 2;
     using Raw = Fetch<D, R, FP8, kWiden, false>;
     static constexpr int kWideBytes = 2 * kTileN * D * 2;
     static constexpr int kShareBytes = kStages * Raw::kBytes + (kWiden ? kStep * kWideBytes : 0);
@@ -116,7 +159,10 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
     const uint32_t item = blockIdx.x / (uint32_t)p.batch.kv_heads;
     const int head = (int)(blockIdx.x - item * (uint32_t)p.batch.kv_heads);
     Place at;
-    if (!find_item<false>(p, item, lane, &at)) return;
+    Cut cut;
+    const SeqLens lens = make_cut(p, lane, &cut);
+    if (blockIdx.x == 0 && tid == 0) *p.run_length = cut.longest;        // (the join reads it)
+    if (!find_item<false>(p, lens, cut, item, lane, &at)) return;
     const SeqLens s = at.s;
 
     // this unit's tiles of keys
@@ -133,7 +179,8 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
     const int half = rows.half, ql = rows.ql;
     const int my_row = group_of_rows * 32 + ql;                     // in the tile
     const bool has_rows = group_of_rows * 32 < rows_left;
-    const Rows mine = rows_of(p, s, head, row0, rows_left, group_of_rows * 32, ql);
+    Rows mine = rows_of(p, s, head, row0, rows_left, group_of_rows * 32, ql);
+    mine.sight.keep(p);
     rows.load_q(static_cast<const uint16_t*>(p.q) + (int64_t)(s.start + mine.token) * p.q_token_stride + (int64_t)mine.q_head * p.q_head_stride);
     rows.reset();
 
@@ -160,6 +207,7 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
     int issued = 0;
     if (my_tiles > 0) { issue(0); issued = 1; }
     rows.await_q();
+    mine.sight.await_kept();
     // A wave that has a ring of its own refills a slot as soon as it is done with it; waves that share one, behind the next barrier.
     constexpr int kFill = R == 1 ? kStages : kStages - kStep;
     for (; issued < my_tiles && issued < kFill; ++issued) issue(issued);
@@ -324,7 +372,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
     const uint32_t item = blockIdx.x / (uint32_t)p.batch.kv_heads;
     const int head = (int)(blockIdx.x - item * (uint32_t)p.batch.kv_heads);
     Place at;
-    if (!find_item<true>(p, item, lane, &at)) return;
+    if (!find_item<true>(p, seq_lens(p.batch, lane), Cut{*p.run_length}, item, lane, &at)) return;
     const int rows = min(at.s.fresh * p.group - (at.row_tile << p.row_shift), p.tile_rows);
     const int runs = max(min(at.runs, p.parts / p.batch.kv_heads - at.part), 0);
     const int my = tid / kLanes, sub = my / ROWS, col = 4 * (tid % kLanes);
@@ -397,29 +445,45 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
 
-// Rows of a workgroup's tile by the most rows a sequence can have: up to 32 rows the keys are all there is to read and its
-// waves share them out; from 128 rows on every wave has rows of its own.
-int rows_of_tile(int64_t most_rows) { return most_rows <= 32 ? 32 : most_rows <= 64 ? 64 : 128; }
+// Rows of a workgroup's tile.  Up to 32 rows a sequence the keys are all there is to read, and the waves share them out; 64 rows: in
+// pairs; from 128 rows on every wave has rows of its own.  256 rows where that means that every key is read once (trees of 256 nodes,
+// 32 heads: 41 -> 37 us), or where there are two rounds of such tiles (4096 after 16384: 1221 -> 1189 us; with one round the last
+// tiles of a causal chunk are waited for: 2048 tokens 63 -> 71 us).  8-bit tiles are widened by all waves together, behind a barrier
+// more, which two workgroups per CU hide and one does not (348 -> 384 us); head_dim 64 fits three workgroups of 128 rows on a CU.
+int rows_of_tile(int64_t most_rows, int64_t all_rows, int32_t kv_heads, int32_t head_dim, bool fp8) {
+    if (most_rows <= 32) return 32;
+    if (most_rows <= 64) return 64;
+    if (most_rows <= 128 || head_dim == 64 || fp8) return 128;
+    return most_rows <= 256 || all_rows / 256 * kv_heads >= 2 * kCus ? 256 : 128;
+}
+
+// What find_item weighs, in the time a workgroup takes for a tile of keys (0.66 us alone on its CU with up to 64 rows; with 128 rows
+// 0.9 us alone, and two share a CU at 1.05 us): a unit's start and end 4 to 5 us, the join's launch 5.5 us and more with more rows
+struct Costs { float slots, unit, cut; };
+Costs costs_of(int tile_rows) { return tile_rows >= 128 ? Costs{(tile_rows == 256 ? 1.f : 2.f) * kCus, 6.f, 12.f} : Costs{kCus, 7.f, 8.f}; }
 
 struct Sizes {
     int tile_rows;
     int64_t most_rows;          // of a sequence, as far as the host knows
     int64_t row_tiles;          // at most, over the batch
-    int64_t items, parts;
-    int run_units, least_tiles;
+    int64_t items, parts;       // of all heads: parts
+    int64_t cut_tiles;          // a head's
+    int run_units[3], least_tiles;
 };
-Sizes sizes_of(int32_t batch, int32_t tokens, int32_t max_q_len, int32_t heads, int32_t kv_heads) {
+Sizes sizes_of(int32_t batch, int32_t tokens, int32_t max_q_len, int32_t heads, int32_t kv_heads, int32_t head_dim, bool fp8) {
     Sizes z;
     const int group = heads / kv_heads;
     z.most_rows = (int64_t)(max_q_len > 0 && max_q_len < tokens ? max_q_len : tokens) * group;
-    z.tile_rows = rows_of_tile(z.most_rows);
+    z.tile_rows = rows_of_tile(z.most_rows, (int64_t)tokens * group, kv_heads, head_dim, fp8);
     z.row_tiles = ((int64_t)tokens * group + (int64_t)(batch < tokens ? batch : tokens) * (z.tile_rows - 1)) / z.tile_rows;
-    z.run_units = z.tile_rows == 32 ? kDecodeUnits : z.tile_rows == 64 ? kMiddleUnits : kChunkUnits;
+    for (int i = 0; i < 3; ++i) z.run_units[i] = z.tile_rows == 256 ? kCus / 2 << i : (i + 1) * kCus;
     z.least_tiles = z.tile_rows == 32 ? kDecodeLeast : kChunkLeast;
-    // a run has at least cost / run_units tiles (rounded: 2^-20 more), and a tile of rows one run more than whole ones
-    const int64_t runs = (z.run_units + z.run_units / 1024 + kv_heads) / kv_heads;
+    // a run has at least cost / run_units tiles (rounded: 2^-20 more), a tile of rows at most one run more than whole ones, and
+    // no more tiles of rows are cut than there are, or than units were wanted
+    const int64_t most = z.run_units[2], runs = (most + most / 256 + kv_heads) / kv_heads;
     z.items = z.row_tiles + runs;
-    z.parts = 2 * runs * kv_heads;      // a cut tile of t key tiles has fewer than 2 t / longest runs
+    z.cut_tiles = z.row_tiles < runs ? z.row_tiles : runs;
+    z.parts = (runs + z.cut_tiles) * kv_heads;
     return z;
 }
 
@@ -446,9 +510,11 @@ template <bool BF16, int D, int R, int S, bool FP8> int launch_units(const Paged
 }
 
 template <bool BF16, int D, int ROWS> int launch_join(const PagedAttnParams& p, const Sizes& z, hipStream_t stream) {
-    const int64_t items = (z.run_units + z.run_units / 1024 + p.batch.kv_heads) / p.batch.kv_heads;      // more than there are cut tiles
+    const int64_t items = z.cut_tiles;
     const int64_t rows = z.most_rows < z.tile_rows ? z.most_rows : z.tile_rows;
-    const dim3 grid((unsigned)(items * p.batch.kv_heads), (unsigned)((rows + ROWS - 1) / ROWS));
+    // (most of them find that there is nothing to do)
+    const int64_t wanted = (rows + ROWS - 1) / ROWS, room = 4 * kCus / (items * p.batch.kv_heads) + 1;
+    const dim3 grid((unsigned)(items * p.batch.kv_heads), (unsigned)(wanted < room ? wanted : room));
     hipLaunchKernelGGL((paged_join_kernel<BF16, D, ROWS>), grid, dim3(256), 0, stream, p);
     FSTA_HIP_OK(hipGetLastError());
     return FSTA_OK;
@@ -459,7 +525,9 @@ template <bool BF16, int D, bool FP8> int launch_attention(const PagedAttnParams
     int rc;
     if (z.tile_rows == 32) rc = launch_units<BF16, D, 1, 4, FP8>(p, units, z, stream);
     else if (z.tile_rows == 64) rc = launch_units<BF16, D, 2, 2, FP8>(p, units, z, stream);
-    else rc = launch_units<BF16, D, 4, 1, FP8>(p, units, z, stream);
+    else if (z.tile_rows == 128) rc = launch_units<BF16, D, 4, 1, FP8>(p, units, z, stream);
+    else if constexpr (D == 128 && !FP8) rc = launch_units<BF16, D, 8, 1, FP8>(p, units, z, stream);
+    else rc = FSTA_EUNSUPPORTED;
     if (rc != FSTA_OK) return rc;
     // nothing is cut where no sequence can have more tiles than the shortest run has
     const int64_t most_tiles = (((int64_t)p.batch.width << p.batch.page_shift) + kTileN - 1) / kTileN;
@@ -482,10 +550,10 @@ int check_heads(const char* who, int32_t batch, int32_t tokens, int32_t heads, i
 using namespace fsta;
 
 extern "C" size_t fsta_paged_attention_workspace_bytes(int32_t batch, int32_t tokens, int32_t max_q_len, int32_t heads, int32_t kv_heads,
-                                                       int32_t head_dim) {
+                                                       int32_t head_dim, int32_t cache_dtype) {
     if (batch <= 0 || tokens <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
-    const Sizes z = sizes_of(batch, tokens, max_q_len, heads, kv_heads);
-    return (size_t)z.parts * (size_t)z.tile_rows * (size_t)(head_dim + 1) * sizeof(float);
+    const Sizes z = sizes_of(batch, tokens, max_q_len, heads, kv_heads, head_dim, cache_dtype == FSTA_FP8);
+    return ((size_t)z.parts * (size_t)z.tile_rows * (size_t)(head_dim + 1) + 4) * sizeof(float);
 }
 
 extern "C" int fsta_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
@@ -514,8 +582,8 @@ extern "C" int fsta_paged_attention(const void* q, int64_t q_token_stride, int64
         return fail(FSTA_EINVAL, "%s: rows of q, o and the cache must be 16-byte aligned", who);
     if (misaligned(k_exponent, 4) || misaligned(v_exponent, 4) || misaligned(lse, 4) || misaligned(tree_bits, 4))
         return fail(FSTA_EINVAL, "%s: exponents, lse and tree_bits must be 4-byte aligned", who);
-    const Sizes z = sizes_of(batch, tokens, max_q_len, heads, kv_heads);
-    const size_t need = fsta_paged_attention_workspace_bytes(batch, tokens, max_q_len, heads, kv_heads, head_dim);
+    const Sizes z = sizes_of(batch, tokens, max_q_len, heads, kv_heads, head_dim, cache_dtype == FSTA_FP8);
+    const size_t need = fsta_paged_attention_workspace_bytes(batch, tokens, max_q_len, heads, kv_heads, head_dim, cache_dtype);
     if (!workspace || workspace_bytes < need) return fail(FSTA_EINVAL, "%s: needs %zu bytes of workspace, got %zu", who, need, workspace_bytes);
     if (misaligned(workspace, 16)) return fail(FSTA_EINVAL, "%s: the workspace must be 16-byte aligned", who);
     while ((1 << p.batch.page_shift) < page_size) ++p.batch.page_shift;
@@ -523,10 +591,14 @@ extern "C" int fsta_paged_attention(const void* q, int64_t q_token_stride, int64
     p.k = k_cache; p.v = v_cache; p.k_exponent = k_exponent; p.v_exponent = v_exponent;
     p.o = o; p.lse = lse;
     p.tree_bits = tree_bits; p.tree_words = mask == FSTA_PAGED_TREE ? tree_words : 0; p.mask = mask;
-    p.group = heads / kv_heads; p.tile_rows = z.tile_rows; p.row_shift = z.tile_rows == 32 ? 5 : z.tile_rows == 64 ? 6 : 7; p.parts = (int32_t)z.parts; p.run_units = z.run_units; p.least_tiles = z.least_tiles;
+    p.group = heads / kv_heads; p.tile_rows = z.tile_rows; p.row_shift = z.tile_rows == 32 ? 5 : z.tile_rows == 64 ? 6 : z.tile_rows == 128 ? 7 : 8; p.parts = (int32_t)z.parts; p.least_tiles = z.least_tiles;
+    for (int i = 0; i < 3; ++i) p.run_units[i] = z.run_units[i];
+    const Costs costs = costs_of(z.tile_rows);
+    p.slots = costs.slots; p.unit_cost = costs.unit; p.cut_cost = costs.cut;
     p.scale_log2e = sm_scale * kLog2e;
     p.part_o = static_cast<float*>(workspace);
     p.part_lse = p.part_o + (size_t)z.parts * z.tile_rows * head_dim;
+    p.run_length = reinterpret_cast<uint32_t*>(p.part_lse + (size_t)z.parts * z.tile_rows);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const bool fp8 = cache_dtype == FSTA_FP8;
     if (dtype == FSTA_BF16) {

@@ -175,7 +175,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, k
         max_q_len = max(tokens - batch + 1, 1)
     o = torch.empty((tokens, heads, d), dtype=q.dtype, device=q.device)
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
-    need = lib.fsta_paged_attention_workspace_bytes(batch, tokens, max_q_len, heads, heads_kv, d)
+    need = lib.fsta_paged_attention_workspace_bytes(batch, tokens, max_q_len, heads, heads_kv, d, code)
     work = torch.empty((need,), dtype=torch.uint8, device=q.device)
     with _on_device(q.device):
         _lib.check(lib.fsta_paged_attention(q.data_ptr(), *q_strides, cache.k.data_ptr(), cache.v.data_ptr(), k_exp, v_exp,

@@ -497,7 +497,8 @@ int fsta_paged_read(const void* k_cache, const void* v_cache, const uint8_t* k_e
  * `stream` has run.  tokens * heads < 2^30, batch <= 65536.
  */
 size_t fsta_paged_attention_workspace_bytes(int32_t batch, int32_t tokens, int32_t max_q_len,
-                                            int32_t heads, int32_t kv_heads, int32_t head_dim);
+                                            int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                            int32_t cache_dtype);
 int fsta_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                          const void* k_cache, const void* v_cache, const uint8_t* k_exponent,
                          const uint8_t* v_exponent, const int32_t* page_table, const int32_t* kv_lens,
