@@ -18,6 +18,7 @@
 
 #include <pybind11/pybind11.h>
 
+#include <algorithm>
 #include <cstring>
 
 #include "../../include/fsta.h"
@@ -412,6 +413,188 @@ PyObject* setup(PyObject*, PyObject* args) {
     Py_RETURN_NONE;
 }
 
+// ---- the paged KV cache: calls that paged.py has nothing to complain about; it judges and raises for all others --------
+
+int half_code(at::ScalarType t) { return t == at::kHalf ? FSTA_F16 : t == at::kBFloat16 ? FSTA_BF16 : -1; }
+
+struct Pool {      // paged.PagedKV
+    const at::Tensor *k, *v;
+    uint8_t *k_exp, *v_exp;
+    int32_t pages, heads, page_size, head_dim, code;
+};
+
+bool read_pool(PyObject* o, Pool* p) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
+    p->k = gpu_tensor(PyTuple_GET_ITEM(o, 0));
+    p->v = gpu_tensor(PyTuple_GET_ITEM(o, 1));
+    if (!p->k || !p->v || p->k->dim() != 4 || p->v->sizes() != p->k->sizes() || p->v->scalar_type() != p->k->scalar_type() ||
+        p->v->device() != p->k->device() || !p->k->is_contiguous() || !p->v->is_contiguous())
+        return false;
+    const bool fp8 = p->k->scalar_type() == at::kFloat8_e4m3fn;
+    p->code = fp8 ? FSTA_FP8 : half_code(p->k->scalar_type());
+    uint8_t* exps[2] = {nullptr, nullptr};
+    for (int i = 0; i < 2; ++i) {
+        PyObject* item = PyTuple_GET_ITEM(o, 2 + i);
+        if (fp8 != (item != Py_None)) return false;
+        if (!fp8) continue;
+        const at::Tensor* e = gpu_tensor(item);
+        if (!e || e->scalar_type() != at::kByte || e->sizes() != p->k->sizes().slice(0, 3) || !e->is_contiguous() || e->device() != p->k->device())
+            return false;
+        exps[i] = static_cast<uint8_t*>(e->data_ptr());
+    }
+    p->k_exp = exps[0];
+    p->v_exp = exps[1];
+    for (int64_t i = 0; i < 4; ++i)
+        if (p->k->size(i) > INT32_MAX) return false;
+    p->pages = (int32_t)p->k->size(0);
+    p->heads = (int32_t)p->k->size(1);
+    p->page_size = (int32_t)p->k->size(2);
+    p->head_dim = (int32_t)p->k->size(3);
+    return p->code >= 0;
+}
+
+const int32_t* int32_array(PyObject* o, const at::Tensor& like, int64_t dims, int64_t size) {
+    const at::Tensor* t = gpu_tensor(o);
+    return t && t->scalar_type() == at::kInt && t->dim() == dims && t->size(0) == size && t->is_contiguous() && t->device() == like.device()
+               ? static_cast<const int32_t*>(t->data_ptr())
+               : nullptr;
+}
+
+struct Batch {
+    const int32_t *table, *lens, *starts;
+    int32_t batch, width;
+};
+// starts == null: not wanted
+bool read_batch(const Pool& pool, PyObject* table, PyObject* lens, PyObject* starts, Batch* b) {
+    const at::Tensor* t = gpu_tensor(table);
+    if (!t || t->dim() != 2 || t->size(0) == 0 || t->size(1) == 0 || t->size(0) > INT32_MAX || t->size(1) > INT32_MAX) return false;
+    b->batch = (int32_t)t->size(0);
+    b->width = (int32_t)t->size(1);
+    b->table = int32_array(table, *pool.k, 2, b->batch);
+    b->lens = int32_array(lens, *pool.k, 1, b->batch);
+    b->starts = starts ? int32_array(starts, *pool.k, 1, (int64_t)b->batch + 1) : nullptr;
+    return b->table && b->lens && (b->starts || !starts);
+}
+
+// Packed rows [tokens, heads, head_dim], at least one
+const at::Tensor* read_rows(PyObject* o, const Pool& pool) {
+    const at::Tensor* t = gpu_tensor(o);
+    if (!t || t->dim() != 3 || t->numel() == 0 || t->size(0) > INT32_MAX || t->size(2) != pool.head_dim || t->stride(2) != 1 ||
+        t->device() != pool.k->device() || (c10::GradMode::is_enabled() && wants_grad(*t)))
+        return nullptr;
+    const int code = half_code(t->scalar_type());
+    return code >= 0 && (pool.code == FSTA_FP8 || pool.code == code) ? t : nullptr;
+}
+int64_t stride_of(const at::Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
+// paged_write(cache, k, v, page_table, kv_lens, q_starts) -> None
+PyObject* paged_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Pool pool;
+    Batch b;
+    if (n != 6 || !plain_context() || !read_pool(args[0], &pool) || !read_batch(pool, args[3], args[4], args[5], &b)) return not_implemented();
+    const at::Tensor *k = read_rows(args[1], pool), *v = read_rows(args[2], pool);
+    if (!k || !v || k->sizes() != v->sizes() || k->size(1) != pool.heads || k->scalar_type() != v->scalar_type()) return not_implemented();
+    try {
+        const OnStream on(*pool.k);
+        if (fsta_paged_write(k->data_ptr(), v->data_ptr(), stride_of(*k, 0), stride_of(*k, 1), stride_of(*v, 0), stride_of(*v, 1),
+                             pool.k->data_ptr(), pool.v->data_ptr(), pool.k_exp, pool.v_exp, b.table, b.lens, b.starts, b.batch, b.width,
+                             (int32_t)k->size(0), pool.pages, pool.page_size, pool.heads, pool.head_dim, half_code(k->scalar_type()),
+                             pool.code, on.stream) != FSTA_OK)
+            return not_implemented();
+    } catch (const std::exception&) {
+        return not_implemented();
+    }
+    Py_RETURN_NONE;
+}
+
+// paged_read(cache, page_table, kv_lens, max_len, dtype or None) -> (k, v)
+PyObject* paged_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Pool pool;
+    Batch b;
+    int64_t max_len;
+    if (n != 5 || !plain_context() || !read_pool(args[0], &pool) || !read_batch(pool, args[1], args[2], nullptr, &b) || !as_int(args[3], &max_len) ||
+        max_len < 0 || max_len > INT32_MAX)
+        return not_implemented();
+    at::ScalarType type = pool.code == FSTA_FP8 ? at::kBFloat16 : pool.k->scalar_type();
+    if (args[4] != Py_None) {
+        if (!THPDtype_Check(args[4])) return not_implemented();
+        const at::ScalarType asked = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
+        if (half_code(asked) < 0 || (pool.code != FSTA_FP8 && asked != type)) return not_implemented();
+        type = asked;
+    }
+    try {
+        const OnStream on(*pool.k);
+        const at::Tensor k = fresh({b.batch, pool.heads, max_len, pool.head_dim}, type, *pool.k), v = fresh(k.sizes(), type, *pool.k);
+        if (fsta_paged_read(pool.k->data_ptr(), pool.v->data_ptr(), pool.k_exp, pool.v_exp, b.table, b.lens, k.data_ptr(), v.data_ptr(), b.batch,
+                            b.width, (int32_t)max_len, pool.pages, pool.page_size, pool.heads, pool.head_dim, half_code(type), pool.code,
+                            on.stream) != FSTA_OK)
+            return not_implemented();
+        return as_tuple(k, v);
+    } catch (const std::exception&) {
+        return not_implemented();
+    }
+}
+
+// paged_attention(q, cache, page_table, kv_lens, q_starts, sm_scale, causal, tree_bits or None, max_q_len or None, return_lse)
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Pool pool;
+    Batch b;
+    if (n != 10 || !plain_context() || !read_pool(args[1], &pool) || !read_batch(pool, args[2], args[3], args[4], &b) || !PyFloat_Check(args[5]))
+        return not_implemented();
+    const at::Tensor* q = read_rows(args[0], pool);
+    const double sm_scale = PyFloat_AS_DOUBLE(args[5]);
+    if (!q || q->size(1) % std::max(pool.heads, 1) || pool.heads == 0 || pool.pages == 0 || !(sm_scale > 0)) return not_implemented();
+    const int32_t tokens = (int32_t)q->size(0), heads = (int32_t)std::min<int64_t>(q->size(1), INT32_MAX);
+    if (!PyBool_Check(args[6]) || !PyBool_Check(args[9])) return not_implemented();
+    const uint32_t* bits = nullptr;
+    int32_t words = 0, mask = args[6] == Py_True ? FSTA_PAGED_CAUSAL : FSTA_PAGED_ALL;
+    if (args[7] != Py_None) {
+        bits = reinterpret_cast<const uint32_t*>(int32_array(args[7], *q, 2, tokens));
+        if (!bits) return not_implemented();
+        words = (int32_t)THPVariable_Unpack(args[7]).size(1);
+        mask = FSTA_PAGED_TREE;
+    }
+    int64_t most = std::max(tokens - b.batch + 1, 1);
+    if (args[8] != Py_None && (!as_int(args[8], &most) || most < 0 || most > INT32_MAX)) return not_implemented();
+    try {
+        const OnStream on(*q);
+        const at::Tensor o = fresh(q->sizes(), q->scalar_type(), *q);
+        const at::Tensor lse = args[9] == Py_True ? fresh({tokens, heads}, at::kFloat, *q) : at::Tensor();
+        const size_t need = fsta_paged_attention_workspace_bytes(b.batch, tokens, (int32_t)most, heads, pool.heads, pool.head_dim, pool.code);
+        const at::Tensor work = fresh({(int64_t)need}, at::kByte, *q);
+        if (fsta_paged_attention(q->data_ptr(), stride_of(*q, 0), stride_of(*q, 1), pool.k->data_ptr(), pool.v->data_ptr(), pool.k_exp, pool.v_exp,
+                                 b.table, b.lens, b.starts, bits, words, o.data_ptr(), data_or_null<float>(lse), b.batch, b.width, tokens,
+                                 (int32_t)most, pool.pages, pool.page_size, heads, pool.heads, pool.head_dim, half_code(q->scalar_type()), pool.code,
+                                 mask, (float)sm_scale, work.data_ptr(), need, on.stream) != FSTA_OK)
+            return not_implemented();
+        return lse.defined() ? as_tuple(o, lse) : THPVariable_Wrap(o);
+    } catch (const std::exception&) {
+        return not_implemented();
+    }
+}
+
+// tree_bits(parent, q_starts, max_nodes): paged.tree_mask_bits of a batch
+PyObject* tree_bits(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    int64_t most;
+    if (n != 3 || !plain_context() || !as_int(args[2], &most) || most <= 0 || most > INT32_MAX - 32) return not_implemented();
+    const at::Tensor *parent = gpu_tensor(args[0]), *starts = gpu_tensor(args[1]);
+    if (!parent || !starts || parent->dim() != 1 || parent->scalar_type() != at::kLong || parent->size(0) == 0 || parent->size(0) > INT32_MAX ||
+        !parent->is_contiguous() || starts->dim() != 1 || starts->size(0) < 2 || starts->size(0) > INT32_MAX)
+        return not_implemented();
+    const int32_t* first = int32_array(args[1], *parent, 1, starts->size(0));
+    if (!first) return not_implemented();
+    try {
+        const OnStream on(*parent);
+        const at::Tensor bits = fresh({parent->size(0), (most + 31) / 32}, at::kInt, *parent);
+        if (fsta_tree_bits(parent->data_ptr<int64_t>(), first, (int32_t)(starts->size(0) - 1), (int32_t)parent->size(0), (int32_t)bits.size(1),
+                           static_cast<uint32_t*>(bits.data_ptr()), on.stream) != FSTA_OK)
+            return not_implemented();
+        return THPVariable_Wrap(bits);
+    } catch (const std::exception&) {
+        return not_implemented();
+    }
+}
+
 #define FSTA_FASTCALL(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&f)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
     FSTA_FASTCALL(attention),
@@ -421,6 +604,10 @@ PyMethodDef kMethods[] = {
     FSTA_FASTCALL(medusa_parents),
     FSTA_FASTCALL(shift_index),
     FSTA_FASTCALL(quantizes),
+    FSTA_FASTCALL(paged_write),
+    FSTA_FASTCALL(paged_read),
+    FSTA_FASTCALL(paged_attention),
+    FSTA_FASTCALL(tree_bits),
     {"setup", &setup, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

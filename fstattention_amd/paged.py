@@ -18,6 +18,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
+from . import attention as _attention
 from .attention import _on_device, _stream_ptr
 
 _HALF = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
@@ -31,6 +32,12 @@ class PagedKV(NamedTuple):
     v: torch.Tensor
     k_exponent: Optional[torch.Tensor] = None
     v_exponent: Optional[torch.Tensor] = None
+
+
+def _calls():
+    """The module of plain C functions: what it takes of a call it has launched, for anything else it answers NotImplemented and
+    the checks below say why (or launch what it did not want to judge)."""
+    return _attention._CALLS or _attention._calls()
 
 
 def paged_kv_cache(num_pages: int, kv_heads: int, page_size: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
@@ -102,6 +109,8 @@ def write_paged_kv(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, page_table:
 
     An 8-bit cache gets, per row, the smallest exponent ``e`` with ``max |x| <= 448 * 2**e`` over the row's finite values
     (kept within [-110, 120]; 0 for a row of zeros) and bytes rounded to nearest even; infinities and NaNs become NaN."""
+    if _calls().paged_write(cache, k, v, page_table, kv_lens, q_starts) is None:
+        return
     pages, heads, page_size, d, code, k_exp, v_exp = _check_cache(cache)
     batch, width = _check_arrays(cache, page_table, kv_lens, q_starts)
     k_strides, v_strides = _check_rows(k, "k", cache), _check_rows(v, "v", cache)
@@ -118,6 +127,9 @@ def read_paged_kv(cache: PagedKV, page_table: torch.Tensor, kv_lens: torch.Tenso
                   dtype: Optional[torch.dtype] = None):
     """The pages of a batch as dense ``k, v [B, Hkv, max_len, D]`` (the layout ``fst_attention`` takes), zeros where a sequence
     has no position.  ``dtype``: the cache's, or float16 / bfloat16 for an 8-bit one (bfloat16 if not given)."""
+    out = _calls().paged_read(cache, page_table, kv_lens, max_len, dtype)
+    if out is not NotImplemented:
+        return out
     pages, heads, page_size, d, code, k_exp, v_exp = _check_cache(cache)
     batch, width = _check_arrays(cache, page_table, kv_lens)
     fp8 = cache.k.dtype == torch.float8_e4m3fn
@@ -152,6 +164,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, k
     Tokens that see nothing get zeros (and ``-inf``); rows of tokens that ``q_starts`` gives to no sequence are not written.
     Sums and softmax statistics are float32; up to 64 rows (tokens times query heads per K/V head) a sequence, bfloat16 weights
     go to the matrix cores as pairs (2^-16 relative at most), beyond that rounded once (2^-8 at most, as the output itself)."""
+    out = _calls().paged_attention(q, cache, page_table, kv_lens, q_starts, sm_scale, causal, tree_bits, max_q_len, return_lse)
+    if out is not NotImplemented:
+        return out
     pages, heads_kv, page_size, d, code, k_exp, v_exp = _check_cache(cache)
     batch, width = _check_arrays(cache, page_table, kv_lens, q_starts)
     q_strides = _check_rows(q, "q", cache)
@@ -193,6 +208,9 @@ def tree_mask_bits(parent: torch.Tensor, q_starts: Optional[torch.Tensor] = None
     ``parent`` int64 ``[T]``: every node's parent by its number within its tree, smaller than its own, -1 for a root (as in
     ``lineage_from_parents``; anything else counts as a root).  ``q_starts`` int32 ``[B + 1]``: tree ``b``'s nodes (one tree if
     not given).  ``max_nodes``: the most nodes a tree has (``T`` if not given); bits beyond it are dropped."""
+    bits = _calls().tree_bits(parent, q_starts, max_nodes)
+    if bits is not NotImplemented:
+        return bits
     if parent.dim() != 1 or parent.dtype != torch.int64:
         raise ValueError("parent must be int64 [tokens]")
     if not parent.is_cuda:
