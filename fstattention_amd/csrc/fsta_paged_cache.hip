@@ -16,6 +16,8 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
+constexpr int kTreeRows = 64;             // rows of a tree's masks per workgroup
+constexpr int kTreeNodes = 8192;          // nodes of a tree in LDS at most (64 KB)
 constexpr int kUnits = 4;                 // 16-byte pieces of 16-bit rows per thread
 
 struct RowArgs {
@@ -196,42 +198,82 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(RowArgs a) {
     }
 }
 
-// Draft trees to masks: bit j of a token's row is set where j is the token itself or one of its ancestors (numbers within its
-// tree).  A parent is a smaller number (anything else counts as a root), so the walk to the root meets the words of the row from
-// the token's own downwards: a word is complete when the walk leaves it, and nothing is collected anywhere but in one register.
+// Draft trees to masks: bit j of a node's row is set where j is the node itself or one of its ancestors (numbers within its
+// tree).  A parent is a smaller number (anything else counts as a root), so a walk to the root meets the words of a row from the
+// node's own downwards, and what one node of a word contributes to it is the same for every walk that enters the word there: the
+// bits of its ancestors among the word's 32 nodes, and the number at which the walk leaves them.  Both come from five rounds of
+// doubling between the lanes of half a wave, for all nodes up to the workgroup's own; they stay in LDS, and a row is then a walk
+// over words, one LDS read each, instead of one dependent read of global memory per ancestor.  Rows are cleared first, 16 bytes
+// a lane, since most words of a deep tree's rows are empty.  Nodes that LDS has no room for (their numbers are the largest ones)
+// are walked in global memory until the walk reaches those that it holds.
+struct TreeNode { uint32_t bits; int32_t exit; };
+
 __global__ __launch_bounds__(kThreads) void tree_bits_kernel(const int64_t* parent, const int32_t* q_starts, int32_t batch,
-                                                             int32_t tokens, int32_t words, uint32_t* bits) {
-    for (int t = blockIdx.x * kThreads + threadIdx.x; t < tokens; t += gridDim.x * kThreads) {
-        int lo = 0, hi = batch;                    // the sequence whose run holds t
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (q_starts[mid] <= t) lo = mid; else hi = mid;
-        }
-        const int start = min(max(q_starts[lo], 0), tokens), end = min(q_starts[lo + 1], tokens);
-        uint32_t* row = bits + (size_t)t * words;
-        if (t < start || t >= end) {               // a token of no tree
-            for (int w = 0; w < words; ++w) row[w] = 0u;
-            continue;
-        }
-        int node = t - start;
-        int at = words - 1;
-        for (; at > node / 32; --at) row[at] = 0u;
-        uint32_t word = 0u;
-        while (true) {
-            if (node / 32 < words) {
-                if (node / 32 != at) {
-                    row[at] = word;
-                    word = 0u;
-                    for (--at; at > node / 32; --at) row[at] = 0u;
+                                                             int32_t tokens, int32_t words, int32_t room, uint32_t* bits) {
+    extern __shared__ TreeNode nodes[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    {   // tokens of no tree
+        const int first = min(max(q_starts[0], 0), tokens), end = min(max(q_starts[batch], 0), tokens);
+        const int64_t none = (int64_t)(first + max(tokens - max(first, end), 0)) * words;
+        for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < none; i += (int64_t)gridDim.x * kThreads)
+            bits[i < (int64_t)first * words ? i : i + (int64_t)(max(first, end) - first) * words] = 0u;
+    }
+    const int chunks = (words * 32 + kTreeRows - 1) / kTreeRows;
+    for (int64_t item = blockIdx.x; item < (int64_t)chunks * batch; item += gridDim.x) {
+        const int b = (int)(item / chunks), start = min(max(q_starts[b], 0), tokens);
+        const int count = min(max(q_starts[b + 1], 0), tokens) - start;
+        // The last chunk of a tree takes what a tree of more nodes than the rows have bits has over
+        const int chunk = (int)(item % chunks);
+        for (int64_t node0 = (int64_t)chunk * kTreeRows; node0 < count && (node0 / kTreeRows == chunk || chunk == chunks - 1); node0 += kTreeRows) {
+            const int own = (int)min((int64_t)count - node0, (int64_t)kTreeRows);
+            const int known = ((int)min(node0 + own, (int64_t)room) + 31) & ~31;
+            const int64_t* up = parent + start;
+            uint32_t* rows = bits + (start + node0) * words;
+            const auto parent_of = [&](int n) {
+                const int64_t p = up[n];
+                return p >= 0 && p < n ? (int)p : -1;
+            };
+            for (int n = tid; n < known; n += kThreads) {   // whole half waves: known is a multiple of 32
+                const int p = n < count ? parent_of(n) : -1;
+                const int base = n & ~31, inside = p >= base;
+                uint32_t mask = 1u << (n & 31);
+                int link = inside ? (lane & 32) + (p & 31) : lane;
+#pragma unroll
+                for (int round = 0; round < 5; ++round) {
+                    mask |= (uint32_t)__shfl((int)mask, link);
+                    link = __shfl(link, link);
                 }
-                word |= 1u << (node % 32);
+                nodes[n] = {mask, __shfl(p, link)};
             }
-            const int64_t up = parent[start + node];
-            if (up < 0 || up >= node) break;
-            node = (int)up;
+            const int total = own * words;
+            if ((reinterpret_cast<uintptr_t>(rows) & 15) == 0) {
+                for (int i = tid; i < total / 4; i += kThreads) reinterpret_cast<u32x4*>(rows)[i] = u32x4{0u, 0u, 0u, 0u};
+                for (int i = (total & ~3) + tid; i < total; i += kThreads) rows[i] = 0u;
+            } else {
+                for (int i = tid; i < total; i += kThreads) rows[i] = 0u;
+            }
+            __syncthreads();
+            if (tid < own) {
+                uint32_t* row = rows + (int64_t)tid * words;
+                int node = (int)node0 + tid;
+                uint32_t word = 0u;
+                while (node >= known) {
+                    word |= 1u << (node & 31);
+                    const int next = parent_of(node);
+                    if (next < (node & ~31)) {
+                        if (node / 32 < words) row[node / 32] = word;
+                        word = 0u;
+                    }
+                    node = next;
+                }
+                while (node >= 0) {
+                    const TreeNode at = nodes[node];
+                    if (node / 32 < words) row[node / 32] = at.bits;
+                    node = at.exit;
+                }
+            }
+            __syncthreads();
         }
-        row[at] = word;
-        for (--at; at >= 0; --at) row[at] = 0u;
     }
 }
 
@@ -365,9 +407,11 @@ extern "C" int fsta_tree_bits(const int64_t* parent, const int32_t* q_starts, in
     if (!parent || !q_starts || !bits) return fail(FSTA_EINVAL, "%s: null pointer", who);
     if (misaligned(parent, 8) || misaligned(q_starts, 4) || misaligned(bits, 4))
         return fail(FSTA_EINVAL, "%s: parent must be 8-byte, q_starts and bits 4-byte aligned", who);
-    const int64_t want = ((int64_t)tokens + kThreads - 1) / kThreads;
-    hipLaunchKernelGGL(tree_bits_kernel, dim3((unsigned)(want < 65536 ? want : 65536)), dim3(kThreads), 0, static_cast<hipStream_t>(stream),
-                       parent, q_starts, batch, tokens, words, bits);
+    const int64_t bits_of_row = (int64_t)words * 32, chunks = (bits_of_row + kTreeRows - 1) / kTreeRows, want = chunks * batch;
+    if (bits_of_row > INT32_MAX - kTreeRows) return fail(FSTA_EUNSUPPORTED, "%s: words=%d", who, words);
+    const int32_t room = (int32_t)(bits_of_row < kTreeNodes ? bits_of_row : kTreeNodes);
+    hipLaunchKernelGGL(tree_bits_kernel, dim3((unsigned)(want < 65536 ? want : 65536)), dim3(kThreads), room * sizeof(TreeNode),
+                       static_cast<hipStream_t>(stream), parent, q_starts, batch, tokens, words, room, bits);
     FSTA_HIP_OK(hipGetLastError());
     return FSTA_OK;
 }
