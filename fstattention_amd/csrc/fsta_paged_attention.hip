@@ -361,8 +361,8 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
 }
 
 // Joins the runs of a tile's keys, in an order that the run count alone decides: D / 4 lanes take a row and every SUBS-th run of
-// it, four runs' loads in flight at a time; what they have is joined through LDS.  A workgroup takes ROWS rows at a time of a
-// (tile whose keys are cut, K/V head).
+// it, four runs' loads in flight at a time; what they have is joined through LDS (tiles of 128 rows and more are in few runs: one
+// share).  A workgroup takes ROWS rows at a time of a (tile whose keys are cut, K/V head).
 template <bool BF16, int D, int ROWS>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
     constexpr int kLanes = D / 4, kSubs = 256 / kLanes / ROWS;
@@ -512,8 +512,10 @@ template <bool BF16, int D, int R, int S, bool FP8> int launch_units(const Paged
 template <bool BF16, int D, int ROWS> int launch_join(const PagedAttnParams& p, const Sizes& z, hipStream_t stream) {
     const int64_t items = z.cut_tiles;
     const int64_t rows = z.most_rows < z.tile_rows ? z.most_rows : z.tile_rows;
-    // (most of them find that there is nothing to do)
-    const int64_t wanted = (rows + ROWS - 1) / ROWS, room = 4 * kCus / (items * p.batch.kv_heads) + 1;
+    // Most of them find that there is nothing to do, and one that has rows waits for two round trips: as many as are on the card
+    // at a time.  (Half as many: 17 sequences of 28 heads, chunks and single tokens, 55.1 -> 53.5 us with the attention; 16
+    // sequences of 4 tokens 55.1 -> 52.5; twice as many 53.0 and 53.2.)
+    const int64_t wanted = (rows + ROWS - 1) / ROWS, room = 8 * kCus / (items * p.batch.kv_heads) + 1;
     const dim3 grid((unsigned)(items * p.batch.kv_heads), (unsigned)(wanted < room ? wanted : room));
     hipLaunchKernelGGL((paged_join_kernel<BF16, D, ROWS>), grid, dim3(256), 0, stream, p);
     FSTA_HIP_OK(hipGetLastError());
@@ -534,7 +536,7 @@ template <bool BF16, int D, bool FP8> int launch_attention(const PagedAttnParams
     if (most_tiles <= z.least_tiles) return FSTA_OK;
     if (z.tile_rows == 32) return launch_join<BF16, D, 1>(p, z, stream);
     if (z.tile_rows == 64) return launch_join<BF16, D, 2>(p, z, stream);
-    return launch_join<BF16, D, 8>(p, z, stream);
+    return launch_join<BF16, D, 1024 / D>(p, z, stream);
 }
 
 int check_heads(const char* who, int32_t batch, int32_t tokens, int32_t heads, int32_t kv_heads) {
