@@ -260,9 +260,14 @@ template <bool BF16, int D, bool DIRECT, bool SPLIT> struct RowGroup {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float a = pw[8 * k2 + 2 * e], b = pw[8 * k2 + 2 * e + 1];
-                const uint32_t hi = PV::pack(a, b);
-                hi4[e] = hi;
-                if (SPLIT) lo4[e] = PV::pack(a - PV::low(hi), b - PV::high(hi));
+                // A pair's high part is cut off, not rounded, and 2^-23 of the weight is added to the low one: it is greater than
+                // zero where the weight is, and both parts' products with an infinity have the same sign.
+                if (SPLIT) {
+                    hi4[e] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
+                    lo4[e] = PV::pack(__builtin_fmaf(a, 1.f + 0x1p-23f, -PV::low(hi4[e])), __builtin_fmaf(b, 1.f + 0x1p-23f, -PV::high(hi4[e])));
+                } else {
+                    hi4[e] = PV::pack(a, b);
+                }
             }
             ph[k2] = __builtin_bit_cast(PFrag, hi4);
             if (SPLIT) pl[k2] = __builtin_bit_cast(PFrag, lo4);
