@@ -445,22 +445,35 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
 
-// Rows of a workgroup's tile.  Up to 32 rows a sequence the keys are all there is to read, and the waves share them out; 64 rows: in
-// pairs; from 128 rows on every wave has rows of its own.  256 rows where that means that every key is read once (trees of 256 nodes,
-// 32 heads: 41 -> 37 us), or where there are two rounds of such tiles (4096 after 16384: 1221 -> 1189 us; with one round the last
-// tiles of a causal chunk are waited for: 2048 tokens 63 -> 71 us).  8-bit tiles are widened by all waves together, behind a barrier
-// more, which two workgroups per CU hide and one does not (348 -> 384 us); head_dim 64 fits three workgroups of 128 rows on a CU.
-int rows_of_tile(int64_t most_rows, int64_t all_rows, int32_t kv_heads, int32_t head_dim, bool fp8) {
+// Rows of a workgroup's tile where there is much to do.  Up to 32 rows a sequence the keys are all there is to read, and the waves
+// share them out; 64 rows: in pairs; from 128 rows on every wave has rows of its own.  256 rows where there are two rounds of such
+// tiles (4096 after 16384: 1221 -> 1189 us; with one round the last tiles of a causal chunk are waited for: 2048 tokens 63 -> 71 us).
+// 8-bit tiles are widened by all waves together, behind a barrier more, which two workgroups per CU hide and one does not (348 ->
+// 384 us); head_dim 64 fits three workgroups of 128 rows on a CU.
+int rows_for_rate(int64_t most_rows, int64_t all_rows, int32_t kv_heads, int32_t head_dim, bool fp8) {
     if (most_rows <= 32) return 32;
     if (most_rows <= 64) return 64;
-    if (most_rows <= 128 || head_dim == 64 || fp8) return 128;
-    return most_rows <= 256 || all_rows / 256 * kv_heads >= 2 * kCus ? 256 : 128;
+    return head_dim == 128 && !fp8 && all_rows / 256 * kv_heads >= 2 * kCus ? 256 : 128;
 }
 
-// What find_item weighs, in the time a workgroup takes for a tile of keys (0.66 us alone on its CU with up to 64 rows; with 128 rows
-// 0.9 us alone, and two share a CU at 1.05 us): a unit's start and end 4 to 5 us, the join's launch 5.5 us and more with more rows
+// Where there is little, a call lasts as long as one workgroup, and smaller tiles, whose waves share out the keys, are done sooner
+// as long as they are not much more than a card's worth.  (32 query on 8 K/V heads of 128, rows 128 / 64 / 32: 64 tokens on 256 keys
+// 12.5 / 10.5 / 9.3 us, of 8 bits 16.0 / 11.4 / 9.6; 256 tokens on 256 keys 12.6 / 10.8 / 13.2, on 1024 keys 19.8 / 23.1 / 22.3; 5 x 38
+// tokens of 4 K/V heads on 362 keys 17.5 / 15.8 / 13.9; 16 x 64 tokens on 250 keys 15.0 / 17.5 / 41; 32 tokens on 16384 keys 42 / 32 /
+// 34; 64 tokens on 16384 keys 42 / 48 / 50.)  What the host knows of the keys is that the page table's rows hold no more.
+int rows_of_tile(int rate, int64_t all_rows, int64_t most_keys, int32_t kv_heads) {
+    const int64_t units32 = (all_rows + 31) / 32 * kv_heads, units64 = (all_rows + 63) / 64 * kv_heads;
+    if (rate > 32 && most_keys <= kDecodeLeast * kTileN && units32 <= kCus * 3 / 4) return 32;
+    if (rate > 64 && (units64 <= kCus / 16 || (units64 <= kCus / 2 && units64 * most_keys < kCus * kDecodeLeast * kTileN))) return 64;
+    return rate;
+}
+
+// What choose weighs, in the time a workgroup takes for a tile of keys (0.66 us alone on its CU with up to 64 rows; with 128 rows
+// 0.9 us alone, and two share a CU at 1.05 us): a unit's start and end 4 to 5 us, the join's launch 5 us, and with many rows the
+// results of the runs, which go to memory and back (4 sequences of 256 tokens, 32 K/V heads, 1256 to 1500 keys: cut 65 us, whole 49;
+// from 16 to 20 nothing else that was timed changes, at 30 one sequence of 256 tokens on 1024 keys of 8 K/V heads 20 -> 31 us).
 struct Costs { float slots, unit, cut; };
-Costs costs_of(int tile_rows) { return tile_rows >= 128 ? Costs{(tile_rows == 256 ? 1.f : 2.f) * kCus, 6.f, 12.f} : Costs{kCus, 7.f, 8.f}; }
+Costs costs_of(int tile_rows) { return tile_rows >= 128 ? Costs{(tile_rows == 256 ? 1.f : 2.f) * kCus, 6.f, 18.f} : Costs{kCus, 7.f, 8.f}; }
 
 struct Sizes {
     int tile_rows;
@@ -468,13 +481,17 @@ struct Sizes {
     int64_t row_tiles;          // at most, over the batch
     int64_t items, parts;       // of all heads: parts
     int64_t cut_tiles;          // a head's
+    int64_t floats;             // of workspace
     int run_units[3], least_tiles;
 };
-Sizes sizes_of(int32_t batch, int32_t tokens, int32_t max_q_len, int32_t heads, int32_t kv_heads, int32_t head_dim, bool fp8) {
+// most_keys: a sequence's, by the page table's width; shrink: by them
+Sizes sizes_of(int32_t batch, int32_t tokens, int32_t max_q_len, int64_t most_keys, bool shrink, int32_t heads, int32_t kv_heads, int32_t head_dim,
+               bool fp8) {
     Sizes z;
     const int group = heads / kv_heads;
     z.most_rows = (int64_t)(max_q_len > 0 && max_q_len < tokens ? max_q_len : tokens) * group;
-    z.tile_rows = rows_of_tile(z.most_rows, (int64_t)tokens * group, kv_heads, head_dim, fp8);
+    z.tile_rows = rows_for_rate(z.most_rows, (int64_t)tokens * group, kv_heads, head_dim, fp8);
+    if (shrink) z.tile_rows = rows_of_tile(z.tile_rows, (int64_t)tokens * group, most_keys, kv_heads);
     z.row_tiles = ((int64_t)tokens * group + (int64_t)(batch < tokens ? batch : tokens) * (z.tile_rows - 1)) / z.tile_rows;
     for (int i = 0; i < 3; ++i) z.run_units[i] = z.tile_rows == 256 ? kCus / 2 << i : (i + 1) * kCus;
     z.least_tiles = z.tile_rows == 32 ? kDecodeLeast : kChunkLeast;
@@ -484,6 +501,7 @@ Sizes sizes_of(int32_t batch, int32_t tokens, int32_t max_q_len, int32_t heads, 
     z.items = z.row_tiles + runs;
     z.cut_tiles = z.row_tiles < runs ? z.row_tiles : runs;
     z.parts = (runs + z.cut_tiles) * kv_heads;
+    z.floats = z.parts * z.tile_rows * (head_dim + 1) + 4;
     return z;
 }
 
@@ -554,8 +572,9 @@ using namespace fsta;
 extern "C" size_t fsta_paged_attention_workspace_bytes(int32_t batch, int32_t tokens, int32_t max_q_len, int32_t heads, int32_t kv_heads,
                                                        int32_t head_dim, int32_t cache_dtype) {
     if (batch <= 0 || tokens <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
-    const Sizes z = sizes_of(batch, tokens, max_q_len, heads, kv_heads, head_dim, cache_dtype == FSTA_FP8);
-    return ((size_t)z.parts * (size_t)z.tile_rows * (size_t)(head_dim + 1) + 4) * sizeof(float);
+    // (the width of the page table may choose smaller tiles than these: a quarter of the rows, or half, and never more parts than
+    // four times as many, or twice)
+    return (size_t)sizes_of(batch, tokens, max_q_len, 0, false, heads, kv_heads, head_dim, cache_dtype == FSTA_FP8).floats * sizeof(float);
 }
 
 extern "C" int fsta_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
@@ -584,7 +603,7 @@ extern "C" int fsta_paged_attention(const void* q, int64_t q_token_stride, int64
         return fail(FSTA_EINVAL, "%s: rows of q, o and the cache must be 16-byte aligned", who);
     if (misaligned(k_exponent, 4) || misaligned(v_exponent, 4) || misaligned(lse, 4) || misaligned(tree_bits, 4))
         return fail(FSTA_EINVAL, "%s: exponents, lse and tree_bits must be 4-byte aligned", who);
-    const Sizes z = sizes_of(batch, tokens, max_q_len, heads, kv_heads, head_dim, cache_dtype == FSTA_FP8);
+    const Sizes z = sizes_of(batch, tokens, max_q_len, (int64_t)width * page_size, true, heads, kv_heads, head_dim, cache_dtype == FSTA_FP8);
     const size_t need = fsta_paged_attention_workspace_bytes(batch, tokens, max_q_len, heads, kv_heads, head_dim, cache_dtype);
     if (!workspace || workspace_bytes < need) return fail(FSTA_EINVAL, "%s: needs %zu bytes of workspace, got %zu", who, need, workspace_bytes);
     if (misaligned(workspace, 16)) return fail(FSTA_EINVAL, "%s: the workspace must be 16-byte aligned", who);
