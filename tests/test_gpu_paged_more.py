@@ -98,3 +98,48 @@ def test_few_rows_on_few_keys(dtype, d, new, keys, heads, kv_heads, page, width)
         want = (score.softmax(-1) @ v).permute(1, 0, 2)
         top = v.abs().amax()
         torch.testing.assert_close(got[starts[b] : starts[b + 1]], want, rtol=_UNIT[dtype], atol=float(1.1 * _UNIT[dtype] * top))
+
+
+# The model of the example has logits of standard deviation 1, the largest of 512 about 3.  Some ten roundings to bfloat16 (2^-8
+# each) on a token's way move a logit by 0.03 or so; 8-bit keys and values (2^-4 of a value, averaged over the keys seen, times the
+# 0.3 that a layer's result counts, four layers) by 0.04.  Eight times that is asked for, far below what a wrong key would do.
+@pytest.mark.parametrize("fp8,off", [(False, 0.25), (True, 0.5)])
+def test_speculative_decoding_over_pages(fp8, off):
+    """The example's answers against its model in float32 on the CPU, whole sequences at a time and without a cache: every token is
+    the likeliest one but for roundings, and trees say more than a token a step."""
+    from fstattention_amd.examples import speculative_decoding as example
+    model = example.make_model()
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(512, (n,), generator=g).tolist() for n in (7, 130, 64, 33)]
+    steps = 24
+    answers, talk = example.answer(model, prompts, steps, draft=32, fp8=fp8)
+    assert talk.lens.tolist() == [len(p) + len(a) - 1 for p, a in zip(prompts, answers)]
+    assert all(steps < len(a) - 1 < 5 * steps for a in answers)
+    embed, unembed = model.embed.cpu().float(), model.unembed.cpu().float()
+    norm = lambda x: x * (x.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+    h, hk, d = model.heads, model.kv_heads, model.head_dim
+    for prompt, said in zip(prompts, answers):
+        tokens = torch.tensor(prompt + said[:-1])
+        n = len(tokens)
+        x = embed[tokens] + 0.1 * example._place(torch.arange(n), embed.shape[1]).float()
+        hidden = torch.ones(n, n, dtype=torch.bool).triu(1)
+        for w_qkv, w_out in zip(model.qkv, model.out):
+            fused = (norm(x) @ w_qkv.cpu().float()).view(n, h + 2 * hk, d).permute(1, 0, 2)
+            k, v = (t.repeat_interleave(h // hk, 0) for t in (fused[h:h + hk], fused[h + hk:]))
+            weights = (fused[:h] @ k.transpose(1, 2) * d ** -0.5).masked_fill(hidden, -math.inf).softmax(-1)
+            x = x + 0.3 * ((weights @ v).permute(1, 0, 2).reshape(n, h * d) @ w_out.cpu().float())
+        logits = (norm(x) @ unembed)[len(prompt) - 1:]
+        short = logits.amax(-1) - logits.gather(1, torch.tensor(said)[:, None])[:, 0]
+        assert short.max() <= off
+
+
+def test_speculative_decoding_one_token_a_step():
+    """The example without trees says one token a step, and leaves as many rows in its pages as there were tokens."""
+    from fstattention_amd.examples import speculative_decoding as example
+    model = example.make_model()
+    prompts = [[5, 6, 7], [9] * 100]
+    answers, talk = example.answer(model, prompts, 6, draft=0)
+    assert [len(a) for a in answers] == [7, 7] and talk.lens.tolist() == [9, 106]
+    dense, _ = fsta.read_paged_kv(talk.pools[0], talk.page_table, talk.lens, 110)
+    used = dense.abs().amax((1, 3)).cpu() > 0
+    assert torch.equal(used, torch.arange(110)[None, :] < talk.lens.cpu()[:, None])
