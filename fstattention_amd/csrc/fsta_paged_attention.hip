@@ -136,7 +136,7 @@ template <int D, int R, int S, bool FP8> struct Shape {
     using Raw = Fetch<D, R, FP8, kWiden, false>;
     static constexpr int kWideBytes = 2 * kTileN * D * 2;
     static constexpr int kShareBytes = kStages * Raw::kBytes + (kWiden ? kStep * kWideBytes : 0);
-    static constexpr size_t kJoin = (size_t)(S - 1) * R * (32 * D + 64) * 4;
+    static constexpr size_t kJoin = S > 1 ? (size_t)S * R * (32 * D + 64) * 4 : 0;
     static constexpr size_t kLds = (size_t)S * kShareBytes > kJoin ? (size_t)S * kShareBytes : kJoin;
 };
 
@@ -295,68 +295,78 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
         }
     }
 
-    // ---- join of the shares: through LDS, in the order of the shares --------------------------------------------------------
-    float l_tot = rows.row_sum(), m_i = rows.m_i;
+    // ---- rows out: a lane has O[row][32 dt + 8 j + 4 half .. + 3], quad 4 dt + j ----------------------------------------------
+    // (a row's first element for this lane: in o or in the workspace; null: nowhere)
+    auto open_row = [&](float m_i, float l_tot, bool first) -> unsigned char* {
+        const float lse = l_tot == 0.f ? -INFINITY : m_i + log2f(l_tot);
+        if (at.part < 0) {
+            // (worked out again: kept over the loop they cost registers that it needs)
+            const int token = (int)((uint32_t)(row0 + my_row) / (uint32_t)p.group);
+            const int64_t row = (int64_t)(s.start + token) * (p.batch.kv_heads * p.group) + head * p.group + (row0 + my_row) - token * p.group;
+            if (p.lse && first && half == 0) p.lse[row] = lse;
+            return reinterpret_cast<unsigned char*>(static_cast<uint16_t*>(p.o) + row * D + 4 * half);
+        }
+        if ((at.part + at.run + 1) * p.batch.kv_heads <= p.parts) {
+            const int64_t row = ((int64_t)(at.part + at.run) * p.batch.kv_heads + head) * p.tile_rows + my_row;
+            if (first && half == 0) p.part_lse[row] = lse;
+            return reinterpret_cast<unsigned char*>(p.part_o + row * D + 4 * half);
+        }
+        return nullptr;
+    };
+    auto put = [&](unsigned char* to, int quad, f32x4 x) {
+        if (at.part < 0) store_row<BF16>(reinterpret_cast<uint16_t*>(to) + 8 * quad, x[0], x[1], x[2], x[3]);
+        else if (to) *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(to) + 8 * quad) = x;
+    };
+    auto inverse = [](float l) { return l > 0.f ? 1.f / l : l == 0.f ? 0.f : l; };      // (NaN stays)
     auto& o = rows.o;
+    auto quad_of = [&](int quad) {
+        const int dt = quad / 4, j = quad % 4;
+        return f32x4{o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]};
+    };
     if constexpr (S > 1) {
-        float* area = reinterpret_cast<float*>(smem);
-        constexpr int kWaveFloats = 32 * D + 64;
+        // The shares' sums meet in LDS, in the order of the shares; every wave joins and writes its part of the head dims, 16 bytes a
+        // lane at a time.  (One wave joining all of it: 64 tokens on 256 keys 9.3 us instead of 8.4, 64 sequences of a token 59.5
+        // instead of 57.3.)
+        constexpr int kQuads = 4 * kDTiles, kPer = kQuads / S, kWaveFloats = 32 * D + 64;
+        float* area = reinterpret_cast<float*>(smem) + (size_t)group_of_rows * kWaveFloats;
+        float* mine_at = area + (size_t)share * R * kWaveFloats;
+        const float l_mine = rows.row_sum();
         __syncthreads();
-        if (share > 0) {
-            float* to = area + (size_t)((share - 1) * R + group_of_rows) * kWaveFloats;
 #pragma unroll
-            for (int dt = 0; dt < kDTiles; ++dt)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) to[(dt * 16 + e) * 64 + lane] = o[dt][e];
-            if (half == 0) {
-                to[32 * D + ql] = m_i;
-                to[32 * D + 32 + ql] = l_tot;
-            }
+        for (int quad = 0; quad < kQuads; ++quad) reinterpret_cast<f32x4*>(mine_at)[quad * 64 + lane] = quad_of(quad);
+        if (half == 0) {
+            mine_at[32 * D + ql] = rows.m_i;
+            mine_at[32 * D + 32 + ql] = l_mine;
         }
         __syncthreads();
-        if (share > 0) return;
-#pragma unroll 1
-        for (int other = 1; other < S; ++other) {
-            const float* theirs = area + (size_t)((other - 1) * R + group_of_rows) * kWaveFloats;
-            const float m_b = theirs[32 * D + ql], l_b = theirs[32 * D + 32 + ql];
-            const float m = fmaxf(m_i, m_b);
-            const float fa = m_i == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_i - m);
-            const float fb = m_b == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_b - m);
-            m_i = m;
-            l_tot = l_tot * fa + l_b * fb;
+        if (my_row >= rows_left) return;
+        float m[S], f[S];
 #pragma unroll
-            for (int dt = 0; dt < kDTiles; ++dt)
+        for (int i = 0; i < S; ++i) m[i] = area[(size_t)i * R * kWaveFloats + 32 * D + ql];
+        float m_i = m[0], l_tot = 0.f;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * fa + theirs[(dt * 16 + e) * 64 + lane] * fb;
+        for (int i = 1; i < S; ++i) m_i = fmaxf(m_i, m[i]);
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            f[i] = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - m_i);
+            l_tot += area[(size_t)i * R * kWaveFloats + 32 * D + 32 + ql] * f[i];
         }
-    }
-    if (my_row >= rows_left) return;
-
-    // ---- rows out: lane has O[row][32 dt + 8 j + 4 half .. + 3] -------------------------------------------------------------
-    const float inv = l_tot > 0.f ? 1.f / l_tot : l_tot == 0.f ? 0.f : l_tot;      // (NaN stays)
-    const float lse = l_tot == 0.f ? -INFINITY : m_i + log2f(l_tot);
-    if (at.part < 0) {
-        // (worked out again: kept over the loop they cost registers that it needs)
-        const int token = (int)((uint32_t)(row0 + my_row) / (uint32_t)p.group);
-        const int64_t out_row = (int64_t)(s.start + token) * (p.batch.kv_heads * p.group) + head * p.group + (row0 + my_row) - token * p.group;
-        if (p.lse && half == 0) p.lse[out_row] = lse;
-        uint16_t* dst = static_cast<uint16_t*>(p.o) + out_row * D + 4 * half;
+        unsigned char* to = open_row(m_i, l_tot, share == 0);
+        const float inv = inverse(l_tot);
 #pragma unroll
-        for (int dt = 0; dt < kDTiles; ++dt)
+        for (int k = 0; k < kPer; ++k) {
+            const int quad = share * kPer + k;
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                store_row<BF16>(dst + 32 * dt + 8 * j, o[dt][4 * j] * inv, o[dt][4 * j + 1] * inv, o[dt][4 * j + 2] * inv, o[dt][4 * j + 3] * inv);
-    } else if ((at.part + at.run + 1) * p.batch.kv_heads <= p.parts) {
-        const int64_t part_row = ((int64_t)(at.part + at.run) * p.batch.kv_heads + head) * p.tile_rows + my_row;
-        if (half == 0) p.part_lse[part_row] = lse;
-        float* dst = p.part_o + part_row * D + 4 * half;
+            for (int i = 0; i < S; ++i) x += reinterpret_cast<const f32x4*>(area + (size_t)i * R * kWaveFloats)[quad * 64 + lane] * f[i];
+            put(to, quad, x * inv);
+        }
+    } else {
+        if (my_row >= rows_left) return;
+        const float l_tot = rows.row_sum(), inv = inverse(l_tot);
+        unsigned char* to = open_row(rows.m_i, l_tot, true);
 #pragma unroll
-        for (int dt = 0; dt < kDTiles; ++dt)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const f32x4 w = {o[dt][4 * j] * inv, o[dt][4 * j + 1] * inv, o[dt][4 * j + 2] * inv, o[dt][4 * j + 3] * inv};
-                *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * j) = w;
-            }
+        for (int quad = 0; quad < 4 * kDTiles; ++quad) put(to, quad, quad_of(quad) * inv);
     }
 }
 
