@@ -235,8 +235,7 @@ def test_many_sequences():
 @pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64)])
 @pytest.mark.parametrize("batch,kv_heads,low,high", [(3, 1, 500, 9000), (5, 8, 1, 3000), (70, 2, 1, 1500), (200, 4, 300, 700), (130, 1, 1, 40)])
 def test_keys_dealt_evenly(batch, kv_heads, low, high, dtype, d, fp8):
-    """Lengths of all kinds under the kernel whose workgroups take equal runs of the batch's keys: runs that end inside a head, at
-    its ends, span many sequences, or are empty."""
+    """Lengths of all kinds in one batch, cut into runs of keys or not, sequences without keys among them."""
     g = torch.Generator().manual_seed(batch + high)
     new = torch.randint(0, 3, (batch,), generator=g).tolist()
     keys = [n + int(torch.randint(low, high, (1,), generator=g)) for n in new]
