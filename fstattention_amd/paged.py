@@ -162,8 +162,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, k
     (it steers the choice of kernel, not the result).
 
     Tokens that see nothing get zeros (and ``-inf``); rows of tokens that ``q_starts`` gives to no sequence are not written.
-    Sums and softmax statistics are float32; up to 64 rows (tokens times query heads per K/V head) a sequence, bfloat16 weights
-    go to the matrix cores as pairs (2^-16 relative at most), beyond that rounded once (2^-8 at most, as the output itself)."""
+    Sums and softmax statistics are float32.  Where a workgroup takes up to 64 rows (tokens times query heads per K/V head: short
+    chunks, and small calls), bfloat16 weights go to the matrix cores as pairs (2^-16 relative at most), elsewhere rounded once
+    (2^-8 at most, as the output itself)."""
     out = _calls().paged_attention(q, cache, page_table, kv_lens, q_starts, sm_scale, causal, tree_bits, max_q_len, return_lse)
     if out is not NotImplemented:
         return out
