@@ -14,6 +14,8 @@
 // TFLOP/s, where a large matrix product reaches 1200 to 1300); one short sequence, one launch and four round trips (9.8 us).
 #include "fsta_paged_attention.h"
 
+#include <algorithm>
+
 namespace fsta {
 namespace {
 
@@ -498,14 +500,14 @@ struct Sizes {
     int64_t floats;             // of workspace
     int run_units[3], least_tiles;
 };
-// most_keys: a sequence's, by the page table's width; shrink: by them
-Sizes sizes_of(int32_t batch, int32_t tokens, int32_t max_q_len, int64_t most_keys, bool shrink, int32_t heads, int32_t kv_heads, int32_t head_dim,
-               bool fp8) {
+int64_t most_rows_of(int32_t tokens, int32_t max_q_len, int group) {
+    return (int64_t)(max_q_len > 0 && max_q_len < tokens ? max_q_len : tokens) * group;
+}
+Sizes sizes_of(int tile_rows, int32_t batch, int32_t tokens, int32_t max_q_len, int32_t heads, int32_t kv_heads, int32_t head_dim) {
     Sizes z;
     const int group = heads / kv_heads;
-    z.most_rows = (int64_t)(max_q_len > 0 && max_q_len < tokens ? max_q_len : tokens) * group;
-    z.tile_rows = rows_for_rate(z.most_rows, (int64_t)tokens * group, kv_heads, head_dim, fp8);
-    if (shrink) z.tile_rows = rows_of_tile(z.tile_rows, (int64_t)tokens * group, most_keys, kv_heads);
+    z.most_rows = most_rows_of(tokens, max_q_len, group);
+    z.tile_rows = tile_rows;
     z.row_tiles = ((int64_t)tokens * group + (int64_t)(batch < tokens ? batch : tokens) * (z.tile_rows - 1)) / z.tile_rows;
     for (int i = 0; i < 3; ++i) z.run_units[i] = z.tile_rows == 256 ? kCus / 2 << i : (i + 1) * kCus;
     z.least_tiles = z.tile_rows == 32 ? kDecodeLeast : kChunkLeast;
@@ -586,9 +588,13 @@ using namespace fsta;
 extern "C" size_t fsta_paged_attention_workspace_bytes(int32_t batch, int32_t tokens, int32_t max_q_len, int32_t heads, int32_t kv_heads,
                                                        int32_t head_dim, int32_t cache_dtype) {
     if (batch <= 0 || tokens <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
-    // (the width of the page table may choose smaller tiles than these: a quarter of the rows, or half, and never more parts than
-    // four times as many, or twice)
-    return (size_t)sizes_of(batch, tokens, max_q_len, 0, false, heads, kv_heads, head_dim, cache_dtype == FSTA_FP8).floats * sizeof(float);
+    // (whichever of its answers rows_of_tile gives)
+    const int group = heads / kv_heads;
+    const int rate = rows_for_rate(most_rows_of(tokens, max_q_len, group), (int64_t)tokens * group, kv_heads, head_dim, cache_dtype == FSTA_FP8);
+    int64_t floats = 0;
+    for (const int rows : {32, 64, rate})
+        if (rows <= rate) floats = std::max(floats, sizes_of(rows, batch, tokens, max_q_len, heads, kv_heads, head_dim).floats);
+    return (size_t)floats * sizeof(float);
 }
 
 extern "C" int fsta_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
@@ -617,8 +623,10 @@ extern "C" int fsta_paged_attention(const void* q, int64_t q_token_stride, int64
         return fail(FSTA_EINVAL, "%s: rows of q, o and the cache must be 16-byte aligned", who);
     if (misaligned(k_exponent, 4) || misaligned(v_exponent, 4) || misaligned(lse, 4) || misaligned(tree_bits, 4))
         return fail(FSTA_EINVAL, "%s: exponents, lse and tree_bits must be 4-byte aligned", who);
-    const Sizes z = sizes_of(batch, tokens, max_q_len, (int64_t)width * page_size, true, heads, kv_heads, head_dim, cache_dtype == FSTA_FP8);
-    const size_t need = fsta_paged_attention_workspace_bytes(batch, tokens, max_q_len, heads, kv_heads, head_dim, cache_dtype);
+    const int64_t all_rows = (int64_t)tokens * (heads / kv_heads);
+    const int rate = rows_for_rate(most_rows_of(tokens, max_q_len, heads / kv_heads), all_rows, kv_heads, head_dim, cache_dtype == FSTA_FP8);
+    const Sizes z = sizes_of(rows_of_tile(rate, all_rows, (int64_t)width * page_size, kv_heads), batch, tokens, max_q_len, heads, kv_heads, head_dim);
+    const size_t need = (size_t)z.floats * sizeof(float);
     if (!workspace || workspace_bytes < need) return fail(FSTA_EINVAL, "%s: needs %zu bytes of workspace, got %zu", who, need, workspace_bytes);
     if (misaligned(workspace, 16)) return fail(FSTA_EINVAL, "%s: the workspace must be 16-byte aligned", who);
     while ((1 << p.batch.page_shift) < page_size) ++p.batch.page_shift;
