@@ -143,3 +143,33 @@ def test_speculative_decoding_one_token_a_step():
     dense, _ = fsta.read_paged_kv(talk.pools[0], talk.page_table, talk.lens, 110)
     used = dense.abs().amax((1, 3)).cpu() > 0
     assert torch.equal(used, torch.arange(110)[None, :] < talk.lens.cpu()[:, None])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_pages_beyond_32_bits(dtype):
+    """A pool of more than 2^32 elements: rows written to its last pages are read from there, by both kernels that read."""
+    pages, heads, page, d = (1 << 20) + 40, 2, 16, 128
+    shape = (pages, heads, page, d)
+    exps = (None, None) if dtype == torch.bfloat16 else tuple(torch.full(shape[:3], 127, dtype=torch.uint8, device="cuda") for _ in range(2))
+    cache = fsta.PagedKV(torch.empty(shape, dtype=dtype, device="cuda"), torch.empty(shape, dtype=dtype, device="cuda"), *exps)
+    keys = 300
+    need = -(-keys // page)
+    places = [pages - 1 - 2 * i for i in range(need)]
+    low = [p - (1 << 20) for p in places]                        # where they would lie by 32-bit offsets
+    table = torch.tensor([places, low], dtype=torch.int32).cuda()
+    lens = torch.tensor([keys, keys], dtype=torch.int32).cuda()
+    starts = torch.tensor([0, keys, 2 * keys], dtype=torch.int32).cuda()
+    g = torch.Generator().manual_seed(5)
+    k, v = (torch.randn((2 * keys, heads, d), generator=g).bfloat16().cuda() for _ in range(2))
+    fsta.write_paged_kv(cache, k, v, table, lens, starts)
+    near = fsta.PagedKV(*(None if t is None else t[torch.tensor(places + low, device="cuda")].clone() for t in cache))
+    near_table = torch.arange(2 * need, dtype=torch.int32).view(2, need).cuda()
+    got, want = (fsta.read_paged_kv(c, t, lens, keys, torch.bfloat16) for c, t in ((cache, table), (near, near_table)))
+    if dtype == torch.bfloat16:
+        assert torch.equal(got[0].transpose(1, 2).reshape(2 * keys, heads, d), k) and torch.equal(got[1].transpose(1, 2).reshape(2 * keys, heads, d), v)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for new in (1, 40, 300):
+        q = torch.randn((2 * new, 4, d), generator=g).bfloat16().cuda()
+        q_starts = torch.tensor([0, new, 2 * new], dtype=torch.int32).cuda()
+        outs = [fsta.paged_attention(q, c, t, lens, q_starts, d ** -0.5, max_q_len=new) for c, t in ((cache, table), (near, near_table))]
+        assert torch.equal(*outs) and outs[0].isfinite().all()
