@@ -27,7 +27,8 @@ struct PagedAttnParams {
     uint32_t* run_length;          // the cut's, behind the parts
     int32_t tree_words, mask, group, tile_rows, row_shift, parts;
     int32_t run_units[3], least_tiles;   // units that a launch may be cut into, the least tiles of a run
-    float slots, unit_cost, cut_cost;    // workgroups that run at once; what a unit and the joining cost, in tiles
+    float slots, unit_cost;              // workgroups that run at once; what a unit costs, in tiles
+    float cut_cost, cut_unit_cost;       // .. the joining, and per unit
     float scale_log2e;
 };
 

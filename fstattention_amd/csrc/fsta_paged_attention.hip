@@ -75,7 +75,7 @@ __device__ __forceinline__ uint32_t choose(const PagedAttnParams& p, const SeqLe
         const float runs = ceilf(keys * __builtin_amdgcn_rcpf((float)run));
         const float units = (float)lane_of(wave_prefix_sum(tiles * (uint32_t)runs), 63) * (float)p.batch.kv_heads;
         const float lasts = fminf(most, (float)run) + p.unit_cost;
-        const float done = (ceilf(units / p.slots) - 1.f) * (work / fmaxf(units, 1.f) + p.unit_cost) + lasts + (most > (float)run ? p.cut_cost : 0.f);
+        const float done = (ceilf(units / p.slots) - 1.f) * (work / fmaxf(units, 1.f) + p.unit_cost) + lasts + (most > (float)run ? p.cut_cost + units * p.cut_unit_cost : 0.f);
         if (done < best) {
             best = done;
             longest = run;
@@ -485,11 +485,12 @@ int rows_of_tile(int rate, int64_t all_rows, int64_t most_keys, int32_t kv_heads
 }
 
 // What choose weighs, in the time a workgroup takes for a tile of keys (0.66 us alone on its CU with up to 64 rows; with 128 rows
-// 0.9 us alone, and two share a CU at 1.05 us): a unit's start and end 4 to 5 us, the join's launch 5 us, and with many rows the
-// results of the runs, which go to memory and back (4 sequences of 256 tokens, 32 K/V heads, 1256 to 1500 keys: cut 65 us, whole 49;
-// from 16 to 20 nothing else that was timed changes, at 30 one sequence of 256 tokens on 1024 keys of 8 K/V heads 20 -> 31 us).
-struct Costs { float slots, unit, cut; };
-Costs costs_of(int tile_rows) { return tile_rows >= 128 ? Costs{(tile_rows == 256 ? 1.f : 2.f) * kCus, 6.f, 18.f} : Costs{kCus, 7.f, 8.f}; }
+// 0.9 us alone, and two share a CU at 1.05 us): a unit's start and end 4 to 5 us, the join's launch 5 us; with many rows it is the
+// results of the runs, which go to memory and back, 64 KB a unit (4 sequences of 256 tokens, 32 K/V heads, 1256 to 1500 keys: cut
+// 65 us, whole 49; the same 18 tiles for any number of units: 4 sequences of 256 tokens, 8 heads, 1500 keys 28.1 us instead of 24.5,
+// 6 sequences of 1 to 130 tokens on up to 700 keys, 40 heads of 64, 20.7 instead of 15.2; 30 tiles: 256 tokens on 1024 keys 31 instead of 20).
+struct Costs { float slots, unit, cut, cut_unit; };
+Costs costs_of(int tile_rows) { return tile_rows >= 128 ? Costs{(tile_rows == 256 ? 1.f : 2.f) * kCus, 6.f, 0.f, 18.f / 512.f} : Costs{kCus, 7.f, 8.f, 0.f}; }
 
 struct Sizes {
     int tile_rows;
@@ -637,7 +638,7 @@ extern "C" int fsta_paged_attention(const void* q, int64_t q_token_stride, int64
     p.group = heads / kv_heads; p.tile_rows = z.tile_rows; p.row_shift = z.tile_rows == 32 ? 5 : z.tile_rows == 64 ? 6 : z.tile_rows == 128 ? 7 : 8; p.parts = (int32_t)z.parts; p.least_tiles = z.least_tiles;
     for (int i = 0; i < 3; ++i) p.run_units[i] = z.run_units[i];
     const Costs costs = costs_of(z.tile_rows);
-    p.slots = costs.slots; p.unit_cost = costs.unit; p.cut_cost = costs.cut;
+    p.slots = costs.slots; p.unit_cost = costs.unit; p.cut_cost = costs.cut; p.cut_unit_cost = costs.cut_unit;
     p.scale_log2e = sm_scale * kLog2e;
     p.part_o = static_cast<float*>(workspace);
     p.part_lse = p.part_o + (size_t)z.parts * z.tile_rows * head_dim;
