@@ -8,7 +8,7 @@
 // Keys and values come page by page straight into an LDS ring (global -> LDS transfers of 1 KiB) through a buffer resource per 16
 // rows; rows past the sequence's end read as zeros, pages outside the cache from a row of zeros, so that what lies in unused rows of
 // a page can not turn a weight of zero into a NaN.
-// What bounds it: few rows, reading keys once (64 sequences of 16 to 8192 keys, 8 K/V heads of 128, 251 MB: 52 us of 56 with the join,
+// What bounds it: few rows, reading keys once (64 sequences of 16 to 8192 keys, 8 K/V heads of 128, 251 MB: 52 us with the join,
 // 4.8 TB/s with the start of 3.8 us in it; 8-bit, 16 of 8192 to 32768 keys, 607 MB: 114 of 117 us, 5.3 TB/s); many rows, the matrix
 // cores, whose products wait for the exponentials in between (4096 tokens after 16384, 32 heads: 1.24e12 operations in 1180 us, 1050
 // TFLOP/s, where a large matrix product reaches 1200 to 1300); one short sequence, one launch and four round trips (9.8 us).
@@ -461,13 +461,17 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
 
-// Rows of a workgroup's tile where there is much to do.  Up to 32 rows a sequence the keys are all there is to read, and the waves
-// share them out; 64 rows: in pairs; from 128 rows on every wave has rows of its own.  256 rows where there are two rounds of such
+// Rows of a workgroup's tile where there is much to do.  Up to 64 rows a sequence the keys are all there is to read, and pairs of waves
+// share them out, at two workgroups per CU, so that one's start lies under the other's keys.  (Up to 32 rows tiles of 32, whose four
+// waves have a ring each, fill the CU's LDS with one workgroup where rows are of 128 in 16 bits: 64 sequences of a token and 16 to 8192
+// keys 57.9 us, by pairs 51.9; 200 of 64 to 128 keys 57.4 and 35.3; 124 of up to 40 keys, 16 K/V heads, 49.6 and 27.5; only a CU that
+// has one unit misses the longer ring, 32 sequences of 4096 keys 92.3 and 97.2.  Of 64 or 8 bits two of them fit, and they are faster:
+// 40.0 and 45.6 for 32 sequences of 500 to 8192 keys of 64.)  From 128 rows on every wave has rows of its own.  256 rows where there are two rounds of such
 // tiles (4096 after 16384: 1221 -> 1189 us; with one round the last tiles of a causal chunk are waited for: 2048 tokens 63 -> 71 us).
 // 8-bit tiles are widened by all waves together, behind a barrier more, which two workgroups per CU hide and one does not (348 ->
 // 384 us); head_dim 64 fits three workgroups of 128 rows on a CU.
 int rows_for_rate(int64_t most_rows, int64_t all_rows, int32_t kv_heads, int32_t head_dim, bool fp8) {
-    if (most_rows <= 32) return 32;
+    if (most_rows <= 32 && (head_dim == 64 || fp8)) return 32;
     if (most_rows <= 64) return 64;
     return head_dim == 128 && !fp8 && all_rows / 256 * kv_heads >= 2 * kCus ? 256 : 128;
 }
@@ -477,20 +481,21 @@ int rows_for_rate(int64_t most_rows, int64_t all_rows, int32_t kv_heads, int32_t
 // 12.5 / 10.5 / 9.3 us, of 8 bits 16.0 / 11.4 / 9.6; 256 tokens on 256 keys 12.6 / 10.8 / 13.2, on 1024 keys 19.8 / 23.1 / 22.3; 5 x 38
 // tokens of 4 K/V heads on 362 keys 17.5 / 15.8 / 13.9; 16 x 64 tokens on 250 keys 15.0 / 17.5 / 41; 32 tokens on 16384 keys 42 / 32 /
 // 34; 64 tokens on 16384 keys 42 / 48 / 50.)  What the host knows of the keys is that the page table's rows hold no more.
-int rows_of_tile(int rate, int64_t all_rows, int64_t most_keys, int32_t kv_heads) {
-    const int64_t units32 = (all_rows + 31) / 32 * kv_heads, units64 = (all_rows + 63) / 64 * kv_heads;
+int rows_of_tile(int rate, int64_t seqs, int64_t all_rows, int64_t most_keys, int32_t kv_heads) {
+    const int64_t units32 = std::max((all_rows + 31) / 32, seqs) * kv_heads, units64 = std::max((all_rows + 63) / 64, seqs) * kv_heads;
     if (rate > 32 && most_keys <= kDecodeLeast * kTileN && units32 <= kCus * 3 / 4) return 32;
     if (rate > 64 && (units64 <= kCus / 16 || (units64 <= kCus / 2 && units64 * most_keys < kCus * kDecodeLeast * kTileN))) return 64;
     return rate;
 }
 
 // What choose weighs, in the time a workgroup takes for a tile of keys (0.66 us alone on its CU with up to 64 rows; with 128 rows
-// 0.9 us alone, and two share a CU at 1.05 us): a unit's start and end 4 to 5 us, the join's launch 5 us; with many rows it is the
+// 0.9 us alone, and two share a CU at 1.05 us): a unit's start and end 4 to 5 us, with few rows
+// half hidden under another's keys (2 tiles; 7: 16 sequences of 4 tokens 47.5 us instead of 45.7), the join's launch 5 us; with many rows it is the
 // results of the runs, which go to memory and back, 64 KB a unit (4 sequences of 256 tokens, 32 K/V heads, 1256 to 1500 keys: cut
 // 65 us, whole 49; the same 18 tiles for any number of units: 4 sequences of 256 tokens, 8 heads, 1500 keys 28.1 us instead of 24.5,
 // 6 sequences of 1 to 130 tokens on up to 700 keys, 40 heads of 64, 20.7 instead of 15.2; 30 tiles: 256 tokens on 1024 keys 31 instead of 20).
 struct Costs { float slots, unit, cut, cut_unit; };
-Costs costs_of(int tile_rows) { return tile_rows >= 128 ? Costs{(tile_rows == 256 ? 1.f : 2.f) * kCus, 6.f, 0.f, 18.f / 512.f} : Costs{kCus, 7.f, 8.f, 0.f}; }
+Costs costs_of(int tile_rows) { return tile_rows >= 128 ? Costs{(tile_rows == 256 ? 1.f : 2.f) * kCus, 6.f, 0.f, 18.f / 512.f} : Costs{kCus, 2.f, 8.f, 0.f}; }
 
 struct Sizes {
     int tile_rows;
@@ -626,7 +631,7 @@ extern "C" int fsta_paged_attention(const void* q, int64_t q_token_stride, int64
         return fail(FSTA_EINVAL, "%s: exponents, lse and tree_bits must be 4-byte aligned", who);
     const int64_t all_rows = (int64_t)tokens * (heads / kv_heads);
     const int rate = rows_for_rate(most_rows_of(tokens, max_q_len, heads / kv_heads), all_rows, kv_heads, head_dim, cache_dtype == FSTA_FP8);
-    const Sizes z = sizes_of(rows_of_tile(rate, all_rows, (int64_t)width * page_size, kv_heads), batch, tokens, max_q_len, heads, kv_heads, head_dim);
+    const Sizes z = sizes_of(rows_of_tile(rate, batch < tokens ? batch : tokens, all_rows, (int64_t)width * page_size, kv_heads), batch, tokens, max_q_len, heads, kv_heads, head_dim);
     const size_t need = (size_t)z.floats * sizeof(float);
     if (!workspace || workspace_bytes < need) return fail(FSTA_EINVAL, "%s: needs %zu bytes of workspace, got %zu", who, need, workspace_bytes);
     if (misaligned(workspace, 16)) return fail(FSTA_EINVAL, "%s: the workspace must be 16-byte aligned", who);
