@@ -8,8 +8,8 @@
 // Keys and values come page by page straight into an LDS ring (global -> LDS transfers of 1 KiB) through a buffer resource per 16
 // rows; rows past the sequence's end read as zeros, pages outside the cache from a row of zeros, so that what lies in unused rows of
 // a page can not turn a weight of zero into a NaN.
-// What bounds it: few rows, reading keys once (64 sequences of 16 to 8192 keys, 8 K/V heads of 128, 251 MB: 52 us with the join,
-// 4.8 TB/s with the start of 3.8 us in it; 8-bit, 16 of 8192 to 32768 keys, 607 MB: 114 of 117 us, 5.3 TB/s); many rows, the matrix
+// What bounds it: few rows, reading keys once (64 sequences of 16 to 8192 keys, 8 K/V heads of 128, 251 MB: 50.4 us with
+// the join, 5.0 TB/s; 8-bit, 16 of 8192 to 32768 keys, 607 MB: 114 of 117 us, 5.3 TB/s); many rows, the matrix
 // cores, whose products wait for the exponentials in between (4096 tokens after 16384, 32 heads: 1.24e12 operations in 1180 us, 1050
 // TFLOP/s, where a large matrix product reaches 1200 to 1300); one short sequence, one launch and four round trips (9.8 us).
 #include "fsta_paged_attention.h"
