@@ -277,12 +277,12 @@ __global__ __launch_bounds__(kThreads) void tree_bits_kernel(const int64_t* pare
                 }
                 nodes[n] = {mask, __shfl(p, link)};
             }
-            const int total = own * words;
+            const int64_t total = (int64_t)own * words;         // (64 rows of 2^25 words are accepted)
             if ((reinterpret_cast<uintptr_t>(rows) & 15) == 0) {
-                for (int i = tid; i < total / 4; i += kThreads) reinterpret_cast<u32x4*>(rows)[i] = u32x4{0u, 0u, 0u, 0u};
-                for (int i = (total & ~3) + tid; i < total; i += kThreads) rows[i] = 0u;
+                for (int64_t i = tid; i < total / 4; i += kThreads) reinterpret_cast<u32x4*>(rows)[i] = u32x4{0u, 0u, 0u, 0u};
+                for (int64_t i = (total & ~(int64_t)3) + tid; i < total; i += kThreads) rows[i] = 0u;
             } else {
-                for (int i = tid; i < total; i += kThreads) rows[i] = 0u;
+                for (int64_t i = tid; i < total; i += kThreads) rows[i] = 0u;
             }
             __syncthreads();
             if (tid < own) {
