@@ -222,7 +222,7 @@ def tree_mask_bits(parent: torch.Tensor, q_starts: Optional[torch.Tensor] = None
     if q_starts.dim() != 1 or q_starts.dtype != torch.int32 or q_starts.shape[0] < 2 or q_starts.device != parent.device:
         raise ValueError("q_starts must be int32 [batch + 1] on parent's device, of at least one sequence")
     max_nodes = tokens if max_nodes is None else max_nodes
-    if max_nodes < 0:
+    if not 0 <= max_nodes < 2 ** 31:
         raise ValueError(f"max_nodes={max_nodes}")
     lib = _lib.load()
     parent, q_starts = parent.contiguous(), q_starts.contiguous()

@@ -19,3 +19,10 @@ def test_masks_wider_than_32_bits_count():
     assert bits[:, :2].tolist() == [[signed(x & 0xffffffff), signed(x >> 32)] for x in chain]
     for row in bits:
         assert int(row[2:].count_nonzero()) == 0
+
+
+@pytest.mark.parametrize("most", [-1, 1 << 31, 1 << 37])
+def test_more_nodes_than_a_tree_can_have_are_refused(most):
+    """2^37 nodes are 2^32 words, which the library's 32-bit count would take for none."""
+    with pytest.raises(ValueError, match="max_nodes"):
+        fsta.tree_mask_bits(torch.zeros(1, dtype=torch.int64).cuda(), max_nodes=most)
