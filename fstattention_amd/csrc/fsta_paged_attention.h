@@ -83,15 +83,15 @@ template <> struct VRaw<true> { u32x2 x[2]; };
 //     S^T = K_tile . Q^T      O^T += V_tile^T . P^T        (32x32x16 matrix instructions)
 // A lane holds 16 scores of row lane & 31: keys 8 (e / 4) + 4 (lane >> 5) + e % 4, which is also how the transposing reads hand
 // it the values' rows, so that the weights go to the second product from the registers they are in.
-// DIRECT: tiles are 8-bit, widened here.  SPLIT: weights go to the matrix cores as pairs of bfloat16, hi + lo.
-template <bool BF16, int D, bool DIRECT, bool SPLIT> struct RowGroup {
+// FP8: the cache is 8-bit.  DIRECT: so are the tiles, widened here.  SPLIT: weights go to the matrix cores as pairs of bfloat16, hi + lo.
+template <bool BF16, int D, bool FP8, bool DIRECT, bool SPLIT> struct RowGroup {
     using MM = Mma<BF16>;
-    using PV = Mma<BF16 || DIRECT>;           // weights times values: 8-bit values are exact in bfloat16 whatever their scale
+    using PV = Mma<BF16 || FP8>;              // weights times values: 8-bit values are exact in bfloat16 whatever their scale
     using Frag = typename MM::frag;
     using PFrag = typename PV::frag;
     static constexpr int kSteps = D / 16;     // matrix instructions of a tile's scores
     static constexpr int kDTiles = D / 32;    // 32-row tiles of O^T
-    static constexpr float kTrustedSum = BF16 || DIRECT ? 16777216.f : 32768.f;
+    static constexpr float kTrustedSum = BF16 || FP8 ? 16777216.f : 32768.f;
     static constexpr uint32_t kVBytes = kTileN * D * (DIRECT ? 1 : 2);      // values behind keys
     static constexpr uint32_t kExps = 2 * kTileN * D;                       // 8-bit tiles: exponents of the keys, of the values
 
@@ -135,7 +135,7 @@ template <bool BF16, int D, bool DIRECT, bool SPLIT> struct RowGroup {
     }
     // Sign bits of the halves whose exponent is all ones (adding the exponent's lowest bit carries into the sign's place)
     __device__ __forceinline__ static uint32_t not_finite(PFrag a, PFrag b) {
-        constexpr uint32_t kTop = BF16 || DIRECT ? 0x7f807f80u : 0x7c007c00u, kLow = BF16 || DIRECT ? 0x00800080u : 0x04000400u;
+        constexpr uint32_t kTop = BF16 || FP8 ? 0x7f807f80u : 0x7c007c00u, kLow = BF16 || FP8 ? 0x00800080u : 0x04000400u;
         const u32x4 x = __builtin_bit_cast(u32x4, a), y = __builtin_bit_cast(u32x4, b);
         uint32_t bits = 0u;
 #pragma unroll
@@ -144,7 +144,7 @@ template <bool BF16, int D, bool DIRECT, bool SPLIT> struct RowGroup {
     }
     // The values' fragment with what is not finite replaced by 0
     __device__ __forceinline__ static PFrag only_finite(PFrag f) {
-        constexpr uint32_t kTop = BF16 || DIRECT ? 0x7f80u : 0x7c00u;
+        constexpr uint32_t kTop = BF16 || FP8 ? 0x7f80u : 0x7c00u;
         u32x4 w = __builtin_bit_cast(u32x4, f);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -155,7 +155,7 @@ template <bool BF16, int D, bool DIRECT, bool SPLIT> struct RowGroup {
     }
     // 1 where it is +inf (sign 0) / -inf (sign 1) or NaN, 0 elsewhere
     __device__ __forceinline__ static PFrag infinite(PFrag f, uint32_t sign) {
-        constexpr uint32_t kTop = BF16 || DIRECT ? 0x7f80u : 0x7c00u, kOne = BF16 || DIRECT ? 0x3f80u : 0x3c00u;
+        constexpr uint32_t kTop = BF16 || FP8 ? 0x7f80u : 0x7c00u, kOne = BF16 || FP8 ? 0x3f80u : 0x3c00u;
         u32x4 w = __builtin_bit_cast(u32x4, f);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -311,7 +311,7 @@ template <bool BF16, int D, bool DIRECT, bool SPLIT> struct RowGroup {
             // A value that is not finite must reach the rows that see its key and no other, although a weight of zero times it
             // is a NaN: where the tile is masked, such values are taken out and put back row by row, by their signs.
             if (masked && __ballot(not_finite(f[0], f[1]) != 0u) != 0ull) {
-                constexpr uint32_t kOne = BF16 || DIRECT ? 0x3f80u : 0x3c00u;
+                constexpr uint32_t kOne = BF16 || FP8 ? 0x3f80u : 0x3c00u;
 #pragma unroll 1
                 for (uint32_t sign = 0; sign < 2; ++sign) {
                     f32x16 touched;

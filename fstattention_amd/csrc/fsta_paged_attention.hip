@@ -152,7 +152,7 @@ template <bool BF16, int D, int R, int S, bool FP8, bool SPLIT, bool ONCE>
 __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnParams p) {
     using SH = Shape<D, R, S, FP8>;
     using F = Fetch<D, R, FP8, SH::kWiden, ONCE>;
-    using G = RowGroup<BF16, D, FP8 && !SH::kWiden, SPLIT>;
+    using G = RowGroup<BF16, D, FP8, FP8 && !SH::kWiden, SPLIT>;
     constexpr int kStages = SH::kStages, kStep = SH::kStep, kDTiles = G::kDTiles;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
 
@@ -245,13 +245,13 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
         for (int j = 0; j < kPieces; ++j) {
             const int piece = (group_of_rows * kPieces + j) * 64 + lane;
             const int r = piece / (D / 16), c = piece % (D / 16);      // r: 0..31 keys, 32..63 values
-            const bool is_v = r >= kTileN;
+            const bool is_v = group_of_rows * kPieces + j >= kTileN * D / 16 / 64;      // (r >= kTileN, said for the whole wave)
             lds_tie(bytes[j]);
             lds_tie(E[j]);
             const float scale = __builtin_bit_cast(float, min(E[j], 254u) << 23);     // (exponents of unused rows may be anything)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const u32x4 w = widen8<BF16>(bytes[j][2 * h], bytes[j][2 * h + 1], scale);
+                const u32x4 w = is_v ? widen8<true>(bytes[j][2 * h], bytes[j][2 * h + 1], scale) : widen8<BF16>(bytes[j][2 * h], bytes[j][2 * h + 1], scale);
                 const int rr = r & (kTileN - 1);
                 const int chunk = is_v ? v_chunk<D>(rr, 2 * c + h) : k_chunk<D>(rr, 2 * c + h);
                 lds_write_b128(wide + (uint32_t)((is_v ? kTileN * D * 2 : 0) + rr * D * 2 + chunk * 16), w);
@@ -529,8 +529,9 @@ Sizes sizes_of(int tile_rows, int32_t batch, int32_t tokens, int32_t max_q_len, 
 
 template <bool BF16, int D, int R, int S, bool FP8, bool ONCE>
 int launch_units_of(const PagedAttnParams& p, int64_t units, hipStream_t stream) {
-    // bfloat16 weights as pairs where the matrix cores wait for keys anyway
-    constexpr bool kSplit = R < 4 && (BF16 || FP8);
+    // bfloat16 weights as pairs where the matrix cores wait for keys anyway, and where queries and results are float16: over 8-bit
+    // values, which only bfloat16 holds whatever their scale
+    constexpr bool kSplit = FP8 ? R < 4 || !BF16 : R < 4 && BF16;
     constexpr auto kernel = &paged_attn_kernel<BF16, D, R, S, FP8, kSplit, ONCE>;
     constexpr size_t lds = Shape<D, R, S, FP8>::kLds;
     if (units * R * S * 64 >= (int64_t)1 << 32) return fail(FSTA_EUNSUPPORTED, "fsta_paged_attention: %d tokens", p.batch.tokens);

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import fstattention_amd as fsta
+from test_gpu_paged import check, cuda, make_batch, make_cache, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +27,29 @@ def test_more_nodes_than_a_tree_can_have_are_refused(most):
     """2^37 nodes are 2^32 words, which the library's 32-bit count would take for none."""
     with pytest.raises(ValueError, match="max_nodes"):
         fsta.tree_mask_bits(torch.zeros(1, dtype=torch.int64).cuda(), max_nodes=most)
+
+
+# ---- float16 queries over 8-bit rows of any range ------------------------------------------------------------------------
+# Rows written from bfloat16 may be larger than float16 holds; the queries and the result are float16.  Tolerances: those of
+# test_gpu_paged.check, per unit of the attention over |v| (the largest value here is 4.5 * 2^17).
+
+def _wide_batch(new, keys, columns, seed):
+    """A batch whose page table is as wide as a server's: `columns` more that no sequence uses"""
+    tab, lens, starts, pages = make_batch(new, keys, 16, seed)
+    return torch.cat([tab, torch.full((len(new), columns), -1, dtype=torch.int32)], 1), lens, starts, pages
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new,columns", [([1, 1], 0), ([15, 9], 0), ([500, 70], 1000)])
+def test_float16_queries_over_large_8_bit_values(d, new, columns):
+    """Every 50th key's values beyond float16's range: the weighted means are within it, at every size of tile."""
+    keys = [700, 333]
+    tab, lens, starts, pages = _wide_batch(new, keys, columns, 61)
+    cache = make_cache(pages, 2, 16, d, torch.bfloat16, 62, fp8=True)
+    cache.v_exponent[:, :, 5] += torch.where(torch.arange(pages) % 3 == 0, 17, 0).to(torch.uint8)[:, None]
+    q = (torch.randn((sum(new), 8, d), generator=torch.Generator().manual_seed(63)) * 0.5).half()
+    out, lse = fsta.paged_attention(q.cuda(), cuda(cache), tab.cuda(), lens.cuda(), starts.cuda(), d ** -0.5, causal=False, max_q_len=max(new),
+                                    return_lse=True)
+    want, want_lse, size = reference(q, cache, tab, lens, starts, d ** -0.5, "all")
+    assert want.abs().max() > 500 and out.isfinite().all()
+    check(out, lse, want, want_lse, size, keys, torch.float16, max(new) * 4, 0.0)
