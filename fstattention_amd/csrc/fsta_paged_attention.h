@@ -94,6 +94,8 @@ template <bool BF16, int D, bool FP8, bool DIRECT, bool SPLIT> struct RowGroup {
     static constexpr float kTrustedSum = BF16 || FP8 ? 16777216.f : 32768.f;
     static constexpr uint32_t kVBytes = kTileN * D * (DIRECT ? 1 : 2);      // values behind keys
     static constexpr uint32_t kExps = 2 * kTileN * D;                       // 8-bit tiles: exponents of the keys, of the values
+    // float16 holds bytes, but not every byte times its power of two: the keys' powers go to the scores
+    static constexpr bool kScaleScores = FP8 && !BF16;
 
     int ql, half;
     uint32_t k_lane0, v_lane0;                // this lane's addresses in a tile
@@ -166,21 +168,30 @@ template <bool BF16, int D, bool FP8, bool DIRECT, bool SPLIT> struct RowGroup {
         return __builtin_bit_cast(PFrag, w);
     }
 
-    // One tile at LDS address `at` (keys, values, exponents).  masked (uniform): word() is the row's bits of the keys it sees.
-    template <typename Word> __device__ __forceinline__ void tile(uint32_t at, float sc, bool masked, Word word) {
+    // One tile at LDS address `at` (keys, values), 8-bit ones' exponents at `exps` (widened ones': the keys' powers of two).  masked
+    // (uniform): word() is the row's bits of the keys it sees.
+    template <typename Word> __device__ __forceinline__ void tile(uint32_t at, uint32_t exps, float sc, bool masked, Word word) {
         // S^T (K fragments: all requested, then used as they arrive; LDS reads come back in order)
         f32x16 sv;
 #pragma unroll
         for (int e = 0; e < 16; ++e) sv[e] = 0.f;
-        uint32_t v_exp[4];
+        uint32_t v_exp[4], k_exp[4];
+        u32x4 k_power[4];
+        if constexpr (kScaleScores) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if constexpr (DIRECT) k_exp[j] = lds_read_b32(exps + 8 * j + 4 * half);
+                else k_power[j] = lds_read_b128(exps + 4 * (8 * j + 4 * half));
+        }
         if constexpr (DIRECT) {
-            uint32_t E;
-            asm volatile("ds_read_u8 %0, %1" : "=v"(E) : "v"(at + kExps + ql) : "memory");
+            uint32_t E = 127u;
+            if constexpr (!kScaleScores) asm volatile("ds_read_u8 %0, %1" : "=v"(E) : "v"(exps + ql) : "memory");
             u32x2 raw[kSteps];
 #pragma unroll
             for (int ks = 0; ks < kSteps; ++ks) raw[ks] = lds_read_b64((at + k_lane0) ^ (uint32_t)(ks << 4));
+            if constexpr (kScaleScores) wait_lds<kSteps>();                        // (the counter of LDS accesses goes up to 15)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v_exp[j] = lds_read_b32(at + kExps + kTileN + 8 * j + 4 * half);
+            for (int j = 0; j < 4; ++j) v_exp[j] = lds_read_b32(exps + kTileN + 8 * j + 4 * half);
             wait_lds<kSteps + 4>();
             lds_tie(E);
             const float scale = __builtin_bit_cast(float, min(E, 254u) << 23);     // (exponents of unused rows may be anything)
@@ -203,6 +214,18 @@ template <bool BF16, int D, bool FP8, bool DIRECT, bool SPLIT> struct RowGroup {
                 lds_tie(raw[k]);
                 sv = MM::mfma(__builtin_bit_cast(Frag, raw[k]), qf[k], sv);
             });
+        }
+        if constexpr (kScaleScores) {         // (requested in front of the keys: they are here)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (DIRECT) lds_tie(k_exp[j]);
+                else lds_tie(k_power[j]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (DIRECT) k_power[j][e] = min((k_exp[j] >> (8 * e)) & 255u, 254u) << 23;
+                    sv[4 * j + e] *= __builtin_bit_cast(float, (uint32_t)k_power[j][e]);
+                }
+            }
         }
         uint32_t mine = ~0u;                  // bit 8 (e / 4) + e % 4: this lane's score e counts
         if (masked) {

@@ -141,7 +141,9 @@ template <int D, int R, int S, bool FP8> struct Shape {
     static constexpr int kStages = R == 8 ? 9 : R == 4 ? 5 : FP8 && R == 2 ? 4 : 2;
     using Raw = Fetch<D, R, FP8, kWiden, false>;
     static constexpr int kWideBytes = 2 * kTileN * D * 2;
-    static constexpr int kShareBytes = kStages * Raw::kBytes + (kWiden ? kStep * kWideBytes : 0);
+    static constexpr int kPowerBytes = kTileN * 4;                          // behind a widened tile: its keys' powers of two
+    static constexpr int kShareBytes = kStages * Raw::kBytes + (kWiden ? kWideBytes + kPowerBytes : 0);
+    static_assert(!kWiden || kStep == 1, "one widened tile");
     static constexpr size_t kJoin = S > 1 ? (size_t)S * R * (32 * D + 64) * 4 : 0;
     static constexpr size_t kLds = (size_t)S * kShareBytes > kJoin ? (size_t)S * kShareBytes : kJoin;
 };
@@ -220,15 +222,16 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
 
     const uint32_t ring_lds = lds_addr(ring), wide_lds = ring_lds + kStages * F::kBytes;
     auto bad_of = [&](int i) { return (bad_halves >> (2 * (int)((uint32_t)i % kStages))) & 3u; };
-    auto lies_at = [&](int i) { return SH::kWiden ? wide_lds + (uint32_t)((i % kStep) * SH::kWideBytes) : ring_lds + ((uint32_t)i % kStages) * F::kBytes; };
+    auto lies_at = [&](int i) { return SH::kWiden ? wide_lds : ring_lds + ((uint32_t)i % kStages) * F::kBytes; };
     auto first_of = [&](int i) { return (tile0 + share + i * S) * kTileN; };
     auto compute = [&](int i) {
         const int first = first_of(i);
         if (first > mine.sight.high_limit) return;
         const uint32_t bad = bad_of(i);
-        rows.tile(lies_at(i), p.scale_log2e, bad || !mine.sight.whole(p, first), [&] { return mine.sight.word(p, first, bad); });
+        rows.tile(lies_at(i), lies_at(i) + (SH::kWiden ? SH::kWideBytes : F::kDma * 1024), p.scale_log2e, bad || !mine.sight.whole(p, first), [&] { return mine.sight.word(p, first, bad); });
     };
-    // 8-bit rows: the share's waves widen the landed tile into the 16-bit layout, once for all row groups
+    // 8-bit rows: the share's waves widen the landed tile into the 16-bit layout, once for all row groups: values times their powers
+    // of two in bfloat16, keys in the type of Q (in float16 without their powers, which are laid down as floats)
     auto widen = [&](int i) {
         const uint32_t raw = ring_lds + ((uint32_t)i % kStages) * F::kBytes, wide = lies_at(i);
         constexpr int kPieces = 2 * kTileN * D / 16 / 64 / R;          // 16-byte pieces per lane
@@ -248,10 +251,14 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
             const bool is_v = group_of_rows * kPieces + j >= kTileN * D / 16 / 64;      // (r >= kTileN, said for the whole wave)
             lds_tie(bytes[j]);
             lds_tie(E[j]);
-            const float scale = __builtin_bit_cast(float, min(E[j], 254u) << 23);     // (exponents of unused rows may be anything)
+            const uint32_t power = min(E[j], 254u) << 23;              // (exponents of unused rows may be anything)
+            const float scale = __builtin_bit_cast(float, power);
+            if constexpr (G::kScaleScores)
+                if (!is_v && c == 0) lds_write_b32(wide + SH::kWideBytes + 4 * r, power);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const u32x4 w = is_v ? widen8<true>(bytes[j][2 * h], bytes[j][2 * h + 1], scale) : widen8<BF16>(bytes[j][2 * h], bytes[j][2 * h + 1], scale);
+                const uint32_t lo = bytes[j][2 * h], hi = bytes[j][2 * h + 1];
+                const u32x4 w = is_v || BF16 ? widen8<true>(lo, hi, scale) : widen8<false>(lo, hi, 1.f);
                 const int rr = r & (kTileN - 1);
                 const int chunk = is_v ? v_chunk<D>(rr, 2 * c + h) : k_chunk<D>(rr, 2 * c + h);
                 lds_write_b128(wide + (uint32_t)((is_v ? kTileN * D * 2 : 0) + rr * D * 2 + chunk * 16), w);

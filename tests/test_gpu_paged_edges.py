@@ -53,3 +53,19 @@ def test_float16_queries_over_large_8_bit_values(d, new, columns):
     want, want_lse, size = reference(q, cache, tab, lens, starts, d ** -0.5, "all")
     assert want.abs().max() > 500 and out.isfinite().all()
     check(out, lse, want, want_lse, size, keys, torch.float16, max(new) * 4, 0.0)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new,columns", [([1, 1], 0), ([15, 9], 0), ([500, 70], 1000)])
+@pytest.mark.parametrize("power", [17, -30])
+def test_float16_queries_over_8_bit_keys_of_any_range(power, d, new, columns):
+    """Keys beyond float16's range, or below its smallest numbers, whose scores are ordinary: sm_scale makes up for it."""
+    keys = [700, 333]
+    tab, lens, starts, pages = _wide_batch(new, keys, columns, 64)
+    cache = make_cache(pages, 2, 16, d, torch.bfloat16, 65, fp8=True)
+    cache.k_exponent.copy_((cache.k_exponent.int() + power).to(torch.uint8))
+    q = torch.randn((sum(new), 8, d), generator=torch.Generator().manual_seed(66)).half()
+    scale = d ** -0.5 * 2.0 ** -power
+    out, lse = fsta.paged_attention(q.cuda(), cuda(cache), tab.cuda(), lens.cuda(), starts.cuda(), scale, max_q_len=max(new), return_lse=True)
+    want, want_lse, size = reference(q, cache, tab, lens, starts, scale, "causal")
+    check(out, lse, want, want_lse, size, keys, torch.float16, max(new) * 4, 0.0)
