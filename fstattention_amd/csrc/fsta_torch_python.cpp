@@ -428,7 +428,8 @@ bool read_pool(PyObject* o, Pool* p) {
     p->k = gpu_tensor(PyTuple_GET_ITEM(o, 0));
     p->v = gpu_tensor(PyTuple_GET_ITEM(o, 1));
     if (!p->k || !p->v || p->k->dim() != 4 || p->v->sizes() != p->k->sizes() || p->v->scalar_type() != p->k->scalar_type() ||
-        p->v->device() != p->k->device() || !p->k->is_contiguous() || !p->v->is_contiguous())
+        p->v->device() != p->k->device() || !p->k->is_contiguous() || !p->v->is_contiguous() ||
+        (c10::GradMode::is_enabled() && (wants_grad(*p->k) || wants_grad(*p->v))))
         return false;
     const bool fp8 = p->k->scalar_type() == at::kFloat8_e4m3fn;
     p->code = fp8 ? FSTA_FP8 : half_code(p->k->scalar_type());

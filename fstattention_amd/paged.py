@@ -64,6 +64,8 @@ def _check_cache(cache: PagedKV):
         raise ValueError("a paged cache lives on the GPU (no CPU fallback)")
     if not (k.is_contiguous() and v.is_contiguous()):
         raise ValueError("the cache's k and v must be contiguous")
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+        raise ValueError("the cache's k or v requires a gradient: the paged cache's operators have no backward pass")
     exponents = (cache.k_exponent, cache.v_exponent)
     if k.dtype == torch.float8_e4m3fn:
         for e in exponents:

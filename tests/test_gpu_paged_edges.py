@@ -1,4 +1,6 @@
 """The operators of the paged KV cache at the ends of what they accept."""
+import types
+
 import pytest
 import torch
 
@@ -69,3 +71,32 @@ def test_float16_queries_over_8_bit_keys_of_any_range(power, d, new, columns):
     out, lse = fsta.paged_attention(q.cuda(), cuda(cache), tab.cuda(), lens.cuda(), starts.cuda(), scale, max_q_len=max(new), return_lse=True)
     want, want_lse, size = reference(q, cache, tab, lens, starts, scale, "causal")
     check(out, lse, want, want_lse, size, keys, torch.float16, max(new) * 4, 0.0)
+
+
+# ---- gradients and what autograd keeps --------------------------------------------------------------------------------------
+
+def _small_call():
+    tab, lens, starts, pages = (t.cuda() if torch.is_tensor(t) else t for t in make_batch([2, 1], [20, 3], 16, 71))
+    cache = cuda(make_cache(pages, 2, 16, 64, torch.bfloat16, 72))
+    q, k = (torch.randn((3, h, 64), device="cuda").bfloat16() for h in (4, 2))
+    return cache, tab, lens, starts, q, k
+
+
+def _without_plain_calls(monkeypatch):
+    """Every call through the checks in Python"""
+    calls = types.SimpleNamespace(**{name: lambda *args: NotImplemented for name in ("paged_attention", "paged_read", "paged_write", "tree_bits")})
+    monkeypatch.setattr("fstattention_amd.paged._calls", lambda: calls)
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_a_cache_that_requires_a_gradient_is_refused(which):
+    """A learned prefix among the pages: no operator has a backward pass, so none takes it for one that has."""
+    cache, tab, lens, starts, q, k = _small_call()
+    learned = cache._replace(**{which: getattr(cache, which).clone().requires_grad_()})
+    calls = (lambda: fsta.write_paged_kv(learned, k, k, tab, lens, starts), lambda: fsta.read_paged_kv(learned, tab, lens, 20),
+             lambda: fsta.paged_attention(q, learned, tab, lens, starts, 0.1))
+    for call in calls:
+        with pytest.raises(ValueError, match="backward"):
+            call()
+        with torch.no_grad():
+            call()
