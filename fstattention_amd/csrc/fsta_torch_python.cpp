@@ -54,6 +54,8 @@ bool plain_dispatch() {
 bool plain_context() { return plain_dispatch() && !at::impl::torch_function_mode_enabled(); }
 
 bool wants_grad(const at::Tensor& t) { return t.requires_grad(); }
+// .. a gradient now, or forward-mode derivatives
+bool wants_derivative(const at::Tensor& t) { return (c10::GradMode::is_enabled() && wants_grad(t)) || t._fw_grad(0).defined(); }
 
 bool as_int(PyObject* o, int64_t* out) {
     if (!PyLong_Check(o)) return false;
@@ -390,7 +392,7 @@ PyObject* quantizes(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     const at::Tensor* t[2];
     for (int i = 0; i < 2; ++i) {
         t[i] = gpu_tensor(args[i]);
-        if (!t[i] || (c10::GradMode::is_enabled() && wants_grad(*t[i])) || t[i]->_fw_grad(0).defined()) Py_RETURN_FALSE;
+        if (!t[i] || wants_derivative(*t[i])) Py_RETURN_FALSE;
     }
     const at::Tensor &k = *t[0], &v = *t[1];
     if (k.dim() != 4 || v.sizes() != k.sizes() || v.device() != k.device() || v.scalar_type() != k.scalar_type() ||
@@ -429,7 +431,7 @@ bool read_pool(PyObject* o, Pool* p) {
     p->v = gpu_tensor(PyTuple_GET_ITEM(o, 1));
     if (!p->k || !p->v || p->k->dim() != 4 || p->v->sizes() != p->k->sizes() || p->v->scalar_type() != p->k->scalar_type() ||
         p->v->device() != p->k->device() || !p->k->is_contiguous() || !p->v->is_contiguous() ||
-        (c10::GradMode::is_enabled() && (wants_grad(*p->k) || wants_grad(*p->v))))
+        wants_derivative(*p->k) || wants_derivative(*p->v))
         return false;
     const bool fp8 = p->k->scalar_type() == at::kFloat8_e4m3fn;
     p->code = fp8 ? FSTA_FP8 : half_code(p->k->scalar_type());
@@ -481,7 +483,7 @@ bool read_batch(const Pool& pool, PyObject* table, PyObject* lens, PyObject* sta
 const at::Tensor* read_rows(PyObject* o, const Pool& pool) {
     const at::Tensor* t = gpu_tensor(o);
     if (!t || t->dim() != 3 || t->numel() == 0 || t->size(0) > INT32_MAX || t->size(2) != pool.head_dim || t->stride(2) != 1 ||
-        t->device() != pool.k->device() || (c10::GradMode::is_enabled() && wants_grad(*t)))
+        t->device() != pool.k->device() || wants_derivative(*t))
         return nullptr;
     const int code = half_code(t->scalar_type());
     return code >= 0 && (pool.code == FSTA_FP8 || pool.code == code) ? t : nullptr;

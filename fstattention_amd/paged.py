@@ -16,6 +16,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from . import attention as _attention
@@ -53,6 +54,13 @@ def paged_kv_cache(num_pages: int, kv_heads: int, page_size: int, head_dim: int,
     return PagedKV(k, v, *(torch.full(shape[:3], 127, dtype=torch.uint8, device=device) for _ in range(2)))
 
 
+def _refuse_derivatives(name: str, t: torch.Tensor):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: the paged cache's operators have no backward pass")
+    if forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} carries a tangent: the paged cache's operators have no forward-mode derivative")
+
+
 def _check_cache(cache: PagedKV):
     """(num_pages, kv_heads, page_size, head_dim, dtype code, exponent pointers)"""
     k, v = cache.k, cache.v
@@ -64,8 +72,8 @@ def _check_cache(cache: PagedKV):
         raise ValueError("a paged cache lives on the GPU (no CPU fallback)")
     if not (k.is_contiguous() and v.is_contiguous()):
         raise ValueError("the cache's k and v must be contiguous")
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
-        raise ValueError("the cache's k or v requires a gradient: the paged cache's operators have no backward pass")
+    _refuse_derivatives("the cache's k", k)
+    _refuse_derivatives("the cache's v", v)
     exponents = (cache.k_exponent, cache.v_exponent)
     if k.dtype == torch.float8_e4m3fn:
         for e in exponents:
@@ -96,8 +104,7 @@ def _check_rows(t: torch.Tensor, name: str, cache: PagedKV):
         raise ValueError(f"{name} must be float16 or bfloat16, and of the cache's dtype unless that is 8 bits")
     if t.device != cache.k.device:
         raise ValueError("all tensors must live on the same device")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires a gradient: the paged cache's operators have no backward pass")
+    _refuse_derivatives(name, t)
     strides = [t.stride(d) if t.shape[d] > 1 else 0 for d in (0, 1)]
     if t.numel() and (t.stride(2) != 1 or any(s % 8 for s in strides) or t.data_ptr() % 16):
         raise ValueError(f"{name}'s rows must be contiguous and 16-byte aligned (strides that are multiples of 8)")

@@ -100,3 +100,20 @@ def test_a_cache_that_requires_a_gradient_is_refused(which):
             call()
         with torch.no_grad():
             call()
+
+
+def test_tangents_are_refused():
+    """Forward-mode derivatives of new rows or of the cache: dropped without a word otherwise."""
+    from torch.autograd import forward_ad
+    cache, tab, lens, starts, q, k = _small_call()
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t.clone(), torch.ones_like(t))
+        learned = cache._replace(v=dual(cache.v))
+        calls = (lambda: fsta.paged_attention(dual(q), cache, tab, lens, starts, 0.1), lambda: fsta.write_paged_kv(cache, dual(k), k, tab, lens, starts),
+                 lambda: fsta.write_paged_kv(cache, k, dual(k), tab, lens, starts), lambda: fsta.paged_attention(q, learned, tab, lens, starts, 0.1),
+                 lambda: fsta.write_paged_kv(learned, k, k, tab, lens, starts), lambda: fsta.read_paged_kv(learned, tab, lens, 20))
+        for call in calls:
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        fsta.write_paged_kv(cache, k, k, tab, lens, starts)
+        assert fsta.paged_attention(q, cache, tab, lens, starts, 0.1).shape == q.shape
