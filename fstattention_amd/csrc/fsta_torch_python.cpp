@@ -420,7 +420,7 @@ PyObject* setup(PyObject*, PyObject* args) {
 int half_code(at::ScalarType t) { return t == at::kHalf ? FSTA_F16 : t == at::kBFloat16 ? FSTA_BF16 : -1; }
 
 struct Pool {      // paged.PagedKV
-    const at::Tensor *k, *v;
+    const at::Tensor *k, *v, *exps[2];      // exps: null but for 8-bit rows
     uint8_t *k_exp, *v_exp;
     int32_t pages, heads, page_size, head_dim, code;
 };
@@ -436,6 +436,7 @@ bool read_pool(PyObject* o, Pool* p) {
     const bool fp8 = p->k->scalar_type() == at::kFloat8_e4m3fn;
     p->code = fp8 ? FSTA_FP8 : half_code(p->k->scalar_type());
     uint8_t* exps[2] = {nullptr, nullptr};
+    p->exps[0] = p->exps[1] = nullptr;
     for (int i = 0; i < 2; ++i) {
         PyObject* item = PyTuple_GET_ITEM(o, 2 + i);
         if (fp8 != (item != Py_None)) return false;
@@ -443,6 +444,7 @@ bool read_pool(PyObject* o, Pool* p) {
         const at::Tensor* e = gpu_tensor(item);
         if (!e || e->scalar_type() != at::kByte || e->sizes() != p->k->sizes().slice(0, 3) || !e->is_contiguous() || e->device() != p->k->device())
             return false;
+        p->exps[i] = e;
         exps[i] = static_cast<uint8_t*>(e->data_ptr());
     }
     p->k_exp = exps[0];
@@ -504,6 +506,9 @@ PyObject* paged_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
                              (int32_t)k->size(0), pool.pages, pool.page_size, pool.heads, pool.head_dim, half_code(k->scalar_type()),
                              pool.code, on.stream) != FSTA_OK)
             return not_implemented();
+        // autograd is told, as by torch's own operations in place (inference tensors have no version counter)
+        for (const at::Tensor* t : {pool.k, pool.v, pool.exps[0], pool.exps[1]})
+            if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
     } catch (const std::exception&) {
         return not_implemented();
     }

@@ -17,6 +17,7 @@ from typing import NamedTuple, Optional
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from . import attention as _attention
@@ -130,6 +131,8 @@ def write_paged_kv(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, page_table:
         _lib.check(lib.fsta_paged_write(k.data_ptr(), v.data_ptr(), *k_strides, *v_strides, cache.k.data_ptr(), cache.v.data_ptr(),
                                         k_exp, v_exp, page_table.data_ptr(), kv_lens.data_ptr(), q_starts.data_ptr(), batch, width,
                                         k.shape[0], pages, page_size, heads, d, _HALF[k.dtype], code, _stream_ptr(cache.k.device)))
+    # autograd is told, as by torch's own operations in place (inference tensors have no version counter)
+    increment_version([t for t in cache if t is not None and not t.is_inference()])
 
 
 def read_paged_kv(cache: PagedKV, page_table: torch.Tensor, kv_lens: torch.Tensor, max_len: int,

@@ -117,3 +117,28 @@ def test_tangents_are_refused():
                 call()
         fsta.write_paged_kv(cache, k, k, tab, lens, starts)
         assert fsta.paged_attention(q, cache, tab, lens, starts, 0.1).shape == q.shape
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("plain_call", [True, False])
+def test_writing_moves_the_version_counters(plain_call, fp8, monkeypatch):
+    """Autograd notices that a tensor it has kept for a backward pass was written to; inference tensors have no counter."""
+    cache, tab, lens, starts, q, k = _small_call()
+    if not plain_call:
+        _without_plain_calls(monkeypatch)
+    if fp8:
+        cache = fsta.paged_kv_cache(*cache.k.shape, torch.float8_e4m3fn)
+    before = [t._version for t in cache if t is not None]
+    fsta.write_paged_kv(cache, k, k, tab, lens, starts)
+    assert [t._version for t in cache if t is not None] == [n + 1 for n in before]
+    if not fp8:
+        w = torch.ones_like(cache.k).requires_grad_()
+        kept = (w * cache.k).sum()
+        fsta.write_paged_kv(cache, k, k, tab, lens, starts)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            kept.backward()
+    with torch.inference_mode():
+        fresh = fsta.paged_kv_cache(*cache.k.shape, cache.k.dtype)
+        fsta.write_paged_kv(fresh, k, k, tab, lens, starts)
+    got, want = (fsta.read_paged_kv(c, tab, lens, 20)[0][0, :, 18:] for c in (fresh, cache))
+    assert torch.equal(got, want) and got.abs().amax() > 0
