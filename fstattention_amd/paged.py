@@ -230,7 +230,7 @@ def tree_mask_bits(parent: torch.Tensor, q_starts: Optional[torch.Tensor] = None
         raise ValueError("tree_mask_bits runs on the GPU only (no CPU fallback)")
     tokens = parent.shape[0]
     if q_starts is None:
-        q_starts = torch.tensor([0, tokens], dtype=torch.int32, device=parent.device)
+        q_starts = torch.arange(2, dtype=torch.int32, device=parent.device) * tokens      # (made there: a copy cannot be captured)
     if q_starts.dim() != 1 or q_starts.dtype != torch.int32 or q_starts.shape[0] < 2 or q_starts.device != parent.device:
         raise ValueError("q_starts must be int32 [batch + 1] on parent's device, of at least one sequence")
     max_nodes = tokens if max_nodes is None else max_nodes

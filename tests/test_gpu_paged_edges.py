@@ -142,3 +142,20 @@ def test_writing_moves_the_version_counters(plain_call, fp8, monkeypatch):
         fsta.write_paged_kv(fresh, k, k, tab, lens, starts)
     got, want = (fsta.read_paged_kv(c, tab, lens, 20)[0][0, :, 18:] for c in (fresh, cache))
     assert torch.equal(got, want) and got.abs().amax() > 0
+
+
+def test_masks_of_one_tree_in_a_captured_call():
+    """Without ``q_starts`` the operator makes them itself, on the GPU: nothing comes from the host, so a capture takes it."""
+    parent = torch.tensor([-1, 0, 0, 1, 2, 2, 4, -1]).cuda()
+    want = fsta.tree_mask_bits(parent)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = fsta.tree_mask_bits(parent)
+    for shift in range(4):
+        parent.copy_(torch.tensor([-1, 0, 0, 1, 2, 2, 4, -1]).roll(shift))
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, fsta.tree_mask_bits(parent)), shift
+        assert shift > 0 or torch.equal(got, want)
