@@ -576,10 +576,10 @@ __device__ __forceinline__ int page_at(const PagedAttnParams& p, const_i32 table
 }
 
 // Transfers of a tile's keys and values (and exponents) from its pages to a ring slot, as wave `part` of PARTS.
-// WIDENED: an 8-bit tile that is copied into the 16-bit layout afterwards lies in LDS as it does in memory.  ONCE: past the caches.
+// WIDENED: an 8-bit tile that is copied into the 16-bit layout afterwards lies in LDS as it does in memory.
 constexpr int kRawBuffer = 0x00020000;        // buffer resource, word 3: raw 32-bit data
 
-template <int D, int PARTS, bool FP8, bool WIDENED, bool ONCE> struct Fetch {
+template <int D, int PARTS, bool FP8, bool WIDENED> struct Fetch {
     static constexpr int kRowBytes = FP8 ? D : 2 * D;             // a key's or a value's row in the cache
     static constexpr int kDma = 2 * kTileN * kRowBytes / 1024;    // transfers of 1 KiB
     static constexpr int kPer = kDma / PARTS;                     // of them this wave's
@@ -621,7 +621,9 @@ template <int D, int PARTS, bool FP8, bool WIDENED, bool ONCE> struct Fetch {
 
     // p0, p1: pages of the tile's 16-key halves; returns the halves that are on none.  A half's rows are a buffer of as many bytes
     // as there are rows: what a lane asks for behind its end the hardware answers with zeros, and no lane needs an address.
-    __device__ __forceinline__ uint32_t tile(const PagedAttnParams& p, int keys, int head, int first, int p0, int p1, unsigned char* dst, int lane) const {
+    // once (a bool, or one known to the compiler): nobody else reads these keys, past the caches.
+    template <typename Once>
+    __device__ __forceinline__ uint32_t tile(const PagedAttnParams& p, int keys, int head, int first, int p0, int p1, unsigned char* dst, int lane, Once once) const {
         typedef const void __attribute__((address_space(1))) * global_ptr;
         typedef void __attribute__((address_space(3))) * lds_ptr;
         const uint32_t page_mask = (1u << p.batch.page_shift) - 1u;
@@ -640,17 +642,23 @@ template <int D, int PARTS, bool FP8, bool WIDENED, bool ONCE> struct Fetch {
         const unsigned char* v_from = kOneSide ? side : v_side;
         const auto k0 = rows_at(side, kOneHalf ? half_of(0) : 0), k1 = kOneHalf ? k0 : rows_at(side, 1);
         const auto v0 = kOneSide ? k0 : rows_at(v_from, 0), v1 = kOneSide ? k1 : rows_at(v_from, 1);
-        static_for<kPer>([&](auto index) {
-            constexpr int j = decltype(index)::value, in_half = j % kRun;
-            constexpr bool v = !kOneSide && j >= kDma / 2;
-            constexpr int half = kOneHalf ? 0 : j % (kDma / 2) / kPerHalf;
-            const uint32_t off = v ? v_off : k_off ^ (in_half * turn);
-            lds_ptr to = (lds_ptr)(dst + (first_unit + j - in_half) * 1024);
-            if constexpr (v && half) __builtin_amdgcn_raw_ptr_buffer_load_lds(v1, to, 16, off, 0, in_half * 1024, ONCE ? 2 : 0);
-            else if constexpr (v) __builtin_amdgcn_raw_ptr_buffer_load_lds(v0, to, 16, off, 0, in_half * 1024, ONCE ? 2 : 0);
-            else if constexpr (half) __builtin_amdgcn_raw_ptr_buffer_load_lds(k1, to, 16, off, 0, in_half * 1024, ONCE ? 2 : 0);
-            else __builtin_amdgcn_raw_ptr_buffer_load_lds(k0, to, 16, off, 0, in_half * 1024, ONCE ? 2 : 0);
-        });
+        auto transfers = [&](auto policy) {
+            constexpr int kPolicy = decltype(policy)::value;
+            static_for<kPer>([&](auto index) {
+                constexpr int j = decltype(index)::value, in_half = j % kRun;
+                constexpr bool v = !kOneSide && j >= kDma / 2;
+                constexpr int half = kOneHalf ? 0 : j % (kDma / 2) / kPerHalf;
+                const uint32_t off = v ? v_off : k_off ^ (in_half * turn);
+                lds_ptr to = (lds_ptr)(dst + (first_unit + j - in_half) * 1024);
+                if constexpr (v && half) __builtin_amdgcn_raw_ptr_buffer_load_lds(v1, to, 16, off, 0, in_half * 1024, kPolicy);
+                else if constexpr (v) __builtin_amdgcn_raw_ptr_buffer_load_lds(v0, to, 16, off, 0, in_half * 1024, kPolicy);
+                else if constexpr (half) __builtin_amdgcn_raw_ptr_buffer_load_lds(k1, to, 16, off, 0, in_half * 1024, kPolicy);
+                else __builtin_amdgcn_raw_ptr_buffer_load_lds(k0, to, 16, off, 0, in_half * 1024, kPolicy);
+            });
+        };
+        if constexpr (!std::is_same_v<Once, bool>) transfers(std::integral_constant<int, Once::value ? 2 : 0>{});
+        else if (once) transfers(std::integral_constant<int, 2>{});
+        else transfers(std::integral_constant<int, 0>{});
 #endif
         if constexpr (FP8) {                  // exponents of the 32 keys, then of the 32 values, four to a lane
             const int l = lane & 15, g = (l >> 2) & 1;

@@ -139,7 +139,7 @@ template <int D, int R, int S, bool FP8> struct Shape {
     static constexpr bool kWiden = FP8 && R > 2;
     static constexpr int kStep = R >= 4 && !FP8 ? 2 : 1;                   // tiles worked on between barriers
     static constexpr int kStages = R == 8 ? 9 : R == 4 ? 5 : FP8 && R == 2 ? 4 : 2;
-    using Raw = Fetch<D, R, FP8, kWiden, false>;
+    using Raw = Fetch<D, R, FP8, kWiden>;
     static constexpr int kWideBytes = 2 * kTileN * D * 2;
     static constexpr int kPowerBytes = kTileN * 4;                          // behind a widened tile: its keys' powers of two
     static constexpr int kShareBytes = kStages * Raw::kBytes + (kWiden ? kWideBytes + kPowerBytes : 0);
@@ -148,12 +148,13 @@ template <int D, int R, int S, bool FP8> struct Shape {
     static constexpr size_t kLds = (size_t)S * kShareBytes > kJoin ? (size_t)S * kShareBytes : kJoin;
 };
 
-// SPLIT: weights go to the matrix cores as pairs of bfloat16, hi + lo.  ONCE: every key is read by one workgroup only, past the
-// caches.
+// SPLIT: weights go to the matrix cores as pairs of bfloat16, hi + lo.  ONCE: no sequence has more rows than a tile, so nobody else
+// reads a workgroup's keys.  Up to 64 rows that is asked for every sequence on its own, whatever the host knows; asked at every
+// tile of 128 rows and more it costs 1 to 4 % (4096 tokens after 16384 1257 -> 1289 us, head_dim 64 460 -> 477).
 template <bool BF16, int D, int R, int S, bool FP8, bool SPLIT, bool ONCE>
 __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnParams p) {
     using SH = Shape<D, R, S, FP8>;
-    using F = Fetch<D, R, FP8, SH::kWiden, ONCE>;
+    using F = typename SH::Raw;
     using G = RowGroup<BF16, D, FP8, FP8 && !SH::kWiden, SPLIT>;
     constexpr int kStages = SH::kStages, kStep = SH::kStep, kDTiles = G::kDTiles;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -195,6 +196,10 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
     // ---- ring of tiles ----------------------------------------------------------------------------------------------------
     unsigned char* ring = smem + share * SH::kShareBytes;
     const F fetch(p, head, group_of_rows, lane);
+    const auto once = [&] {
+        if constexpr (R < 4) return s.fresh * p.group <= p.tile_rows;
+        else return std::bool_constant<ONCE>{};
+    }();
     const const_i32 table = table_of(p, at.seq);
     int next_p0 = 0, next_p1 = 0;             // pages of the share's tile that is fetched next
     auto look_up = [&](int i) {
@@ -208,7 +213,7 @@ __global__ __launch_bounds__(R * S * 64, 2) void paged_attn_kernel(PagedAttnPara
     auto issue = [&](int i) {                 // the share's i-th tile into slot i % kStages
         const int slot = (int)((uint32_t)i % kStages), p0 = next_p0, p1 = next_p1;
         look_up(i + 1);
-        const uint32_t bad = fetch.tile(p, s.keys, head, (tile0 + share + i * S) * kTileN, p0, p1, ring + slot * F::kBytes, lane);
+        const uint32_t bad = fetch.tile(p, s.keys, head, (tile0 + share + i * S) * kTileN, p0, p1, ring + slot * F::kBytes, lane, once);
         bad_halves = (bad_halves & ~(3u << (2 * slot))) | (bad << (2 * slot));
     };
     look_up(0);
@@ -506,20 +511,24 @@ Costs costs_of(int tile_rows) { return tile_rows >= 128 ? Costs{(tile_rows == 25
 
 struct Sizes {
     int tile_rows;
-    int64_t most_rows;          // of a sequence, as far as the host knows
+    int64_t most_rows;          // of a sequence, as far as the host can guess
+    int64_t sure_rows;          // .. and as it knows
     int64_t row_tiles;          // at most, over the batch
     int64_t items, parts;       // of all heads: parts
     int64_t cut_tiles;          // a head's
     int64_t floats;             // of workspace
     int run_units[3], least_tiles;
 };
-int64_t most_rows_of(int32_t tokens, int32_t max_q_len, int group) {
-    return (int64_t)(max_q_len > 0 && max_q_len < tokens ? max_q_len : tokens) * group;
+// Most rows of a sequence: by max_q_len, else as if every sequence had new tokens, where that can be
+int64_t most_rows_of(int32_t batch, int32_t tokens, int32_t max_q_len, int group) {
+    const int32_t most = max_q_len > 0 ? max_q_len : tokens >= batch ? tokens - batch + 1 : tokens;
+    return (int64_t)std::min(most, tokens) * group;
 }
 Sizes sizes_of(int tile_rows, int32_t batch, int32_t tokens, int32_t max_q_len, int32_t heads, int32_t kv_heads, int32_t head_dim) {
     Sizes z;
     const int group = heads / kv_heads;
-    z.most_rows = most_rows_of(tokens, max_q_len, group);
+    z.most_rows = most_rows_of(batch, tokens, max_q_len, group);
+    z.sure_rows = max_q_len > 0 ? z.most_rows : (int64_t)tokens * group;
     z.tile_rows = tile_rows;
     z.row_tiles = ((int64_t)tokens * group + (int64_t)(batch < tokens ? batch : tokens) * (z.tile_rows - 1)) / z.tile_rows;
     for (int i = 0; i < 3; ++i) z.run_units[i] = z.tile_rows == 256 ? kCus / 2 << i : (i + 1) * kCus;
@@ -551,10 +560,10 @@ int launch_units_of(const PagedAttnParams& p, int64_t units, hipStream_t stream)
     return FSTA_OK;
 }
 
-// (a sequence whose rows fit one tile has its keys read once)
 template <bool BF16, int D, int R, int S, bool FP8> int launch_units(const PagedAttnParams& p, int64_t units, const Sizes& z, hipStream_t stream) {
-    return z.most_rows <= z.tile_rows ? launch_units_of<BF16, D, R, S, FP8, true>(p, units, stream)
-                                      : launch_units_of<BF16, D, R, S, FP8, false>(p, units, stream);
+    if constexpr (R >= 4)
+        if (z.sure_rows <= z.tile_rows) return launch_units_of<BF16, D, R, S, FP8, true>(p, units, stream);
+    return launch_units_of<BF16, D, R, S, FP8, false>(p, units, stream);
 }
 
 template <bool BF16, int D, int ROWS> int launch_join(const PagedAttnParams& p, const Sizes& z, hipStream_t stream) {
@@ -604,7 +613,7 @@ extern "C" size_t fsta_paged_attention_workspace_bytes(int32_t batch, int32_t to
     if (batch <= 0 || tokens <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
     // (whichever of its answers rows_of_tile gives)
     const int group = heads / kv_heads;
-    const int rate = rows_for_rate(most_rows_of(tokens, max_q_len, group), (int64_t)tokens * group, kv_heads, head_dim, cache_dtype == FSTA_FP8);
+    const int rate = rows_for_rate(most_rows_of(batch, tokens, max_q_len, group), (int64_t)tokens * group, kv_heads, head_dim, cache_dtype == FSTA_FP8);
     int64_t floats = 0;
     for (const int rows : {32, 64, rate})
         if (rows <= rate) floats = std::max(floats, sizes_of(rows, batch, tokens, max_q_len, heads, kv_heads, head_dim).floats);
@@ -638,7 +647,7 @@ extern "C" int fsta_paged_attention(const void* q, int64_t q_token_stride, int64
     if (misaligned(k_exponent, 4) || misaligned(v_exponent, 4) || misaligned(lse, 4) || misaligned(tree_bits, 4))
         return fail(FSTA_EINVAL, "%s: exponents, lse and tree_bits must be 4-byte aligned", who);
     const int64_t all_rows = (int64_t)tokens * (heads / kv_heads);
-    const int rate = rows_for_rate(most_rows_of(tokens, max_q_len, heads / kv_heads), all_rows, kv_heads, head_dim, cache_dtype == FSTA_FP8);
+    const int rate = rows_for_rate(most_rows_of(batch, tokens, max_q_len, heads / kv_heads), all_rows, kv_heads, head_dim, cache_dtype == FSTA_FP8);
     const Sizes z = sizes_of(rows_of_tile(rate, batch < tokens ? batch : tokens, all_rows, (int64_t)width * page_size, kv_heads), batch, tokens, max_q_len, heads, kv_heads, head_dim);
     const size_t need = (size_t)z.floats * sizeof(float);
     if (!workspace || workspace_bytes < need) return fail(FSTA_EINVAL, "%s: needs %zu bytes of workspace, got %zu", who, need, workspace_bytes);

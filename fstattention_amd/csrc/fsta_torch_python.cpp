@@ -562,7 +562,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         words = (int32_t)THPVariable_Unpack(args[7]).size(1);
         mask = FSTA_PAGED_TREE;
     }
-    int64_t most = std::max(tokens - b.batch + 1, 1);
+    int64_t most = 0;
     if (args[8] != Py_None && (!as_int(args[8], &most) || most < 0 || most > INT32_MAX)) return not_implemented();
     try {
         const OnStream on(*q);

@@ -170,8 +170,10 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, k
     tree.  With ``causal`` a token sees the positions up to its own; with ``tree_bits`` (:func:`tree_mask_bits`: int32
     ``[T, words]``) all positions in front of the new tokens and, among those, the ones of its row of bits; with neither, every
     position of its sequence.  ``return_lse``: also the base-2 log-sum-exp ``[T, H]`` float32, e.g. to join the result with
-    another part's by :func:`merge_attention_states`.  ``max_q_len``: the most new tokens a sequence has, if the caller knows
-    (it steers the choice of kernel, not the result).
+    another part's by :func:`merge_attention_states`.  ``max_q_len``: the most new tokens a sequence has, if the caller knows.  It
+    steers the choice of kernel, and by that the rounding of the weights (below), nothing else; without it every sequence is taken
+    to bring a token, unless there are fewer tokens than sequences: a batch of mostly empty slots is faster with it (256 slots,
+    260 tokens of one behind 8000 keys: 73 us instead of 111).
 
     Tokens that see nothing get zeros (and ``-inf``); rows of tokens that ``q_starts`` gives to no sequence are not written.
     Sums and softmax statistics are float32.  Where a workgroup takes up to 64 rows (tokens times query heads per K/V head: short
@@ -199,8 +201,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, k
     if tokens and (batch == 0 or width == 0 or pages == 0):
         raise ValueError(f"{tokens} tokens need sequences and a cache with pages")
     lib = _lib.load()
-    if max_q_len is None:
-        max_q_len = max(tokens - batch + 1, 1)
+    max_q_len = max_q_len or 0
     o = torch.empty((tokens, heads, d), dtype=q.dtype, device=q.device)
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
     need = lib.fsta_paged_attention_workspace_bytes(batch, tokens, max_q_len, heads, heads_kv, d, code)

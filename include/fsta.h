@@ -491,8 +491,9 @@ int fsta_paged_read(const void* k_cache, const void* v_cache, const uint8_t* k_e
  * token that sees nothing has o = 0 and lse = -inf; rows of tokens of no sequence are not written.
  * FSTA_PAGED_TREE: the token sees all positions in front of its sequence's new tokens, and the j-th
  * new one where bit j % 32 of word j / 32 of its row of tree_bits [tokens, tree_words] is set (bits
- * past the row are 0).  sm_scale > 0.  max_q_len: the most new tokens a sequence has, or 0; it
- * steers the choice of kernel only.  The workspace (16-byte aligned, always needed) holds the parts
+ * past the row are 0).  sm_scale > 0.  max_q_len: the most new tokens a sequence has, or 0 (then
+ * every sequence is taken to have one, unless tokens < batch).  It steers the choice of kernel, and
+ * by that whether bfloat16 weights are rounded once or kept as pairs, nothing else.  The workspace (16-byte aligned, always needed) holds the parts
  * of sequences whose keys are dealt to several workgroups; it is free again when the work queued on
  * `stream` has run.  tokens * heads < 2^30, batch <= 65536.
  */

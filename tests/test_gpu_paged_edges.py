@@ -159,3 +159,16 @@ def test_masks_of_one_tree_in_a_captured_call():
         torch.cuda.synchronize()
         assert torch.equal(got, fsta.tree_mask_bits(parent)), shift
         assert shift > 0 or torch.equal(got, want)
+
+
+@pytest.mark.parametrize("tokens,most", [(200, None), (200, 0), (300, None), (300, 300), (1, None), (40, 3)])
+def test_slots_without_new_tokens(tokens, most):
+    """A server's fixed slots, one of which brings a chunk, without a word about its length (or with a wrong one)."""
+    new, keys = [0] * 256, [16] * 256
+    new[7], keys[7] = tokens, 500 + tokens
+    tab, lens, starts, pages = make_batch(new, keys, 16, 81)
+    cache = make_cache(pages, 2, 16, 64, torch.bfloat16, 82)
+    q = torch.randn((tokens, 8, 64), generator=torch.Generator().manual_seed(83)).bfloat16()
+    out, lse = fsta.paged_attention(q.cuda(), cuda(cache), tab.cuda(), lens.cuda(), starts.cuda(), 0.125, max_q_len=most, return_lse=True)
+    want, want_lse, size = reference(q, cache, tab, lens, starts, 0.125, "causal")
+    check(out, lse, want, want_lse, size, keys, torch.bfloat16, tokens * 4, 5.0)
