@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import fstattention_amd as fsta
-from test_gpu_paged import check, cuda, make_batch, make_cache, reference
+from test_gpu_paged import check, cuda, make_batch, make_cache, reference, values
 
 pytestmark = pytest.mark.gpu
 
@@ -172,3 +172,28 @@ def test_slots_without_new_tokens(tokens, most):
     out, lse = fsta.paged_attention(q.cuda(), cuda(cache), tab.cuda(), lens.cuda(), starts.cuda(), 0.125, max_q_len=most, return_lse=True)
     want, want_lse, size = reference(q, cache, tab, lens, starts, 0.125, "causal")
     check(out, lse, want, want_lse, size, keys, torch.bfloat16, tokens * 4, 5.0)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("new,columns", [([1, 1], 0), ([15, 9], 0), ([500, 70], 1000)])
+def test_values_as_large_as_documented(new, columns, fp8):
+    """Values up to 1e24, whose weights grow along the keys: the float32 sums in front of the division by the weights' sum hold them."""
+    keys = [700, 333]
+    tab, lens, starts, pages = _wide_batch(new, keys, columns, 91)
+    cache = make_cache(pages, 2, 16, 128, torch.bfloat16, 92, fp8)
+    if fp8:
+        cache.v_exponent.copy_((cache.v_exponent.int() + 77).to(torch.uint8))
+    else:
+        cache.v.mul_(2.0 ** 77)
+    # (scores of the later keys are greater by up to 7: the running maximum is raised from 8 powers of two on)
+    q = (torch.randn((sum(new), 8, 128), generator=torch.Generator().manual_seed(93)) * 0.5).bfloat16()
+    for b in range(2):
+        for p in range(keys[b]):
+            place = (int(tab[b, p // 16]), slice(None), p % 16)
+            if not fp8:
+                cache.k[place] = cache.k[place] * (0.1 + 2.0 * p / keys[b])
+    assert values(cache.v, cache.v_exponent).abs().max() < 1e24
+    out, lse = fsta.paged_attention(q.cuda(), cuda(cache), tab.cuda(), lens.cuda(), starts.cuda(), 128 ** -0.5, max_q_len=max(new), return_lse=True)
+    want, want_lse, size = reference(q, cache, tab, lens, starts, 128 ** -0.5, "causal")
+    assert want.abs().max() > 2.0 ** 70 and out.isfinite().all()
+    check(out, lse, want, want_lse, size, keys, torch.bfloat16, max(new) * 4, 0.0)
