@@ -8,8 +8,9 @@
 // Keys and values come page by page straight into an LDS ring (global -> LDS transfers of 1 KiB) through a buffer resource per 16
 // rows; rows past the sequence's end read as zeros, pages outside the cache from a row of zeros, so that what lies in unused rows of
 // a page can not turn a weight of zero into a NaN.
-// What bounds it: few rows, reading keys once (64 sequences of 16 to 8192 keys, 8 K/V heads of 128, 251 MB: 50.4 us with
-// the join, 5.0 TB/s; 8-bit, 16 of 8192 to 32768 keys, 607 MB: 114 of 117 us, 5.3 TB/s); many rows, the matrix
+// 8-bit rows are widened to the type of Q and V to bfloat16; where Q is float16 the keys' powers of two go to the scores.
+// What bounds it: few rows, reading keys once (64 sequences of 16 to 8192 keys, 8 K/V heads of 128, 251 MB: 50.8 us with
+// the join, 4.9 TB/s; 8-bit, 16 of 8192 to 32768 keys, 607 MB: 119 us with the join, 5.1 TB/s); many rows, the matrix
 // cores, whose products wait for the exponentials in between (4096 tokens after 16384, 32 heads: 1.24e12 operations in 1180 us, 1050
 // TFLOP/s, where a large matrix product reaches 1200 to 1300); one short sequence, one launch and four round trips (9.8 us).
 #include "fsta_paged_attention.h"
@@ -28,9 +29,13 @@ constexpr int kDecodeLeast = 16, kChunkLeast = 8;          // tiles of a run, at
 // The cut is a function of the lengths alone; every wave works it out for itself from the arrays (64 sequences at a time, a lane
 // each: one round trip and a few prefix sums), so that no launch has to come before this one and the host never waits for a length.
 // Of four cuts (none, and runs for 1, 2 or 3 rounds' worth of units) the one is taken whose units would be done first: rounds of
-// workgroups times what a unit lasts, its start included, and joining the runs.  (Measured with every cut forced: 32 sequences of
-// 4096 keys, 8 K/V heads, whole 88.7 us, in runs for two rounds 94; 40 sequences 132 whole, 121; 128 tiles of 128 rows 45 us whole and
-// 38 in two runs; 256 of them 51 whole and 66 in two.)
+// workgroups times what a unit lasts, its start included, and joining the runs.  (Measured with every cut forced, us whole / for one,
+// two, three rounds, 8 K/V heads of 128, a token each: 64 sequences of 16 to 8192 keys 153 / 55 / 57 / 51, 32 of 4096 keys 96 / 97 / 90 /
+// 98, 40 of them 111 / 112 / 133 / 114, one of 16384 287 / 22 / 21 / 21; 2 sequences of 256 tokens on 1256 to 1500 keys, 32 heads: 45 /
+// 35 / 38 / 50, 4 of them 47 / 61 / 61 / 63.  The estimate takes three, whole, three, one; two, whole: up to a tenth from the best.)
+// From 65 sequences on, whose lengths a wave does not hold all at once, runs are for two rounds,
+// in which few keys stay whole: 70 sequences of 16 to 8192 keys 178 / 102 / 95 / 86, 128 of 2048 to 4096 266 / 268 / 268 / 282, 256 of 16 to
+// 2048 103 / 113 / 106 / 101.
 struct Cut {
     uint32_t longest;              // tiles of keys in a run
     // (a batch has fewer than 2^30 rows; tile_rows is a power of two)
@@ -480,8 +485,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
 // has one unit misses the longer ring, 32 sequences of 4096 keys 92.3 and 97.2.  Of 64 or 8 bits two of them fit, and they are faster:
 // 40.0 and 45.6 for 32 sequences of 500 to 8192 keys of 64.)  From 128 rows on every wave has rows of its own.  256 rows where there are two rounds of such
 // tiles (4096 after 16384: 1221 -> 1189 us; with one round the last tiles of a causal chunk are waited for: 2048 tokens 63 -> 71 us).
-// 8-bit tiles are widened by all waves together, behind a barrier more, which two workgroups per CU hide and one does not (348 ->
-// 384 us); head_dim 64 fits three workgroups of 128 rows on a CU.
+// 8-bit tiles are widened by all waves together, behind a barrier more, which two workgroups per CU hide and one does not (2048
+// tokens on 8192 keys, 32 query on 8 K/V heads, 348 -> 384 us; 343 now, with float16 queries and pairs of weights 461); head_dim 64 fits three workgroups of 128 rows on a CU.
 int rows_for_rate(int64_t most_rows, int64_t all_rows, int32_t kv_heads, int32_t head_dim, bool fp8) {
     if (most_rows <= 32 && (head_dim == 64 || fp8)) return 32;
     if (most_rows <= 64) return 64;
@@ -500,7 +505,9 @@ int rows_of_tile(int rate, int64_t seqs, int64_t all_rows, int64_t most_keys, in
     return rate;
 }
 
-// What choose weighs, in the time a workgroup takes for a tile of keys (0.66 us alone on its CU with up to 64 rows; with 128 rows
+// What choose weighs (slots: workgroups at a time, one per CU up to 64 rows, as tiles of 32 rows of 128 in 16 bits have it; two of 64 rows
+// or of smaller tiles fit, and three of 128 rows at head_dim 64, which the estimate does not know), in the time a workgroup takes
+// for a tile of keys (0.66 us alone on its CU with up to 64 rows; with 128 rows
 // 0.9 us alone, and two share a CU at 1.05 us): a unit's start and end 4 to 5 us, with few rows
 // half hidden under another's keys (2 tiles; 7: 16 sequences of 4 tokens 47.5 us instead of 45.7), the join's launch 5 us; with many rows it is the
 // results of the runs, which go to memory and back, 64 KB a unit (4 sequences of 256 tokens, 32 K/V heads, 1256 to 1500 keys: cut

@@ -3,8 +3,9 @@
 //
 // Memory-bound, element-wise.  An 8-bit row x of head_dim values is kept as bytes b and one exponent byte E: x ~ b 2^(E - 127)
 // with the smallest power under which max |x| <= 448.  A power of two and not max |x| / 448: e4m3 is a floating-point format,
-// so where in a binade its largest value falls costs nothing but the last subnormal bit, and b 2^(E - 127) is exact in the
-// 16-bit type that it is widened to, by the conversion instruction itself (it takes a scale).
+// so where in a binade its largest value falls costs nothing but the last subnormal bit, and b 2^(E - 127) is exact in bfloat16, to
+// which the conversion instruction itself widens it (it takes a scale).  float16 holds every b, but not every b 2^(E - 127): above
+// 65504 it is infinite, below 2^-14 it loses bits (rows read as float16; the attention keeps the powers apart).
 #include "fsta_paged.h"
 
 namespace fsta {

@@ -9,7 +9,8 @@ several sequences keeps theirs in pages.  Three arrays describe a batch, on the 
 * ``q_starts`` int32 ``[B + 1]``, ascending: tokens ``q_starts[b]`` to ``q_starts[b + 1] - 1`` of the packed tensors
   (``q [T, H, D]``, ``k, v [T, Hkv, D]``) are sequence ``b``'s new ones, at its last positions.
 
-The compute is ``libfsta.so``'s (``include/fsta.h``), on torch's current stream; there is no CPU fallback.
+The compute is ``libfsta.so``'s (``include/fsta.h``), on torch's current stream; there is no CPU fallback.  No operator has a
+derivative: rows or caches that require a gradient, or carry a tangent, are refused.
 """
 from __future__ import annotations
 
@@ -118,7 +119,8 @@ def write_paged_kv(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, page_table:
     fused projection) to their places in the pages; tokens without a place are left out.
 
     An 8-bit cache gets, per row, the smallest exponent ``e`` with ``max |x| <= 448 * 2**e`` over the row's finite values
-    (kept within [-110, 120]; 0 for a row of zeros) and bytes rounded to nearest even; infinities and NaNs become NaN."""
+    (kept within [-110, 120]; 0 for a row of zeros) and bytes rounded to nearest even; infinities and NaNs become NaN.  The version
+    counters of the tensors written to move, as by an operation in place of torch's own."""
     if _calls().paged_write(cache, k, v, page_table, kv_lens, q_starts) is None:
         return
     pages, heads, page_size, d, code, k_exp, v_exp = _check_cache(cache)
@@ -138,7 +140,8 @@ def write_paged_kv(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, page_table:
 def read_paged_kv(cache: PagedKV, page_table: torch.Tensor, kv_lens: torch.Tensor, max_len: int,
                   dtype: Optional[torch.dtype] = None):
     """The pages of a batch as dense ``k, v [B, Hkv, max_len, D]`` (the layout ``fst_attention`` takes), zeros where a sequence
-    has no position.  ``dtype``: the cache's, or float16 / bfloat16 for an 8-bit one (bfloat16 if not given)."""
+    has no position.  ``dtype``: the cache's, or float16 / bfloat16 for an 8-bit one (bfloat16 if not given, which holds its values
+    exactly; float16 rounds them, beyond 65504 to infinities)."""
     out = _calls().paged_read(cache, page_table, kv_lens, max_len, dtype)
     if out is not NotImplemented:
         return out
@@ -176,9 +179,11 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, k
     260 tokens of one behind 8000 keys: 73 us instead of 111).
 
     Tokens that see nothing get zeros (and ``-inf``); rows of tokens that ``q_starts`` gives to no sequence are not written.
-    Sums and softmax statistics are float32.  Where a workgroup takes up to 64 rows (tokens times query heads per K/V head: short
-    chunks, and small calls), bfloat16 weights go to the matrix cores as pairs (2^-16 relative at most), elsewhere rounded once
-    (2^-8 at most, as the output itself)."""
+    Sums and softmax statistics are float32 (finite values of up to 1e24 in magnitude do not leave it).  The weights' rounding: where
+    a workgroup takes up to 64 rows (tokens times query heads per K/V head: short chunks, and small calls; the longest chunk of a
+    batch decides for all), bfloat16 weights go to the matrix cores as pairs (2^-16 relative at most), elsewhere rounded once (2^-8
+    at most, as the output itself).  float16 weights over a 16-bit cache are rounded once everywhere (2^-11, those below 2^-14 of the
+    running maximum's to 2^-25 of it), over an 8-bit cache they are pairs of bfloat16."""
     out = _calls().paged_attention(q, cache, page_table, kv_lens, q_starts, sm_scale, causal, tree_bits, max_q_len, return_lse)
     if out is not NotImplemented:
         return out
@@ -221,7 +226,7 @@ def tree_mask_bits(parent: torch.Tensor, q_starts: Optional[torch.Tensor] = None
 
     ``parent`` int64 ``[T]``: every node's parent by its number within its tree, smaller than its own, -1 for a root (as in
     ``lineage_from_parents``; anything else counts as a root).  ``q_starts`` int32 ``[B + 1]``: tree ``b``'s nodes (one tree if
-    not given).  ``max_nodes``: the most nodes a tree has (``T`` if not given); bits beyond it are dropped."""
+    not given).  ``max_nodes``: the most nodes a tree has (``T`` if not given; below 2^31); bits beyond it are dropped."""
     bits = _calls().tree_bits(parent, q_starts, max_nodes)
     if bits is not NotImplemented:
         return bits

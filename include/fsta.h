@@ -496,6 +496,9 @@ int fsta_paged_read(const void* k_cache, const void* v_cache, const uint8_t* k_e
  * by that whether bfloat16 weights are rounded once or kept as pairs, nothing else.  The workspace (16-byte aligned, always needed) holds the parts
  * of sequences whose keys are dealt to several workgroups; it is free again when the work queued on
  * `stream` has run.  tokens * heads < 2^30, batch <= 65536.
+ * An 8-bit row's value is taken as it stands, also where float16 queries meet rows that float16 could
+ * not hold.  The result is right while finite values are at most 1e24 in magnitude: weights times
+ * values are summed in float32 before they are divided by the sum of the weights, which may be large.
  */
 size_t fsta_paged_attention_workspace_bytes(int32_t batch, int32_t tokens, int32_t max_q_len,
                                             int32_t heads, int32_t kv_heads, int32_t head_dim,
