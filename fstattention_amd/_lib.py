@@ -82,6 +82,16 @@ SIGNATURES = {
     "fsta_paged_attention": (c_int, [c_void_p] + [c_int64] * 2 + [c_void_p] * 8 + [c_int32] + [c_void_p] * 2 + [c_int32] * 12 +
                              [c_float, c_void_p, c_size_t, c_void_p]),
     "fsta_tree_bits": (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
+    "fsta_verify_workspace_bytes": (c_size_t, [c_int32] * 5),
+    "fsta_verify_drafts": (c_int, [c_void_p, c_int64, c_int32] * 2 + [c_void_p] * 6 + [c_float] + [c_void_p] * 3 + [c_int32] * 4 +
+                           [c_void_p, c_size_t, c_void_p]),
+    "fsta_compact_paged_kv": (c_int, [c_void_p] + [c_int32] * 3 + [c_void_p, c_int32] + [c_void_p] * 4 + [c_int32] * 2 + [c_void_p] * 2),
+    "fsta_copy_pages": (c_int, [c_void_p] * 2 + [c_int32] * 4 + [c_void_p] * 2 + [c_int32, c_void_p]),
+    "fsta_fit_pages_workspace_bytes": (c_size_t, [c_int32] * 2),
+    "fsta_fit_pages": (c_int, [c_void_p] + [c_int32] * 3 + [c_void_p] * 3 + [c_int32] * 2 + [c_void_p] * 2 + [c_size_t, c_void_p]),
+    "fsta_fork_pages_workspace_bytes": (c_size_t, [c_int32] * 3),
+    "fsta_fork_pages": (c_int, [c_void_p] + [c_int32] * 3 + [c_void_p] * 3 + [c_int32] * 2 + [c_void_p] * 2 + [c_int32] + [c_void_p] * 2 +
+                        [c_size_t, c_void_p]),
     "fsta_probe_empty_launch": (c_int, [c_int32, c_int32, c_void_p]),
     "fsta_probe_hbm_read": (c_int, [c_void_p, c_size_t, c_int32, c_int32, c_void_p, c_void_p]),
     "fsta_quantize_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int32]),
@@ -90,6 +100,13 @@ SIGNATURES = {
     "fsta_merge_states": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
                                   c_int32, c_int32, c_void_p]),
 }
+
+
+class PagedPool(ctypes.Structure):
+    """fsta_paged_pool"""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_exponent", c_void_p), ("v_exponent", c_void_p),
+                ("kv_heads", c_int32), ("head_dim", c_int32), ("cache_dtype", c_int32), ("reserved", c_int32)]
+
 
 _lib = None
 

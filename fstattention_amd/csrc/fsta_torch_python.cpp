@@ -20,6 +20,8 @@
 
 #include <algorithm>
 #include <cstring>
+#include <limits>
+#include <vector>
 
 #include "../../include/fsta.h"
 #include "fsta_torch.h"
@@ -603,6 +605,214 @@ PyObject* tree_bits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
 }
 
+// ---- what happens between two passes of a model: drafts.py and pages.py judge and raise for all other calls --------------
+
+// A float tensor [nodes, vocabulary] whose rows are contiguous
+const at::Tensor* read_logits(PyObject* o) {
+    const at::Tensor* t = gpu_tensor(o);
+    return t && t->dim() == 2 && t->numel() > 0 && t->size(0) <= INT32_MAX && t->size(1) <= INT32_MAX - 65536 && (t->size(1) == 1 || t->stride(1) == 1) &&
+                   (t->scalar_type() == at::kFloat || half_code(t->scalar_type()) >= 0)
+               ? t
+               : nullptr;
+}
+int float_code(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? FSTA_F32 : half_code(t.scalar_type()); }
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// The data of a contiguous tensor [size] of one type on like's device
+template <typename T> const T* array_of(PyObject* o, const at::Tensor& like, at::ScalarType type, int64_t size) {
+    const at::Tensor* t = gpu_tensor(o);
+    return t && t->scalar_type() == type && t->dim() == 1 && t->size(0) == size && t->is_contiguous() && t->device() == like.device()
+               ? static_cast<const T*>(t->data_ptr())
+               : nullptr;
+}
+
+// verify_drafts(logits, tokens, parent, q_starts, u_accept, u_next, max_path, temperature, draft_probs or None) -> (path, counts, next)
+PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    int64_t most;
+    if (n != 9 || !plain_context() || !as_int(args[6], &most) || most < 1 || most > INT32_MAX) return not_implemented();
+    const at::Tensor *logits = read_logits(args[0]), *starts = gpu_tensor(args[3]), *draft = nullptr;
+    if (!logits || !starts || starts->dim() != 1 || starts->size(0) < 2 || starts->size(0) > INT32_MAX) return not_implemented();
+    const int64_t nodes = logits->size(0), batch = starts->size(0) - 1;
+    const int64_t *tokens = array_of<int64_t>(args[1], *logits, at::kLong, nodes), *parent = array_of<int64_t>(args[2], *logits, at::kLong, nodes);
+    const int32_t* first = array_of<int32_t>(args[3], *logits, at::kInt, batch + 1);
+    const float *u_accept = array_of<float>(args[4], *logits, at::kFloat, nodes), *u_next = array_of<float>(args[5], *logits, at::kFloat, batch);
+    if (!tokens || !parent || !first || !u_accept || !u_next) return not_implemented();
+    const float* temperatures = nullptr;
+    double temperature = 0;
+    if (PyFloat_Check(args[7])) {
+        temperature = PyFloat_AS_DOUBLE(args[7]);
+        if (!(temperature >= 0) || (float)temperature > std::numeric_limits<float>::max()) return not_implemented();
+    } else if (!(temperatures = array_of<float>(args[7], *logits, at::kFloat, batch))) {
+        return not_implemented();
+    }
+    if (args[8] != Py_None) {
+        draft = read_logits(args[8]);
+        if (!draft || draft->sizes() != logits->sizes() || draft->device() != logits->device()) return not_implemented();
+    }
+    try {
+        const OnStream on(*logits);
+        const at::Tensor path = fresh({batch, most}, at::kInt, *logits), counts = fresh({batch}, at::kInt, *logits),
+                         next = fresh({batch}, at::kLong, *logits);
+        const size_t need = fsta_verify_workspace_bytes((int32_t)batch, (int32_t)nodes, (int32_t)logits->size(1), float_code(*logits), draft != nullptr);
+        const at::Tensor work = need ? fresh({(int64_t)need}, at::kByte, *logits) : at::Tensor();
+        if (fsta_verify_drafts(logits->data_ptr(), row_stride(*logits), float_code(*logits), draft ? draft->data_ptr() : nullptr,
+                               draft ? row_stride(*draft) : 0, draft ? float_code(*draft) : FSTA_F32, tokens, parent, first, u_accept, u_next,
+                               temperatures, (float)temperature, path.data_ptr<int32_t>(), counts.data_ptr<int32_t>(), next.data_ptr<int64_t>(),
+                               (int32_t)batch, (int32_t)nodes, (int32_t)logits->size(1), (int32_t)most, need ? work.data_ptr() : nullptr, need,
+                               on.stream) != FSTA_OK)
+            return not_implemented();
+        return as_tuple(path, counts, next);
+    } catch (const std::exception&) {
+        return not_implemented();
+    }
+}
+
+// The caches of all layers: a PagedKV, or a list or tuple of them
+struct Pools {
+    std::vector<fsta_paged_pool> layers;
+    std::vector<const at::Tensor*> tensors;      // what a call that writes to them changes
+    const at::Tensor* k = nullptr;               // of the first
+    int32_t pages = 0, page_size = 0;
+};
+bool read_pools(PyObject* o, Pools* p) {
+    const bool list = PyList_CheckExact(o);
+    if (!list && !PyTuple_Check(o)) return false;
+    PyObject** items = list ? reinterpret_cast<PyListObject*>(o)->ob_item : reinterpret_cast<PyTupleObject*>(o)->ob_item;
+    Py_ssize_t n = Py_SIZE(o);
+    if (n == 0) return false;
+    if (!list && THPVariable_Check(items[0])) items = &o, n = 1;      // a PagedKV itself
+    p->layers.resize(n);
+    p->tensors.reserve(2 * n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        Pool pool;
+        if (!read_pool(items[i], &pool)) return false;
+        if (i == 0) p->k = pool.k, p->pages = pool.pages, p->page_size = pool.page_size;
+        if (pool.pages != p->pages || pool.page_size != p->page_size || pool.k->device() != p->k->device()) return false;
+        p->layers[i] = fsta_paged_pool{pool.k->data_ptr(), pool.v->data_ptr(), pool.k_exp, pool.v_exp, pool.heads, pool.head_dim, pool.code, 0};
+        for (const at::Tensor* t : {pool.k, pool.v, pool.exps[0], pool.exps[1]})
+            if (t) p->tensors.push_back(t);
+    }
+    return true;
+}
+void moved(const at::Tensor* t) {
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+void moved(const Pools& p) {
+    for (const at::Tensor* t : p.tensors) moved(t);
+}
+
+// [batch, width] of a page table on the pools' device, or false
+bool read_table(PyObject* o, const Pools& p, int32_t* batch, int32_t* width, const int32_t** data) {
+    const at::Tensor* t = gpu_tensor(o);
+    if (!t || t->dim() != 2 || t->size(0) == 0 || t->size(0) > INT32_MAX || t->size(1) > INT32_MAX) return false;
+    *batch = (int32_t)t->size(0);
+    *width = (int32_t)t->size(1);
+    *data = int32_array(o, *p.k, 2, *batch);
+    return *data != nullptr;
+}
+
+// compact_paged_kv(caches, path, counts, page_table, kv_lens, q_starts) -> lengths
+PyObject* compact_paged_kv(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    try {
+        Pools pools;
+        int32_t batch, width;
+        const int32_t* table;
+        if (n != 6 || !plain_context() || !read_pools(args[0], &pools) || !read_table(args[3], pools, &batch, &width, &table)) return not_implemented();
+        const int32_t *path = int32_array(args[1], *pools.k, 2, batch), *counts = int32_array(args[2], *pools.k, 1, batch);
+        const int32_t *lens = int32_array(args[4], *pools.k, 1, batch), *starts = int32_array(args[5], *pools.k, 1, (int64_t)batch + 1);
+        if (!path || !counts || !lens || !starts || THPVariable_Unpack(args[1]).size(1) > INT32_MAX) return not_implemented();
+        const OnStream on(*pools.k);
+        const at::Tensor out = fresh({batch}, at::kInt, *pools.k);
+        if (fsta_compact_paged_kv(pools.layers.data(), (int32_t)pools.layers.size(), pools.pages, pools.page_size, path,
+                                  (int32_t)THPVariable_Unpack(args[1]).size(1), counts, table, lens, starts, batch, width, out.data_ptr<int32_t>(),
+                                  on.stream) != FSTA_OK)
+            return not_implemented();
+        moved(pools);
+        return THPVariable_Wrap(out);
+    } catch (const std::exception&) {
+        return not_implemented();
+    }
+}
+
+// copy_pages(caches, sources, targets, into or None) -> None
+PyObject* copy_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    try {
+        Pools pools, others;
+        if (n != 4 || !plain_context() || !read_pools(args[0], &pools)) return not_implemented();
+        const bool elsewhere = args[3] != Py_None;
+        if (elsewhere && (!read_pools(args[3], &others) || others.layers.size() != pools.layers.size() || others.page_size != pools.page_size ||
+                          others.k->device() != pools.k->device()))
+            return not_implemented();
+        const Pools& into = elsewhere ? others : pools;
+        const at::Tensor* t = gpu_tensor(args[1]);
+        if (!t || t->dim() != 1 || t->size(0) > INT32_MAX) return not_implemented();
+        const int32_t *sources = int32_array(args[1], *pools.k, 1, t->size(0)), *targets = int32_array(args[2], *pools.k, 1, t->size(0));
+        if (!sources || !targets) return not_implemented();
+        const OnStream on(*pools.k);
+        if (fsta_copy_pages(pools.layers.data(), into.layers.data(), (int32_t)pools.layers.size(), pools.pages, into.pages, pools.page_size, sources,
+                            targets, (int32_t)t->size(0), on.stream) != FSTA_OK)
+            return not_implemented();
+        moved(into);
+    } catch (const std::exception&) {
+        return not_implemented();
+    }
+    Py_RETURN_NONE;
+}
+
+// fit_pages(caches, refs, page_table, lens) -> missing
+PyObject* fit_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    try {
+        Pools pools;
+        int32_t batch, width;
+        const int32_t* table;
+        if (n != 4 || !plain_context() || !read_pools(args[0], &pools) || !read_table(args[2], pools, &batch, &width, &table)) return not_implemented();
+        const int32_t *refs = int32_array(args[1], *pools.k, 1, pools.pages), *lens = int32_array(args[3], *pools.k, 1, batch);
+        if (!refs || !lens) return not_implemented();
+        const OnStream on(*pools.k);
+        const at::Tensor missing = fresh({batch}, at::kInt, *pools.k);
+        const size_t need = fsta_fit_pages_workspace_bytes(batch, pools.pages);
+        const at::Tensor work = fresh({(int64_t)need}, at::kByte, *pools.k);
+        if (fsta_fit_pages(pools.layers.data(), (int32_t)pools.layers.size(), pools.pages, pools.page_size, const_cast<int32_t*>(refs),
+                           const_cast<int32_t*>(table), lens, batch, width, missing.data_ptr<int32_t>(), work.data_ptr(), need, on.stream) != FSTA_OK)
+            return not_implemented();
+        moved(pools);
+        moved(&THPVariable_Unpack(args[1]));
+        moved(&THPVariable_Unpack(args[2]));
+        return THPVariable_Wrap(missing);
+    } catch (const std::exception&) {
+        return not_implemented();
+    }
+}
+
+// fork_pages(caches, refs, page_table, lens, sources, targets) -> missing
+PyObject* fork_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    try {
+        Pools pools;
+        int32_t batch, width;
+        const int32_t* table;
+        if (n != 6 || !plain_context() || !read_pools(args[0], &pools) || !read_table(args[2], pools, &batch, &width, &table)) return not_implemented();
+        const int32_t *refs = int32_array(args[1], *pools.k, 1, pools.pages), *lens = int32_array(args[3], *pools.k, 1, batch);
+        const at::Tensor* t = gpu_tensor(args[4]);
+        if (!refs || !lens || !t || t->dim() != 1 || t->size(0) > INT32_MAX) return not_implemented();
+        const int32_t pairs = (int32_t)t->size(0);
+        const int32_t *sources = int32_array(args[4], *pools.k, 1, pairs), *targets = int32_array(args[5], *pools.k, 1, pairs);
+        if (!sources || !targets) return not_implemented();
+        const OnStream on(*pools.k);
+        const at::Tensor missing = fresh({pairs}, at::kInt, *pools.k);
+        const size_t need = fsta_fork_pages_workspace_bytes(pairs, width, pools.pages);
+        const at::Tensor work = fresh({(int64_t)need}, at::kByte, *pools.k);
+        if (fsta_fork_pages(pools.layers.data(), (int32_t)pools.layers.size(), pools.pages, pools.page_size, const_cast<int32_t*>(refs),
+                            const_cast<int32_t*>(table), const_cast<int32_t*>(lens), batch, width, sources, targets, pairs, missing.data_ptr<int32_t>(),
+                            work.data_ptr(), need, on.stream) != FSTA_OK)
+            return not_implemented();
+        moved(pools);
+        for (int i : {1, 2, 3}) moved(&THPVariable_Unpack(args[i]));
+        return THPVariable_Wrap(missing);
+    } catch (const std::exception&) {
+        return not_implemented();
+    }
+}
+
 #define FSTA_FASTCALL(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&f)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
     FSTA_FASTCALL(attention),
@@ -616,6 +826,11 @@ PyMethodDef kMethods[] = {
     FSTA_FASTCALL(paged_read),
     FSTA_FASTCALL(paged_attention),
     FSTA_FASTCALL(tree_bits),
+    FSTA_FASTCALL(verify_drafts),
+    FSTA_FASTCALL(compact_paged_kv),
+    FSTA_FASTCALL(copy_pages),
+    FSTA_FASTCALL(fit_pages),
+    FSTA_FASTCALL(fork_pages),
     {"setup", &setup, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

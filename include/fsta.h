@@ -522,6 +522,104 @@ int fsta_tree_bits(const int64_t* parent, const int32_t* q_starts, int32_t batch
                    int32_t words, uint32_t* bits, void* stream);
 
 /*
+ * fsta_verify_drafts: which tokens of a batch of draft trees stand against the model's logits, from
+ * given random numbers, and the token behind each accepted path (no counterpart in the reference).
+ *   logits [nodes, vocabulary] of logits_dtype (FSTA_F32, FSTA_F16, FSTA_BF16; logits_stride elements
+ *   from row to row): row t is what the model says behind node t.  tokens, parent [nodes] int64, q_starts
+ *   [batch + 1]: the trees, as fsta_tree_bits takes them; node 0 of a tree is its root and stands, other
+ *   roots are never reached.  u_accept [nodes], u_next [batch] float32: random numbers in [0, 1).
+ *   temperatures [batch] float32, or NULL: `temperature` for all.  draft [nodes, vocabulary] of
+ *   draft_dtype, or NULL: row t holds the probabilities from which the children of node t were drawn,
+ *   one after the other in the order of their numbers, no token twice.
+ * At an accepted node with row l and temperature T > 0: P(x) = exp((l(x) - max l) / T), W = P, Z = sum W,
+ * r = 1, s = 0.  Its children are asked in order.  One with token x, random number u and draft
+ * probability q(x) > 0 stands where u Z q(x) < W(x) r; if not, s += Z / r, then r -= q(x).  One without
+ * (no draft, q(x) not above 0, or r not above 0) stands where u Z < W(x).  A token that fell leaves P, and
+ * W = max(P - s q, 0), Z = sum W; one whose token is none of the vocabulary's or fell before falls and
+ * changes nothing.  The walk goes on from the first child that stands; where none does, the
+ * next token is the smallest x with W(0) + .. + W(x) > u_next Z (where rounding leaves W no mass, P takes
+ * its place, and where that is empty too, P with the tokens that fell).  Whether a path is kept or not, the
+ * next token is distributed as the model's own.  T <= 0 or NaN: P is 1 for the largest logit (the first of
+ * equals) and 0 elsewhere, the draft's probabilities are not looked at.
+ * A NaN counts as -inf; logits of +inf share all mass; a row of nothing but -inf leaves no token: its
+ * children fall and the next token is -1.  Sums and comparisons are made in 64 bits.
+ *   path [batch, max_path] int32: the accepted nodes' numbers within their tree from the root, -1 behind
+ *   them; a path that reaches max_path (>= 1) nodes ends there.  counts [batch] int32: how many.
+ *   next_tokens [batch] int64.  A sequence of no nodes has none: 0 and -1.  At most
+ *   FSTA_VERIFY_MAX_CHILDREN children of a node are asked, the first ones.
+ * The workspace (16-byte aligned) may be NULL where fsta_verify_workspace_bytes says 0; it is free again
+ * when the work queued on `stream` has run.
+ */
+#define FSTA_VERIFY_MAX_CHILDREN 2048
+size_t fsta_verify_workspace_bytes(int32_t batch, int32_t nodes, int32_t vocabulary, int32_t logits_dtype,
+                                   int32_t draft);
+int fsta_verify_drafts(const void* logits, int64_t logits_stride, int32_t logits_dtype, const void* draft,
+                       int64_t draft_stride, int32_t draft_dtype, const int64_t* tokens,
+                       const int64_t* parent, const int32_t* q_starts, const float* u_accept,
+                       const float* u_next, const float* temperatures, float temperature, int32_t* path,
+                       int32_t* counts, int64_t* next_tokens, int32_t batch, int32_t nodes,
+                       int32_t vocabulary, int32_t max_path, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/*
+ * What a program does with the pages of a paged cache between two passes of its model, all layers in one
+ * call (no counterpart in the reference).  `pools` is HOST memory: one entry per layer, layers >= 1; the
+ * layers share page_size and num_pages, nothing else.
+ *
+ * fsta_compact_paged_kv: of the new tokens of a sequence (its last q_starts[b + 1] - q_starts[b] positions
+ * below kv_lens[b]) the ones that path [batch, max_path] names, counts[b] of them, move to the first of
+ * those positions: position base + path[b][i] to base + i.  A path's numbers ascend (fsta_verify_drafts'
+ * do); others leave the rows it concerns undefined, entries outside the new tokens move nothing.
+ * new_lens [batch] = base + counts[b] (counts kept within [0, new tokens and max_path]).
+ */
+typedef struct fsta_paged_pool {
+    void* k;                 /* [num_pages, kv_heads, page_size, head_dim] */
+    void* v;
+    uint8_t* k_exponent;     /* FSTA_FP8: [num_pages, kv_heads, page_size], else NULL */
+    uint8_t* v_exponent;
+    int32_t kv_heads, head_dim, cache_dtype, reserved;
+} fsta_paged_pool;
+
+int fsta_compact_paged_kv(const fsta_paged_pool* pools, int32_t layers, int32_t num_pages, int32_t page_size,
+                          const int32_t* path, int32_t max_path, const int32_t* counts,
+                          const int32_t* page_table, const int32_t* kv_lens, const int32_t* q_starts,
+                          int32_t batch, int32_t width, int32_t* new_lens, void* stream);
+
+/*
+ * fsta_copy_pages: page sources[i] of `pools` to page targets[i] of `into` (the same pools, or others of
+ * the same layers with into_pages pages).  A pair with an entry that names no page, or one page twice, copies
+ * nothing.  No page may be the target of two pairs, or of one and the source of another.
+ */
+int fsta_copy_pages(const fsta_paged_pool* pools, const fsta_paged_pool* into, int32_t layers,
+                    int32_t num_pages, int32_t into_pages, int32_t page_size, const int32_t* sources,
+                    const int32_t* targets, int32_t pairs, void* stream);
+
+/*
+ * refs [num_pages] int32: by how many entries of page tables a page is held; 0: it is free.
+ * fsta_fit_pages makes a page table fit the lengths lens [batch]: entries behind a sequence's last page
+ * are taken back (-1; the page is held once less), entries up to it that name no page get a free one, and
+ * where a sequence ends inside a page that others hold too, it gets a copy of its rows of that page in all
+ * layers.  Pages are given in order of sequence and position, the lowest-numbered first, among those that
+ * are free before the call.  missing [batch]: pages that a sequence wanted and did not get (its entries name
+ * none, or still the page of others: such a sequence must not be written to).
+ * fsta_fork_pages: slot targets[i] gives up what it holds and becomes a copy of slot sources[i] as it was
+ * before the call: it shares the pages that are full and gets a copy of the rows of the last one, lens too.
+ * Where pairs have one target the first counts; a pair of one slot twice, or outside [0, batch), does
+ * nothing else.  missing [pairs]: 1 where there was no free page for the last rows: that target is empty.
+ * Both change page_table, refs and the pools (fsta_fork_pages: lens too) in place.  The workspaces (16-byte
+ * aligned) are always needed and free again when the work queued on `stream` has run.
+ */
+size_t fsta_fit_pages_workspace_bytes(int32_t batch, int32_t num_pages);
+int fsta_fit_pages(const fsta_paged_pool* pools, int32_t layers, int32_t num_pages, int32_t page_size,
+                   int32_t* refs, int32_t* page_table, const int32_t* lens, int32_t batch, int32_t width,
+                   int32_t* missing, void* workspace, size_t workspace_bytes, void* stream);
+size_t fsta_fork_pages_workspace_bytes(int32_t pairs, int32_t width, int32_t num_pages);
+int fsta_fork_pages(const fsta_paged_pool* pools, int32_t layers, int32_t num_pages, int32_t page_size,
+                    int32_t* refs, int32_t* page_table, int32_t* lens, int32_t batch, int32_t width,
+                    const int32_t* sources, const int32_t* targets, int32_t pairs, int32_t* missing,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Measuring aids (no counterpart in the reference; bench.py reports them beside
  * the attention kernels' figures as this GPU's own ceilings).
  *   fsta_probe_empty_launch: one launch of a kernel that does nothing, `workgroups`
