@@ -1,0 +1,127 @@
+"""Acceptance of drafted tokens where there are too many rows to sum all of them: a launch per step of all walks, and what is left of
+long ones behind them."""
+import numpy as np
+import pytest
+import torch
+
+import fstattention_amd as fsta
+from test_gpu_verify import call, check, expected, make_case, on_gpu
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype,draft,vocabulary", [(torch.bfloat16, None, 50021), (torch.float16, torch.float32, 50021), (torch.float32, None, 32000),
+                                                    (torch.bfloat16, torch.bfloat16, 131072), (torch.float32, torch.float16, 30011)])
+def test_trees(dtype, draft, vocabulary):
+    sizes = [1, 30, 0, 64, 17, 90, 2, 45, 80, 64, 100, 33, 64, 200, 64, 64] + [5] * 20
+    case = make_case(vocabulary + 1, sizes, vocabulary, dtype, 4, draft)
+    assert case["logits"].numel() * case["logits"].element_size() > 70e6
+    gpu = on_gpu(case)
+    check(call(gpu, 40), expected(case, 40))
+    check(call(gpu, 3, 0.8), expected(case, 3, 0.8), "cut")
+    tau = [0.0, 1.0, 0.5, 1.7] * 9
+    check(call(gpu, 12, torch.tensor(tau).cuda()), expected(case, 12, tau), "mixed")
+
+
+@pytest.mark.parametrize("draft", [None, torch.float32])
+def test_long_paths(draft):
+    """Chains whose tokens are all but certain, longer than there are launches."""
+    sizes = [60] * 12 + [7, 1, 0, 40]
+    case = make_case(3, sizes, 24001, torch.float32, 1, draft, likely=1.0)
+    n = case["tokens"].shape[0]
+    starts = case["q_starts"].numpy()
+    for b, size in enumerate(sizes):
+        s = starts[b]
+        for i in range(size):
+            case["parent"][s + i] = i - 1
+            if i:
+                case["logits"][s + i - 1, case["tokens"][s + i]] = 25.0
+                if draft is not None:
+                    case["draft_probs"][s + i - 1, case["tokens"][s + i]] = 0.5
+    assert case["logits"].numel() * 4 > 70e6 and n == 768
+    case["u_accept"][200] = 1.0                                # one falls
+    gpu = on_gpu(case)
+    want = expected(case, 64)
+    assert want[1].max() >= 59
+    check(call(gpu, 64), want)
+    check(call(gpu, 25), expected(case, 25))
+
+
+@pytest.mark.parametrize("draft", [None, torch.float32])
+def test_many_that_fall(draft):
+    """Nodes with a dozen children of which most fall: more sums than launches; little left of a sum, and nothing."""
+    sizes = [40] * 30
+    case = make_case(6, sizes, 16007, torch.float32, 13, draft, likely=0.0, spread=1.0)
+    case["u_accept"][:] = 1.0 - 2.0 ** -24
+    rows = case["logits"].view(30, 40, 16007)
+    for b in range(10):                                        # the first children have nearly all the mass
+        for i in range(1, 4):
+            if case["parent"].view(30, 40)[b, i] == 0:
+                rows[b, 0, case["tokens"].view(30, 40)[b, i]] = 40.0 - i
+    for b in range(10, 15):                                    # the root's children are all there is
+        kids = (case["parent"].view(30, 40)[b] == 0).nonzero()[:, 0]
+        keep = rows[b, 0, case["tokens"].view(30, 40)[b, kids]].clone()
+        rows[b, 0] = -float("inf")
+        rows[b, 0, case["tokens"].view(30, 40)[b, kids]] = keep
+    case["u_accept"].view(30, 40)[10:13] = 1.0                 # and all of them fall
+    assert case["logits"].numel() * 4 > 70e6
+    check(call(on_gpu(case), 9), expected(case, 9))
+    case["u_accept"][::3] = 0.3
+    check(call(on_gpu(case), 9), expected(case, 9))
+
+
+@pytest.mark.parametrize("tau", [0.0, 1.0])
+def test_masked_and_infinite_rows(tau):
+    case = make_case(21, [6] * 400, 16000, torch.bfloat16, 2, None)
+    rows = case["logits"].view(400, 6, 16000)
+    inf = float("inf")
+    rows[0::8] = -inf
+    rows[1::8, :, 8195:] = -inf                                # whole parts without anything
+    rows[2::8, :, :8192] = float("nan")
+    rows[3::8, :, [3, 9000]] = inf
+    rows[4::8, :, 15999] = torch.finfo(torch.bfloat16).max
+    rows[5::8] = torch.finfo(torch.bfloat16).min
+    assert rows.numel() * 2 > 70e6
+    check(call(on_gpu(case), 6, tau), expected(case, 6, tau))
+
+
+def test_captured_and_replayed():
+    cases = [make_case(s, [64] * 20 + [3] * 10, 30000, torch.bfloat16, 3, torch.bfloat16 if s < 9 else None) for s in (1, 2, 3)]
+    held = on_gpu(cases[0])
+    assert held["logits"].numel() * 2 > 70e6
+    call(held, 12)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(held, 12)
+    for case in cases + cases[:2]:
+        for name, t in on_gpu(case).items():
+            held[name].copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out, expected(case, 12))
+        check(call(held, 12), expected(case, 12))
+
+
+def test_the_same_answers_by_either_way():
+    """A batch too large to sum all its rows, and its halves that are not."""
+    sizes = [40] * 32
+    case = make_case(12, sizes, 40000, torch.bfloat16, 4, torch.bfloat16)
+    gpu = on_gpu(case)
+    whole = call(gpu, 10)
+    for b in range(0, 32, 8):
+        s = slice(40 * b, 40 * (b + 8))
+        part = fsta.verify_drafts(gpu["logits"][s], gpu["tokens"][s], gpu["parent"][s], torch.arange(9, dtype=torch.int32, device="cuda") * 40,
+                                  gpu["u_accept"][s], gpu["u_next"][b:b + 8], 10, draft_probs=gpu["draft_probs"][s])
+        for a, w in zip(part, whole):
+            np.testing.assert_array_equal(a.cpu().numpy(), w[b:b + 8].cpu().numpy())
+
+
+def test_rows_longer_than_a_part_can_be():
+    """A row of more than 256 parts of 8192: parts are longer."""
+    vocabulary = 256 * 8192 + 12345
+    case = make_case(2, [4, 3, 5, 2], vocabulary, torch.float16, 2, None)
+    check(call(on_gpu(case), 5), expected(case, 5))
+    case["logits"][:, 20000:] = -float("inf")
+    case["logits"][3, vocabulary - 1] = 30.0
+    check(call(on_gpu(case), 5, 0.5), expected(case, 5, 0.5))
