@@ -19,6 +19,9 @@
 namespace fsta {
 namespace {
 
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
 constexpr int kChildren = FSTA_VERIFY_MAX_CHILDREN;
 constexpr int kRun = 512;                 // tokens that a wave looks at at once, eight a lane
 constexpr int kPart = 4 * kRun;
@@ -71,37 +74,71 @@ __device__ __forceinline__ float value(float x) { return x; }
 __device__ __forceinline__ float value(Half x) { return (float)__builtin_bit_cast(_Float16, x.bits); }
 __device__ __forceinline__ float value(Brain x) { return __builtin_bit_cast(float, (uint32_t)x.bits << 16); }
 
-// Eight values of a row at any address that the type allows (a row of odd length starts anywhere)
+// Eight values of a row at any address that the type allows (a row of odd length starts anywhere), as they come: taking them apart
+// is what waits for them
 template <typename T> struct Eight {
-    T v[8];
+    u32x4 w[sizeof(T) / 2];
 };
+__device__ __forceinline__ float value(const Eight<float>& x, int e) {
+    const uint32_t word = x.w[e / 4][e % 4];
+    return __builtin_bit_cast(float, word);
+}
+__device__ __forceinline__ float value(const Eight<Half>& x, int e) { return value(Half{(unsigned short)(x.w[0][e / 2] >> (e & 1) * 16)}); }
+__device__ __forceinline__ float value(const Eight<Brain>& x, int e) {
+    return __builtin_bit_cast(float, e & 1 ? x.w[0][e / 2] & 0xffff0000u : x.w[0][e / 2] << 16);
+}
 
 // 2^d for d <= 0, exactly 1 for 0; 0 for NaN, -inf and all below -1000.  2^f = 1 + f g(f) over |f| <= 1/2, g the polynomial of degree 9
 // that meets (2^f - 1) / f at the Chebyshev points: off by 6e-16 at most.  Rounding to a whole number and scaling by its power of
 // two go through the bits of the sum with 1.5 2^52: sums, products and their fusions run at full rate in 64 bits, conversions and
-// ldexp do not (by those the exponentials took twice as long).
-__device__ __forceinline__ double power(double d) {
+// ldexp do not.  N at once, step by step: each step waits for the one before, and the few waves that fit beside the registers do not fill
+// that time (one by one a wave took 3.6 us for 2048).
+template <int N> __device__ __forceinline__ void powers(double (&d)[N]) {
     constexpr double kRound = 6755399441055744.0;
-    const double k = d + kRound, f = d - (k - kRound);
-    double p = 7.070977866508138e-09;
-    p = fma(p, f, 1.0205905413765595e-07);
-    p = fma(p, f, 1.3215451633221434e-06);
-    p = fma(p, f, 1.5252672924850737e-05);
-    p = fma(p, f, 0.00015403530424776529);
-    p = fma(p, f, 0.0013333558200794592);
-    p = fma(p, f, 0.009618129107618665);
-    p = fma(p, f, 0.05550410866465167);
-    p = fma(p, f, 0.24022650695910075);
-    p = fma(p, f, 0.6931471805599462);
-    p = fma(p, f, 1.0);
-    const uint64_t bits = __builtin_bit_cast(uint64_t, p);
-    const uint32_t high = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, k) << 20);
-    p = __builtin_bit_cast(double, (uint64_t)high << 32 | (uint32_t)bits);
-    return d > -1000.0 ? p : 0.0;
+    constexpr double kG[10] = {7.070977866508138e-09, 1.0205905413765595e-07, 1.3215451633221434e-06, 1.5252672924850737e-05, 0.00015403530424776529,
+                               0.0013333558200794592, 0.009618129107618665, 0.05550410866465167, 0.24022650695910075, 0.6931471805599462};
+    double k[N], f[N], p[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) k[i] = d[i] + kRound;
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = d[i] - (k[i] - kRound);
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = kG[0];
+#pragma unroll
+    for (int c = 1; c < 10; ++c) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] = fma(p[i], f[i], kG[c]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        u32x2 bits = __builtin_bit_cast(u32x2, fma(p[i], f[i], 1.0));
+        bits[1] += __builtin_bit_cast(u32x2, k[i])[0] << 20;
+        d[i] = d[i] > -1000.0 ? __builtin_bit_cast(double, bits) : 0.0;
+    }
+}
+__device__ __forceinline__ double power(double d) {
+    double one[1] = {d};
+    powers(one);
+    return one[0];
 }
 // exp((l - against) / T), the logit `against` being the largest; infinite ones share all weight
 __device__ __forceinline__ double weight_of(float l, float against, double rate) {
     return against == INFINITY ? (l == INFINITY ? 1.0 : 0.0) : power(((double)l - (double)against) * rate);
+}
+
+// .. of eight logits
+__device__ __forceinline__ void weights_of(const float (&l)[8], float against, double rate, double (&w)[8]) {
+    const bool infinite = against == INFINITY;
+    const double top = infinite ? 0.0 : (double)against;
+#pragma unroll
+    for (int h = 0; h < 8; h += 4) {
+        double d[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = ((double)l[h + e] - top) * rate;
+        powers(d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[h + e] = infinite ? (l[h + e] == INFINITY ? 1.0 : 0.0) : d[e];
+    }
 }
 
 // The weights of one row: P against its largest logit, W with the draft's row
@@ -112,6 +149,17 @@ template <typename L, typename Q> struct Row {
     float top;
     int best;
     double shift;                         // s
+    int n;                                // the vocabulary
+    // of eight tokens as they were loaded
+    __device__ __forceinline__ void eight(const Eight<L>& l, const Eight<Q>& q, double (&w)[8]) const {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = value(l, e);
+        weights_of(x, top, rate, w);
+        if (!draft || !(shift > 0.0)) return;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = fmax(w[e] - shift * fmax((double)value(q, e), 0.0), 0.0);
+    }
     __device__ __forceinline__ double weight(float l, double q) const {
         const double p = weight_of(l, top, rate);
         return shift > 0.0 ? fmax(p - shift * q, 0.0) : p;
@@ -125,112 +173,167 @@ struct Shared {
     int32_t parent[kTree], token[kTree];  // -1: none
     uint32_t fell[kWalkThreads / 64][kPart / 32];     // a wave's part: which tokens fell
     int32_t fallen[kChildren];            // tokens that left P at this node
+    double lost[kChildren];               // .. and their weights
     double wave_sum[kWalkThreads / 64];
     int32_t best[kWalkThreads / 64], last[kWalkThreads / 64];
 };
 
-__device__ __forceinline__ double sum_of(double x) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
-    return x;
+// Steps of a sum (or least, or largest) over the lanes up to each: from 1, 2, 4 and 8 lanes below within rows of 16, then the rows'
+// last lanes to the rows behind them.  Register moves: a shuffle through LDS takes ten times as long, and decisions wait for these.
+template <int STEP> __device__ __forceinline__ uint32_t from_below(uint32_t none, uint32_t x) {
+    constexpr int kControl[6] = {0x111, 0x112, 0x114, 0x118, 0x142, 0x143}, kRows[6] = {0xf, 0xf, 0xf, 0xf, 0xa, 0xc};
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)x, kControl[STEP], kRows[STEP], 0xf, false);
+}
+template <int STEP> __device__ __forceinline__ double from_below(double x) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+    return __builtin_bit_cast(double, (uint64_t)from_below<STEP>(0u, (uint32_t)(bits >> 32)) << 32 | from_below<STEP>(0u, (uint32_t)bits));
+}
+template <typename F> __device__ __forceinline__ void six_steps(F f) {
+    f(std::integral_constant<int, 0>{});
+    f(std::integral_constant<int, 1>{});
+    f(std::integral_constant<int, 2>{});
+    f(std::integral_constant<int, 3>{});
+    f(std::integral_constant<int, 4>{});
+    f(std::integral_constant<int, 5>{});
+}
+// The value of lane l, the same l in all lanes
+__device__ __forceinline__ int of_lane(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
+__device__ __forceinline__ double of_lane(double x, int l) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+    return __builtin_bit_cast(double, (uint64_t)(uint32_t)of_lane((int)(bits >> 32), l) << 32 | (uint32_t)of_lane((int)bits, l));
 }
 __device__ __forceinline__ double sum_up_to(double x) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const double y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
+    six_steps([&](auto step) { x += from_below<decltype(step)::value>(x); });
     return x;
 }
+__device__ __forceinline__ double sum_of(double x) { return of_lane(sum_up_to(x), 63); }
 __device__ __forceinline__ float max_of(float x) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
-    return x;
+    six_steps([&](auto step) {
+        x = fmaxf(x, __builtin_bit_cast(float, from_below<decltype(step)::value>(0xff800000u, __builtin_bit_cast(uint32_t, x))));
+    });
+    return __builtin_bit_cast(float, of_lane(__builtin_bit_cast(int, x), 63));
+}
+__device__ __forceinline__ int min_of(int x) {
+    six_steps([&](auto step) { x = min(x, (int)from_below<decltype(step)::value>((uint32_t)INT32_MAX, (uint32_t)x)); });
+    return of_lane(x, 63);
+}
+__device__ __forceinline__ int max_of(int x) {
+    six_steps([&](auto step) { x = max(x, (int)from_below<decltype(step)::value>((uint32_t)INT32_MIN, (uint32_t)x)); });
+    return of_lane(x, 63);
 }
 __device__ __forceinline__ void first_best(float& top, int& best) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        const float other = __shfl_xor(top, d);
-        const int at = __shfl_xor(best, d);
-        if (other > top || (other == top && at < best)) top = other, best = at;
-    }
+    const float most = max_of(top);
+    best = min_of(top == most ? best : INT32_MAX);
+    top = most;
 }
 
-// Eight values from token i on, `none` at and behind token `to`
-template <typename T> __device__ __forceinline__ void load_eight(const T* row, int i, int to, float none, float (&x)[8]) {
-    if (i + 8 <= to) {
-        Eight<T> w;
-        __builtin_memcpy(&w, row + i, sizeof(w));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = value(w.v[e]);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = i + e < to ? value(row[i + e]) : none;
-    }
+// Eight values of a row of n >= 8 from place first_of(i, n) on: i, or the last at which there are eight
+__device__ __forceinline__ int first_of(int i, int n) { return min(i, n - 8); }
+template <typename T> __device__ __forceinline__ Eight<T> load_eight(const T* row, int i, int n) {
+    Eight<T> x;
+    __builtin_memcpy(&x, row + first_of(i, n), sizeof(x));
+    return x;
 }
 
-// Tokens [from, to) of a row by one wave: the largest logit and the sum against it, in one pass: what is summed so far is
-// scaled when a larger logit comes.  All lanes have the result.
-template <typename L> __device__ Part first_sum(const L* row, double rate, int from, int to) {
-    constexpr int kAtOnce = kPart / kRun;
+// Which of the eight places from `at` on lie outside [i, end), as bits
+__device__ __forceinline__ uint32_t outside(int at, int i, int end) {
+    const int skip = min(i - at, 8), stop = min(max(end - at, 0), 8);
+    return ((1u << skip) - 1u) | ~((1u << stop) - 1u);
+}
+template <typename T> __device__ __forceinline__ void leave_out(uint32_t out, T none, T (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = out >> e & 1u ? none : x[e];
+}
+
+// Parts [p, p_end) of a row by one wave: their largest logits and the sums against them, in one pass: what is summed so far is
+// scaled when a larger logit comes.  The next part's runs are on their way while one's are looked at.
+template <typename L>
+__device__ __forceinline__ void first_sums(const L* row, double rate, int vocabulary, int part_length, int p, int p_end, Part* out) {
     const int lane = threadIdx.x & 63;
+    if (p >= p_end) return;
+    if (vocabulary < 8) {                 // a token per lane
+        const float x = lane < vocabulary ? value(row[lane]) : -INFINITY;
+        Part part{1.0, x == x ? x : -INFINITY, lane};
+        first_best(part.top, part.best);
+        if (rate != 0.0) part.sum = sum_of(part.top > -INFINITY ? weight_of(x, part.top, rate) : 0.0);
+        if (lane == 0) out[p] = part;
+        return;
+    }
+    constexpr int kRing = kPart / kRun;
+    const int last = (int)min((int64_t)p_end * part_length, (int64_t)vocabulary);
+    const auto load = [&](int i) { return load_eight(row, i + lane * 8, vocabulary); };
+    Eight<L> ring[kRing];
+#pragma unroll
+    for (int r = 0; r < kRing; ++r) {
+        ring[r] = load(p * part_length + r * kRun);
+        __builtin_amdgcn_sched_barrier(0);                       // (in this order: the loop waits for one at a time)
+    }
     float top = -INFINITY;
-    int best = INT32_MAX;
+    int best = INT32_MAX, end = min(p * part_length + part_length, last);
     double sum = 0.0;
-    for (int i0 = from; i0 < to; i0 += kPart) {
-        float x[kAtOnce][8];
+#pragma unroll 1
+    for (int i1 = p * part_length; i1 < last; i1 += kPart) {
 #pragma unroll
-        for (int r = 0; r < kAtOnce; ++r) load_eight(row, i0 + r * kRun + lane * 8, to, -INFINITY, x[r]);
-        float m = -INFINITY;              // (fmaxf passes over a NaN)
+        for (int r = 0; r < kRing; ++r) {
+            const int i0 = i1 + r * kRun, i = i0 + lane * 8, at = first_of(i, vocabulary);
+            if (i0 < last) {
+                float x[8], m = -INFINITY;                       // (fmaxf passes over a NaN)
 #pragma unroll
-        for (int r = 0; r < kAtOnce; ++r)
+                for (int e = 0; e < 8; ++e) x[e] = value(ring[r], e);
+                if (i0 + kRun > vocabulary) leave_out(outside(at, i, vocabulary), -INFINITY, x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) m = fmaxf(m, x[r][e]);
-        if (rate == 0.0) {
-            if (m > top) {
-                top = m;
+                for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);
+                if (rate == 0.0) {
+                    if (m > top) {
+                        top = m;
 #pragma unroll
-                for (int r = kAtOnce - 1; r >= 0; --r)
+                        for (int e = 7; e >= 0; --e)
+                            if (x[e] == m) best = at + e;
+                    }
+                } else {
+                    m = max_of(m);
+                    if (m > top) {
+                        if (sum > 0.0) sum *= weight_of(top, m, rate);
+                        top = m;
+                    }
+                    if (top > -INFINITY) {
+                        double w[8];
+                        weights_of(x, top, rate, w);
 #pragma unroll
-                    for (int e = 7; e >= 0; --e)
-                        if (x[r][e] == m) best = i0 + r * kRun + lane * 8 + e;
+                        for (int e = 0; e < 8; ++e) sum += w[e];
+                    }
+                }
             }
-            continue;
+            // (behind the last use of what it replaces, so that it comes to the same registers)
+            ring[r] = load(min(i0 + kPart, last));
+            __builtin_amdgcn_sched_barrier(0);
         }
-        m = max_of(m);
-        if (m > top) {
-            if (sum > 0.0) sum *= weight_of(top, m, rate);
-            top = m;
-        }
-        if (top == INFINITY) {
-#pragma unroll
-            for (int r = 0; r < kAtOnce; ++r)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sum += x[r][e] == INFINITY ? 1.0 : 0.0;
-        } else if (top > -INFINITY) {
-            const double against = top;
-#pragma unroll
-            for (int r = 0; r < kAtOnce; ++r) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sum += power(((double)x[r][e] - against) * rate);
-                __builtin_amdgcn_sched_barrier(0);               // (eight at a time: all at once they need twice the registers)
-            }
-        }
+        if (i1 + kPart < end) continue;
+        Part part{1.0, top, best};
+        if (rate == 0.0) first_best(part.top, part.best);
+        else part.sum = sum_of(sum);
+        if (lane == 0) out[p] = part;
+        ++p;
+        end = (int)min((int64_t)end + part_length, (int64_t)last);
+        top = -INFINITY;
+        best = INT32_MAX;
+        sum = 0.0;
     }
-    if (rate == 0.0) {
-        first_best(top, best);
-        return Part{1.0, top, best};
-    }
-    return Part{sum_of(sum), top, 0};
 }
 
 // Sum of a row's weights over [from, to) without the tokens that fell, by one wave; `fell`: room for kPart bits
 template <typename L, typename Q>
-__device__ double sum_again(const Row<L, Q>& row, int from, int to, const int32_t* fallen, int n_fallen, uint32_t* fell) {
+__device__ __forceinline__ double sum_again(const Row<L, Q>& row, int from, int to, const int32_t* fallen, int n_fallen, uint32_t* fell) {
     const int lane = threadIdx.x & 63;
     const bool drafted = row.draft && row.shift > 0.0;
     double sum = 0.0;
+    if (row.n < 8) {                      // a token per lane
+        const int i = from + lane;
+        if (i < to) sum = row.weight(value(row.logits[i]), row.proposed(i));
+        for (int k = 0; k < n_fallen; ++k)
+            if (fallen[k] == i) sum = 0.0;
+        return sum_of(sum);
+    }
     for (int i0 = from; i0 < to; i0 += kPart) {
         bool any = false;
         for (int k0 = 0; k0 < n_fallen; k0 += 64) {
@@ -245,26 +348,40 @@ __device__ double sum_again(const Row<L, Q>& row, int from, int to, const int32_
             if (here) atomicOr(&fell[x >> 5], 1u << (x & 31));
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        const auto add = [&](const float (&x)[8], const float (&q)[8], uint32_t out) {
+        const int end = min(i0 + kPart, to);
+        const auto logits = [&](int i) { return load_eight(row.logits, i + lane * 8, row.n); };
+        const auto drafts = [&](int i) { return drafted ? load_eight(row.draft, i + lane * 8, row.n) : Eight<Q>{}; };
+        constexpr int kAtOnce = 2;
+        Eight<L> ring[kAtOnce];
+        Eight<Q> draft_ring[kAtOnce];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                double w = weight_of(x[e], row.top, row.rate);
-                if (drafted) w = fmax(w - row.shift * fmax((double)q[e], 0.0), 0.0);
-                sum += out >> e & 1 ? 0.0 : w;
-            }
-        };
-        const auto left_out = [&](int i) { return any ? fell[(i - i0) >> 5] >> ((i - i0) & 31) : 0u; };
-        for (int i = i0 + lane * 8; i < min(i0 + kPart, to); i += 2 * kRun) {
-            float x[8], y[8], q[8] = {}, p[8] = {};
-            load_eight(row.logits, i, to, -INFINITY, x);
-            load_eight(row.logits, min(i + kRun, to), to, -INFINITY, y);
-            if (drafted) {
-                load_eight(row.draft, i, to, 0.f, q);
-                load_eight(row.draft, min(i + kRun, to), to, 0.f, p);
-            }
-            add(x, q, left_out(i));
+        for (int r = 0; r < kAtOnce; ++r) {
+            ring[r] = logits(i0 + r * kRun);
+            draft_ring[r] = drafts(i0 + r * kRun);
             __builtin_amdgcn_sched_barrier(0);
-            add(y, p, left_out(i + kRun));
+        }
+#pragma unroll 1
+        for (int i2 = i0; i2 < end; i2 += kAtOnce * kRun) {
+#pragma unroll
+            for (int r = 0; r < kAtOnce; ++r) {
+                const int i1 = i2 + r * kRun, i = i1 + lane * 8, at = first_of(i, row.n);
+                double w[8];
+                row.eight(ring[r], draft_ring[r], w);
+                if (any || i1 + kRun > end) {
+                    uint32_t out = outside(at, i, end);
+                    if (any) {
+                        const int bit = at - i0, word = min(max(bit, 0) >> 5, kPart / 32 - 2);
+                        const uint64_t bits = (uint64_t)fell[word + 1] << 32 | fell[word];
+                        out |= (uint32_t)(bit < 0 ? bits << min(-bit, 8) : bits >> (bit - 32 * word));
+                    }
+                    leave_out(out, 0.0, w);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum += w[e];
+                ring[r] = logits(i1 + kAtOnce * kRun);
+                draft_ring[r] = drafts(i1 + kAtOnce * kRun);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
@@ -286,10 +403,12 @@ template <typename L, typename Q, int THREADS> struct Walk {
     // the strip of 64 nodes whose children are asked next: a child per lane, and which lanes
     int strip, token;
     uint64_t kids;
-    float logit;
-    double q, u;
+    L logit;
+    Q draft;
+    float u;
+    int early_parent, early_token;        // of node threadIdx.x, on their way
 
-    __device__ Walk(const VerifyArgs& args, Shared& shared, int sequence) : a(args), sh(shared), b(sequence) {
+    __device__ __forceinline__ Walk(const VerifyArgs& args, Shared& shared, int sequence) : a(args), sh(shared), b(sequence) {
         start = min(max(a.q_starts[b], 0), a.nodes);
         nodes = max(min(a.q_starts[b + 1], a.nodes) - start, 0);
         const float tau = a.temperatures ? a.temperatures[b] : a.temperature;
@@ -301,35 +420,49 @@ template <typename L, typename Q, int THREADS> struct Walk {
         row.shift = 0.0;
         row.top = -INFINITY;
         row.best = -1;
-        for (int j = threadIdx.x; j < min(nodes, kTree); j += THREADS) {
+        row.n = a.vocabulary;
+        const bool mine = (int)threadIdx.x < min(nodes, kTree);
+        early_parent = mine ? parent_in_memory(threadIdx.x) : -1;
+        early_token = mine ? token_in_memory(threadIdx.x) : -1;
+    }
+    // The tree is in LDS from here on
+    __device__ __forceinline__ void read_tree() {
+        if ((int)threadIdx.x < min(nodes, kTree)) {
+            sh.parent[threadIdx.x] = early_parent;
+            sh.token[threadIdx.x] = early_token;
+        }
+        for (int j = threadIdx.x + THREADS; j < min(nodes, kTree); j += THREADS) {
             sh.parent[j] = parent_in_memory(j);
             sh.token[j] = token_in_memory(j);
         }
         __syncthreads();
     }
-    __device__ int parent_in_memory(int j) const {
+    __device__ __forceinline__ int parent_in_memory(int j) const {
         const int64_t p = a.parent[start + j];
         return p >= 0 && p < j ? (int)p : -1;
     }
-    __device__ int token_in_memory(int j) const {
+    __device__ __forceinline__ int token_in_memory(int j) const {
         const int64_t x = a.tokens[start + j];
         return x >= 0 && x < a.vocabulary ? (int)x : -1;
     }
-    __device__ bool is_child(int j) const { return j < nodes && (j < kTree ? sh.parent[j] : parent_in_memory(j)) == node; }
-    __device__ int token_of(int j) const { return j < kTree ? sh.token[j] : token_in_memory(j); }
+    __device__ __forceinline__ bool is_child(int j) const { return j < nodes && (j < kTree ? sh.parent[j] : parent_in_memory(j)) == node; }
+    __device__ __forceinline__ int token_of(int j) const { return j < kTree ? sh.token[j] : token_in_memory(j); }
 
     // To the next strip with children of the node, from node `from` on: what they are asked with
-    __device__ void look(int from) {
+    __device__ __forceinline__ void look(int from) {
         const int lane = threadIdx.x & 63;
         kids = 0;
         for (strip = from; strip < nodes && !kids; strip += kids ? 0 : 64) kids = __ballot(is_child(strip + lane));
         const bool mine = kids >> lane & 1;
+        if (!kids) return;
+        // (loads of all lanes, the others' from a place that there is: a branch around them would wait for each)
         token = mine ? token_of(strip + lane) : -1;
-        logit = token >= 0 ? value(row.logits[token]) : -INFINITY;
-        q = token >= 0 ? row.proposed(token) : 0.0;
-        u = mine ? (double)a.u_accept[start + strip + lane] : 0.0;
+        const int x = max(token, 0);
+        logit = row.logits[x];
+        if (row.draft) draft = row.draft[x];
+        u = a.u_accept[start + min(strip + lane, nodes - 1)];
     }
-    __device__ void stand_at(int at, int how_many) {
+    __device__ __forceinline__ void stand_on(int at, int how_many) {
         node = at;
         count = how_many;
         child = summed = at + 1;
@@ -340,39 +473,53 @@ template <typename L, typename Q, int THREADS> struct Walk {
         row.shift = 0.0;
         row.top = -INFINITY;
         row.best = -1;
+    }
+    __device__ __forceinline__ void stand_at(int at, int how_many) {
+        stand_on(at, how_many);
         look(at + 1);
     }
-    __device__ void resume(const State& s) {
-        stand_at(s.node, s.count);
-        if (s.phase == kFirst) return;
-        child = s.child;
-        asked = s.asked;
-        left = s.left;
-        row.shift = s.shift;
-        row.top = s.top;
-        look(child);
+    __device__ __forceinline__ const Part* parts_of(const Part* all, int64_t which) const { return all + which * a.parts_per_row; }
+    __device__ __forceinline__ const Part* parts_of_node() const { return parts_of(a.all_parts, start + (int64_t)node); }
+    __device__ __forceinline__ const Part* parts_of_step(int turn) const { return parts_of(a.parts[turn], b); }
+    __device__ __forceinline__ void take(int what, const Part* parts) {
+        if (what == kFirst) take_first(parts);
+        else take_again(parts);
     }
-    __device__ void part_range(int p, int* from, int* to) const {
+    // Where the state is, with the sum that it waits for (or the last one, at a walk's end); the tree is in LDS behind it
+    __device__ __forceinline__ void resume(const State& s, const Part* parts) {
+        stand_on(s.node, s.count);
+        if (s.phase != kFirst) {
+            child = s.child;
+            asked = s.asked;
+            left = s.left;
+            row.shift = s.shift;
+            row.top = s.top;
+        }
+        if (parts) take(s.phase == kDone ? s.held : s.phase, parts);
+        read_tree();
+        if (s.phase != kDone) look(child);
+    }
+    __device__ __forceinline__ void part_range(int p, int* from, int* to) const {
         *from = (int)min((int64_t)p * a.part_length, (int64_t)a.vocabulary);
         *to = (int)min((int64_t)*from + a.part_length, (int64_t)a.vocabulary);
     }
 
     // The parts of the first sum of the row: its largest logit, Z.  (Every wave writes the same to sh.sum.)
-    __device__ void take_first(const Part* parts) {
+    __device__ __forceinline__ void take_first(const Part* parts) {
         const int lane = threadIdx.x & 63;
-        float top = -INFINITY;
-        int best = INT32_MAX;
-        for (int p = lane; p < a.parts_per_row; p += 64) {
-            const Part part = parts[p];
-            if (part.top > top) top = part.top, best = part.best;
-        }
+        Part mine = parts[min(lane, a.parts_per_row - 1)];
+        if (lane >= a.parts_per_row) mine = Part{0.0, -INFINITY, INT32_MAX};
+        float top = mine.top;
+        int best = mine.best;
+        for (int p = lane + 64; p < a.parts_per_row; p += 64)
+            if (parts[p].top > top) top = parts[p].top, best = parts[p].best;
         first_best(top, best);
         row.top = top;
         row.best = top > -INFINITY ? best : -1;
         double sum = 0.0;
         if (!greedy) {
             for (int p = lane; p < a.parts_per_row; p += 64) {
-                const Part part = parts[p];
+                const Part part = p == lane ? mine : parts[p];
                 const double s = part.sum > 0.0 ? part.sum * weight_of(part.top, top, row.rate) : 0.0;
                 sum += s;
                 sh.sum[p] = s;
@@ -383,7 +530,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
         held = kFirst;
     }
     // .. of a sum of W
-    __device__ void take_again(const Part* parts) {
+    __device__ __forceinline__ void take_again(const Part* parts) {
         double sum = 0.0;
         for (int p = threadIdx.x & 63; p < a.parts_per_row; p += 64) {
             const double s = parts[p].sum;
@@ -396,7 +543,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
     }
 
     // Whether a child before child j has its token x
-    __device__ bool fell_before(int j, int x) const {
+    __device__ __forceinline__ bool fell_before(int j, int x) const {
         for (int i0 = node + 1; i0 < j; i0 += 64) {
             const int i = i0 + (threadIdx.x & 63);
             if (__ballot(i < j && is_child(i) && token_of(i) == x)) return true;
@@ -405,12 +552,12 @@ template <typename L, typename Q, int THREADS> struct Walk {
     }
 
     // Asks children until one stands (kFirst: `node` is that one now), a sum of W is wanted (kAgain) or there are no more (kDone)
-    __device__ int ask() {
+    __device__ __forceinline__ int ask() {
         if (row.top == -INFINITY) return kDone;                  // nothing to choose: all children fall
         while (kids && count < a.max_path && asked < kChildren) {
-            const double w = row.weight(logit, q);
+            const double q = row.draft ? fmax((double)value(draft), 0.0) : 0.0, w = row.weight(value(logit), q);
             for (; kids && asked < kChildren; kids &= kids - 1) {
-                const int l = __ffsll((unsigned long long)kids) - 1, x = __shfl(token, l), j = strip + l;
+                const int l = __ffsll((unsigned long long)kids) - 1, x = of_lane(token, l), j = strip + l;
                 ++asked;
                 child = j + 1;
                 if (x < 0) continue;
@@ -420,7 +567,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
                     return kFirst;
                 }
                 if (fell_before(j, x)) continue;
-                const double wx = __shfl(w, l), qx = __shfl(q, l), ux = __shfl(u, l);
+                const double wx = of_lane(w, l), qx = of_lane(q, l), ux = of_lane((double)u, l);
                 const bool drawn = qx > 0.0 && left > 0.0;
                 // (W is at most Z: with u at 1 or more only the rounding of Z could let a given child stand)
                 if (drawn ? ux * all * qx < wx * left : ux < 1.0 && ux * all < wx) {
@@ -444,7 +591,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
     }
 
     // The tokens that fell, in sh.fallen; behind those that the sum leaves out (returned: how many) each comes once
-    __device__ int collect() {
+    __device__ __forceinline__ int collect() {
         const int lane = threadIdx.x & 63;
         __syncthreads();
         fallen = 0;
@@ -458,7 +605,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
         for (int i0 = summed; i0 < child; i0 += 64) {
             const int i = i0 + lane, mine = i < child && is_child(i) ? token_of(i) : -1;
             for (uint64_t those = __ballot(mine >= 0); those; those &= those - 1) {
-                const int l = __ffsll((unsigned long long)those) - 1, x = __shfl(mine, l);
+                const int l = __ffsll((unsigned long long)those) - 1, x = of_lane(mine, l);
                 if (fell_before(i0 + l, x)) continue;
                 if (threadIdx.x == 0) sh.fallen[fallen] = x;
                 ++fallen;
@@ -468,59 +615,72 @@ template <typename L, typename Q, int THREADS> struct Walk {
         return before;
     }
 
-    // Sums over the whole row by this workgroup alone, a part a wave: into sh.part
-    __device__ void sum_alone(bool first) {
-        const int wave = threadIdx.x >> 6;
-        __syncthreads();
-        for (int p = wave; p < a.parts_per_row; p += kWaves) {
+    // The share of wave `which` of `waves` in the row's sums: into out[part]
+    __device__ __forceinline__ void sum_parts(bool first, int which, int waves, Part* out) {
+        const int p0 = (int)((int64_t)a.parts_per_row * which / waves), p1 = (int)((int64_t)a.parts_per_row * (which + 1) / waves);
+        if (first) {
+            first_sums(row.logits, row.rate, a.vocabulary, a.part_length, p0, p1, out);
+            return;
+        }
+        for (int p = p0; p < p1; ++p) {
             int from, to;
             part_range(p, &from, &to);
-            const Part part = first ? first_sum(row.logits, row.rate, from, to) : Part{sum_again(row, from, to, sh.fallen, fallen, sh.fell[wave]), row.top, 0};
-            if ((threadIdx.x & 63) == 0) sh.part[p] = part;
+            const double sum = sum_again(row, from, to, sh.fallen, fallen, sh.fell[threadIdx.x >> 6]);
+            if ((threadIdx.x & 63) == 0) out[p] = Part{sum, row.top, 0};
         }
+    }
+    // Sums over the whole row by this workgroup alone, a part a wave: into sh.part
+    __device__ __forceinline__ void sum_alone(bool first) {
+        const int wave = threadIdx.x >> 6;
+        __syncthreads();
+        sum_parts(first, wave, kWaves, sh.part);
         __syncthreads();
     }
 
     // The smallest token at which the running sum of the weights passes u of all of it, the last one with any weight where rounding
     // (or u >= 1) lets none; -1 where there is no weight
-    __device__ int pick(double u) {
+    __device__ __forceinline__ int pick(double u) {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
         __syncthreads();                  // sh.sum
         if (child > summed) {
             // a part loses the terms that fell since its sum was taken; where little is left of it, its sum is taken again
             const int old = collect();
-            for (int p = wave; p < a.parts_per_row; p += kWaves) {
-                int from, to;
-                part_range(p, &from, &to);
+            for (int k = old + tid; k < fallen; k += THREADS) {
+                const int x = sh.fallen[k];
+                sh.lost[k] = row.weight(value(row.logits[x]), row.proposed(x));
+            }
+            __syncthreads();
+            for (int p = tid; p < a.parts_per_row; p += THREADS) {
                 double lost = 0.0;
-                for (int k = old + lane; k < fallen; k += 64) {
-                    const int x = sh.fallen[k];
-                    if (x >= from && x < to) lost += row.weight(value(row.logits[x]), row.proposed(x));
-                }
-                lost = sum_of(lost);
-                double s = sh.sum[p];
-                if (lost > 0.0) s = s - lost > s * 0x1p-10 ? s - lost : sum_again(row, from, to, sh.fallen, fallen, sh.fell[wave]);
-                if (lane == 0) sh.sum[p] = s;
+                for (int k = old; k < fallen; ++k)
+                    if (sh.fallen[k] / a.part_length == p) lost += sh.lost[k];
+                const double s = sh.sum[p];
+                if (lost > 0.0) sh.sum[p] = s - lost > s * 0x1p-10 ? s - lost : -1.0;
             }
             __syncthreads();
         } else {
             collect();
         }
-        // the part that holds it: the first whose end passes the target, or the last with weight
-        const auto total = [&] {
-            double sum = 0.0;
+        double sum;
+        for (int resort = 0;; ++resort) {
+            for (int p = wave; p < a.parts_per_row; p += kWaves) {
+                if (sh.sum[p] >= 0.0) continue;
+                int from, to;
+                part_range(p, &from, &to);
+                const double s = sum_again(row, from, to, sh.fallen, fallen, sh.fell[wave]);
+                if (lane == 0) sh.sum[p] = s;
+            }
+            __syncthreads();
+            sum = 0.0;
             for (int p = lane; p < a.parts_per_row; p += 64) sum += sh.sum[p];
-            return sum_of(sum);
-        };
-        double sum = total();
-        for (int resort = 0; !(sum > 0.0); ++resort) {           // rounding left nothing: P without what fell, then P
-            if (resort == 2) return -1;
+            sum = sum_of(sum);
+            if (sum > 0.0) break;
+            if (resort == 2) return -1;                          // rounding left nothing: P without what fell, then P
             row.shift = 0.0;
             if (resort == 1) fallen = 0;
-            sum_alone(false);
-            for (int p = tid; p < a.parts_per_row; p += THREADS) sh.sum[p] = sh.part[p].sum;
             __syncthreads();
-            sum = total();
+            for (int p = tid; p < a.parts_per_row; p += THREADS) sh.sum[p] = -1.0;
+            __syncthreads();
         }
         double target = u * sum;
         int chosen = -1, last = -1;
@@ -533,9 +693,9 @@ template <typename L, typename Q, int THREADS> struct Walk {
             if (passes) {
                 const int l = __ffsll((unsigned long long)passes) - 1;
                 chosen = p0 + l;
-                at_chosen = before + (__shfl(up_to, l) - __shfl(s, l));
+                at_chosen = before + (of_lane(up_to, l) - of_lane(s, l));
             }
-            before += __shfl(up_to, 63);
+            before += of_lane(up_to, 63);
         }
         if (chosen < 0) chosen = last, at_chosen = 0.0, target = INFINITY;
         target -= at_chosen;
@@ -570,18 +730,22 @@ template <typename L, typename Q, int THREADS> struct Walk {
             to = min(from + each, to);
         }
         double w[8], mine = 0.0;
-        const int i = min(from + tid * 8, to);
-        float x[8], qs[8];
-        load_eight(row.logits, i, to, -INFINITY, x);
-        const bool drafted = row.draft && row.shift > 0.0;
-        if (drafted) load_eight(row.draft, i, to, 0.f, qs);
+        int i = from + tid * 8, at = i;
+        if (row.n < 8) {                  // a token per thread
+            at = i = from + tid;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = i + e < to ? row.weight(x[e], drafted ? fmax((double)qs[e], 0.0) : 0.0) : 0.0;
+            for (int e = 0; e < 8; ++e) w[e] = 0.0;
+            if (i < to) w[0] = row.weight(value(row.logits[i]), row.proposed(i));
+        } else {
+            at = first_of(i, row.n);
+            Eight<Q> draft = {};
+            if (row.draft && row.shift > 0.0) draft = load_eight(row.draft, i, row.n);
+            row.eight(load_eight(row.logits, i, row.n), draft, w);
+            leave_out(outside(at, i, to), 0.0, w);
+        }
         for (int k = 0; k < fallen; ++k) {
-            const int f = sh.fallen[k] - i;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (f == e) w[e] = 0.0;
+            const int f = sh.fallen[k] - at;
+            if (f >= 0 && f < 8) leave_out(1u << f, 0.0, w);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) mine += w[e];
@@ -597,15 +761,12 @@ template <typename L, typename Q, int THREADS> struct Walk {
         for (int e = 0; e < 8; ++e) {
             run += w[e];
             if (w[e] > 0.0) {
-                weighs = i + e;
-                if (run > target && passes == INT32_MAX) passes = i + e;
+                weighs = at + e;
+                if (run > target && passes == INT32_MAX) passes = at + e;
             }
         }
-#pragma unroll
-        for (int d = 32; d; d >>= 1) {
-            passes = min(passes, __shfl_xor(passes, d));
-            weighs = max(weighs, __shfl_xor(weighs, d));
-        }
+        passes = min_of(passes);
+        weighs = max_of(weighs);
         if (lane == 0) sh.best[wave] = passes, sh.last[wave] = weighs;
         __syncthreads();
         for (int k = 0; k < kWaves; ++k) {
@@ -616,7 +777,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
     }
 
     // The end of a sequence's walk
-    __device__ void answer() {
+    __device__ __forceinline__ void answer() {
         int next = -1;
         if (nodes == 0) count = 0;
         else if (row.top > -INFINITY) next = greedy ? row.best : pick(a.u_next[b]);
@@ -626,35 +787,29 @@ template <typename L, typename Q, int THREADS> struct Walk {
         }
         for (int i = count + threadIdx.x; i < a.max_path; i += THREADS) a.path[(int64_t)b * a.max_path + i] = -1;
     }
-    __device__ void note() const {
+    __device__ __forceinline__ void note() const {
         if (threadIdx.x == 0) a.path[(int64_t)b * a.max_path + count - 1] = node;
     }
 
-    __device__ const Part* parts_of_node() const { return a.all_parts + (start + (int64_t)node) * a.parts_per_row; }
-    __device__ const Part* parts_of_step(int turn) const { return a.parts[turn] + (int64_t)b * a.parts_per_row; }
-    __device__ void take(int what, const Part* parts) {
-        if (what == kFirst) take_first(parts);
-        else take_again(parts);
-    }
-    // Takes decisions for as long as the sums are there; `parts`: the one that the state waits for, or null
-    __device__ int go_on(int phase, const Part* parts, bool noting) {
+    // Takes decisions for as long as the sums are there; `taken`: the state's is
+    __device__ __forceinline__ int go_on(int phase, bool taken, bool noting) {
         for (;;) {
-            if (phase == kFirst && !parts && a.all_parts && kids) {
-                parts = parts_of_node();
+            if (!taken) {
+                if (phase != kFirst || !a.all_parts || !kids) return phase;
+                take_first(parts_of_node());
                 where = kOfNode;
             }
-            if (!parts) return phase;
-            take(phase, parts);
-            parts = nullptr;
+            taken = false;
             phase = ask();
             if (phase == kFirst && noting) note();
-            if (phase != kFirst) return phase;
+            if (phase == kDone) return phase;
         }
     }
 };
 
-// blockIdx.x: parts in fours, .y: node
+// blockIdx.x: parts of a row, .y: node
 template <typename L> __global__ __launch_bounds__(kStepThreads, 4) void stats_kernel(VerifyArgs a) {
+    constexpr int kWaves = kStepThreads / 64;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     for (int64_t t = blockIdx.y; t < a.nodes; t += gridDim.y) {
         // the node's sequence: how many start at or before it
@@ -667,16 +822,15 @@ template <typename L> __global__ __launch_bounds__(kStepThreads, 4) void stats_k
         if (!any) continue;
         const float tau = a.temperatures ? a.temperatures[b] : a.temperature;
         const double rate = tau > 0.f ? fmax(1.4426950408889634074 / (double)tau, 1e-300) : 0.0;
-        const int p = blockIdx.x * (kStepThreads / 64) + wave;
-        if (p >= a.parts_per_row) continue;
-        const int from = (int)min((int64_t)p * a.part_length, (int64_t)a.vocabulary), to = (int)min((int64_t)from + a.part_length, (int64_t)a.vocabulary);
-        const Part part = first_sum(static_cast<const L*>(a.logits) + t * a.logits_stride, rate, from, to);
-        if (lane == 0) a.parts_out[t * a.parts_per_row + p] = part;
+        const int which = blockIdx.x * kWaves + wave, waves = gridDim.x * kWaves;
+        first_sums(static_cast<const L*>(a.logits) + t * a.logits_stride, rate, a.vocabulary, a.part_length,
+                   (int)((int64_t)a.parts_per_row * which / waves), (int)((int64_t)a.parts_per_row * (which + 1) / waves), a.parts_out + t * a.parts_per_row);
     }
 }
 
-// blockIdx.x: parts in fours, .y: sequence
-template <typename L, typename Q> __global__ __launch_bounds__(kStepThreads, 3) void step_kernel(VerifyArgs a) {
+// blockIdx.x: parts of a row, .y: sequence
+template <typename L, typename Q> __global__ __launch_bounds__(kStepThreads, 2) void step_kernel(VerifyArgs a) {
+    constexpr int kWaves = kStepThreads / 64;
     __shared__ Shared sh;
     const int wave = threadIdx.x >> 6;
     const bool speaks = blockIdx.x == 0;
@@ -692,10 +846,10 @@ template <typename L, typename Q> __global__ __launch_bounds__(kStepThreads, 3) 
         if (w.nodes == 0) {
             s.phase = kDone;
         } else {
-            w.resume(s);
             w.where = a.turn ^ 1;
+            w.resume(s, a.fresh ? nullptr : w.parts_of_step(a.turn ^ 1));
             if (a.fresh && speaks) w.note();
-            s.phase = w.go_on(s.phase, a.fresh ? nullptr : w.parts_of_step(a.turn ^ 1), speaks);
+            s.phase = w.go_on(s.phase, !a.fresh, speaks);
         }
         if (speaks && threadIdx.x == 0)
             a.states[a.turn][b] = State{w.node, w.count, w.child, w.asked, w.summed, s.phase, w.held, w.where, w.row.shift, w.left, w.row.top, 0};
@@ -704,13 +858,7 @@ template <typename L, typename Q> __global__ __launch_bounds__(kStepThreads, 3) 
             w.summed = w.child;
             w.collect();
         }
-        const int p = blockIdx.x * (kStepThreads / 64) + wave;
-        if (p >= a.parts_per_row) continue;
-        int from, to;
-        w.part_range(p, &from, &to);
-        const Part part = s.phase == kFirst ? first_sum(w.row.logits, w.row.rate, from, to)
-                                            : Part{sum_again(w.row, from, to, sh.fallen, w.fallen, sh.fell[wave]), w.row.top, 0};
-        if ((threadIdx.x & 63) == 0) a.parts[a.turn][(int64_t)b * a.parts_per_row + p] = part;
+        w.sum_parts(s.phase == kFirst, blockIdx.x * kWaves + wave, gridDim.x * kWaves, a.parts[a.turn] + (int64_t)b * a.parts_per_row);
     }
 }
 
@@ -718,25 +866,24 @@ template <typename L, typename Q> __global__ __launch_bounds__(kWalkThreads, 2) 
     __shared__ Shared sh;
     for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
         __syncthreads();
+        State s{0, 1, 1, 0, 1, kFirst, kFirst, 0, 0.0, 1.0, 0.f, 0};
+        if (!a.fresh) s = a.states[a.turn][b];
         Walk<L, Q, kWalkThreads> w(a, sh, b);
-        if (w.nodes > 0) {
-            State s{0, 1, 1, 0, 1, kFirst, kFirst, 0, 0.0, 1.0, 0.f, 0};
-            if (!a.fresh) s = a.states[a.turn][b];
-            w.resume(s);
-            if (s.phase == kDone) {
-                w.take(s.held, s.where == kOfNode ? w.parts_of_node() : w.parts_of_step(s.where));
-                w.summed = s.summed;
-            } else {
-                if (a.fresh) w.note();
-                const Part* parts = a.fresh ? nullptr : w.parts_of_step(a.turn);
-                while ((s.phase = w.go_on(s.phase, parts, true)) != kDone) {
-                    if (s.phase == kAgain) {
-                        w.summed = w.child;
-                        w.collect();
-                    }
-                    w.sum_alone(s.phase == kFirst);
-                    parts = sh.part;
+        if (w.nodes > 0 && s.phase == kDone) {
+            w.resume(s, s.where == kOfNode ? w.parts_of(a.all_parts, w.start + s.node) : w.parts_of_step(s.where));
+            w.summed = s.summed;
+        } else if (w.nodes > 0) {
+            w.resume(s, a.fresh ? nullptr : w.parts_of_step(a.turn));
+            if (a.fresh) w.note();
+            bool taken = !a.fresh;
+            while ((s.phase = w.go_on(s.phase, taken, true)) != kDone) {
+                if (s.phase == kAgain) {
+                    w.summed = w.child;
+                    w.collect();
                 }
+                w.sum_alone(s.phase == kFirst);
+                w.take(s.phase, sh.part);
+                taken = true;
             }
         }
         w.answer();
@@ -754,6 +901,7 @@ struct Plan {
 size_t rounded(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
 constexpr int kMostSteps = 10;
+constexpr int kStatsGroups = 2048, kStepGroups = 512;
 constexpr double kAllBytes = 128e6;
 
 Plan plan_of(int64_t batch, int64_t nodes, int64_t vocabulary, int size, bool draft, int32_t max_path) {
@@ -769,12 +917,16 @@ Plan plan_of(int64_t batch, int64_t nodes, int64_t vocabulary, int size, bool dr
 
 template <typename L, typename Q> int launch(VerifyArgs a, const Plan& plan, void* workspace, hipStream_t stream) {
     uint8_t* work = static_cast<uint8_t*>(workspace);
-    const unsigned groups = (unsigned)((a.parts_per_row + kStepThreads / 64 - 1) / (kStepThreads / 64));
+    // as many workgroups as the GPU holds, and no more: what comes before a workgroup's first sum takes as long as one
+    const auto groups = [&](int64_t rows, int64_t most) {
+        const int64_t needed = (a.parts_per_row + kStepThreads / 64 - 1) / (kStepThreads / 64), fit = (most + rows - 1) / rows;
+        return dim3((unsigned)(needed < fit ? needed : fit), (unsigned)(rows < 65535 ? rows : 65535));
+    };
     if (plan.all && a.nodes > 0) {
         a.parts_out = reinterpret_cast<Part*>(work);
         a.all_parts = a.parts_out;
         work += rounded(sizeof(Part) * (size_t)a.nodes * a.parts_per_row);
-        hipLaunchKernelGGL((stats_kernel<L>), dim3(groups, (unsigned)(a.nodes < 65535 ? a.nodes : 65535)), dim3(kStepThreads), 0, stream, a);
+        hipLaunchKernelGGL((stats_kernel<L>), groups(a.nodes, kStatsGroups), dim3(kStepThreads), 0, stream, a);
     }
     for (int i = 0; i < 2; ++i) {
         a.parts[i] = reinterpret_cast<Part*>(work);
@@ -785,7 +937,7 @@ template <typename L, typename Q> int launch(VerifyArgs a, const Plan& plan, voi
     a.fresh = 1;
     for (int i = 0; i < plan.steps; ++i) {
         a.turn = i & 1;
-        hipLaunchKernelGGL((step_kernel<L, Q>), dim3(groups, (unsigned)(a.batch < 65535 ? a.batch : 65535)), dim3(kStepThreads), 0, stream, a);
+        hipLaunchKernelGGL((step_kernel<L, Q>), groups(a.batch, kStepGroups), dim3(kStepThreads), 0, stream, a);
         a.fresh = 0;
     }
     hipLaunchKernelGGL((walk_kernel<L, Q>), dim3((unsigned)(a.batch < 65536 ? a.batch : 65536)), dim3(kWalkThreads), 0, stream, a);

@@ -349,3 +349,19 @@ def test_no_sequences_and_no_nodes():
     none = {k: v[:0] for k, v in case.items() if v is not None and k not in ("q_starts", "u_next")}
     got = call({**case, **none}, 4, q_starts=torch.zeros(2, dtype=torch.int32, device="cuda"))
     assert got.counts.tolist() == [0] and got.next_tokens.tolist() == [-1] and got.path.tolist() == [[-1] * 4]
+
+
+@pytest.mark.parametrize("draft", [None, torch.float32])
+def test_a_token_with_nearly_all_mass_falls(draft):
+    """The sum without it is taken again, wherever in the row it stands."""
+    vocabulary = 24001
+    places = list(range(20)) + [31, 32, 63, 504, 511, 512, 1023, 1024, 1500, 2047, 2048, 5000, 9999, 10000, 20479, 20480, 23551, 23552, 23992, 23993, 24000]
+    n = len(places)
+    case = make_case(5, [2] * n, vocabulary, torch.float32, 1, None, spread=1.0)
+    case["parent"] = torch.tensor([-1, 0] * n)
+    case["tokens"] = torch.tensor([t for x in places for t in (0, x)])
+    case["logits"][torch.arange(0, 2 * n, 2), torch.tensor(places)] = 25.0
+    case["u_accept"][:] = 1.0                                  # it falls all the same
+    if draft is not None:
+        case["draft_probs"] = torch.zeros((2 * n, vocabulary))
+    check(call(on_gpu(case), 3), expected(case, 3))
