@@ -43,11 +43,12 @@ struct State {
     int32_t child, asked, summed;         // as in Walk
     int32_t phase;                        // kFirst, kAgain: what the parts of this step are; kDone: no child stands
     int32_t held, where;                  // kDone: what the last parts were, and whose: of the steps' buffers 0 and 1, or kOfNode
+    int32_t ready, exact;                 // whether the parts are there; whether they have to be 64 bits
     double shift, left;                   // s, r
     float top;                            // of the node's row, in kAgain
     int32_t pad;
 };
-enum { kFirst = 0, kAgain = 1, kDone = 2 };
+enum { kFirst = 0, kAgain = 1, kDone = 2, kQuick = 3 };
 enum { kOfNode = 2 };
 
 struct VerifyArgs {
@@ -88,11 +89,10 @@ __device__ __forceinline__ float value(const Eight<Brain>& x, int e) {
     return __builtin_bit_cast(float, e & 1 ? x.w[0][e / 2] & 0xffff0000u : x.w[0][e / 2] << 16);
 }
 
-// 2^d for d <= 0, exactly 1 for 0; 0 for NaN, -inf and all below -1000.  2^f = 1 + f g(f) over |f| <= 1/2, g the polynomial of degree 9
-// that meets (2^f - 1) / f at the Chebyshev points: off by 6e-16 at most.  Rounding to a whole number and scaling by its power of
-// two go through the bits of the sum with 1.5 2^52: sums, products and their fusions run at full rate in 64 bits, conversions and
-// ldexp do not.  N at once, step by step: each step waits for the one before, and the few waves that fit beside the registers do not fill
-// that time (one by one a wave took 3.6 us for 2048).
+// 2^d for -1000 <= d <= 0, exactly 1 for 0.  2^f = 1 + f g(f) over |f| <= 1/2, g the polynomial of degree 9 that meets (2^f - 1) / f at
+// the Chebyshev points: off by 6e-16 at most.  Rounding to a whole number and scaling by its power of two go through the bits of the
+// sum with 1.5 2^52: sums, products and their fusions run at full rate in 64 bits, conversions and ldexp do not.  A wave takes 90 to 100
+// cycles for its 64, alone on its SIMD or not.
 template <int N> __device__ __forceinline__ void powers(double (&d)[N]) {
     constexpr double kRound = 6755399441055744.0;
     constexpr double kG[10] = {7.070977866508138e-09, 1.0205905413765595e-07, 1.3215451633221434e-06, 1.5252672924850737e-05, 0.00015403530424776529,
@@ -113,23 +113,26 @@ template <int N> __device__ __forceinline__ void powers(double (&d)[N]) {
     for (int i = 0; i < N; ++i) {
         u32x2 bits = __builtin_bit_cast(u32x2, fma(p[i], f[i], 1.0));
         bits[1] += __builtin_bit_cast(u32x2, k[i])[0] << 20;
-        d[i] = d[i] > -1000.0 ? __builtin_bit_cast(double, bits) : 0.0;
+        d[i] = __builtin_bit_cast(double, bits);
     }
 }
-__device__ __forceinline__ double power(double d) {
-    double one[1] = {d};
-    powers(one);
-    return one[0];
-}
-// exp((l - against) / T), the logit `against` being the largest; infinite ones share all weight
+// exp((l - against) / T), the logit `against` being the largest: any l (NaN: as -inf); infinite ones share all weight
 __device__ __forceinline__ double weight_of(float l, float against, double rate) {
-    return against == INFINITY ? (l == INFINITY ? 1.0 : 0.0) : power(((double)l - (double)against) * rate);
+    if (against == INFINITY) return l == INFINITY ? 1.0 : 0.0;
+    const double d = ((double)l - (double)against) * rate;
+    const bool far = d < -1000.0;         // (scaled in two steps: the result may have fewer bits)
+    double p[1] = {far ? fmax(d, -1200.0) + 200.0 : d};
+    powers(p);
+    return d > -1200.0 ? (far ? p[0] * 0x1p-200 : p[0]) : 0.0;
 }
-
 // .. of eight logits
 __device__ __forceinline__ void weights_of(const float (&l)[8], float against, double rate, double (&w)[8]) {
     const bool infinite = against == INFINITY;
     const double top = infinite ? 0.0 : (double)against;
+    float least = INFINITY;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) least = fminf(least, fmaxf(l[e], -INFINITY));       // (fmaxf takes the number of the two)
+    const bool far = infinite || !(((double)least - top) * rate >= -1000.0);
 #pragma unroll
     for (int h = 0; h < 8; h += 4) {
         double d[4];
@@ -137,7 +140,22 @@ __device__ __forceinline__ void weights_of(const float (&l)[8], float against, d
         for (int e = 0; e < 4; ++e) d[e] = ((double)l[h + e] - top) * rate;
         powers(d);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[h + e] = infinite ? (l[h + e] == INFINITY ? 1.0 : 0.0) : d[e];
+        for (int e = 0; e < 4; ++e) w[h + e] = d[e];
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if (!far) return;
+#pragma unroll
+    for (int h = 0; h < 8; h += 2) {
+        double d[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) d[e] = fmax(fmin(((double)l[h + e] - top) * rate, 0.0), -1200.0) + 200.0;
+        powers(d);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float x = l[h + e];
+            w[h + e] = infinite ? (x == INFINITY ? 1.0 : 0.0) : ((double)x - top) * rate > -1200.0 ? d[e] * 0x1p-200 : 0.0;
+        }
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -171,11 +189,13 @@ struct Shared {
     double sum[kMaxParts];                // parts' sums against the row's largest logit
     Part part[kMaxParts];                 // walk_kernel's own
     int32_t parent[kTree], token[kTree];  // -1: none
+    float logit[kTree], draft[kTree], u[kTree];       // .. of a token at its parent; only where the first sums of all rows are there
     uint32_t fell[kWalkThreads / 64][kPart / 32];     // a wave's part: which tokens fell
     int32_t fallen[kChildren];            // tokens that left P at this node
     double lost[kChildren];               // .. and their weights
     double wave_sum[kWalkThreads / 64];
     int32_t best[kWalkThreads / 64], last[kWalkThreads / 64];
+    int32_t sure;
 };
 
 // Steps of a sum (or least, or largest) over the lanes up to each: from 1, 2, 4 and 8 lanes below within rows of 16, then the rows'
@@ -245,9 +265,15 @@ template <typename T> __device__ __forceinline__ void leave_out(uint32_t out, T 
     for (int e = 0; e < 8; ++e) x[e] = out >> e & 1u ? none : x[e];
 }
 
+// A sum in 32 bits is off by less than kDoubt of itself: a weight 2^-t by three roundings of its exponent, 1.3e-7 t of itself, and a step
+// of the exponential, 1.2e-7; the mean of t over the weights is at most log2 of the vocabulary (it is the entropy of W / Z less log2 Z, and
+// Z is 1 at least), 31, so 4.1e-6 in all; eight weights at a time are added in 32 bits, 2e-7, the rest in 64.
+constexpr double kDoubt = 0x1p-17;
+constexpr double kQuickRate = 1e6;        // log2(e) / T at most: (l - top) log2(e) / T is a number then
+
 // Parts [p, p_end) of a row by one wave: their largest logits and the sums against them, in one pass: what is summed so far is
-// scaled when a larger logit comes.  The next part's runs are on their way while one's are looked at.
-template <typename L>
+// scaled when a larger logit comes.  The next part's runs are on their way while one's are looked at.  QUICK: weights in 32 bits.
+template <bool QUICK, typename L>
 __device__ __forceinline__ void first_sums(const L* row, double rate, int vocabulary, int part_length, int p, int p_end, Part* out) {
     const int lane = threadIdx.x & 63;
     if (p >= p_end) return;
@@ -296,7 +322,14 @@ __device__ __forceinline__ void first_sums(const L* row, double rate, int vocabu
                         if (sum > 0.0) sum *= weight_of(top, m, rate);
                         top = m;
                     }
-                    if (top > -INFINITY) {
+                    if constexpr (QUICK) {
+                        float w[8];
+                        const float by = fmaxf((float)rate, 1e-30f);     // (times -inf: -inf)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            w[e] = top < INFINITY ? __builtin_amdgcn_exp2f(fmaxf(x[e] - top, -INFINITY) * by) : x[e] == top ? 1.f : 0.f;
+                        sum += (double)(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+                    } else if (top > -INFINITY) {
                         double w[8];
                         weights_of(x, top, rate, w);
 #pragma unroll
@@ -398,14 +431,13 @@ template <typename L, typename Q, int THREADS> struct Walk {
     Row<L, Q> row;
     int node, count, child, asked;        // children below `child` have fallen, `asked` of them
     int summed, fallen;                   // children below `summed` were left out of the sum; entries of sh.fallen
-    int held, where;                      // the last sum, as in State
+    int held, where;                      // the last sum: kFirst, kAgain or kQuick; as in State
+    bool exact, always_exact;             // the node's first sum has to be 64 bits
     double all, whole, left;              // Z, Z when the sum was taken, r
     // the strip of 64 nodes whose children are asked next: a child per lane, and which lanes
     int strip, token;
     uint64_t kids;
-    L logit;
-    Q draft;
-    float u;
+    float logit, draft, u;
     int early_parent, early_token;        // of node threadIdx.x, on their way
 
     __device__ __forceinline__ Walk(const VerifyArgs& args, Shared& shared, int sequence) : a(args), sh(shared), b(sequence) {
@@ -421,6 +453,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
         row.top = -INFINITY;
         row.best = -1;
         row.n = a.vocabulary;
+        always_exact = exact = !a.draft && row.rate > kQuickRate;
         const bool mine = (int)threadIdx.x < min(nodes, kTree);
         early_parent = mine ? parent_in_memory(threadIdx.x) : -1;
         early_token = mine ? token_in_memory(threadIdx.x) : -1;
@@ -448,6 +481,21 @@ template <typename L, typename Q, int THREADS> struct Walk {
     __device__ __forceinline__ bool is_child(int j) const { return j < nodes && (j < kTree ? sh.parent[j] : parent_in_memory(j)) == node; }
     __device__ __forceinline__ int token_of(int j) const { return j < kTree ? sh.token[j] : token_in_memory(j); }
 
+    // Every node's token's logit and probability at its parent, all at once: a walk through sums that are there waits for memory
+    // once, not at every node
+    __device__ __forceinline__ void gather() {
+        for (int j = threadIdx.x; j < min(nodes, kTree); j += THREADS) {
+            const int64_t parent = start + max(sh.parent[j], 0);
+            const int x = max(sh.token[j], 0);
+            const L logit = (static_cast<const L*>(a.logits) + parent * a.logits_stride)[x];
+            Q draft{};
+            if (a.draft) draft = (static_cast<const Q*>(a.draft) + parent * a.draft_stride)[x];
+            sh.u[j] = a.u_accept[start + j];
+            sh.logit[j] = value(logit);
+            sh.draft[j] = value(draft);
+        }
+        __syncthreads();
+    }
     // To the next strip with children of the node, from node `from` on: what they are asked with
     __device__ __forceinline__ void look(int from) {
         const int lane = threadIdx.x & 63;
@@ -457,10 +505,20 @@ template <typename L, typename Q, int THREADS> struct Walk {
         if (!kids) return;
         // (loads of all lanes, the others' from a place that there is: a branch around them would wait for each)
         token = mine ? token_of(strip + lane) : -1;
+        if (a.all_parts && strip + 64 <= kTree) {
+            const int j = strip + lane;
+            logit = sh.logit[j];
+            draft = sh.draft[j];
+            u = sh.u[j];
+            return;
+        }
         const int x = max(token, 0);
-        logit = row.logits[x];
-        if (row.draft) draft = row.draft[x];
+        const L l = row.logits[x];
+        Q q{};
+        if (row.draft) q = row.draft[x];
         u = a.u_accept[start + min(strip + lane, nodes - 1)];
+        logit = value(l);
+        draft = value(q);
     }
     __device__ __forceinline__ void stand_on(int at, int how_many) {
         node = at;
@@ -468,6 +526,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
         child = summed = at + 1;
         fallen = asked = 0;
         left = 1.0;
+        exact = always_exact;
         row.logits = static_cast<const L*>(a.logits) + (start + (int64_t)node) * a.logits_stride;
         row.draft = a.draft && !greedy ? static_cast<const Q*>(a.draft) + (start + (int64_t)node) * a.draft_stride : nullptr;
         row.shift = 0.0;
@@ -482,12 +541,14 @@ template <typename L, typename Q, int THREADS> struct Walk {
     __device__ __forceinline__ const Part* parts_of_node() const { return parts_of(a.all_parts, start + (int64_t)node); }
     __device__ __forceinline__ const Part* parts_of_step(int turn) const { return parts_of(a.parts[turn], b); }
     __device__ __forceinline__ void take(int what, const Part* parts) {
-        if (what == kFirst) take_first(parts);
-        else take_again(parts);
+        if (what == kAgain) take_again(parts);
+        else take_first(parts);
+        held = what;
     }
     // Where the state is, with the sum that it waits for (or the last one, at a walk's end); the tree is in LDS behind it
     __device__ __forceinline__ void resume(const State& s, const Part* parts) {
         stand_on(s.node, s.count);
+        exact |= s.exact != 0;
         if (s.phase != kFirst) {
             child = s.child;
             asked = s.asked;
@@ -495,8 +556,9 @@ template <typename L, typename Q, int THREADS> struct Walk {
             row.shift = s.shift;
             row.top = s.top;
         }
-        if (parts) take(s.phase == kDone ? s.held : s.phase, parts);
+        if (parts) take(s.phase == kDone ? s.held : s.phase == kFirst && !exact && !a.draft ? kQuick : s.phase, parts);
         read_tree();
+        if (s.phase != kDone && a.all_parts) gather();
         if (s.phase != kDone) look(child);
     }
     __device__ __forceinline__ void part_range(int p, int* from, int* to) const {
@@ -527,7 +589,6 @@ template <typename L, typename Q, int THREADS> struct Walk {
         }
         whole = all = sum_of(sum);
         summed = child;
-        held = kFirst;
     }
     // .. of a sum of W
     __device__ __forceinline__ void take_again(const Part* parts) {
@@ -539,7 +600,6 @@ template <typename L, typename Q, int THREADS> struct Walk {
         }
         whole = all = sum_of(sum);
         summed = child;
-        held = kAgain;
     }
 
     // Whether a child before child j has its token x
@@ -555,7 +615,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
     __device__ __forceinline__ int ask() {
         if (row.top == -INFINITY) return kDone;                  // nothing to choose: all children fall
         while (kids && count < a.max_path && asked < kChildren) {
-            const double q = row.draft ? fmax((double)value(draft), 0.0) : 0.0, w = row.weight(value(logit), q);
+            const double q = row.draft ? fmax((double)draft, 0.0) : 0.0, w = row.weight(logit, q);
             for (; kids && asked < kChildren; kids &= kids - 1) {
                 const int l = __ffsll((unsigned long long)kids) - 1, x = of_lane(token, l), j = strip + l;
                 ++asked;
@@ -569,6 +629,12 @@ template <typename L, typename Q, int THREADS> struct Walk {
                 if (fell_before(j, x)) continue;
                 const double wx = of_lane(w, l), qx = of_lane(q, l), ux = of_lane((double)u, l);
                 const bool drawn = qx > 0.0 && left > 0.0;
+                // Too near to tell by a sum in 32 bits: once more, in 64
+                if (held == kQuick && fabs(ux * all - wx) <= kDoubt * whole) {
+                    stand_at(node, count);
+                    exact = true;
+                    return kFirst;
+                }
                 // (W is at most Z: with u at 1 or more only the rounding of Z could let a given child stand)
                 if (drawn ? ux * all * qx < wx * left : ux < 1.0 && ux * all < wx) {
                     stand_at(j, count + 1);
@@ -615,11 +681,12 @@ template <typename L, typename Q, int THREADS> struct Walk {
         return before;
     }
 
+    __device__ __forceinline__ int share(int which, int waves) const { return (int)((int64_t)a.parts_per_row * which / waves); }
     // The share of wave `which` of `waves` in the row's sums: into out[part]
-    __device__ __forceinline__ void sum_parts(bool first, int which, int waves, Part* out) {
-        const int p0 = (int)((int64_t)a.parts_per_row * which / waves), p1 = (int)((int64_t)a.parts_per_row * (which + 1) / waves);
+    template <bool QUICK> __device__ __forceinline__ void sum_parts(bool first, int which, int waves, Part* out) {
+        const int p0 = share(which, waves), p1 = share(which + 1, waves);
         if (first) {
-            first_sums(row.logits, row.rate, a.vocabulary, a.part_length, p0, p1, out);
+            first_sums<QUICK>(row.logits, row.rate, a.vocabulary, a.part_length, p0, p1, out);
             return;
         }
         for (int p = p0; p < p1; ++p) {
@@ -633,12 +700,13 @@ template <typename L, typename Q, int THREADS> struct Walk {
     __device__ __forceinline__ void sum_alone(bool first) {
         const int wave = threadIdx.x >> 6;
         __syncthreads();
-        sum_parts(first, wave, kWaves, sh.part);
+        sum_parts<false>(first, wave, kWaves, sh.part);
         __syncthreads();
     }
 
     // The smallest token at which the running sum of the weights passes u of all of it, the last one with any weight where rounding
-    // (or u >= 1) lets none; -1 where there is no weight
+    // (or u >= 1) lets none; -1 where there is no weight, kUnsure where sums in 32 bits do not tell
+    static constexpr int kUnsure = -2;
     __device__ __forceinline__ int pick(double u) {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
         __syncthreads();                  // sh.sum
@@ -682,7 +750,8 @@ template <typename L, typename Q, int THREADS> struct Walk {
             for (int p = tid; p < a.parts_per_row; p += THREADS) sh.sum[p] = -1.0;
             __syncthreads();
         }
-        double target = u * sum;
+        const double doubt = held == kQuick ? 2.0 * kDoubt * whole : 0.0;       // of the target, and of what comes before a part
+        double target = u < 1.0 ? u * sum : INFINITY;
         int chosen = -1, last = -1;
         double before = 0.0, at_chosen = 0.0;
         for (int p0 = 0; p0 < a.parts_per_row && chosen < 0; p0 += 64) {
@@ -697,7 +766,12 @@ template <typename L, typename Q, int THREADS> struct Walk {
             }
             before += of_lane(up_to, 63);
         }
-        if (chosen < 0) chosen = last, at_chosen = 0.0, target = INFINITY;
+        if (chosen < 0) {
+            if (held == kQuick) return kUnsure;
+            chosen = last;
+            at_chosen = 0.0;
+            target = INFINITY;
+        }
         target -= at_chosen;
         int from, to;
         part_range(chosen, &from, &to);
@@ -755,6 +829,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
         __syncthreads();
         double run = up_to - mine;
         for (int k = 0; k < wave; ++k) run += sh.wave_sum[k];
+        bool sure = false;
         // Every thread names its first token that passes the target; the smallest counts.  None: the largest with any weight.
         int passes = INT32_MAX, weighs = -1;
 #pragma unroll
@@ -762,9 +837,13 @@ template <typename L, typename Q, int THREADS> struct Walk {
             run += w[e];
             if (w[e] > 0.0) {
                 weighs = at + e;
-                if (run > target && passes == INT32_MAX) passes = at + e;
+                if (run > target && passes == INT32_MAX) {
+                    passes = at + e;
+                    sure = run - target > doubt && target - (run - w[e]) > doubt;
+                }
             }
         }
+        const int own = passes;
         passes = min_of(passes);
         weighs = max_of(weighs);
         if (lane == 0) sh.best[wave] = passes, sh.last[wave] = weighs;
@@ -773,6 +852,12 @@ template <typename L, typename Q, int THREADS> struct Walk {
             passes = min(passes, sh.best[k]);
             weighs = max(weighs, sh.last[k]);
         }
+        if (held == kQuick) {
+            if (passes == INT32_MAX) return kUnsure;
+            if (own == passes) sh.sure = sure;
+            __syncthreads();
+            if (!sh.sure) return kUnsure;
+        }
         return passes != INT32_MAX ? passes : weighs;
     }
 
@@ -780,7 +865,14 @@ template <typename L, typename Q, int THREADS> struct Walk {
     __device__ __forceinline__ void answer() {
         int next = -1;
         if (nodes == 0) count = 0;
-        else if (row.top > -INFINITY) next = greedy ? row.best : pick(a.u_next[b]);
+        else if (row.top > -INFINITY && greedy) next = row.best;
+        else if (row.top > -INFINITY) {
+            while ((next = pick(a.u_next[b])) == kUnsure) {
+                sum_alone(true);
+                take(kFirst, sh.part);
+                summed = node + 1;
+            }
+        }
         if (threadIdx.x == 0) {
             a.counts[b] = count;
             a.next[b] = next;
@@ -795,20 +887,20 @@ template <typename L, typename Q, int THREADS> struct Walk {
     __device__ __forceinline__ int go_on(int phase, bool taken, bool noting) {
         for (;;) {
             if (!taken) {
-                if (phase != kFirst || !a.all_parts || !kids) return phase;
-                take_first(parts_of_node());
+                if (phase != kFirst || !a.all_parts || !kids || exact) return phase;
+                take(a.draft ? kFirst : kQuick, parts_of_node());
                 where = kOfNode;
             }
             taken = false;
             phase = ask();
-            if (phase == kFirst && noting) note();
+            if (phase == kFirst && noting) note();               // (a node that is summed once more is noted once more)
             if (phase == kDone) return phase;
         }
     }
 };
 
 // blockIdx.x: parts of a row, .y: node
-template <typename L> __global__ __launch_bounds__(kStepThreads, 4) void stats_kernel(VerifyArgs a) {
+template <typename L, bool QUICK> __global__ __launch_bounds__(kStepThreads, QUICK ? 4 : 3) void stats_kernel(VerifyArgs a) {
     constexpr int kWaves = kStepThreads / 64;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     for (int64_t t = blockIdx.y; t < a.nodes; t += gridDim.y) {
@@ -823,21 +915,22 @@ template <typename L> __global__ __launch_bounds__(kStepThreads, 4) void stats_k
         const float tau = a.temperatures ? a.temperatures[b] : a.temperature;
         const double rate = tau > 0.f ? fmax(1.4426950408889634074 / (double)tau, 1e-300) : 0.0;
         const int which = blockIdx.x * kWaves + wave, waves = gridDim.x * kWaves;
-        first_sums(static_cast<const L*>(a.logits) + t * a.logits_stride, rate, a.vocabulary, a.part_length,
+        first_sums<QUICK>(static_cast<const L*>(a.logits) + t * a.logits_stride, rate, a.vocabulary, a.part_length,
                    (int)((int64_t)a.parts_per_row * which / waves), (int)((int64_t)a.parts_per_row * (which + 1) / waves), a.parts_out + t * a.parts_per_row);
     }
 }
 
-// blockIdx.x: parts of a row, .y: sequence
-template <typename L, typename Q> __global__ __launch_bounds__(kStepThreads, 2) void step_kernel(VerifyArgs a) {
+// blockIdx.x: parts of a row, .y: sequence.  DRAWN: there are the draft's probabilities, and sums are 64 bits.  Without them a first
+// sum of 32 bits is enough for almost every decision; what is not (and sums once more without what fell) waits for walk_kernel.
+template <typename L, typename Q, bool DRAWN> __global__ __launch_bounds__(kStepThreads, DRAWN ? 2 : 3) void step_kernel(VerifyArgs a) {
     constexpr int kWaves = kStepThreads / 64;
     __shared__ Shared sh;
     const int wave = threadIdx.x >> 6;
     const bool speaks = blockIdx.x == 0;
     for (int b = blockIdx.y; b < a.batch; b += gridDim.y) {
-        State s{0, 1, 1, 0, 1, kFirst, kFirst, 0, 0.0, 1.0, 0.f, 0};
+        State s{0, 1, 1, 0, 1, kFirst, kFirst, 0, 0, 0, 0.0, 1.0, 0.f, 0};
         if (!a.fresh) s = a.states[a.turn ^ 1][b];
-        if (s.phase == kDone) {
+        if (!a.fresh && (s.phase == kDone || !s.ready)) {
             if (speaks && threadIdx.x == 0) a.states[a.turn][b] = s;
             continue;
         }
@@ -851,14 +944,18 @@ template <typename L, typename Q> __global__ __launch_bounds__(kStepThreads, 2) 
             if (a.fresh && speaks) w.note();
             s.phase = w.go_on(s.phase, !a.fresh, speaks);
         }
+        const bool sums = s.phase != kDone && (DRAWN || (s.phase == kFirst && !w.exact));
         if (speaks && threadIdx.x == 0)
-            a.states[a.turn][b] = State{w.node, w.count, w.child, w.asked, w.summed, s.phase, w.held, w.where, w.row.shift, w.left, w.row.top, 0};
-        if (s.phase == kDone) continue;
-        if (s.phase == kAgain) {
+            a.states[a.turn][b] = State{w.node, w.count, w.child, w.asked, w.summed, s.phase, w.held, w.where, sums, w.exact, w.row.shift, w.left, w.row.top, 0};
+        if (!sums) continue;
+        if (DRAWN && s.phase == kAgain) {
             w.summed = w.child;
             w.collect();
         }
-        w.sum_parts(s.phase == kFirst, blockIdx.x * kWaves + wave, gridDim.x * kWaves, a.parts[a.turn] + (int64_t)b * a.parts_per_row);
+        Part* out = a.parts[a.turn] + (int64_t)b * a.parts_per_row;
+        const int which = blockIdx.x * kWaves + wave, waves = gridDim.x * kWaves;
+        if constexpr (DRAWN) w.template sum_parts<false>(s.phase == kFirst, which, waves, out);
+        else first_sums<true>(w.row.logits, w.row.rate, a.vocabulary, a.part_length, w.share(which, waves), w.share(which + 1, waves), out);
     }
 }
 
@@ -866,16 +963,17 @@ template <typename L, typename Q> __global__ __launch_bounds__(kWalkThreads, 2) 
     __shared__ Shared sh;
     for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
         __syncthreads();
-        State s{0, 1, 1, 0, 1, kFirst, kFirst, 0, 0.0, 1.0, 0.f, 0};
+        State s{0, 1, 1, 0, 1, kFirst, kFirst, 0, 0, 0, 0.0, 1.0, 0.f, 0};
         if (!a.fresh) s = a.states[a.turn][b];
         Walk<L, Q, kWalkThreads> w(a, sh, b);
         if (w.nodes > 0 && s.phase == kDone) {
             w.resume(s, s.where == kOfNode ? w.parts_of(a.all_parts, w.start + s.node) : w.parts_of_step(s.where));
             w.summed = s.summed;
         } else if (w.nodes > 0) {
-            w.resume(s, a.fresh ? nullptr : w.parts_of_step(a.turn));
+            bool taken = !a.fresh && s.ready;
+            w.where = a.turn;
+            w.resume(s, taken ? w.parts_of_step(a.turn) : nullptr);
             if (a.fresh) w.note();
-            bool taken = !a.fresh;
             while ((s.phase = w.go_on(s.phase, taken, true)) != kDone) {
                 if (s.phase == kAgain) {
                     w.summed = w.child;
@@ -901,7 +999,7 @@ struct Plan {
 size_t rounded(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
 constexpr int kMostSteps = 10;
-constexpr int kStatsGroups = 2048, kStepGroups = 512;
+constexpr int kStatsGroups = 2048, kDrawnGroups = 512, kGivenGroups = 768;
 constexpr double kAllBytes = 128e6;
 
 Plan plan_of(int64_t batch, int64_t nodes, int64_t vocabulary, int size, bool draft, int32_t max_path) {
@@ -926,7 +1024,8 @@ template <typename L, typename Q> int launch(VerifyArgs a, const Plan& plan, voi
         a.parts_out = reinterpret_cast<Part*>(work);
         a.all_parts = a.parts_out;
         work += rounded(sizeof(Part) * (size_t)a.nodes * a.parts_per_row);
-        hipLaunchKernelGGL((stats_kernel<L>), groups(a.nodes, kStatsGroups), dim3(kStepThreads), 0, stream, a);
+        if (a.draft) hipLaunchKernelGGL((stats_kernel<L, false>), groups(a.nodes, kStatsGroups), dim3(kStepThreads), 0, stream, a);
+        else hipLaunchKernelGGL((stats_kernel<L, true>), groups(a.nodes, kStatsGroups), dim3(kStepThreads), 0, stream, a);
     }
     for (int i = 0; i < 2; ++i) {
         a.parts[i] = reinterpret_cast<Part*>(work);
@@ -937,7 +1036,8 @@ template <typename L, typename Q> int launch(VerifyArgs a, const Plan& plan, voi
     a.fresh = 1;
     for (int i = 0; i < plan.steps; ++i) {
         a.turn = i & 1;
-        hipLaunchKernelGGL((step_kernel<L, Q>), groups(a.batch, kStepGroups), dim3(kStepThreads), 0, stream, a);
+        if (a.draft) hipLaunchKernelGGL((step_kernel<L, Q, true>), groups(a.batch, kDrawnGroups), dim3(kStepThreads), 0, stream, a);
+        else hipLaunchKernelGGL((step_kernel<L, float, false>), groups(a.batch, kGivenGroups), dim3(kStepThreads), 0, stream, a);
         a.fresh = 0;
     }
     hipLaunchKernelGGL((walk_kernel<L, Q>), dim3((unsigned)(a.batch < 65536 ? a.batch : 65536)), dim3(kWalkThreads), 0, stream, a);

@@ -125,3 +125,33 @@ def test_rows_longer_than_a_part_can_be():
     case["logits"][:, 20000:] = -float("inf")
     case["logits"][3, vocabulary - 1] = 30.0
     check(call(on_gpu(case), 5, 0.5), expected(case, 5, 0.5))
+
+
+@pytest.mark.parametrize("tau", [1e-7, 1e-4, 1.0, 1e8])
+def test_random_numbers_next_to_what_decides(tau):
+    """Random numbers within some 1e-7 of the place where a child stands or falls, or the next token changes: sums in 32 bits do not tell, and
+    every answer is that of 64."""
+    sizes, vocabulary = [3] * 64, 9001
+    case = make_case(77, sizes, vocabulary, torch.float32, 2, None, spread=2.0, likely=0.3)
+    case["parent"] = torch.tensor([-1, 0, 0] * 64)
+    rows = case["logits"].double()[0::3]
+    scaled = (rows - rows.amax(1, keepdim=True)) / float(np.float32(tau))
+    p = torch.exp(scaled)
+    first = p.gather(1, case["tokens"][1::3, None])[:, 0] / p.sum(1)
+    near = torch.linspace(-2e-7, 2e-7, 64, dtype=torch.float64)
+    case["u_accept"][1::3] = (first + near).clamp(0, 1).float()
+    case["u_accept"][2::3] = 1.0
+    case["tokens"][2::3] = case["tokens"][1::3]                # once fallen, it falls
+    rest = p.scatter(1, case["tokens"][1::3, None], 0.0)
+    run = rest.cumsum(1) / rest.sum(1, keepdim=True)
+    case["u_next"] = (run[torch.arange(64), torch.arange(64) * 140] + near).clamp(0, 1).float()
+    check(call(on_gpu(case), 2, tau), expected(case, 2, tau))
+    more = make_case(78, [2] * 4000, 3000, torch.float32, 1, None)                            # and where each step is a launch
+    more["logits"][:192] = case["logits"][:, :3000]
+    assert more["logits"].numel() * 4 > 70e6
+    p = torch.exp((more["logits"].double()[0::2] - more["logits"].double()[0::2].amax(1, keepdim=True)) / float(np.float32(tau)))
+    run = p.cumsum(1) / p.sum(1, keepdim=True)
+    places = torch.arange(4000) % 3000
+    more["u_next"] = (run[torch.arange(4000), places] + torch.linspace(-2e-7, 2e-7, 4000, dtype=torch.float64)).clamp(0, 1).float()
+    more["u_accept"][:] = 1.0
+    check(call(on_gpu(more), 1, tau), expected(more, 1, tau))
