@@ -195,7 +195,6 @@ struct Shared {
     double lost[kChildren];               // .. and their weights
     double wave_sum[kWalkThreads / 64];
     int32_t best[kWalkThreads / 64], last[kWalkThreads / 64];
-    int32_t sure;
 };
 
 // Steps of a sum (or least, or largest) over the lanes up to each: from 1, 2, 4 and 8 lanes below within rows of 16, then the rows'
@@ -536,6 +535,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
     __device__ __forceinline__ void stand_at(int at, int how_many) {
         stand_on(at, how_many);
         look(at + 1);
+        exact |= !a.draft && !kids;       // nothing to ask: its sum is the one that the next token is picked from
     }
     __device__ __forceinline__ const Part* parts_of(const Part* all, int64_t which) const { return all + which * a.parts_per_row; }
     __device__ __forceinline__ const Part* parts_of_node() const { return parts_of(a.all_parts, start + (int64_t)node); }
@@ -560,6 +560,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
         read_tree();
         if (s.phase != kDone && a.all_parts) gather();
         if (s.phase != kDone) look(child);
+        if (s.phase == kFirst) exact |= !a.draft && !kids;
     }
     __device__ __forceinline__ void part_range(int p, int* from, int* to) const {
         *from = (int)min((int64_t)p * a.part_length, (int64_t)a.vocabulary);
@@ -705,8 +706,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
     }
 
     // The smallest token at which the running sum of the weights passes u of all of it, the last one with any weight where rounding
-    // (or u >= 1) lets none; -1 where there is no weight, kUnsure where sums in 32 bits do not tell
-    static constexpr int kUnsure = -2;
+    // (or u >= 1) lets none; -1 where there is no weight
     __device__ __forceinline__ int pick(double u) {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
         __syncthreads();                  // sh.sum
@@ -750,7 +750,6 @@ template <typename L, typename Q, int THREADS> struct Walk {
             for (int p = tid; p < a.parts_per_row; p += THREADS) sh.sum[p] = -1.0;
             __syncthreads();
         }
-        const double doubt = held == kQuick ? 2.0 * kDoubt * whole : 0.0;       // of the target, and of what comes before a part
         double target = u < 1.0 ? u * sum : INFINITY;
         int chosen = -1, last = -1;
         double before = 0.0, at_chosen = 0.0;
@@ -767,7 +766,6 @@ template <typename L, typename Q, int THREADS> struct Walk {
             before += of_lane(up_to, 63);
         }
         if (chosen < 0) {
-            if (held == kQuick) return kUnsure;
             chosen = last;
             at_chosen = 0.0;
             target = INFINITY;
@@ -775,104 +773,68 @@ template <typename L, typename Q, int THREADS> struct Walk {
         target -= at_chosen;
         int from, to;
         part_range(chosen, &from, &to);
-        // the same among the waves' shares of it, until a thread has eight tokens
-        while (to - from > THREADS * 8) {
-            const int each = ((to - from + kWaves - 1) / kWaves + 7) & ~7;
-            int lo = (int)min((int64_t)from + (int64_t)wave * each, (int64_t)to);
-            const double mine = sum_again(row, lo, min(lo + each, to), sh.fallen, fallen, sh.fell[wave]);
-            __syncthreads();
-            if (lane == 0) sh.wave_sum[wave] = mine;
-            __syncthreads();
-            before = 0.0;
-            chosen = last = -1;
-            for (int w = 0; w < kWaves && chosen < 0; ++w) {
-                const double s = sh.wave_sum[w];
-                if (s > 0.0) {
-                    last = w;
-                    if (before + s > target) chosen = w, at_chosen = before;
-                }
-                before += s;
+        int found = -1;
+        for (; from < to; from += THREADS * 8) {
+            // eight tokens a thread: threads' sums, then the tokens of each thread
+            double w[8], mine = 0.0;
+            int i = from + tid * 8, at = i;
+            if (row.n < 8) {              // a token per thread
+                at = i = from + tid;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = 0.0;
+                if (i < to) w[0] = row.weight(value(row.logits[i]), row.proposed(i));
+            } else {
+                at = first_of(i, row.n);
+                Eight<Q> draft = {};
+                if (row.draft && row.shift > 0.0) draft = load_eight(row.draft, i, row.n);
+                row.eight(load_eight(row.logits, i, row.n), draft, w);
+                leave_out(outside(at, i, to), 0.0, w);
             }
-            if (chosen < 0) {
-                if (last < 0) return -1;
-                chosen = last;
-                at_chosen = 0.0;
-                target = INFINITY;
+            for (int k = 0; k < fallen; ++k) {
+                const int f = sh.fallen[k] - at;
+                if (f >= 0 && f < 8) leave_out(1u << f, 0.0, w);
             }
-            target -= at_chosen;
-            from = (int)min((int64_t)from + (int64_t)chosen * each, (int64_t)to);
-            to = min(from + each, to);
-        }
-        double w[8], mine = 0.0;
-        int i = from + tid * 8, at = i;
-        if (row.n < 8) {                  // a token per thread
-            at = i = from + tid;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = 0.0;
-            if (i < to) w[0] = row.weight(value(row.logits[i]), row.proposed(i));
-        } else {
-            at = first_of(i, row.n);
-            Eight<Q> draft = {};
-            if (row.draft && row.shift > 0.0) draft = load_eight(row.draft, i, row.n);
-            row.eight(load_eight(row.logits, i, row.n), draft, w);
-            leave_out(outside(at, i, to), 0.0, w);
-        }
-        for (int k = 0; k < fallen; ++k) {
-            const int f = sh.fallen[k] - at;
-            if (f >= 0 && f < 8) leave_out(1u << f, 0.0, w);
-        }
+            for (int e = 0; e < 8; ++e) mine += w[e];
+            const double up_to = sum_up_to(mine);
+            __syncthreads();
+            if (lane == 63) sh.wave_sum[wave] = up_to;
+            __syncthreads();
+            double run = up_to - mine, here = 0.0;
+            for (int k = 0; k < kWaves; ++k) {
+                if (k < wave) run += sh.wave_sum[k];
+                here += sh.wave_sum[k];
+            }
+            // Every thread names its first token that passes the target; the smallest counts.  None: the largest with any weight.
+            int passes = INT32_MAX, weighs = -1;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mine += w[e];
-        const double up_to = sum_up_to(mine);
-        __syncthreads();
-        if (lane == 63) sh.wave_sum[wave] = up_to;
-        __syncthreads();
-        double run = up_to - mine;
-        for (int k = 0; k < wave; ++k) run += sh.wave_sum[k];
-        bool sure = false;
-        // Every thread names its first token that passes the target; the smallest counts.  None: the largest with any weight.
-        int passes = INT32_MAX, weighs = -1;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            run += w[e];
-            if (w[e] > 0.0) {
-                weighs = at + e;
-                if (run > target && passes == INT32_MAX) {
-                    passes = at + e;
-                    sure = run - target > doubt && target - (run - w[e]) > doubt;
+            for (int e = 0; e < 8; ++e) {
+                run += w[e];
+                if (w[e] > 0.0) {
+                    weighs = at + e;
+                    if (run > target && passes == INT32_MAX) passes = at + e;
                 }
             }
-        }
-        const int own = passes;
-        passes = min_of(passes);
-        weighs = max_of(weighs);
-        if (lane == 0) sh.best[wave] = passes, sh.last[wave] = weighs;
-        __syncthreads();
-        for (int k = 0; k < kWaves; ++k) {
-            passes = min(passes, sh.best[k]);
-            weighs = max(weighs, sh.last[k]);
-        }
-        if (held == kQuick) {
-            if (passes == INT32_MAX) return kUnsure;
-            if (own == passes) sh.sure = sure;
+            passes = min_of(passes);
+            weighs = max_of(weighs);
+            if (lane == 0) sh.best[wave] = passes, sh.last[wave] = weighs;
             __syncthreads();
-            if (!sh.sure) return kUnsure;
+            for (int k = 0; k < kWaves; ++k) {
+                passes = min(passes, sh.best[k]);
+                weighs = max(weighs, sh.last[k]);
+            }
+            if (weighs >= 0) found = weighs;
+            if (passes != INT32_MAX) return passes;
+            target -= here;
         }
-        return passes != INT32_MAX ? passes : weighs;
+        return found;
     }
 
     // The end of a sequence's walk
     __device__ __forceinline__ void answer() {
         int next = -1;
         if (nodes == 0) count = 0;
-        else if (row.top > -INFINITY && greedy) next = row.best;
-        else if (row.top > -INFINITY) {
-            while ((next = pick(a.u_next[b])) == kUnsure) {
-                sum_alone(true);
-                take(kFirst, sh.part);
-                summed = node + 1;
-            }
-        }
+        else if (row.top > -INFINITY) next = greedy ? row.best : pick(a.u_next[b]);
         if (threadIdx.x == 0) {
             a.counts[b] = count;
             a.next[b] = next;
@@ -921,7 +883,8 @@ template <typename L, bool QUICK> __global__ __launch_bounds__(kStepThreads, QUI
 }
 
 // blockIdx.x: parts of a row, .y: sequence.  DRAWN: there are the draft's probabilities, and sums are 64 bits.  Without them a first
-// sum of 32 bits is enough for almost every decision; what is not (and sums once more without what fell) waits for walk_kernel.
+// sum of 32 bits is enough for almost every decision; rows whose sum has to be 64 bits wait for last_kernel, sums without what fell for
+// walk_kernel.
 template <typename L, typename Q, bool DRAWN> __global__ __launch_bounds__(kStepThreads, DRAWN ? 2 : 3) void step_kernel(VerifyArgs a) {
     constexpr int kWaves = kStepThreads / 64;
     __shared__ Shared sh;
@@ -959,6 +922,29 @@ template <typename L, typename Q, bool DRAWN> __global__ __launch_bounds__(kStep
     }
 }
 
+// Sums of 64 bits where steps made none: of the row that a sequence's next token is picked from, and of rows whose children's fate
+// sums of 32 bits do not tell.  They go to the buffer that the last step did not write.  blockIdx.x: parts of a row, .y: sequence
+__device__ __forceinline__ bool wants_last(const State& s, double rate) {
+    return s.phase == kDone ? s.held == kQuick && rate != 0.0 : s.phase == kFirst && !s.ready;
+}
+__device__ __forceinline__ double rate_of(const VerifyArgs& a, int b) {
+    const float tau = a.temperatures ? a.temperatures[b] : a.temperature;
+    return tau > 0.f ? fmax(1.4426950408889634074 / (double)tau, 1e-300) : 0.0;
+}
+template <typename L> __global__ __launch_bounds__(kStepThreads, 3) void last_kernel(VerifyArgs a) {
+    constexpr int kWaves = kStepThreads / 64;
+    const int which = blockIdx.x * kWaves + (threadIdx.x >> 6), waves = gridDim.x * kWaves;
+    for (int b = blockIdx.y; b < a.batch; b += gridDim.y) {
+        const State s = a.states[a.turn][b];
+        const int start = min(max(a.q_starts[b], 0), a.nodes), nodes = min(a.q_starts[b + 1], a.nodes) - start;
+        const double rate = rate_of(a, b);
+        if (nodes <= 0 || !wants_last(s, rate)) continue;
+        first_sums<false>(static_cast<const L*>(a.logits) + (start + (int64_t)s.node) * a.logits_stride, rate, a.vocabulary, a.part_length,
+                          (int)((int64_t)a.parts_per_row * which / waves), (int)((int64_t)a.parts_per_row * (which + 1) / waves),
+                          a.parts[a.turn ^ 1] + (int64_t)b * a.parts_per_row);
+    }
+}
+
 template <typename L, typename Q> __global__ __launch_bounds__(kWalkThreads, 2) void walk_kernel(VerifyArgs a) {
     __shared__ Shared sh;
     for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
@@ -966,13 +952,16 @@ template <typename L, typename Q> __global__ __launch_bounds__(kWalkThreads, 2) 
         State s{0, 1, 1, 0, 1, kFirst, kFirst, 0, 0, 0, 0.0, 1.0, 0.f, 0};
         if (!a.fresh) s = a.states[a.turn][b];
         Walk<L, Q, kWalkThreads> w(a, sh, b);
+        const bool last = w.nodes > 0 && !a.fresh && !a.draft && wants_last(s, w.row.rate);
         if (w.nodes > 0 && s.phase == kDone) {
-            w.resume(s, s.where == kOfNode ? w.parts_of(a.all_parts, w.start + s.node) : w.parts_of_step(s.where));
+            if (last) s.held = kFirst;
+            w.resume(s, last ? w.parts_of_step(a.turn ^ 1) : s.where == kOfNode ? w.parts_of(a.all_parts, w.start + s.node) : w.parts_of_step(s.where));
             w.summed = s.summed;
         } else if (w.nodes > 0) {
-            bool taken = !a.fresh && s.ready;
+            if (last) s.exact = 1;
+            bool taken = last || (!a.fresh && s.ready);
             w.where = a.turn;
-            w.resume(s, taken ? w.parts_of_step(a.turn) : nullptr);
+            w.resume(s, taken ? w.parts_of_step(last ? a.turn ^ 1 : a.turn) : nullptr);
             if (a.fresh) w.note();
             while ((s.phase = w.go_on(s.phase, taken, true)) != kDone) {
                 if (s.phase == kAgain) {
@@ -982,6 +971,11 @@ template <typename L, typename Q> __global__ __launch_bounds__(kWalkThreads, 2) 
                 w.sum_alone(s.phase == kFirst);
                 w.take(s.phase, sh.part);
                 taken = true;
+            }
+            if (w.held == kQuick && !w.greedy && w.row.top > -INFINITY) {       // the sum that the next token is picked from
+                w.sum_alone(true);
+                w.take(kFirst, sh.part);
+                w.summed = w.node + 1;
             }
         }
         w.answer();
@@ -999,7 +993,7 @@ struct Plan {
 size_t rounded(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
 constexpr int kMostSteps = 10;
-constexpr int kStatsGroups = 2048, kDrawnGroups = 512, kGivenGroups = 768;
+constexpr int kStatsGroups = 2048, kDrawnGroups = 512, kGivenGroups = 768, kLastGroups = 768;
 constexpr double kAllBytes = 128e6;
 
 Plan plan_of(int64_t batch, int64_t nodes, int64_t vocabulary, int size, bool draft, int32_t max_path) {
@@ -1037,9 +1031,10 @@ template <typename L, typename Q> int launch(VerifyArgs a, const Plan& plan, voi
     for (int i = 0; i < plan.steps; ++i) {
         a.turn = i & 1;
         if (a.draft) hipLaunchKernelGGL((step_kernel<L, Q, true>), groups(a.batch, kDrawnGroups), dim3(kStepThreads), 0, stream, a);
-        else hipLaunchKernelGGL((step_kernel<L, float, false>), groups(a.batch, kGivenGroups), dim3(kStepThreads), 0, stream, a);
+        else hipLaunchKernelGGL((step_kernel<L, float, false>), groups(a.batch, plan.all ? 1 : kGivenGroups), dim3(kStepThreads), 0, stream, a);
         a.fresh = 0;
     }
+    if (!a.draft) hipLaunchKernelGGL((last_kernel<L>), groups(a.batch, kLastGroups), dim3(kStepThreads), 0, stream, a);
     hipLaunchKernelGGL((walk_kernel<L, Q>), dim3((unsigned)(a.batch < 65536 ? a.batch : 65536)), dim3(kWalkThreads), 0, stream, a);
     FSTA_HIP_OK(hipGetLastError());
     return FSTA_OK;
