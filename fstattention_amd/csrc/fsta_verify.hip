@@ -434,10 +434,12 @@ template <typename L, typename Q, int THREADS> struct Walk {
     bool exact, always_exact;             // the node's first sum has to be 64 bits
     double all, whole, left;              // Z, Z when the sum was taken, r
     // the strip of 64 nodes whose children are asked next: a child per lane, and which lanes
-    int strip, token;
-    uint64_t kids;
-    float logit, draft, u;
+    int strip = 0, token = -1;
+    uint64_t kids = 0;
+    float logit = 0.f, draft = 0.f, u = 0.f;
     int early_parent, early_token;        // of node threadIdx.x, on their way
+    const Part* ahead_of = nullptr;       // the sums of the first child's row, which the walk is likely to need next
+    Part ahead{0.0, 0.f, 0};
 
     __device__ __forceinline__ Walk(const VerifyArgs& args, Shared& shared, int sequence) : a(args), sh(shared), b(sequence) {
         start = min(max(a.q_starts[b], 0), a.nodes);
@@ -570,7 +572,12 @@ template <typename L, typename Q, int THREADS> struct Walk {
     // The parts of the first sum of the row: its largest logit, Z.  (Every wave writes the same to sh.sum.)
     __device__ __forceinline__ void take_first(const Part* parts) {
         const int lane = threadIdx.x & 63;
-        Part mine = parts[min(lane, a.parts_per_row - 1)];
+        Part mine = ahead;
+        if (ahead_of != parts) mine = parts[min(lane, a.parts_per_row - 1)];
+        if (a.all_parts && kids) {        // (on their way while the children are asked)
+            ahead_of = parts_of(a.all_parts, start + (int64_t)strip + __ffsll((unsigned long long)kids) - 1);
+            ahead = ahead_of[min(lane, a.parts_per_row - 1)];
+        }
         if (lane >= a.parts_per_row) mine = Part{0.0, -INFINITY, INT32_MAX};
         float top = mine.top;
         int best = mine.best;
@@ -970,6 +977,7 @@ template <typename L, typename Q> __global__ __launch_bounds__(kWalkThreads, 2) 
                 }
                 w.sum_alone(s.phase == kFirst);
                 w.take(s.phase, sh.part);
+                if (s.phase == kAgain) w.look(w.child);
                 taken = true;
             }
             if (w.held == kQuick && !w.greedy && w.row.top > -INFINITY) {       // the sum that the next token is picked from
@@ -993,8 +1001,8 @@ struct Plan {
 size_t rounded(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
 constexpr int kMostSteps = 10;
-constexpr int kStatsGroups = 2048, kDrawnGroups = 512, kGivenGroups = 768, kLastGroups = 768;
-constexpr double kAllBytes = 128e6;
+constexpr int kStatsGroups = 2048, kDrawnGroups = 512, kGivenGroups = 2048, kLastGroups = 768;
+constexpr double kAllBytes = 160e6;
 
 Plan plan_of(int64_t batch, int64_t nodes, int64_t vocabulary, int size, bool draft, int32_t max_path) {
     Plan p;

@@ -365,3 +365,28 @@ def test_a_token_with_nearly_all_mass_falls(draft):
     if draft is not None:
         case["draft_probs"] = torch.zeros((2 * n, vocabulary))
     check(call(on_gpu(case), 3), expected(case, 3))
+
+
+@pytest.mark.parametrize("draft", [None, torch.float32])
+@pytest.mark.parametrize("vocabulary", [40, 3000])
+def test_more_fall_than_there_are_launches(draft, vocabulary):
+    """Twenty children of one node, drawn or given, of which any number falls; the ones behind those that fell are asked as well."""
+    n = 40
+    case = make_case(9, [21] * n, vocabulary, torch.float32, 20, None, spread=1.5)
+    case["parent"] = torch.tensor(([-1] + [0] * 20) * n)
+    g = torch.Generator().manual_seed(4)
+    case["tokens"] = torch.stack([torch.randperm(vocabulary, generator=g)[:21] for _ in range(n)]).reshape(-1)
+    if draft is not None:
+        case["draft_probs"] = torch.softmax(case["logits"] + torch.randn((21 * n, vocabulary), generator=g), -1)
+    else:                                                      # the first ones have all but a thousandth of what is left, each
+        rows = case["logits"].view(n, 21, vocabulary)
+        for b in range(n):
+            for i in range(1, 1 + b % 6):
+                rows[b, 0, case["tokens"].view(n, 21)[b, i]] = 70.0 - 10.0 * i
+    u = case["u_accept"].view(n, 21)
+    u[:] = 1.0 - 2.0 ** -24
+    for b in range(n):
+        u[b, 1 + b % 20] = 0.0                                 # stands, if anything is left of it
+    check(call(on_gpu(case), 3), expected(case, 3))
+    u[:] = 1.0 - 2.0 ** -24
+    check(call(on_gpu(case), 3), expected(case, 3))
