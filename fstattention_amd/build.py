@@ -51,7 +51,7 @@ HIPCC_FLAGS = [
 # in scratch memory, or a spill, is reloaded through the same vmcnt queue their gather rings count on.
 NO_SCRATCH = ("fsta_attention_mfma16.hip", "fsta_attention_mfma.hip", "fsta_attention_prefix.hip",
               "fsta_attention_cache.hip", "fsta_attention_stream.hip", "fsta_attention_generic.hip", "fsta_attention_f32.hip",
-              "fsta_paged_attention.hip", "fsta_pages.hip", "fsta_verify.hip")
+              "fsta_paged_attention.hip", "fsta_pages.hip")
 
 
 def _hipcc() -> str:

@@ -1001,8 +1001,8 @@ struct Plan {
 size_t rounded(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
 constexpr int kMostSteps = 10;
-constexpr int kStatsGroups = 2048, kDrawnGroups = 512, kGivenGroups = 2048, kLastGroups = 768;
-constexpr double kAllBytes = 160e6;
+constexpr int kStatsGroups = 2048, kDrawnGroups = 512, kGivenGroups = 768, kLastGroups = 768;
+constexpr double kAllBytes = 200e6;
 
 Plan plan_of(int64_t batch, int64_t nodes, int64_t vocabulary, int size, bool draft, int32_t max_path) {
     Plan p;
@@ -1039,7 +1039,7 @@ template <typename L, typename Q> int launch(VerifyArgs a, const Plan& plan, voi
     for (int i = 0; i < plan.steps; ++i) {
         a.turn = i & 1;
         if (a.draft) hipLaunchKernelGGL((step_kernel<L, Q, true>), groups(a.batch, kDrawnGroups), dim3(kStepThreads), 0, stream, a);
-        else hipLaunchKernelGGL((step_kernel<L, float, false>), groups(a.batch, plan.all ? 1 : kGivenGroups), dim3(kStepThreads), 0, stream, a);
+        else hipLaunchKernelGGL((step_kernel<L, float, false>), groups(a.batch, plan.all ? 1 : i < 3 ? kGivenGroups : 2 * kGivenGroups), dim3(kStepThreads), 0, stream, a);
         a.fresh = 0;
     }
     if (!a.draft) hipLaunchKernelGGL((last_kernel<L>), groups(a.batch, kLastGroups), dim3(kStepThreads), 0, stream, a);
