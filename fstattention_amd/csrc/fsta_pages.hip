@@ -195,19 +195,30 @@ __device__ __forceinline__ void list_copy(const TableArgs& a, int from, int to, 
     a.list[atomicAdd(a.listed, 1)] = Copy{from, to, rows};      // (their order is nobody's concern: no two touch one page)
 }
 
-// One wave: which of a group's pages are free
+// One wave: which of a group's pages are free, 32 a lane
 __device__ void survey_group(const TableArgs& a, int g) {
     const int lane = threadIdx.x & 63;
+    const int64_t first = (int64_t)g * kGroup + lane * 32, pages = a.num_pages;
+    int4 refs[8];                         // (all on their way at once; places behind the last page are read at its own)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int64_t p = first + 4 * i;
+        if (pages >= 4) __builtin_memcpy(&refs[i], a.refs + min(p, pages - 4), sizeof(int4));
+    }
     uint32_t word = 0;
-    int total = 0;
-#pragma unroll 8
-    for (int i = 0; i < kGroup / 64; ++i) {
-        const int64_t p = (int64_t)g * kGroup + i * 64 + lane;
-        const uint64_t free = __ballot(p < a.num_pages && a.refs[p] <= 0);
-        total += __popcll(free);
-        if (lane >> 1 == i) word = (uint32_t)(lane & 1 ? free >> 32 : free);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int held[4] = {refs[i].x, refs[i].y, refs[i].z, refs[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) word |= (uint32_t)(held[e] <= 0) << (4 * i + e);
+    }
+    if (first + 32 > pages) {             // the last pages, one by one
+        word = 0;
+        for (int e = 0; e < 32; ++e)
+            if (first + e < pages && a.refs[first + e] <= 0) word |= 1u << e;
     }
     a.free_bits[(int64_t)g * (kGroup / 32) + lane] = word;
+    const int total = __shfl((int)wave_prefix_sum((uint32_t)__popc(word)), 63);
     if (lane == 0) a.group_free[g] = total;
 }
 
@@ -225,8 +236,10 @@ struct FreePages {
     __device__ bool seek(const TableArgs& a, int rank) {
         const int lane = threadIdx.x & 63, groups = groups_of(a);
         int base = first + count;
+        int next = group + 1 + lane < groups ? a.group_free[group + 1 + lane] : 0;
         for (int g0 = group + 1; g0 < groups; g0 += 64) {
-            const int mine = g0 + lane < groups ? a.group_free[g0 + lane] : 0;
+            const int mine = next;
+            next = g0 + 64 + lane < groups ? a.group_free[g0 + 64 + lane] : 0;
             const int up_to = (int)wave_prefix_sum((uint32_t)mine);
             const uint64_t hit = __ballot(base + up_to > rank);
             if (hit) {
@@ -266,7 +279,13 @@ struct FreePages {
 
 __device__ __forceinline__ int needed_before(const TableArgs& a, int i) {
     int sum = 0;
-    for (int j = threadIdx.x & 63; j < i; j += 64) sum += a.need[j];
+    for (int j = threadIdx.x & 63; j < i; j += 8 * 64) {
+        int some[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) some[k] = a.need[min(j + 64 * k, i - 1)];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum += j + 64 * k < i ? some[k] : 0;
+    }
     return sum_of(sum);
 }
 
@@ -282,53 +301,72 @@ __device__ __forceinline__ Entry judge(const TableArgs& a, int n, int slot, int 
     return e;
 }
 
+// Entries s0 + 64 k + lane of a row, for eight k at once; -1 behind its end
+constexpr int kStrips = 8;
+__device__ __forceinline__ void load_strips(const int32_t* row, int s0, int end, int (&page)[kStrips]) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int k = 0; k < kStrips; ++k) page[k] = row[min(s0 + 64 * k + lane, end - 1)];
+#pragma unroll
+    for (int k = 0; k < kStrips; ++k)
+        if (s0 + 64 * k + lane >= end) page[k] = -1;
+}
+
 __device__ void survey_fit(const TableArgs& a, int b) {
     const int lane = threadIdx.x & 63;
     const int n = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.width << a.page_shift);
     const int keep = (int)(((int64_t)n + (1 << a.page_shift) - 1) >> a.page_shift);
-    int need = 0;
-    for (int s = lane; s < keep; s += 64) {
-        const int page = a.table[(int64_t)b * a.width + s];
-        const Entry e = judge(a, n, s, page);
-        need += e.wanted || (e.tail && a.refs[page] > 1);
+    const int32_t* row = a.table + (int64_t)b * a.width;
+    int need = 0, last = -1;
+    if (keep > 0) last = row[keep - 1];   // (meanwhile the others come)
+    for (int s0 = 0; s0 < keep; s0 += 64 * kStrips) {
+        int page[kStrips];
+        load_strips(row, s0, keep, page);
+#pragma unroll
+        for (int k = 0; k < kStrips; ++k) need += s0 + 64 * k + lane < keep && (page[k] < 0 || page[k] >= a.num_pages);
     }
     need = sum_of(need);
-    if (lane == 0) a.need[b] = need;
+    const bool copies = judge(a, n, keep - 1, last).tail && a.refs[last] > 1;
+    if (lane == 0) {
+        a.need[b] = need + copies;
+        a.row_lens[b] = copies;           // the last page is one that others hold too (refs change in the next launch)
+    }
 }
 
 __device__ void assign_fit(const TableArgs& a, int b, uint16_t* ids) {
     const int lane = threadIdx.x & 63;
     const int n = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.width << a.page_shift);
     const int need = a.need[b];
+    const bool copies = a.row_lens[b] != 0;
+    int32_t* row = a.table + (int64_t)b * a.width;
     int next = need ? needed_before(a, b) : 0, missing = 0;
     FreePages free{ids, -1, 0, 0};
-    bool over = false;                    // need says whether a tail that others hold is among it: refs change by now
-    int open = 0;
-    {
-        const int keep = (int)(((int64_t)n + (1 << a.page_shift) - 1) >> a.page_shift);
-        if (need)
-            for (int s = lane; s < keep; s += 64) open += judge(a, n, s, a.table[(int64_t)b * a.width + s]).wanted;
-        over = sum_of(open) < need;
-    }
-    for (int s0 = 0; s0 < a.width; s0 += 64) {
-        const int s = s0 + lane;
-        const int page = s < a.width ? a.table[(int64_t)b * a.width + s] : -1;
-        const Entry e = judge(a, n, s, page);
-        const bool copied = e.tail && over, wanted = s < a.width && (e.wanted || copied);
-        const uint64_t all = __ballot(wanted);
-        int fresh = -1;
-        if (all) {
-            fresh = free.take(a, wanted, next + __popcll(all & ((1ull << lane) - 1)));
-            next += __popcll(all);
-            missing += __popcll(__ballot(wanted && fresh < 0));
+    for (int s0 = 0; s0 < a.width; s0 += 64 * kStrips) {
+        int page[kStrips];
+        load_strips(row, s0, a.width, page);
+#pragma unroll 1
+        for (int k = 0; k < kStrips; ++k) {
+            int own = page[0];            // (one after the other to the front: a register cannot be chosen by a number)
+#pragma unroll
+            for (int j = 0; j < kStrips - 1; ++j) page[j] = page[j + 1];
+            const int s = s0 + 64 * k + lane;
+            const Entry e = judge(a, n, s, own);
+            const bool copied = e.tail && copies, wanted = s < a.width && (e.wanted || copied);
+            const uint64_t all = __ballot(wanted);
+            int fresh = -1;
+            if (all) {
+                fresh = free.take(a, wanted, next + __popcll(all & ((1ull << lane) - 1)));
+                next += __popcll(all);
+                missing += __popcll(__ballot(wanted && fresh < 0));
+            }
+            if (s >= a.width) continue;
+            const int now = fresh >= 0 ? fresh : e.inside && e.named ? own : -1;
+            if (now == own) continue;
+            row[s] = now;
+            if (fresh >= 0) a.refs[fresh] = 1;
+            if (e.named) atomicSub(a.refs + own, 1);
+            if (copied) list_copy(a, own, fresh, n & ((1 << a.page_shift) - 1));
         }
-        if (s >= a.width) continue;
-        const int now = fresh >= 0 ? fresh : e.inside && e.named ? page : -1;
-        if (now == page) continue;
-        a.table[(int64_t)b * a.width + s] = now;
-        if (fresh >= 0) a.refs[fresh] = 1;
-        if (e.named) atomicSub(a.refs + page, 1);
-        if (copied) list_copy(a, page, fresh, n & ((1 << a.page_shift) - 1));
     }
     if (lane == 0) a.missing[b] = missing;
 }
@@ -526,7 +564,7 @@ template <bool FORK> int launch_table(const TableArgs& a, const fsta_paged_pool*
     c.listed = a.listed;
     c.num_pages = c.into_pages = a.num_pages;
     c.page_shift = a.page_shift;
-    return launch_copies(c, (int32_t)rows, FORK ? 65536 : 2048, pools, pools, layers, stream);
+    return launch_copies(c, (int32_t)rows, FORK ? 65536 : 512, pools, pools, layers, stream);
 }
 
 int check_table(const char* who, int32_t batch, int32_t width, int32_t page_size, const void* refs, const void* table, const void* lens,
