@@ -367,9 +367,7 @@ def test_a_token_with_nearly_all_mass_falls(draft):
     check(call(on_gpu(case), 3), expected(case, 3))
 
 
-@pytest.mark.parametrize("draft", [None, torch.float32])
-@pytest.mark.parametrize("vocabulary", [40, 3000])
-def test_more_fall_than_there_are_launches(draft, vocabulary):
+def cases_of_more_that_fall(draft, vocabulary):
     """Twenty children of one node, drawn or given, of which any number falls; the ones behind those that fell are asked as well."""
     n = 40
     case = make_case(9, [21] * n, vocabulary, torch.float32, 20, None, spread=1.5)
@@ -387,6 +385,13 @@ def test_more_fall_than_there_are_launches(draft, vocabulary):
     u[:] = 1.0 - 2.0 ** -24
     for b in range(n):
         u[b, 1 + b % 20] = 0.0                                 # stands, if anything is left of it
-    check(call(on_gpu(case), 3), expected(case, 3))
+    yield case
     u[:] = 1.0 - 2.0 ** -24
-    check(call(on_gpu(case), 3), expected(case, 3))
+    yield case
+
+
+@pytest.mark.parametrize("draft", [None, torch.float32])
+@pytest.mark.parametrize("vocabulary", [40, 3000])
+def test_more_fall_than_there_are_launches(draft, vocabulary):
+    for case in cases_of_more_that_fall(draft, vocabulary):
+        check(call(on_gpu(case), 3), expected(case, 3))

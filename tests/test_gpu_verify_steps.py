@@ -1,13 +1,37 @@
-"""Acceptance of drafted tokens where there are too many rows to sum all of them: a launch per step of all walks, and what is left of
-long ones behind them."""
+"""Acceptance of drafted tokens where there are too many rows to sum all of them first: a launch per step of all walks, and what is left
+of long ones behind them.  Each case also runs with its rows alone, most of them few enough to be summed first."""
 import numpy as np
 import pytest
 import torch
 
 import fstattention_amd as fsta
-from test_gpu_verify import call, check, expected, make_case, on_gpu
+from fstattention_amd import _lib
+from test_gpu_verify import call, cases_of_more_that_fall, check, expected, make_case, on_gpu
 
 pytestmark = pytest.mark.gpu
+
+
+def by_steps(case):
+    """The case on the GPU with rows behind the last sequence, until there are too many to sum all."""
+    gpu = on_gpu(case)
+    nodes, vocabulary = gpu["logits"].shape
+    size = gpu["logits"].element_size()
+    more = max(int(200e6 / (vocabulary * size)) + 1 - nodes, 0)
+    pad = lambda t, x: torch.cat([t, torch.full((more, *t.shape[1:]), x, dtype=t.dtype, device="cuda")])
+    gpu = {**gpu, "logits": pad(gpu["logits"], 7.0), "tokens": pad(gpu["tokens"], 0), "parent": pad(gpu["parent"], 0), "u_accept": pad(gpu["u_accept"], 0.0),
+           "draft_probs": None if gpu["draft_probs"] is None else pad(gpu["draft_probs"], 0.5)}
+    # no room for a sum of every row
+    code = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}[case["logits"].dtype]
+    work = [_lib.load().fsta_verify_workspace_bytes(1, nodes + more + i, vocabulary, code, case["draft_probs"] is not None) for i in range(2)]
+    assert work[0] == work[1]
+    return gpu
+
+
+def check_both(case, *args, what=""):
+    want = expected(case, *args)
+    tau = [torch.tensor(a).cuda() if isinstance(a, list) else a for a in args]
+    check(call(by_steps(case), *tau), want, what + " by steps")
+    check(call(on_gpu(case), *tau), want, what + " alone")
 
 
 @pytest.mark.parametrize("dtype,draft,vocabulary", [(torch.bfloat16, None, 50021), (torch.float16, torch.float32, 50021), (torch.float32, None, 32000),
@@ -15,12 +39,9 @@ pytestmark = pytest.mark.gpu
 def test_trees(dtype, draft, vocabulary):
     sizes = [1, 30, 0, 64, 17, 90, 2, 45, 80, 64, 100, 33, 64, 200, 64, 64] + [5] * 20
     case = make_case(vocabulary + 1, sizes, vocabulary, dtype, 4, draft)
-    assert case["logits"].numel() * case["logits"].element_size() > 70e6
-    gpu = on_gpu(case)
-    check(call(gpu, 40), expected(case, 40))
-    check(call(gpu, 3, 0.8), expected(case, 3, 0.8), "cut")
-    tau = [0.0, 1.0, 0.5, 1.7] * 9
-    check(call(gpu, 12, torch.tensor(tau).cuda()), expected(case, 12, tau), "mixed")
+    check_both(case, 40)
+    check_both(case, 3, 0.8, what="cut")
+    check_both(case, 12, [0.0, 1.0, 0.5, 1.7] * 9, what="mixed")
 
 
 @pytest.mark.parametrize("draft", [None, torch.float32])
@@ -38,13 +59,11 @@ def test_long_paths(draft):
                 case["logits"][s + i - 1, case["tokens"][s + i]] = 25.0
                 if draft is not None:
                     case["draft_probs"][s + i - 1, case["tokens"][s + i]] = 0.5
-    assert case["logits"].numel() * 4 > 70e6 and n == 768
+    assert n == 768
     case["u_accept"][200] = 1.0                                # one falls
-    gpu = on_gpu(case)
-    want = expected(case, 64)
-    assert want[1].max() >= 59
-    check(call(gpu, 64), want)
-    check(call(gpu, 25), expected(case, 25))
+    assert expected(case, 64)[1].max() >= 59
+    check_both(case, 64)
+    check_both(case, 25)
 
 
 @pytest.mark.parametrize("draft", [None, torch.float32])
@@ -64,15 +83,15 @@ def test_many_that_fall(draft):
         rows[b, 0] = -float("inf")
         rows[b, 0, case["tokens"].view(30, 40)[b, kids]] = keep
     case["u_accept"].view(30, 40)[10:13] = 1.0                 # and all of them fall
-    assert case["logits"].numel() * 4 > 70e6
-    check(call(on_gpu(case), 9), expected(case, 9))
+    check_both(case, 9)
     case["u_accept"][::3] = 0.3
-    check(call(on_gpu(case), 9), expected(case, 9))
+    check_both(case, 9)
 
 
 @pytest.mark.parametrize("tau", [0.0, 1.0])
-def test_masked_and_infinite_rows(tau):
-    case = make_case(21, [6] * 400, 16000, torch.bfloat16, 2, None)
+@pytest.mark.parametrize("draft", [None, torch.bfloat16])
+def test_masked_and_infinite_rows(tau, draft):
+    case = make_case(21, [6] * 400, 16000, torch.bfloat16, 2, draft)
     rows = case["logits"].view(400, 6, 16000)
     inf = float("inf")
     rows[0::8] = -inf
@@ -81,22 +100,22 @@ def test_masked_and_infinite_rows(tau):
     rows[3::8, :, [3, 9000]] = inf
     rows[4::8, :, 15999] = torch.finfo(torch.bfloat16).max
     rows[5::8] = torch.finfo(torch.bfloat16).min
-    assert rows.numel() * 2 > 70e6
-    check(call(on_gpu(case), 6, tau), expected(case, 6, tau))
+    check_both(case, 6, tau)
 
 
-def test_captured_and_replayed():
-    cases = [make_case(s, [64] * 20 + [3] * 10, 30000, torch.bfloat16, 3, torch.bfloat16 if s < 9 else None) for s in (1, 2, 3)]
-    held = on_gpu(cases[0])
-    assert held["logits"].numel() * 2 > 70e6
+@pytest.mark.parametrize("draft", [None, torch.bfloat16])
+def test_captured_and_replayed(draft):
+    cases = [make_case(s, [64] * 20 + [3] * 10, 30000, torch.bfloat16, 3, draft) for s in (1, 2, 3)]
+    held = by_steps(cases[0])
     call(held, 12)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         out = call(held, 12)
     for case in cases + cases[:2]:
-        for name, t in on_gpu(case).items():
-            held[name].copy_(t)
+        for name, t in by_steps(case).items():
+            if t is not None:
+                held[name].copy_(t)
         graph.replay()
         torch.cuda.synchronize()
         check(out, expected(case, 12))
@@ -107,8 +126,7 @@ def test_the_same_answers_by_either_way():
     """A batch too large to sum all its rows, and its halves that are not."""
     sizes = [40] * 32
     case = make_case(12, sizes, 40000, torch.bfloat16, 4, torch.bfloat16)
-    gpu = on_gpu(case)
-    whole = call(gpu, 10)
+    whole, gpu = call(by_steps(case), 10), on_gpu(case)
     for b in range(0, 32, 8):
         s = slice(40 * b, 40 * (b + 8))
         part = fsta.verify_drafts(gpu["logits"][s], gpu["tokens"][s], gpu["parent"][s], torch.arange(9, dtype=torch.int32, device="cuda") * 40,
@@ -121,10 +139,10 @@ def test_rows_longer_than_a_part_can_be():
     """A row of more than 256 parts of 8192: parts are longer."""
     vocabulary = 256 * 8192 + 12345
     case = make_case(2, [4, 3, 5, 2], vocabulary, torch.float16, 2, None)
-    check(call(on_gpu(case), 5), expected(case, 5))
+    check_both(case, 5)
     case["logits"][:, 20000:] = -float("inf")
     case["logits"][3, vocabulary - 1] = 30.0
-    check(call(on_gpu(case), 5, 0.5), expected(case, 5, 0.5))
+    check_both(case, 5, 0.5)
 
 
 @pytest.mark.parametrize("tau", [1e-7, 1e-4, 1.0, 1e8])
@@ -145,13 +163,19 @@ def test_random_numbers_next_to_what_decides(tau):
     rest = p.scatter(1, case["tokens"][1::3, None], 0.0)
     run = rest.cumsum(1) / rest.sum(1, keepdim=True)
     case["u_next"] = (run[torch.arange(64), torch.arange(64) * 140] + near).clamp(0, 1).float()
-    check(call(on_gpu(case), 2, tau), expected(case, 2, tau))
-    more = make_case(78, [2] * 4000, 3000, torch.float32, 1, None)                            # and where each step is a launch
+    check_both(case, 2, tau)
+    more = make_case(78, [2] * 4000, 3000, torch.float32, 1, None)                            # and where only the last sum counts
     more["logits"][:192] = case["logits"][:, :3000]
-    assert more["logits"].numel() * 4 > 70e6
     p = torch.exp((more["logits"].double()[0::2] - more["logits"].double()[0::2].amax(1, keepdim=True)) / float(np.float32(tau)))
     run = p.cumsum(1) / p.sum(1, keepdim=True)
     places = torch.arange(4000) % 3000
     more["u_next"] = (run[torch.arange(4000), places] + torch.linspace(-2e-7, 2e-7, 4000, dtype=torch.float64)).clamp(0, 1).float()
     more["u_accept"][:] = 1.0
-    check(call(on_gpu(more), 1, tau), expected(more, 1, tau))
+    check_both(more, 1, tau)
+
+
+@pytest.mark.parametrize("draft", [None, torch.float32])
+@pytest.mark.parametrize("vocabulary", [301, 9001])
+def test_more_fall_than_there_are_launches(draft, vocabulary):
+    for case in cases_of_more_that_fall(draft, vocabulary):
+        check_both(case, 3)
