@@ -294,7 +294,7 @@ __device__ __forceinline__ void first_sums(const L* row, double rate, int vocabu
         __builtin_amdgcn_sched_barrier(0);                       // (in this order: the loop waits for one at a time)
     }
     float top = -INFINITY;
-    int best = INT32_MAX, end = min(p * part_length + part_length, last);
+    int best = INT32_MAX, end = (int)min((int64_t)p * part_length + part_length, (int64_t)last);
     double sum = 0.0;
 #pragma unroll 1
     for (int i1 = p * part_length; i1 < last; i1 += kPart) {
@@ -1078,7 +1078,7 @@ extern "C" int fsta_verify_drafts(const void* logits, int64_t logits_stride, int
     if (!temperatures && (temperature < 0.f || temperature != temperature || temperature == INFINITY))
         return fail(FSTA_EINVAL, "%s: temperature=%g", who, (double)temperature);
     if (logits_stride < 0 || (draft && draft_stride < 0)) return fail(FSTA_EINVAL, "%s: negative stride", who);
-    if (vocabulary > INT32_MAX - 65536) return fail(FSTA_EUNSUPPORTED, "%s: vocabulary=%d", who, vocabulary);
+    if (vocabulary > INT32_MAX - 65536 || batch > INT32_MAX - 65536) return fail(FSTA_EUNSUPPORTED, "%s: batch=%d vocabulary=%d", who, batch, vocabulary);
     if (batch == 0) return FSTA_OK;
     if (!q_starts || !u_next || !path || !counts || !next_tokens || (nodes > 0 && (!logits || !tokens || !parent || !u_accept)))
         return fail(FSTA_EINVAL, "%s: null pointer", who);

@@ -241,6 +241,21 @@ def test_far_rows():
 
 
 @pytest.mark.parametrize("draft", [False, True])
+def test_the_longest_rows(draft):
+    """Rows of as many tokens as there may be, whose parts' ends pass 31 bits; three of them have weight."""
+    vocabulary, middle = 2 ** 31 - 1 - 65536, 2 ** 30 + 3
+    row = torch.full((1, vocabulary), -math.inf, dtype=torch.float16, device="cuda")
+    row[0, [5, middle, vocabulary - 1]] = 0.5
+    drafts = torch.zeros((1, vocabulary), dtype=torch.float16, device="cuda") if draft else None
+    if draft:
+        drafts[0, middle] = 1.0
+    for u, u_next, path, following in ((0.9, 0.75, [0, -1], vocabulary - 1), (0.9, 0.25, [0, -1], 5), (0.2, 0.99, [0, 1], vocabulary - 1), (0.2, 0.5, [0, 1], middle)):
+        got = fsta.verify_drafts(row.expand(2, -1), torch.tensor([0, middle]).cuda(), torch.tensor([-1, 0]).cuda(), torch.tensor([0, 2]).int().cuda(),
+                                 torch.tensor([0.0, u]).cuda(), torch.tensor([u_next]).cuda(), 2, draft_probs=drafts.expand(2, -1) if draft else None)
+        assert got.path.tolist() == [path] and got.next_tokens.tolist() == [following]
+
+
+@pytest.mark.parametrize("draft", [False, True])
 def test_answers_are_distributed_as_the_models_own(draft):
     """What stands behind the root is a sample of the model's own distribution, whatever was drafted: 200000 trees of up to three children,
     Pearson's statistic over 12 tokens (11 degrees of freedom) below 46 (1 - chi2.cdf = 3e-6; the seed is fixed)."""

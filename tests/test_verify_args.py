@@ -42,7 +42,7 @@ def _refused(entry, base, change, word, pool=None):
 @pytest.mark.parametrize("change,word", [
     (dict(logits=None), "null"), (dict(tokens=None), "null"), (dict(parent=None), "null"), (dict(starts=None), "null"), (dict(u_accept=None), "null"),
     (dict(u_next=None), "null"), (dict(path=None), "null"), (dict(counts=None), "null"), (dict(next=None), "null"), (dict(batch=-1), "batch"),
-    (dict(nodes=-1), "nodes"), (dict(vocabulary=0), "vocabulary"), (dict(vocabulary=2 ** 31 - 1), "vocabulary"), (dict(max_path=0), "max_path"),
+    (dict(nodes=-1), "nodes"), (dict(vocabulary=0), "vocabulary"), (dict(vocabulary=2 ** 31 - 1), "vocabulary"), (dict(batch=2 ** 31 - 1), "batch"), (dict(max_path=0), "max_path"),
     (dict(dtype=_lib.FP8), "logits_dtype"), (dict(dtype=_lib.F64), "logits_dtype"), (dict(draft=P, draft_dtype=_lib.FP8), "draft_dtype"),
     (dict(temperature=-0.5), "temperature"), (dict(temperature=float("nan")), "temperature"), (dict(temperature=float("inf")), "temperature"),
     (dict(stride=-1), "stride"), (dict(draft=P, draft_stride=-4), "stride"), (dict(logits=P + 1), "aligned"), (dict(draft=P + 2), "aligned"),
