@@ -90,6 +90,13 @@ def test_tables(entry, base, change, word):
     _refused(entry, base, change, word)
 
 
+def test_more_rows_than_31_bits_count():
+    for entry, base, change, word in (("fsta_fit_pages", FIT, dict(batch=2 ** 31 - 1), "batch"), ("fsta_fit_pages", FIT, dict(batch=1 << 24, width=128), "width"),
+                                      ("fsta_fork_pages", FORK, dict(batch=1 << 24, width=128), "width"), ("fsta_fork_pages", FORK, dict(pairs=1 << 25), "pairs"),
+                                      ("fsta_copy_pages", COPY, dict(pairs=2 ** 31 - 1), "pairs"), ("fsta_compact_paged_kv", COMPACT, dict(batch=1 << 25), "batch")):
+        _refused(entry, base, change, word)
+
+
 @pytest.mark.parametrize("change,word", [(dict(sources=None), "null"), (dict(targets=None), "null"), (dict(targets=P + 1), "aligned"), (dict(pairs=-1), "pairs")])
 def test_fork(change, word):
     _refused("fsta_fork_pages", FORK, change, word)
