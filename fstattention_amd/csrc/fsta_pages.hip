@@ -598,6 +598,13 @@ extern "C" int fsta_compact_paged_kv(const fsta_paged_pool* pools, int32_t layer
     if (misaligned(path, 4) || misaligned(counts, 4) || misaligned(page_table, 4) || misaligned(kv_lens, 4) || misaligned(q_starts, 4) || misaligned(new_lens, 4))
         return fail(FSTA_EINVAL, "%s: path, counts, page_table, kv_lens, q_starts and new_lens must be 4-byte aligned", who);
     if (batch > kMaxRows) return fail(FSTA_EUNSUPPORTED, "%s: batch=%d", who, batch);
+    // rows move in place: of two workgroups with the same pool one would read what the other has moved
+    for (int32_t l = 0; l < layers && num_pages > 0; ++l) {
+        bool twice = pools[l].k == pools[l].v;
+        for (int32_t i = 0; i < l; ++i)
+            twice |= (pools[i].k == pools[l].k) | (pools[i].v == pools[l].v) | (pools[i].k == pools[l].v) | (pools[i].v == pools[l].k);
+        if (twice) return fail(FSTA_EINVAL, "%s: layer %d has a pool that is there twice", who, l);
+    }
     const CompactArgs a{path, counts, page_table, kv_lens, q_starts, new_lens, max_path, batch, width, num_pages, shift_of(page_size)};
     for (int32_t first = 0; first < layers; first += kMaxLayers) {
         Layers l;

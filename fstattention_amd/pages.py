@@ -3,7 +3,7 @@ shared among them, copied, taken back.
 
 The arrays are those of :mod:`fstattention_amd.paged`, and like there the host reads none of them: nothing here waits for the GPU.
 Beside them a program keeps ``refs`` int32 ``[num_pages]``: by how many entries of the page table a page is held.  A page with 0 is free,
-so ``torch.zeros`` (and a page table of -1) is where a server starts.  ``caches`` is a :class:`PagedKV` or a list or tuple of them,
+so ``torch.zeros`` (and a page table of -1) is where a server starts; from then on only the calls here change it.  ``caches`` is a :class:`PagedKV` or a list or tuple of them,
 one per layer (a plain tuple of its four tensors will do); they share ``num_pages`` and ``page_size``, so that one page table serves all, and
 may differ in heads, head_dim and dtype.  All layers go in one launch (32 at a time).
 
@@ -58,7 +58,8 @@ def compact_paged_kv(caches: Caches, path: torch.Tensor, counts: torch.Tensor, p
 
     ``kv_lens`` and ``q_starts`` are those of the pass that wrote the tree (new tokens included); ``path`` int32 ``[B, P]`` and ``counts`` int32
     ``[B]`` are :func:`verify_drafts`' (node numbers within each tree, ascending): row ``base + path[b, i]`` goes to ``base + i`` for the first
-    ``counts[b]``, ``base = kv_lens[b]`` minus its new tokens.  Entries outside the new tokens, and rows without a page, move nothing."""
+    ``counts[b]``, ``base = kv_lens[b]`` minus its new tokens.  Entries outside the new tokens, and rows without a page, move nothing.
+    Rows move in place: no layer may be there twice."""
     out = _calls().compact_paged_kv(caches, path, counts, page_table, kv_lens, q_starts)
     if out is not NotImplemented:
         return out
@@ -105,7 +106,9 @@ def fit_pages(caches: Caches, refs: torch.Tensor, page_table: torch.Tensor, lens
 
     Entries up to a sequence's last page that name none get a free one (the lowest-numbered, in order of sequence and position); entries
     behind it become -1, and their pages are held once less.  Where a sequence ends inside a page that others hold too
-    (:func:`fork_pages`, then shortened), it gets its own copy of the rows it has there.  Pages given back by a call are free for the next one.
+    (:func:`fork_pages`, then shortened), it gets its own copy of the rows it has there; so a sequence that shares pages and is cut short
+    is fitted to the shorter length before it grows again.  Pages given back by a call are free for the next one.  Lengths are cut to
+    what ``W`` entries hold.
 
     Returns int32 ``[B]``: how many pages each sequence wanted and did not get.  One with any must not be written to: nothing is
     given to it in another's place, and it may still end in a page of others."""

@@ -570,7 +570,8 @@ int fsta_verify_drafts(const void* logits, int64_t logits_stride, int32_t logits
  * below kv_lens[b]) the ones that path [batch, max_path] names, counts[b] of them, move to the first of
  * those positions: position base + path[b][i] to base + i.  A path's numbers ascend (fsta_verify_drafts'
  * do); others leave the rows it concerns undefined, entries outside the new tokens move nothing.
- * new_lens [batch] = base + counts[b] (counts kept within [0, new tokens and max_path]).
+ * new_lens [batch] = base + counts[b] (counts kept within [0, new tokens and max_path]).  Rows move in place:
+ * a pool that is there twice is refused, and no page may hold new tokens of two sequences.
  */
 typedef struct fsta_paged_pool {
     void* k;                 /* [num_pages, kv_heads, page_size, head_dim] */
@@ -595,13 +596,16 @@ int fsta_copy_pages(const fsta_paged_pool* pools, const fsta_paged_pool* into, i
                     const int32_t* targets, int32_t pairs, void* stream);
 
 /*
- * refs [num_pages] int32: by how many entries of page tables a page is held; 0: it is free.
+ * refs [num_pages] int32: by how many entries of page tables a page is held; 0: it is free.  It has to agree
+ * with the tables (zeros and a table of -1 do): one that does not gives pages away that are in use.
  * fsta_fit_pages makes a page table fit the lengths lens [batch]: entries behind a sequence's last page
  * are taken back (-1; the page is held once less), entries up to it that name no page get a free one, and
  * where a sequence ends inside a page that others hold too, it gets a copy of its rows of that page in all
  * layers.  Pages are given in order of sequence and position, the lowest-numbered first, among those that
  * are free before the call.  missing [batch]: pages that a sequence wanted and did not get (its entries name
- * none, or still the page of others: such a sequence must not be written to).
+ * none, or still the page of others: such a sequence must not be written to); lengths are cut to what `width`
+ * entries hold.  A sequence that shares pages and is cut short has to be fitted to the shorter length before it
+ * grows again: between its two ends only the page that it ends in is looked at.
  * fsta_fork_pages: slot targets[i] gives up what it holds and becomes a copy of slot sources[i] as it was
  * before the call: it shares the pages that are full and gets a copy of the rows of the last one, lens too.
  * Where pairs have one target the first counts; a pair of one slot twice, or outside [0, batch), does

@@ -392,6 +392,9 @@ def test_refusals():
                          (dict(lens=lens.float()), "kv_lens")):
         with pytest.raises(ValueError, match=word):
             compact(**change)
+    for bad in ([caches[0], caches[1], caches[0]], [caches[0]._replace(v=caches[0].k)], [caches[0], caches[0]._replace(k=caches[0].v, v=caches[0].k)]):
+        with pytest.raises(Exception, match="twice"):
+            compact(caches=bad)
     for into, word in (([caches[0]], "layers"), (make_pools(9, 32, [(2, 64, BF16), (2, 64, FP8)]), "layers"), (make_pools(9, 16, [(2, 64, BF16), (3, 64, FP8)]), "layers"),
                        (make_pools(9, 16, [(2, 64, F16), (2, 64, FP8)]), "layers"), (make_pools(9, 16, [(2, 128, BF16), (2, 64, FP8)]), "layers")):
         with pytest.raises(ValueError, match=word):

@@ -90,6 +90,14 @@ def test_tables(entry, base, change, word):
     _refused(entry, base, change, word)
 
 
+def test_compact_with_a_pool_twice():
+    for at in ((1, 2, 1, 3), (1, 2, 3, 2), (1, 2, 2, 3), (1, 2, 3, 1), (1, 1, 2, 3), (1, 2, 3, 3)):
+        pools = _pools()
+        for pool, k, v in zip(pools, at[::2], at[1::2]):
+            pool.k, pool.v = k * P, v * P
+        _refused("fsta_compact_paged_kv", COMPACT, dict(pools=pools), "twice")
+
+
 def test_more_rows_than_31_bits_count():
     for entry, base, change, word in (("fsta_fit_pages", FIT, dict(batch=2 ** 31 - 1), "batch"), ("fsta_fit_pages", FIT, dict(batch=1 << 24, width=128), "width"),
                                       ("fsta_fork_pages", FORK, dict(batch=1 << 24, width=128), "width"), ("fsta_fork_pages", FORK, dict(pairs=1 << 25), "pairs"),
