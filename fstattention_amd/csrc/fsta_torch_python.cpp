@@ -653,7 +653,7 @@ PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const OnStream on(*logits);
         const at::Tensor path = fresh({batch, most}, at::kInt, *logits), counts = fresh({batch}, at::kInt, *logits),
                          next = fresh({batch}, at::kLong, *logits);
-        const size_t need = fsta_verify_workspace_bytes((int32_t)batch, (int32_t)nodes, (int32_t)logits->size(1), float_code(*logits), draft != nullptr);
+        const size_t need = fsta_verify_workspace_bytes((int32_t)batch, (int32_t)nodes, (int32_t)logits->size(1), (int32_t)most, draft != nullptr);
         const at::Tensor work = need ? fresh({(int64_t)need}, at::kByte, *logits) : at::Tensor();
         if (fsta_verify_drafts(logits->data_ptr(), row_stride(*logits), float_code(*logits), draft ? draft->data_ptr() : nullptr,
                                draft ? row_stride(*draft) : 0, draft ? float_code(*draft) : FSTA_F32, tokens, parent, first, u_accept, u_next,

@@ -62,7 +62,8 @@ struct VerifyArgs {
     int64_t* next;
     int32_t batch, nodes, vocabulary, max_path;
     int32_t parts_per_row, part_length;
-    const Part* all_parts;                // of every node with children, or null
+    const Part* all_parts;                // of every node with children, or null ..
+    int32_t* stands;                      // .. and the child that stands there, -1: none, or sums of W have to be asked
     Part *parts_out;                      // stats_kernel
     Part* parts[2];                       // of every sequence, by steps in turn
     State* states[2];
@@ -189,7 +190,7 @@ struct Shared {
     double sum[kMaxParts];                // parts' sums against the row's largest logit
     Part part[kMaxParts];                 // walk_kernel's own
     int32_t parent[kTree], token[kTree];  // -1: none
-    float logit[kTree], draft[kTree], u[kTree];       // .. of a token at its parent; only where the first sums of all rows are there
+    int32_t stands[kTree];
     uint32_t fell[kWalkThreads / 64][kPart / 32];     // a wave's part: which tokens fell
     int32_t fallen[kChildren];            // tokens that left P at this node
     double lost[kChildren];               // .. and their weights
@@ -420,28 +421,29 @@ __device__ __forceinline__ double sum_again(const Row<L, Q>& row, int from, int 
     return sum_of(sum);
 }
 
-// One sequence's walk, by a workgroup.  Every wave takes all decisions itself, from the same numbers.
+// One sequence's walk, by a workgroup.  Every wave takes all decisions itself, from the same numbers.  Of a wave that looks at one
+// node only (THREADS 64) there is no Shared.
 template <typename L, typename Q, int THREADS> struct Walk {
     static constexpr int kWaves = THREADS / 64;
+    static constexpr bool kOneNode = THREADS == 64;
     const VerifyArgs& a;
-    Shared& sh;
+    Shared* const sh;
+    const bool notes;                     // this workgroup writes the path
     int b, start, nodes;
     bool greedy;
     Row<L, Q> row;
     int node, count, child, asked;        // children below `child` have fallen, `asked` of them
-    int summed, fallen;                   // children below `summed` were left out of the sum; entries of sh.fallen
+    int summed, fallen;                   // children below `summed` were left out of the sum; entries of sh->fallen
     int held, where;                      // the last sum: kFirst, kAgain or kQuick; as in State
     bool exact, always_exact;             // the node's first sum has to be 64 bits
     double all, whole, left;              // Z, Z when the sum was taken, r
     // the strip of 64 nodes whose children are asked next: a child per lane, and which lanes
     int strip = 0, token = -1;
-    uint64_t kids = 0;
+    uint64_t kids = 0, all_kids = 0;      // .. are left, were there
     float logit = 0.f, draft = 0.f, u = 0.f;
-    int early_parent, early_token;        // of node threadIdx.x, on their way
-    const Part* ahead_of = nullptr;       // the sums of the first child's row, which the walk is likely to need next
-    Part ahead{0.0, 0.f, 0};
+    int early_parent, early_token, early_stands;      // of node threadIdx.x, on their way
 
-    __device__ __forceinline__ Walk(const VerifyArgs& args, Shared& shared, int sequence) : a(args), sh(shared), b(sequence) {
+    __device__ __forceinline__ Walk(const VerifyArgs& args, Shared* shared, int sequence, bool writes) : a(args), sh(shared), notes(writes), b(sequence) {
         start = min(max(a.q_starts[b], 0), a.nodes);
         nodes = max(min(a.q_starts[b + 1], a.nodes) - start, 0);
         const float tau = a.temperatures ? a.temperatures[b] : a.temperature;
@@ -455,19 +457,22 @@ template <typename L, typename Q, int THREADS> struct Walk {
         row.best = -1;
         row.n = a.vocabulary;
         always_exact = exact = !a.draft && row.rate > kQuickRate;
-        const bool mine = (int)threadIdx.x < min(nodes, kTree);
+        const bool mine = !kOneNode && (int)threadIdx.x < min(nodes, kTree);
         early_parent = mine ? parent_in_memory(threadIdx.x) : -1;
         early_token = mine ? token_in_memory(threadIdx.x) : -1;
+        early_stands = mine && a.all_parts ? a.stands[start + threadIdx.x] : -1;
     }
     // The tree is in LDS from here on
     __device__ __forceinline__ void read_tree() {
         if ((int)threadIdx.x < min(nodes, kTree)) {
-            sh.parent[threadIdx.x] = early_parent;
-            sh.token[threadIdx.x] = early_token;
+            sh->parent[threadIdx.x] = early_parent;
+            sh->token[threadIdx.x] = early_token;
+            sh->stands[threadIdx.x] = early_stands;
         }
         for (int j = threadIdx.x + THREADS; j < min(nodes, kTree); j += THREADS) {
-            sh.parent[j] = parent_in_memory(j);
-            sh.token[j] = token_in_memory(j);
+            sh->parent[j] = parent_in_memory(j);
+            sh->token[j] = token_in_memory(j);
+            sh->stands[j] = a.all_parts ? a.stands[start + j] : -1;
         }
         __syncthreads();
     }
@@ -479,40 +484,31 @@ template <typename L, typename Q, int THREADS> struct Walk {
         const int64_t x = a.tokens[start + j];
         return x >= 0 && x < a.vocabulary ? (int)x : -1;
     }
-    __device__ __forceinline__ bool is_child(int j) const { return j < nodes && (j < kTree ? sh.parent[j] : parent_in_memory(j)) == node; }
-    __device__ __forceinline__ int token_of(int j) const { return j < kTree ? sh.token[j] : token_in_memory(j); }
-
-    // Every node's token's logit and probability at its parent, all at once: a walk through sums that are there waits for memory
-    // once, not at every node
-    __device__ __forceinline__ void gather() {
-        for (int j = threadIdx.x; j < min(nodes, kTree); j += THREADS) {
-            const int64_t parent = start + max(sh.parent[j], 0);
-            const int x = max(sh.token[j], 0);
-            const L logit = (static_cast<const L*>(a.logits) + parent * a.logits_stride)[x];
-            Q draft{};
-            if (a.draft) draft = (static_cast<const Q*>(a.draft) + parent * a.draft_stride)[x];
-            sh.u[j] = a.u_accept[start + j];
-            sh.logit[j] = value(logit);
-            sh.draft[j] = value(draft);
-        }
-        __syncthreads();
+    __device__ __forceinline__ bool is_child(int j) const {
+        if (j >= nodes) return false;
+        if constexpr (kOneNode) return parent_in_memory(j) == node;
+        else return (j < kTree ? sh->parent[j] : parent_in_memory(j)) == node;
     }
+    __device__ __forceinline__ int token_of(int j) const {
+        if constexpr (kOneNode) return token_in_memory(j);
+        else return j < kTree ? sh->token[j] : token_in_memory(j);
+    }
+    // (trees that overlap leave entries that nobody wrote: a child comes behind its parent, whatever is there)
+    __device__ __forceinline__ int stands_at(int j) const {
+        const int child = j < kTree ? sh->stands[j] : a.stands[start + j];
+        return child > j && child < nodes ? child : -1;
+    }
+
     // To the next strip with children of the node, from node `from` on: what they are asked with
     __device__ __forceinline__ void look(int from) {
         const int lane = threadIdx.x & 63;
         kids = 0;
         for (strip = from; strip < nodes && !kids; strip += kids ? 0 : 64) kids = __ballot(is_child(strip + lane));
+        all_kids = kids;
         const bool mine = kids >> lane & 1;
         if (!kids) return;
         // (loads of all lanes, the others' from a place that there is: a branch around them would wait for each)
         token = mine ? token_of(strip + lane) : -1;
-        if (a.all_parts && strip + 64 <= kTree) {
-            const int j = strip + lane;
-            logit = sh.logit[j];
-            draft = sh.draft[j];
-            u = sh.u[j];
-            return;
-        }
         const int x = max(token, 0);
         const L l = row.logits[x];
         Q q{};
@@ -534,7 +530,16 @@ template <typename L, typename Q, int THREADS> struct Walk {
         row.top = -INFINITY;
         row.best = -1;
     }
+    // .. from where on it goes on through children that are known to stand
     __device__ __forceinline__ void stand_at(int at, int how_many) {
+        if constexpr (kOneNode) {
+            node = at;
+            return;
+        }
+        note(at, how_many);
+        if (a.all_parts) {
+            for (int j = stands_at(at); j >= 0 && how_many < a.max_path; j = stands_at(j)) note(at = j, ++how_many);
+        }
         stand_on(at, how_many);
         look(at + 1);
         exact |= !a.draft && !kids;       // nothing to ask: its sum is the one that the next token is picked from
@@ -560,8 +565,12 @@ template <typename L, typename Q, int THREADS> struct Walk {
         }
         if (parts) take(s.phase == kDone ? s.held : s.phase == kFirst && !exact && !a.draft ? kQuick : s.phase, parts);
         read_tree();
-        if (s.phase != kDone && a.all_parts) gather();
-        if (s.phase != kDone) look(child);
+        if (s.phase == kFirst && !parts) {
+            stand_at(s.node, s.count);
+            exact |= s.exact != 0;
+        } else if (s.phase != kDone) {
+            look(child);
+        }
         if (s.phase == kFirst) exact |= !a.draft && !kids;
     }
     __device__ __forceinline__ void part_range(int p, int* from, int* to) const {
@@ -569,15 +578,10 @@ template <typename L, typename Q, int THREADS> struct Walk {
         *to = (int)min((int64_t)*from + a.part_length, (int64_t)a.vocabulary);
     }
 
-    // The parts of the first sum of the row: its largest logit, Z.  (Every wave writes the same to sh.sum.)
+    // The parts of the first sum of the row: its largest logit, Z.  (Every wave writes the same to sh->sum.)
     __device__ __forceinline__ void take_first(const Part* parts) {
         const int lane = threadIdx.x & 63;
-        Part mine = ahead;
-        if (ahead_of != parts) mine = parts[min(lane, a.parts_per_row - 1)];
-        if (a.all_parts && kids) {        // (on their way while the children are asked)
-            ahead_of = parts_of(a.all_parts, start + (int64_t)strip + __ffsll((unsigned long long)kids) - 1);
-            ahead = ahead_of[min(lane, a.parts_per_row - 1)];
-        }
+        Part mine = parts[min(lane, a.parts_per_row - 1)];
         if (lane >= a.parts_per_row) mine = Part{0.0, -INFINITY, INT32_MAX};
         float top = mine.top;
         int best = mine.best;
@@ -592,7 +596,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
                 const Part part = p == lane ? mine : parts[p];
                 const double s = part.sum > 0.0 ? part.sum * weight_of(part.top, top, row.rate) : 0.0;
                 sum += s;
-                sh.sum[p] = s;
+                if constexpr (!kOneNode) sh->sum[p] = s;
             }
         }
         whole = all = sum_of(sum);
@@ -604,7 +608,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
         for (int p = threadIdx.x & 63; p < a.parts_per_row; p += 64) {
             const double s = parts[p].sum;
             sum += s;
-            sh.sum[p] = s;
+            sh->sum[p] = s;
         }
         whole = all = sum_of(sum);
         summed = child;
@@ -617,6 +621,11 @@ template <typename L, typename Q, int THREADS> struct Walk {
             if (__ballot(i < j && is_child(i) && token_of(i) == x)) return true;
         }
         return false;
+    }
+
+    // .. of the strip's child of lane l
+    __device__ __forceinline__ bool fell_before_in_strip(int l, int x) const {
+        return __ballot((all_kids >> (threadIdx.x & 63) & 1) && (int)(threadIdx.x & 63) < l && token == x) || fell_before(strip, x);
     }
 
     // Asks children until one stands (kFirst: `node` is that one now), a sum of W is wanted (kAgain) or there are no more (kDone)
@@ -634,7 +643,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
                     stand_at(j, count + 1);
                     return kFirst;
                 }
-                if (fell_before(j, x)) continue;
+                if (fell_before_in_strip(l, x)) continue;
                 const double wx = of_lane(w, l), qx = of_lane(q, l), ux = of_lane((double)u, l);
                 const bool drawn = qx > 0.0 && left > 0.0;
                 // Too near to tell by a sum in 32 bits: once more, in 64
@@ -664,7 +673,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
         return kDone;
     }
 
-    // The tokens that fell, in sh.fallen; behind those that the sum leaves out (returned: how many) each comes once
+    // The tokens that fell, in sh->fallen; behind those that the sum leaves out (returned: how many) each comes once
     __device__ __forceinline__ int collect() {
         const int lane = threadIdx.x & 63;
         __syncthreads();
@@ -672,7 +681,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
         for (int i0 = node + 1; i0 < summed; i0 += 64) {
             const int i = i0 + lane, x = i < summed && is_child(i) ? token_of(i) : -1;
             const uint64_t those = __ballot(x >= 0);
-            if (x >= 0 && threadIdx.x < 64) sh.fallen[fallen + __popcll(those & ((1ull << lane) - 1))] = x;
+            if (x >= 0 && threadIdx.x < 64) sh->fallen[fallen + __popcll(those & ((1ull << lane) - 1))] = x;
             fallen += __popcll(those);
         }
         const int before = fallen;
@@ -681,7 +690,7 @@ template <typename L, typename Q, int THREADS> struct Walk {
             for (uint64_t those = __ballot(mine >= 0); those; those &= those - 1) {
                 const int l = __ffsll((unsigned long long)those) - 1, x = of_lane(mine, l);
                 if (fell_before(i0 + l, x)) continue;
-                if (threadIdx.x == 0) sh.fallen[fallen] = x;
+                if (threadIdx.x == 0) sh->fallen[fallen] = x;
                 ++fallen;
             }
         }
@@ -700,15 +709,15 @@ template <typename L, typename Q, int THREADS> struct Walk {
         for (int p = p0; p < p1; ++p) {
             int from, to;
             part_range(p, &from, &to);
-            const double sum = sum_again(row, from, to, sh.fallen, fallen, sh.fell[threadIdx.x >> 6]);
+            const double sum = sum_again(row, from, to, sh->fallen, fallen, sh->fell[threadIdx.x >> 6]);
             if ((threadIdx.x & 63) == 0) out[p] = Part{sum, row.top, 0};
         }
     }
-    // Sums over the whole row by this workgroup alone, a part a wave: into sh.part
+    // Sums over the whole row by this workgroup alone, a part a wave: into sh->part
     __device__ __forceinline__ void sum_alone(bool first) {
         const int wave = threadIdx.x >> 6;
         __syncthreads();
-        sum_parts<false>(first, wave, kWaves, sh.part);
+        sum_parts<false>(first, wave, kWaves, sh->part);
         __syncthreads();
     }
 
@@ -716,21 +725,21 @@ template <typename L, typename Q, int THREADS> struct Walk {
     // (or u >= 1) lets none; -1 where there is no weight
     __device__ __forceinline__ int pick(double u) {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-        __syncthreads();                  // sh.sum
+        __syncthreads();                  // sh->sum
         if (child > summed) {
             // a part loses the terms that fell since its sum was taken; where little is left of it, its sum is taken again
             const int old = collect();
             for (int k = old + tid; k < fallen; k += THREADS) {
-                const int x = sh.fallen[k];
-                sh.lost[k] = row.weight(value(row.logits[x]), row.proposed(x));
+                const int x = sh->fallen[k];
+                sh->lost[k] = row.weight(value(row.logits[x]), row.proposed(x));
             }
             __syncthreads();
             for (int p = tid; p < a.parts_per_row; p += THREADS) {
                 double lost = 0.0;
                 for (int k = old; k < fallen; ++k)
-                    if (sh.fallen[k] / a.part_length == p) lost += sh.lost[k];
-                const double s = sh.sum[p];
-                if (lost > 0.0) sh.sum[p] = s - lost > s * 0x1p-10 ? s - lost : -1.0;
+                    if (sh->fallen[k] / a.part_length == p) lost += sh->lost[k];
+                const double s = sh->sum[p];
+                if (lost > 0.0) sh->sum[p] = s - lost > s * 0x1p-10 ? s - lost : -1.0;
             }
             __syncthreads();
         } else {
@@ -739,29 +748,29 @@ template <typename L, typename Q, int THREADS> struct Walk {
         double sum;
         for (int resort = 0;; ++resort) {
             for (int p = wave; p < a.parts_per_row; p += kWaves) {
-                if (sh.sum[p] >= 0.0) continue;
+                if (sh->sum[p] >= 0.0) continue;
                 int from, to;
                 part_range(p, &from, &to);
-                const double s = sum_again(row, from, to, sh.fallen, fallen, sh.fell[wave]);
-                if (lane == 0) sh.sum[p] = s;
+                const double s = sum_again(row, from, to, sh->fallen, fallen, sh->fell[wave]);
+                if (lane == 0) sh->sum[p] = s;
             }
             __syncthreads();
             sum = 0.0;
-            for (int p = lane; p < a.parts_per_row; p += 64) sum += sh.sum[p];
+            for (int p = lane; p < a.parts_per_row; p += 64) sum += sh->sum[p];
             sum = sum_of(sum);
             if (sum > 0.0) break;
             if (resort == 2) return -1;                          // rounding left nothing: P without what fell, then P
             row.shift = 0.0;
             if (resort == 1) fallen = 0;
             __syncthreads();
-            for (int p = tid; p < a.parts_per_row; p += THREADS) sh.sum[p] = -1.0;
+            for (int p = tid; p < a.parts_per_row; p += THREADS) sh->sum[p] = -1.0;
             __syncthreads();
         }
         double target = u < 1.0 ? u * sum : INFINITY;
         int chosen = -1, last = -1;
         double before = 0.0, at_chosen = 0.0;
         for (int p0 = 0; p0 < a.parts_per_row && chosen < 0; p0 += 64) {
-            const double s = p0 + lane < a.parts_per_row ? sh.sum[p0 + lane] : 0.0;
+            const double s = p0 + lane < a.parts_per_row ? sh->sum[p0 + lane] : 0.0;
             const double up_to = sum_up_to(s);
             const uint64_t weighs = __ballot(s > 0.0), passes = __ballot(s > 0.0 && before + up_to > target);
             if (weighs) last = p0 + 63 - __builtin_clzll(weighs);
@@ -798,19 +807,19 @@ template <typename L, typename Q, int THREADS> struct Walk {
                 leave_out(outside(at, i, to), 0.0, w);
             }
             for (int k = 0; k < fallen; ++k) {
-                const int f = sh.fallen[k] - at;
+                const int f = sh->fallen[k] - at;
                 if (f >= 0 && f < 8) leave_out(1u << f, 0.0, w);
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) mine += w[e];
             const double up_to = sum_up_to(mine);
             __syncthreads();
-            if (lane == 63) sh.wave_sum[wave] = up_to;
+            if (lane == 63) sh->wave_sum[wave] = up_to;
             __syncthreads();
             double run = up_to - mine, here = 0.0;
             for (int k = 0; k < kWaves; ++k) {
-                if (k < wave) run += sh.wave_sum[k];
-                here += sh.wave_sum[k];
+                if (k < wave) run += sh->wave_sum[k];
+                here += sh->wave_sum[k];
             }
             // Every thread names its first token that passes the target; the smallest counts.  None: the largest with any weight.
             int passes = INT32_MAX, weighs = -1;
@@ -824,11 +833,11 @@ template <typename L, typename Q, int THREADS> struct Walk {
             }
             passes = min_of(passes);
             weighs = max_of(weighs);
-            if (lane == 0) sh.best[wave] = passes, sh.last[wave] = weighs;
+            if (lane == 0) sh->best[wave] = passes, sh->last[wave] = weighs;
             __syncthreads();
             for (int k = 0; k < kWaves; ++k) {
-                passes = min(passes, sh.best[k]);
-                weighs = max(weighs, sh.last[k]);
+                passes = min(passes, sh->best[k]);
+                weighs = max(weighs, sh->last[k]);
             }
             if (weighs >= 0) found = weighs;
             if (passes != INT32_MAX) return passes;
@@ -848,12 +857,12 @@ template <typename L, typename Q, int THREADS> struct Walk {
         }
         for (int i = count + threadIdx.x; i < a.max_path; i += THREADS) a.path[(int64_t)b * a.max_path + i] = -1;
     }
-    __device__ __forceinline__ void note() const {
-        if (threadIdx.x == 0) a.path[(int64_t)b * a.max_path + count - 1] = node;
+    __device__ __forceinline__ void note(int at, int how_many) const {
+        if (notes && threadIdx.x == 0) a.path[(int64_t)b * a.max_path + how_many - 1] = at;
     }
 
     // Takes decisions for as long as the sums are there; `taken`: the state's is
-    __device__ __forceinline__ int go_on(int phase, bool taken, bool noting) {
+    __device__ __forceinline__ int go_on(int phase, bool taken) {
         for (;;) {
             if (!taken) {
                 if (phase != kFirst || !a.all_parts || !kids || exact) return phase;
@@ -862,20 +871,25 @@ template <typename L, typename Q, int THREADS> struct Walk {
             }
             taken = false;
             phase = ask();
-            if (phase == kFirst && noting) note();               // (a node that is summed once more is noted once more)
             if (phase == kDone) return phase;
         }
     }
 };
+
+// A node's sequence: how many start at or before it
+__device__ __forceinline__ int sequence_of(const VerifyArgs& a, int64_t t) {
+    const int lane = threadIdx.x & 63;
+    int b = -1;
+    for (int c = 0; c < a.batch; c += 64) b += __popcll(__ballot(c + lane < a.batch && a.q_starts[c + lane] <= t));
+    return b;
+}
 
 // blockIdx.x: parts of a row, .y: node
 template <typename L, bool QUICK> __global__ __launch_bounds__(kStepThreads, QUICK ? 4 : 3) void stats_kernel(VerifyArgs a) {
     constexpr int kWaves = kStepThreads / 64;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     for (int64_t t = blockIdx.y; t < a.nodes; t += gridDim.y) {
-        // the node's sequence: how many start at or before it
-        int b = -1;
-        for (int c = 0; c < a.batch; c += 64) b += __popcll(__ballot(c + lane < a.batch && a.q_starts[c + lane] <= t));
+        const int b = sequence_of(a, t);
         if (b < 0) continue;
         const int start = max(a.q_starts[b], 0), end = min(a.q_starts[b + 1], a.nodes), node = (int)(t - start);
         uint64_t any = 0;
@@ -886,6 +900,27 @@ template <typename L, bool QUICK> __global__ __launch_bounds__(kStepThreads, QUI
         const int which = blockIdx.x * kWaves + wave, waves = gridDim.x * kWaves;
         first_sums<QUICK>(static_cast<const L*>(a.logits) + t * a.logits_stride, rate, a.vocabulary, a.part_length,
                    (int)((int64_t)a.parts_per_row * which / waves), (int)((int64_t)a.parts_per_row * (which + 1) / waves), a.parts_out + t * a.parts_per_row);
+    }
+}
+
+// Which child stands at each node, by the first sums of all rows, a wave per node: what a walk comes through does not wait for one
+// decision after the other.
+template <typename L, typename Q> __global__ __launch_bounds__(kStepThreads) void stands_kernel(VerifyArgs a) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t t = (int64_t)blockIdx.x * (kStepThreads / 64) + (threadIdx.x >> 6); t < a.nodes; t += (int64_t)gridDim.x * (kStepThreads / 64)) {
+        const int b = sequence_of(a, t);
+        if (b < 0) continue;
+        Walk<L, Q, 64> w(a, nullptr, b, false);
+        const int node = (int)(t - w.start);
+        if (node < 0 || node >= w.nodes) continue;
+        w.stand_on(node, 1);
+        w.look(node + 1);
+        int phase = kDone;
+        if (w.kids && !w.exact) {
+            w.take(a.draft ? kFirst : kQuick, w.parts_of_node());
+            phase = w.ask();
+        }
+        if (lane == 0) a.stands[t] = phase == kFirst && !w.exact ? w.node : -1;
     }
 }
 
@@ -905,14 +940,13 @@ template <typename L, typename Q, bool DRAWN> __global__ __launch_bounds__(kStep
             continue;
         }
         __syncthreads();
-        Walk<L, Q, kStepThreads> w(a, sh, b);
+        Walk<L, Q, kStepThreads> w(a, &sh, b, speaks);
         if (w.nodes == 0) {
             s.phase = kDone;
         } else {
             w.where = a.turn ^ 1;
             w.resume(s, a.fresh ? nullptr : w.parts_of_step(a.turn ^ 1));
-            if (a.fresh && speaks) w.note();
-            s.phase = w.go_on(s.phase, !a.fresh, speaks);
+            s.phase = w.go_on(s.phase, !a.fresh);
         }
         const bool sums = s.phase != kDone && (DRAWN || (s.phase == kFirst && !w.exact));
         if (speaks && threadIdx.x == 0)
@@ -929,9 +963,11 @@ template <typename L, typename Q, bool DRAWN> __global__ __launch_bounds__(kStep
     }
 }
 
-// Sums of 64 bits where steps made none: of the row that a sequence's next token is picked from, and of rows whose children's fate
-// sums of 32 bits do not tell.  They go to the buffer that the last step did not write.  blockIdx.x: parts of a row, .y: sequence
-__device__ __forceinline__ bool wants_last(const State& s, double rate) {
+// Sums of 64 bits where there are none: of the row that a sequence's next token is picked from, and of rows whose children's fate
+// sums of 32 bits do not tell.  They go to the buffer that the last step did not write.  Without steps that is the row of the last child that
+// is known to stand.  blockIdx.x: parts of a row, .y: sequence
+__device__ __forceinline__ bool wants_last(const VerifyArgs& a, const State& s, double rate) {
+    if (a.fresh) return a.all_parts && rate != 0.0;
     return s.phase == kDone ? s.held == kQuick && rate != 0.0 : s.phase == kFirst && !s.ready;
 }
 __device__ __forceinline__ double rate_of(const VerifyArgs& a, int b) {
@@ -940,12 +976,24 @@ __device__ __forceinline__ double rate_of(const VerifyArgs& a, int b) {
 }
 template <typename L> __global__ __launch_bounds__(kStepThreads, 3) void last_kernel(VerifyArgs a) {
     constexpr int kWaves = kStepThreads / 64;
+    __shared__ int32_t stands[kTree];
     const int which = blockIdx.x * kWaves + (threadIdx.x >> 6), waves = gridDim.x * kWaves;
     for (int b = blockIdx.y; b < a.batch; b += gridDim.y) {
-        const State s = a.states[a.turn][b];
+        State s = {};
+        if (!a.fresh) s = a.states[a.turn][b];
         const int start = min(max(a.q_starts[b], 0), a.nodes), nodes = min(a.q_starts[b + 1], a.nodes) - start;
         const double rate = rate_of(a, b);
-        if (nodes <= 0 || !wants_last(s, rate)) continue;
+        if (nodes <= 0 || !wants_last(a, s, rate)) continue;
+        if (a.fresh) {
+            __syncthreads();
+            for (int j = threadIdx.x; j < min(nodes, kTree); j += kStepThreads) stands[j] = a.stands[start + j];
+            __syncthreads();
+            for (int count = 1; count < a.max_path; ++count) {
+                const int child = s.node < kTree ? stands[s.node] : a.stands[start + s.node];
+                if (child <= s.node || child >= nodes) break;
+                s.node = child;
+            }
+        }
         first_sums<false>(static_cast<const L*>(a.logits) + (start + (int64_t)s.node) * a.logits_stride, rate, a.vocabulary, a.part_length,
                           (int)((int64_t)a.parts_per_row * which / waves), (int)((int64_t)a.parts_per_row * (which + 1) / waves),
                           a.parts[a.turn ^ 1] + (int64_t)b * a.parts_per_row);
@@ -958,8 +1006,8 @@ template <typename L, typename Q> __global__ __launch_bounds__(kWalkThreads, 2) 
         __syncthreads();
         State s{0, 1, 1, 0, 1, kFirst, kFirst, 0, 0, 0, 0.0, 1.0, 0.f, 0};
         if (!a.fresh) s = a.states[a.turn][b];
-        Walk<L, Q, kWalkThreads> w(a, sh, b);
-        const bool last = w.nodes > 0 && !a.fresh && !a.draft && wants_last(s, w.row.rate);
+        Walk<L, Q, kWalkThreads> w(a, &sh, b, true);
+        const bool last = w.nodes > 0 && !a.draft && wants_last(a, s, w.row.rate);
         if (w.nodes > 0 && s.phase == kDone) {
             if (last) s.held = kFirst;
             w.resume(s, last ? w.parts_of_step(a.turn ^ 1) : s.where == kOfNode ? w.parts_of(a.all_parts, w.start + s.node) : w.parts_of_step(s.where));
@@ -968,9 +1016,9 @@ template <typename L, typename Q> __global__ __launch_bounds__(kWalkThreads, 2) 
             if (last) s.exact = 1;
             bool taken = last || (!a.fresh && s.ready);
             w.where = a.turn;
-            w.resume(s, taken ? w.parts_of_step(last ? a.turn ^ 1 : a.turn) : nullptr);
-            if (a.fresh) w.note();
-            while ((s.phase = w.go_on(s.phase, taken, true)) != kDone) {
+            w.resume(s, taken && !a.fresh ? w.parts_of_step(last ? a.turn ^ 1 : a.turn) : nullptr);
+            if (taken && a.fresh) w.take(kFirst, w.parts_of_step(a.turn ^ 1));
+            while ((s.phase = w.go_on(s.phase, taken)) != kDone) {
                 if (s.phase == kAgain) {
                     w.summed = w.child;
                     w.collect();
@@ -1000,18 +1048,29 @@ struct Plan {
 };
 size_t rounded(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
-constexpr int kMostSteps = 10;
-constexpr int kStatsGroups = 2048, kDrawnGroups = 512, kGivenGroups = 768, kLastGroups = 768;
-constexpr double kAllBytes = 200e6;
+// Chains: no more nodes than paths have places, and not because those are given generously
+bool chains(int64_t batch, int64_t nodes, int32_t max_path) { return max_path <= 16 && nodes <= batch * max_path; }
 
-Plan plan_of(int64_t batch, int64_t nodes, int64_t vocabulary, int size, bool draft, int32_t max_path) {
+// Sums of all rows first, or only of the rows that walks come to, a launch each?  The first costs with all nodes' tokens, the second a launch
+// (and what comes before its first sum) per node of the longest path.  Measured, all rows / steps, us:
+//   no draft probabilities  16 x 64 nodes of 32000 tokens 53 / 68, 32 x 64 68 / 71, 8 x 64 of 131072 65 / 66, 64 x 23 of 50021 60 / 76, 16 x 64 of 131072 96 / 67
+//   with them               4 x 64 of 50021 73 / 90, 8 x 23 of 131072 76 / 77, 32 x 23 of 32000 79 / 80, 8 x 64 of 50021 105 / 91
+//   chains                  256 x 6 of 131072 152 / 170, with draft probabilities 128 x 6 133 / 171
+constexpr double kAllGiven = 80e6, kAllDrawn = 20e6, kAllChains = 200e6;
+// Steps: one per node of a path, and of each child that falls for draft probabilities some more; behind ten the walks go on alone (a workgroup
+// instead of a row's share of them all, but a launch less).  With all sums there a step is one that falls: a chain has one, trees
+// of four children 105 us with four steps, 112 with three, 100 with six; of three 84, 82 and 90.
+constexpr int kMostSteps = 10, kDrawnSteps = 4;
+constexpr int kStatsGroups = 2048, kDrawnGroups = 512, kGivenGroups = 768, kLastGroups = 768;
+
+Plan plan_of(int64_t batch, int64_t nodes, int64_t vocabulary, bool draft, int32_t max_path) {
     Plan p;
     p.part_length = (int32_t)((vocabulary + (int64_t)kPart * kMaxParts - 1) / ((int64_t)kPart * kMaxParts) * kPart);
     p.parts = (int32_t)((vocabulary + p.part_length - 1) / p.part_length);
-    p.all = (double)nodes * vocabulary * size <= kAllBytes;
+    p.all = (double)nodes * vocabulary <= (chains(batch, nodes, max_path) ? kAllChains : draft ? kAllDrawn : kAllGiven);
     p.steps = max_path + (draft ? 3 : 0) < kMostSteps ? max_path + (draft ? 3 : 0) : kMostSteps;
-    if (p.all) p.steps = draft ? 4 : 1;
-    p.bytes = (p.all ? rounded(sizeof(Part) * (size_t)(nodes * p.parts)) : 0) + 2 * (rounded(sizeof(Part) * (size_t)(batch * p.parts)) + rounded(sizeof(State) * (size_t)batch));
+    if (p.all) p.steps = draft ? (chains(batch, nodes, max_path) ? 1 : kDrawnSteps) : 0;
+    p.bytes = (p.all ? rounded(sizeof(Part) * (size_t)(nodes * p.parts)) + rounded(sizeof(int32_t) * (size_t)nodes) : 0) + 2 * (rounded(sizeof(Part) * (size_t)(batch * p.parts)) + rounded(sizeof(State) * (size_t)batch));
     return p;
 }
 
@@ -1026,8 +1085,12 @@ template <typename L, typename Q> int launch(VerifyArgs a, const Plan& plan, voi
         a.parts_out = reinterpret_cast<Part*>(work);
         a.all_parts = a.parts_out;
         work += rounded(sizeof(Part) * (size_t)a.nodes * a.parts_per_row);
+        a.stands = reinterpret_cast<int32_t*>(work);
+        work += rounded(sizeof(int32_t) * (size_t)a.nodes);
         if (a.draft) hipLaunchKernelGGL((stats_kernel<L, false>), groups(a.nodes, kStatsGroups), dim3(kStepThreads), 0, stream, a);
         else hipLaunchKernelGGL((stats_kernel<L, true>), groups(a.nodes, kStatsGroups), dim3(kStepThreads), 0, stream, a);
+        const unsigned waves = kStepThreads / 64, of_nodes = ((unsigned)a.nodes + waves - 1) / waves;
+        hipLaunchKernelGGL((stands_kernel<L, Q>), dim3(of_nodes < 65536 ? of_nodes : 65536), dim3(kStepThreads), 0, stream, a);
     }
     for (int i = 0; i < 2; ++i) {
         a.parts[i] = reinterpret_cast<Part*>(work);
@@ -1039,7 +1102,7 @@ template <typename L, typename Q> int launch(VerifyArgs a, const Plan& plan, voi
     for (int i = 0; i < plan.steps; ++i) {
         a.turn = i & 1;
         if (a.draft) hipLaunchKernelGGL((step_kernel<L, Q, true>), groups(a.batch, kDrawnGroups), dim3(kStepThreads), 0, stream, a);
-        else hipLaunchKernelGGL((step_kernel<L, float, false>), groups(a.batch, plan.all ? 1 : i < 3 ? kGivenGroups : 2 * kGivenGroups), dim3(kStepThreads), 0, stream, a);
+        else hipLaunchKernelGGL((step_kernel<L, float, false>), groups(a.batch, i < 3 ? kGivenGroups : 2 * kGivenGroups), dim3(kStepThreads), 0, stream, a);
         a.fresh = 0;
     }
     if (!a.draft) hipLaunchKernelGGL((last_kernel<L>), groups(a.batch, kLastGroups), dim3(kStepThreads), 0, stream, a);
@@ -1060,9 +1123,9 @@ bool is_float(int32_t dtype) { return dtype == FSTA_F32 || dtype == FSTA_F16 || 
 
 using namespace fsta;
 
-extern "C" size_t fsta_verify_workspace_bytes(int32_t batch, int32_t nodes, int32_t vocabulary, int32_t logits_dtype, int32_t draft) {
-    if (batch <= 0 || nodes < 0 || vocabulary < 1) return 0;
-    return plan_of(batch, nodes, vocabulary, logits_dtype == FSTA_F32 ? 4 : 2, draft != 0, 1).bytes;
+extern "C" size_t fsta_verify_workspace_bytes(int32_t batch, int32_t nodes, int32_t vocabulary, int32_t max_path, int32_t draft) {
+    if (batch <= 0 || nodes < 0 || vocabulary < 1 || max_path < 1) return 0;
+    return plan_of(batch, nodes, vocabulary, draft != 0, max_path).bytes;
 }
 
 extern "C" int fsta_verify_drafts(const void* logits, int64_t logits_stride, int32_t logits_dtype, const void* draft, int64_t draft_stride,
@@ -1086,7 +1149,7 @@ extern "C" int fsta_verify_drafts(const void* logits, int64_t logits_stride, int
     if (misaligned(logits, size) || (draft && misaligned(draft, draft_size)) || misaligned(tokens, 8) || misaligned(parent, 8) || misaligned(next_tokens, 8) ||
         misaligned(q_starts, 4) || misaligned(u_accept, 4) || misaligned(u_next, 4) || misaligned(temperatures, 4) || misaligned(path, 4) || misaligned(counts, 4))
         return fail(FSTA_EINVAL, "%s: a tensor is not aligned to its elements", who);
-    const Plan plan = plan_of(batch, nodes, vocabulary, (int)size, draft != nullptr, max_path);
+    const Plan plan = plan_of(batch, nodes, vocabulary, draft != nullptr, max_path);
     if (plan.bytes && (!workspace || misaligned(workspace, 16) || workspace_bytes < plan.bytes))
         return fail(FSTA_EINVAL, "%s: workspace of %zu bytes (%zu needed, 16-byte aligned)", who, workspace_bytes, plan.bytes);
     VerifyArgs a = {};

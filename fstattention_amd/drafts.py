@@ -98,7 +98,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parent: torch.Tens
     counts = torch.empty((batch,), dtype=torch.int32, device=dev)
     next_tokens = torch.empty((batch,), dtype=torch.int64, device=dev)
     code = _FLOATS[logits.dtype]
-    need = lib.fsta_verify_workspace_bytes(batch, nodes, vocabulary, code, draft_probs is not None)
+    need = lib.fsta_verify_workspace_bytes(batch, nodes, vocabulary, max_path, draft_probs is not None)
     work = torch.empty((need,), dtype=torch.uint8, device=dev)
     with _on_device(dev):
         _lib.check(lib.fsta_verify_drafts(logits.data_ptr(), stride, code, None if draft_probs is None else draft_probs.data_ptr(), draft_stride,

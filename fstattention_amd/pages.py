@@ -3,9 +3,9 @@ shared among them, copied, taken back.
 
 The arrays are those of :mod:`fstattention_amd.paged`, and like there the host reads none of them: nothing here waits for the GPU.
 Beside them a program keeps ``refs`` int32 ``[num_pages]``: by how many entries of the page table a page is held.  A page with 0 is free,
-so ``torch.zeros`` (and a page table of -1) is where a server starts; from then on only the calls here change it.  ``caches`` is a :class:`PagedKV` or a list or tuple of them,
-one per layer (a plain tuple of its four tensors will do); they share ``num_pages`` and ``page_size``, so that one page table serves all, and
-may differ in heads, head_dim and dtype.  All layers go in one launch (32 at a time).
+so ``torch.zeros`` (and a page table of -1) is where a server starts; from then on only the calls here change both.  ``caches`` is a
+:class:`PagedKV` or a list or tuple of them, one per layer (a plain tuple of its four tensors will do); they share ``num_pages`` and
+``page_size``, so that one page table serves all, and may differ in heads, head_dim and dtype.  All layers go in one launch (32 at a time).
 
 The compute is ``libfsta.so``'s (``include/fsta.h``), on torch's current stream; there is no CPU fallback.  Tensors are changed in place,
 and their version counters move, as by an operation in place of torch's own; caches that require a gradient, or carry a tangent, are refused.

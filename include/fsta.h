@@ -551,7 +551,7 @@ int fsta_tree_bits(const int64_t* parent, const int32_t* q_starts, int32_t batch
  * when the work queued on `stream` has run.
  */
 #define FSTA_VERIFY_MAX_CHILDREN 2048
-size_t fsta_verify_workspace_bytes(int32_t batch, int32_t nodes, int32_t vocabulary, int32_t logits_dtype,
+size_t fsta_verify_workspace_bytes(int32_t batch, int32_t nodes, int32_t vocabulary, int32_t max_path,
                                    int32_t draft);
 int fsta_verify_drafts(const void* logits, int64_t logits_stride, int32_t logits_dtype, const void* draft,
                        int64_t draft_stride, int32_t draft_dtype, const int64_t* tokens,

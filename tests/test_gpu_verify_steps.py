@@ -15,14 +15,12 @@ def by_steps(case):
     """The case on the GPU with rows behind the last sequence, until there are too many to sum all."""
     gpu = on_gpu(case)
     nodes, vocabulary = gpu["logits"].shape
-    size = gpu["logits"].element_size()
-    more = max(int(200e6 / (vocabulary * size)) + 1 - nodes, 0)
+    more = max(int(200e6 / vocabulary) + 1 - nodes, 0)
     pad = lambda t, x: torch.cat([t, torch.full((more, *t.shape[1:]), x, dtype=t.dtype, device="cuda")])
     gpu = {**gpu, "logits": pad(gpu["logits"], 7.0), "tokens": pad(gpu["tokens"], 0), "parent": pad(gpu["parent"], 0), "u_accept": pad(gpu["u_accept"], 0.0),
            "draft_probs": None if gpu["draft_probs"] is None else pad(gpu["draft_probs"], 0.5)}
     # no room for a sum of every row
-    code = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}[case["logits"].dtype]
-    work = [_lib.load().fsta_verify_workspace_bytes(1, nodes + more + i, vocabulary, code, case["draft_probs"] is not None) for i in range(2)]
+    work = [_lib.load().fsta_verify_workspace_bytes(1, nodes + more + i, vocabulary, 8, case["draft_probs"] is not None) for i in range(2)]
     assert work[0] == work[1]
     return gpu
 
