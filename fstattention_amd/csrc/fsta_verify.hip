@@ -299,6 +299,42 @@ __device__ __forceinline__ void first_sums(const L* row, double rate, int vocabu
     double sum = 0.0;
 #pragma unroll 1
     for (int i1 = p * part_length; i1 < last; i1 += kPart) {
+        if (QUICK && rate != 0.0) {
+            // one largest logit for four runs, and the next four on their way as soon as these are taken apart
+            float x[kRing][8], m = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < kRing; ++r) {
+                const int i0 = i1 + r * kRun, i = i0 + lane * 8;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[r][e] = value(ring[r], e);
+                if (i0 + kRun > vocabulary) leave_out(outside(first_of(i, vocabulary), i, vocabulary), -INFINITY, x[r]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m = fmaxf(m, x[r][e]);
+                ring[r] = load(min(i0 + kPart, last));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            m = max_of(m);
+            if (m > top) {
+                if (sum > 0.0) sum *= weight_of(top, m, rate);
+                top = m;
+            }
+            const float by = fmaxf((float)rate, 1e-30f);         // (times -inf: -inf)
+            if (top < INFINITY) {
+#pragma unroll
+                for (int r = 0; r < kRing; ++r) {
+                    float w[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(fmaxf(x[r][e] - top, -INFINITY) * by);
+                    sum += (double)(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < kRing; ++r) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum += x[r][e] == top ? 1.0 : 0.0;
+                }
+            }
+        } else {
 #pragma unroll
         for (int r = 0; r < kRing; ++r) {
             const int i0 = i1 + r * kRun, i = i0 + lane * 8, at = first_of(i, vocabulary);
@@ -322,14 +358,7 @@ __device__ __forceinline__ void first_sums(const L* row, double rate, int vocabu
                         if (sum > 0.0) sum *= weight_of(top, m, rate);
                         top = m;
                     }
-                    if constexpr (QUICK) {
-                        float w[8];
-                        const float by = fmaxf((float)rate, 1e-30f);     // (times -inf: -inf)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            w[e] = top < INFINITY ? __builtin_amdgcn_exp2f(fmaxf(x[e] - top, -INFINITY) * by) : x[e] == top ? 1.f : 0.f;
-                        sum += (double)(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
-                    } else if (top > -INFINITY) {
+                    if (!QUICK && top > -INFINITY) {
                         double w[8];
                         weights_of(x, top, rate, w);
 #pragma unroll
@@ -340,6 +369,7 @@ __device__ __forceinline__ void first_sums(const L* row, double rate, int vocabu
             // (behind the last use of what it replaces, so that it comes to the same registers)
             ring[r] = load(min(i0 + kPart, last));
             __builtin_amdgcn_sched_barrier(0);
+        }
         }
         if (i1 + kPart < end) continue;
         Part part{1.0, top, best};
@@ -885,7 +915,7 @@ __device__ __forceinline__ int sequence_of(const VerifyArgs& a, int64_t t) {
 }
 
 // blockIdx.x: parts of a row, .y: node
-template <typename L, bool QUICK> __global__ __launch_bounds__(kStepThreads, QUICK ? 4 : 3) void stats_kernel(VerifyArgs a) {
+template <typename L, bool QUICK> __global__ __launch_bounds__(kStepThreads, QUICK && sizeof(L) == 2 ? 4 : 3) void stats_kernel(VerifyArgs a) {
     constexpr int kWaves = kStepThreads / 64;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     for (int64_t t = blockIdx.y; t < a.nodes; t += gridDim.y) {
