@@ -973,6 +973,9 @@ template <typename L, typename Q, bool DRAWN> __global__ __launch_bounds__(kStep
         Walk<L, Q, kStepThreads> w(a, &sh, b, speaks);
         if (w.nodes == 0) {
             s.phase = kDone;
+        } else if (a.fresh && !a.all_parts) {         // the roots' sums wait for nothing
+            w.stand_on(0, 1);
+            w.note(0, 1);
         } else {
             w.where = a.turn ^ 1;
             w.resume(s, a.fresh ? nullptr : w.parts_of_step(a.turn ^ 1));
@@ -1091,7 +1094,7 @@ constexpr double kAllGiven = 80e6, kAllDrawn = 20e6, kAllChains = 200e6;
 // instead of a row's share of them all, but a launch less).  With all sums there a step is one that falls: a chain has one, trees
 // of four children 105 us with four steps, 112 with three, 100 with six; of three 84, 82 and 90.
 constexpr int kMostSteps = 10, kDrawnSteps = 4;
-constexpr int kStatsGroups = 2048, kDrawnGroups = 512, kGivenGroups = 768, kLastGroups = 768;
+constexpr int kStatsGroups = 2048, kDrawnGroups = 512, kGivenGroups = 512, kLastGroups = 768;
 
 Plan plan_of(int64_t batch, int64_t nodes, int64_t vocabulary, bool draft, int32_t max_path) {
     Plan p;
