@@ -7,13 +7,23 @@
 // kept per token.  Without the draft's probabilities a child is its own proposal: W loses the token, nothing else.
 //
 // Decisions compare sums over the vocabulary with a random number, and the next token is the place where a running sum passes
-// one: in 32 bits a sum of 10^5 terms is off by more than many of them are large, so weights and sums are 64 bits here.
+// one: in 32 bits a sum of 10^5 terms is off by more than many of them are large, so weights and sums are of 64 bits.  Only a first
+// sum (of P) without draft probabilities may be one of 32 bits with a bound of its error (kDoubt): a decision inside the bound is taken once more
+// by 64, and the token is always picked by 64.
 //
-// A row is summed in parts of 2048 tokens, a wave each.  What depends on a sum comes in a later launch:
-//   stats_kernel  the parts of the rows of all nodes with children (few rows: the walks behind it do not wait for sums);
-//   step_kernel   one step of all sequences: each workgroup takes the decisions that the sums so far allow (all workgroups of a
-//                 sequence the same ones), and its parts of the sum that is wanted next.  Only the rows on accepted paths are read;
-//   walk_kernel   a workgroup per sequence goes on alone from wherever a sequence is to its end, and picks its next token.
+// A row is summed in parts of 2048 tokens, a wave each.  What depends on a sum comes in a later launch.  Where the rows of all nodes
+// are few enough (chains(), kAllGiven):
+//   stats_kernel   the parts of the rows of all nodes with children;
+//   stands_kernel  which child stands at each node by these sums: walks only follow;
+//   step_kernel    with draft probabilities: sums of W where a child fell, one of every sequence's a launch;
+//   last_kernel    without: the row at each walk's end in 64 bits;
+// and where they are not
+//   step_kernel    one step of all sequences: each workgroup takes the decisions that the sums so far allow (all workgroups of a
+//                  sequence the same ones), and its parts of the sum that is wanted next.  Only the rows on accepted paths are read;
+//   last_kernel    as above.  In both cases then
+//   walk_kernel    a workgroup per sequence goes on alone from wherever a sequence is to its end, and picks its next token.
+// What bounds it: few rows, the chain of launches and of loads that need each other (8 to 20 us before the first sum and behind the last);
+// many, the exponentials: 95 cycles of a SIMD for 64 of 64 bits, some 35 for 64 of 32.
 #include "fsta_common.h"
 
 namespace fsta {
@@ -158,6 +168,12 @@ __device__ __forceinline__ void weights_of(const float (&l)[8], float against, d
         }
         __builtin_amdgcn_sched_barrier(0);
     }
+}
+
+// log2(e) / T of a sequence; 0: greedy
+__device__ __forceinline__ double rate_of(const VerifyArgs& a, int b) {
+    const float tau = a.temperatures ? a.temperatures[b] : a.temperature;
+    return tau > 0.f ? fmax(1.4426950408889634074 / (double)tau, 1e-300) : 0.0;
 }
 
 // The weights of one row: P against its largest logit, W with the draft's row
@@ -336,40 +352,40 @@ __device__ __forceinline__ void first_sums(const L* row, double rate, int vocabu
             }
         } else {
 #pragma unroll
-        for (int r = 0; r < kRing; ++r) {
-            const int i0 = i1 + r * kRun, i = i0 + lane * 8, at = first_of(i, vocabulary);
-            if (i0 < last) {
-                float x[8], m = -INFINITY;                       // (fmaxf passes over a NaN)
+            for (int r = 0; r < kRing; ++r) {
+                const int i0 = i1 + r * kRun, i = i0 + lane * 8, at = first_of(i, vocabulary);
+                if (i0 < last) {
+                    float x[8], m = -INFINITY;                       // (fmaxf passes over a NaN)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = value(ring[r], e);
-                if (i0 + kRun > vocabulary) leave_out(outside(at, i, vocabulary), -INFINITY, x);
+                    for (int e = 0; e < 8; ++e) x[e] = value(ring[r], e);
+                    if (i0 + kRun > vocabulary) leave_out(outside(at, i, vocabulary), -INFINITY, x);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);
-                if (rate == 0.0) {
-                    if (m > top) {
-                        top = m;
+                    for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);
+                    if (rate == 0.0) {
+                        if (m > top) {
+                            top = m;
 #pragma unroll
-                        for (int e = 7; e >= 0; --e)
-                            if (x[e] == m) best = at + e;
-                    }
-                } else {
-                    m = max_of(m);
-                    if (m > top) {
-                        if (sum > 0.0) sum *= weight_of(top, m, rate);
-                        top = m;
-                    }
-                    if (!QUICK && top > -INFINITY) {
-                        double w[8];
-                        weights_of(x, top, rate, w);
+                            for (int e = 7; e >= 0; --e)
+                                if (x[e] == m) best = at + e;
+                        }
+                    } else {
+                        m = max_of(m);
+                        if (m > top) {
+                            if (sum > 0.0) sum *= weight_of(top, m, rate);
+                            top = m;
+                        }
+                        if (!QUICK && top > -INFINITY) {
+                            double w[8];
+                            weights_of(x, top, rate, w);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) sum += w[e];
+                            for (int e = 0; e < 8; ++e) sum += w[e];
+                        }
                     }
                 }
+                // (behind the last use of what it replaces, so that it comes to the same registers)
+                ring[r] = load(min(i0 + kPart, last));
+                __builtin_amdgcn_sched_barrier(0);
             }
-            // (behind the last use of what it replaces, so that it comes to the same registers)
-            ring[r] = load(min(i0 + kPart, last));
-            __builtin_amdgcn_sched_barrier(0);
-        }
         }
         if (i1 + kPart < end) continue;
         Part part{1.0, top, best};
@@ -914,7 +930,9 @@ __device__ __forceinline__ int sequence_of(const VerifyArgs& a, int64_t t) {
     return b;
 }
 
-// blockIdx.x: parts of a row, .y: node
+// The first sums of all rows, largest logit and sum in one pass.  blockIdx.x: parts of a row, .y: node.  250 rows of 32000 float32 (16 trees of
+// 64 nodes) 18 us in sums of 32 bits, 32 MB; 32 trees' of 50021 float16 with draft probabilities 22.5 us in 64.  2048 workgroups for all rows: 1024 56
+// us instead of 53.5 for 8 x 64 rows of 131072 tokens, 4096 52 there and 52 instead of 50 for 16 x 64 of 32000.
 template <typename L, bool QUICK> __global__ __launch_bounds__(kStepThreads, QUICK && sizeof(L) == 2 ? 4 : 3) void stats_kernel(VerifyArgs a) {
     constexpr int kWaves = kStepThreads / 64;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -925,16 +943,16 @@ template <typename L, bool QUICK> __global__ __launch_bounds__(kStepThreads, QUI
         uint64_t any = 0;
         for (int64_t j = t + 1; j < end && !any; j += 64) any = __ballot(j + lane < end && a.parent[j + lane] == node);
         if (!any) continue;
-        const float tau = a.temperatures ? a.temperatures[b] : a.temperature;
-        const double rate = tau > 0.f ? fmax(1.4426950408889634074 / (double)tau, 1e-300) : 0.0;
+        const double rate = rate_of(a, b);
         const int which = blockIdx.x * kWaves + wave, waves = gridDim.x * kWaves;
         first_sums<QUICK>(static_cast<const L*>(a.logits) + t * a.logits_stride, rate, a.vocabulary, a.part_length,
                    (int)((int64_t)a.parts_per_row * which / waves), (int)((int64_t)a.parts_per_row * (which + 1) / waves), a.parts_out + t * a.parts_per_row);
     }
 }
 
-// Which child stands at each node, by the first sums of all rows, a wave per node: what a walk comes through does not wait for one
-// decision after the other.
+// Which child stands at each node, by the first sums of all rows, a wave per node: a walk does not wait for one decision after the
+// other (2 us each: parts, largest, sum, the children's logits).  4.4 us for a chain of 6, 7.3 for 16 trees of 64; the call without it 38 instead
+// of 29 us, and 55 instead of 53.
 template <typename L, typename Q> __global__ __launch_bounds__(kStepThreads) void stands_kernel(VerifyArgs a) {
     const int lane = threadIdx.x & 63;
     for (int64_t t = (int64_t)blockIdx.x * (kStepThreads / 64) + (threadIdx.x >> 6); t < a.nodes; t += (int64_t)gridDim.x * (kStepThreads / 64)) {
@@ -956,7 +974,8 @@ template <typename L, typename Q> __global__ __launch_bounds__(kStepThreads) voi
 
 // blockIdx.x: parts of a row, .y: sequence.  DRAWN: there are the draft's probabilities, and sums are 64 bits.  Without them a first
 // sum of 32 bits is enough for almost every decision; rows whose sum has to be 64 bits wait for last_kernel, sums without what fell for
-// walk_kernel.
+// walk_kernel.  128 sequences, 131072 bfloat16: 11 us the roots' step (33 MB), 15 to 10 the next ones while ever fewer go on; 5 to 6 of them pass
+// before the first load of a row (state, tree, the parts so far, the children's logits).  32 sequences of 50021, drawn: 10 us.
 template <typename L, typename Q, bool DRAWN> __global__ __launch_bounds__(kStepThreads, DRAWN ? 2 : 3) void step_kernel(VerifyArgs a) {
     constexpr int kWaves = kStepThreads / 64;
     __shared__ Shared sh;
@@ -998,14 +1017,11 @@ template <typename L, typename Q, bool DRAWN> __global__ __launch_bounds__(kStep
 
 // Sums of 64 bits where there are none: of the row that a sequence's next token is picked from, and of rows whose children's fate
 // sums of 32 bits do not tell.  They go to the buffer that the last step did not write.  Without steps that is the row of the last child that
-// is known to stand.  blockIdx.x: parts of a row, .y: sequence
+// is known to stand.  blockIdx.x: parts of a row, .y: sequence.  128 rows of 131072 bfloat16 23 us, of which the exponentials take half; 16 of
+// 32000 float32 7 us.
 __device__ __forceinline__ bool wants_last(const VerifyArgs& a, const State& s, double rate) {
     if (a.fresh) return a.all_parts && rate != 0.0;
     return s.phase == kDone ? s.held == kQuick && rate != 0.0 : s.phase == kFirst && !s.ready;
-}
-__device__ __forceinline__ double rate_of(const VerifyArgs& a, int b) {
-    const float tau = a.temperatures ? a.temperatures[b] : a.temperature;
-    return tau > 0.f ? fmax(1.4426950408889634074 / (double)tau, 1e-300) : 0.0;
 }
 template <typename L> __global__ __launch_bounds__(kStepThreads, 3) void last_kernel(VerifyArgs a) {
     constexpr int kWaves = kStepThreads / 64;
@@ -1033,6 +1049,9 @@ template <typename L> __global__ __launch_bounds__(kStepThreads, 3) void last_ke
     }
 }
 
+// What is left of every walk, and the next tokens, a workgroup per sequence: sums here are one workgroup's work, so that launches before it
+// leave few.  8 us where nothing is left but to pick, 15 for 128 sequences of 131072 tokens, 19 where the decisions at the last node come first
+// (16 trees): loads that need each other, and ten barriers.
 template <typename L, typename Q> __global__ __launch_bounds__(kWalkThreads, 2) void walk_kernel(VerifyArgs a) {
     __shared__ Shared sh;
     for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
@@ -1087,6 +1106,7 @@ bool chains(int64_t batch, int64_t nodes, int32_t max_path) { return max_path <=
 // Sums of all rows first, or only of the rows that walks come to, a launch each?  The first costs with all nodes' tokens, the second a launch
 // (and what comes before its first sum) per node of the longest path.  Measured, all rows / steps, us:
 //   no draft probabilities  16 x 64 nodes of 32000 tokens 53 / 68, 32 x 64 68 / 71, 8 x 64 of 131072 65 / 66, 64 x 23 of 50021 60 / 76, 16 x 64 of 131072 96 / 67
+//                           (both ways have gained since: 54 the third, 60 the last)
 //   with them               4 x 64 of 50021 73 / 90, 8 x 23 of 131072 76 / 77, 32 x 23 of 32000 79 / 80, 8 x 64 of 50021 105 / 91
 //   chains                  256 x 6 of 131072 152 / 170, with draft probabilities 128 x 6 133 / 171
 constexpr double kAllGiven = 80e6, kAllDrawn = 20e6, kAllChains = 200e6;
@@ -1094,6 +1114,9 @@ constexpr double kAllGiven = 80e6, kAllDrawn = 20e6, kAllChains = 200e6;
 // instead of a row's share of them all, but a launch less).  With all sums there a step is one that falls: a chain has one, trees
 // of four children 105 us with four steps, 112 with three, 100 with six; of three 84, 82 and 90.
 constexpr int kMostSteps = 10, kDrawnSteps = 4;
+// Workgroups that share the rows of a launch.  Steps without draft probabilities: 128 sequences of 131072 tokens 116 us with 512 and twice as many
+// behind the third step, when fewer sequences are left (117 with 512 throughout, 124 with 384, 122 with 768, 131 with 1024); with them
+// 182 with 512, 235 with 384, 229 with 768; last rows 121 with 512, 768 and 1024.
 constexpr int kStatsGroups = 2048, kDrawnGroups = 512, kGivenGroups = 512, kLastGroups = 768;
 
 Plan plan_of(int64_t batch, int64_t nodes, int64_t vocabulary, bool draft, int32_t max_path) {
@@ -1103,7 +1126,8 @@ Plan plan_of(int64_t batch, int64_t nodes, int64_t vocabulary, bool draft, int32
     p.all = (double)nodes * vocabulary <= (chains(batch, nodes, max_path) ? kAllChains : draft ? kAllDrawn : kAllGiven);
     p.steps = max_path + (draft ? 3 : 0) < kMostSteps ? max_path + (draft ? 3 : 0) : kMostSteps;
     if (p.all) p.steps = draft ? (chains(batch, nodes, max_path) ? 1 : kDrawnSteps) : 0;
-    p.bytes = (p.all ? rounded(sizeof(Part) * (size_t)(nodes * p.parts)) + rounded(sizeof(int32_t) * (size_t)nodes) : 0) + 2 * (rounded(sizeof(Part) * (size_t)(batch * p.parts)) + rounded(sizeof(State) * (size_t)batch));
+    p.bytes = 2 * (rounded(sizeof(Part) * (size_t)(batch * p.parts)) + rounded(sizeof(State) * (size_t)batch));
+    if (p.all) p.bytes += rounded(sizeof(Part) * (size_t)(nodes * p.parts)) + rounded(sizeof(int32_t) * (size_t)nodes);
     return p;
 }
 
