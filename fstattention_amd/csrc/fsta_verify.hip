@@ -922,12 +922,18 @@ template <typename L, typename Q, int THREADS> struct Walk {
     }
 };
 
-// A node's sequence: how many start at or before it
+// A node's sequence: how many start at or before it (less one), by 64 places at a time
 __device__ __forceinline__ int sequence_of(const VerifyArgs& a, int64_t t) {
     const int lane = threadIdx.x & 63;
-    int b = -1;
-    for (int c = 0; c < a.batch; c += 64) b += __popcll(__ballot(c + lane < a.batch && a.q_starts[c + lane] <= t));
-    return b;
+    int first = 0, count = a.batch;
+    while (count > 64) {
+        const int step = (count + 63) / 64, at = lane * step;
+        const int before = __popcll(__ballot(at < count && a.q_starts[first + min(at, count - 1)] <= t));
+        if (before == 0) return -1;
+        first += (before - 1) * step;
+        count = min(step, count - (before - 1) * step);
+    }
+    return first - 1 + __popcll(__ballot(lane < count && a.q_starts[first + min(lane, count - 1)] <= t));
 }
 
 // The first sums of all rows, largest logit and sum in one pass.  blockIdx.x: parts of a row, .y: node.  250 rows of 32000 float32 (16 trees of
