@@ -957,7 +957,7 @@ template <typename L, bool QUICK> __global__ __launch_bounds__(kStepThreads, QUI
 }
 
 // Which child stands at each node, by the first sums of all rows, a wave per node: a walk does not wait for one decision after the
-// other (2 us each: parts, largest, sum, the children's logits).  4.4 us for a chain of 6, 7.3 for 16 trees of 64; the call without it 38 instead
+// other (2 us each: parts, largest, sum, the children's logits).  4.4 us for a chain of 6, 7.3 for 16 trees of 64; the calls without it 38 instead
 // of 29 us, and 55 instead of 53.
 template <typename L, typename Q> __global__ __launch_bounds__(kStepThreads) void stands_kernel(VerifyArgs a) {
     const int lane = threadIdx.x & 63;
@@ -1056,7 +1056,7 @@ template <typename L> __global__ __launch_bounds__(kStepThreads, 3) void last_ke
 }
 
 // What is left of every walk, and the next tokens, a workgroup per sequence: sums here are one workgroup's work, so that launches before it
-// leave few.  8 us where nothing is left but to pick, 15 for 128 sequences of 131072 tokens, 19 where the decisions at the last node come first
+// leave few.  8 us where nothing is left but to pick, 14 for 128 sequences of 131072 tokens, 17 where the decisions at the last node come first
 // (16 trees): loads that need each other, and ten barriers.  256 threads look at a part at once, and two workgroups fit a CU: with 512 the call for
 // 500 trees of 32000 tokens takes 110 us instead of 100, for 2000 of 8000 173 instead of 137, for few the same; with 128 one to two more up to
 // 500, 131 for 2000.
