@@ -1118,6 +1118,7 @@ bool chains(int64_t batch, int64_t nodes, int32_t max_path) { return max_path <=
 //   with them               4 x 64 of 50021 73 / 90, 8 x 23 of 131072 76 / 77, 32 x 23 of 32000 79 / 80, 8 x 64 of 50021 105 / 91
 //   chains                  256 x 6 of 131072 152 / 170, with draft probabilities 128 x 6 133 / 171
 constexpr double kAllGiven = 80e6, kAllDrawn = 20e6, kAllChains = 200e6;
+constexpr int64_t kLargeTree = 1 << 17;   // (a node looks for its children through all behind it: walks do that at a few nodes, all rows at each)
 // Steps: one per node of a path, and of each child that falls for draft probabilities some more; behind ten the walks go on alone (a workgroup
 // instead of a row's share of them all, but a launch less).  With all sums there a step is one that falls: a chain has one, trees
 // of four children 105 us with four steps, 112 with three, 100 with six; of three 84, 82 and 90.
@@ -1132,6 +1133,7 @@ Plan plan_of(int64_t batch, int64_t nodes, int64_t vocabulary, bool draft, int32
     p.part_length = (int32_t)((vocabulary + (int64_t)kPart * kMaxParts - 1) / ((int64_t)kPart * kMaxParts) * kPart);
     p.parts = (int32_t)((vocabulary + p.part_length - 1) / p.part_length);
     p.all = (double)nodes * vocabulary <= (chains(batch, nodes, max_path) ? kAllChains : draft ? kAllDrawn : kAllGiven);
+    p.all = p.all && (nodes <= kLargeTree || nodes <= 16 * batch);
     p.steps = max_path + (draft ? 3 : 0) < kMostSteps ? max_path + (draft ? 3 : 0) : kMostSteps;
     if (p.all) p.steps = draft ? (chains(batch, nodes, max_path) ? 1 : kDrawnSteps) : 0;
     p.bytes = 2 * (rounded(sizeof(Part) * (size_t)(batch * p.parts)) + rounded(sizeof(State) * (size_t)batch));

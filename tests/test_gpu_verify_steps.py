@@ -172,6 +172,23 @@ def test_random_numbers_next_to_what_decides(tau):
     check_both(more, 1, tau)
 
 
+def test_a_large_tree():
+    """More nodes than all rows are summed of, whatever they cost."""
+    n, vocabulary = 140000, 41
+    case = make_case(8, [3], vocabulary, torch.float32, 2, None)
+    g = torch.Generator().manual_seed(8)
+    case = {**case, "logits": torch.randn((n, vocabulary), generator=g), "tokens": torch.randint(vocabulary, (n,), generator=g),
+            "u_accept": torch.rand((n,), generator=g), "q_starts": torch.tensor([0, n], dtype=torch.int32), "u_next": torch.rand((1,), generator=g)}
+    case["parent"] = (torch.arange(n) - 1 - (torch.rand((n,), generator=g) * 3000).long()).clamp(min=0)
+    case["parent"][0] = -1
+    case["logits"][case["parent"][1:], case["tokens"][1:]] = 6.0
+    work = [_lib.load().fsta_verify_workspace_bytes(1, n + i, vocabulary, 9, 0) for i in range(2)]
+    assert work[0] == work[1]
+    want = expected(case, 9)
+    assert want[1][0] == 3                                     # the oracle's: nodes 0, 44 and 2255
+    check(call(on_gpu(case), 9), want)
+
+
 @pytest.mark.parametrize("draft", [None, torch.float32])
 @pytest.mark.parametrize("vocabulary", [301, 9001])
 def test_more_fall_than_there_are_launches(draft, vocabulary):
