@@ -536,7 +536,8 @@ int launch_copies(const CopyArgs& a, int32_t most, int32_t most_groups, const fs
 }
 
 constexpr size_t kAlign = 16;
-constexpr int32_t kMaxRows = 1 << 24;     // sequences of a table, pairs of a call
+constexpr int32_t kMaxRows = 1 << 24;     // pairs of pages
+constexpr int32_t kMaxSequences = 1 << 16;            // (each looks at what those before it want)
 size_t rounded(size_t bytes) { return (bytes + kAlign - 1) / kAlign * kAlign; }
 
 size_t table_workspace(int64_t rows, int64_t width, int64_t num_pages, TableArgs* a, void* at) {
@@ -577,8 +578,8 @@ int check_table(const char* who, int32_t batch, int32_t width, int32_t page_size
                 int32_t num_pages, const void* missing, bool any) {
     if (batch < 0 || width < 0) return fail(FSTA_EINVAL, "%s: batch=%d width=%d", who, batch, width);
     if ((int64_t)width * page_size > 0x7fffffc0ll) return fail(FSTA_EUNSUPPORTED, "%s: %d pages of %d keys in a sequence", who, width, page_size);
-    // (pages wanted are counted over the batch, and rows with groups of pages, in 31 bits)
-    if (batch > kMaxRows || (int64_t)batch * width > INT32_MAX) return fail(FSTA_EUNSUPPORTED, "%s: batch=%d width=%d", who, batch, width);
+    // (pages wanted are counted over the batch in 31 bits)
+    if (batch > kMaxSequences || (int64_t)batch * width > INT32_MAX) return fail(FSTA_EUNSUPPORTED, "%s: batch=%d width=%d", who, batch, width);
     if (any && ((num_pages > 0 && !refs) || (width > 0 && !table) || !lens || !missing)) return fail(FSTA_EINVAL, "%s: null pointer", who);
     if (misaligned(refs, 4) || misaligned(table, 4) || misaligned(lens, 4) || misaligned(missing, 4))
         return fail(FSTA_EINVAL, "%s: refs, page_table, lens and missing must be 4-byte aligned", who);
@@ -602,7 +603,7 @@ extern "C" int fsta_compact_paged_kv(const fsta_paged_pool* pools, int32_t layer
     if ((max_path > 0 && !path) || !counts || (width > 0 && !page_table) || !kv_lens || !q_starts || !new_lens) return fail(FSTA_EINVAL, "%s: null pointer", who);
     if (misaligned(path, 4) || misaligned(counts, 4) || misaligned(page_table, 4) || misaligned(kv_lens, 4) || misaligned(q_starts, 4) || misaligned(new_lens, 4))
         return fail(FSTA_EINVAL, "%s: path, counts, page_table, kv_lens, q_starts and new_lens must be 4-byte aligned", who);
-    if (batch > kMaxRows) return fail(FSTA_EUNSUPPORTED, "%s: batch=%d", who, batch);
+    if (batch > kMaxSequences) return fail(FSTA_EUNSUPPORTED, "%s: batch=%d", who, batch);
     // rows move in place: of two workgroups with the same pool one would read what the other has moved
     for (int32_t l = 0; l < layers && num_pages > 0; ++l) {
         bool twice = pools[l].k == pools[l].v;
@@ -682,7 +683,7 @@ extern "C" int fsta_fork_pages(const fsta_paged_pool* pools, int32_t layers, int
     int rc = check_pools(who, pools, pools, layers, num_pages, page_size);
     if (rc != FSTA_OK) return rc;
     if (pairs < 0) return fail(FSTA_EINVAL, "%s: pairs=%d", who, pairs);
-    if (pairs > kMaxRows) return fail(FSTA_EUNSUPPORTED, "%s: pairs=%d", who, pairs);
+    if (pairs > kMaxSequences) return fail(FSTA_EUNSUPPORTED, "%s: pairs=%d", who, pairs);
     rc = check_table(who, batch, width, page_size, refs, page_table, lens, num_pages, missing, pairs > 0 && batch > 0);
     if (rc != FSTA_OK) return rc;
     if (pairs == 0) return FSTA_OK;

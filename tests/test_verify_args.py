@@ -99,9 +99,9 @@ def test_compact_with_a_pool_twice():
 
 
 def test_more_rows_than_31_bits_count():
-    for entry, base, change, word in (("fsta_fit_pages", FIT, dict(batch=2 ** 31 - 1), "batch"), ("fsta_fit_pages", FIT, dict(batch=1 << 24, width=128), "width"),
-                                      ("fsta_fork_pages", FORK, dict(batch=1 << 24, width=128), "width"), ("fsta_fork_pages", FORK, dict(pairs=1 << 25), "pairs"),
-                                      ("fsta_copy_pages", COPY, dict(pairs=2 ** 31 - 1), "pairs"), ("fsta_compact_paged_kv", COMPACT, dict(batch=1 << 25), "batch")):
+    for entry, base, change, word in (("fsta_fit_pages", FIT, dict(batch=2 ** 31 - 1), "batch"), ("fsta_fit_pages", FIT, dict(batch=1 << 16, width=1 << 15), "width"),
+                                      ("fsta_fork_pages", FORK, dict(batch=1 << 16, width=1 << 15), "width"), ("fsta_fork_pages", FORK, dict(pairs=(1 << 16) + 1), "pairs"),
+                                      ("fsta_copy_pages", COPY, dict(pairs=2 ** 31 - 1), "pairs"), ("fsta_compact_paged_kv", COMPACT, dict(batch=(1 << 16) + 1), "batch")):
         _refused(entry, base, change, word)
 
 
