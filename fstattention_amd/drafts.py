@@ -57,13 +57,14 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parent: torch.Tens
     logit, the first of equals.  Tokens that may not be chosen (top-k, top-p, a grammar) have logits of -inf.
 
     ``draft_probs [T, V]``: row ``t`` holds the probabilities from which node ``t``'s children were drawn, one after the other in the
-    order of their numbers, no token twice (rows of leaves are not read).  Without it the children are taken for a given list, such as a draft head's
-    best guesses.  In both cases the token behind what was committed so far is distributed as the model's own: a drafted one where a child
-    stands, ``next_tokens`` otherwise.  Sums and comparisons are made in 64 bits: equal inputs give equal answers, whatever the batch.
+    order of their numbers, no token twice (rows of leaves are not read).  Without it the children are taken for a given list, such as a
+    draft head's best guesses.  In both cases the token behind what was committed so far is distributed as the model's own: a drafted one
+    where a child stands, ``next_tokens`` otherwise.  Answers are those of sums and comparisons in 64 bits: equal inputs give equal answers,
+    whatever the batch.
 
-    A path ends at ``max_path`` nodes (the depth of the trees plus 1 loses nothing); of a node's children the first 2048 are asked.  A row
-    of nothing but -inf (or NaN, which counts as that) leaves no token: ``next_tokens`` is -1; logits of +inf share all mass.  Sequences
-    without nodes have no path and no token (0 and -1).  ``path`` and ``counts`` are what :func:`compact_paged_kv` takes."""
+    A path ends at ``max_path`` nodes (the depth of the trees plus 1 loses nothing, and more costs launches); of a node's children the first
+    2048 are asked.  A row of nothing but -inf (or NaN, which counts as that) leaves no token: ``next_tokens`` is -1; logits of +inf share all
+    mass.  Sequences without nodes have no path and no token (0 and -1).  ``path`` and ``counts`` are what :func:`compact_paged_kv` takes."""
     out = _calls().verify_drafts(logits, tokens, parent, q_starts, u_accept, u_next, max_path, temperature, draft_probs)
     if out is not NotImplemented:
         return Verified(*out)

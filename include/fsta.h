@@ -542,7 +542,7 @@ int fsta_tree_bits(const int64_t* parent, const int32_t* q_starts, int32_t batch
  * next token is distributed as the model's own.  T <= 0 or NaN: P is 1 for the largest logit (the first of
  * equals) and 0 elsewhere, the draft's probabilities are not looked at.
  * A NaN counts as -inf; logits of +inf share all mass; a row of nothing but -inf leaves no token: its
- * children fall and the next token is -1.  Sums and comparisons are made in 64 bits.
+ * children fall and the next token is -1.  Answers are those of sums and comparisons in 64 bits.
  *   path [batch, max_path] int32: the accepted nodes' numbers within their tree from the root, -1 behind
  *   them; a path that reaches max_path (>= 1) nodes ends there.  counts [batch] int32: how many.
  *   next_tokens [batch] int64.  A sequence of no nodes has none: 0 and -1.  At most
